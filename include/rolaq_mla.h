@@ -304,6 +304,74 @@ int rolaq_assemble_rows(const int64_t* slots, int64_t n, const uint8_t* codes, c
                         const int32_t* owner_of_row, const void* rotation, int D, int R, void* out,
                         int64_t out_stride, void* stream);
 
+/*
+ * The 4-bit (MX4) latent cache: no counterpart in the reference, whose cache is
+ * INT2 with a BF16 window. A layer's buffers, by token slot (0 .. num_slots - 1):
+ *   codes  u8 [num_slots, D / 2]: E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6; bit 3 the
+ *          sign), element 2 j in the low nibble of byte j, 2 j + 1 in the high one;
+ *   scales u8 [num_slots, D / 32]: byte s of elements 32 i .. 32 i + 31 stands for
+ *          2^(s - 127), 63 <= s <= 159; 255: all 32 are NaN;
+ *   rope   bf16 [num_slots, R].
+ * All three 16-byte aligned. An element is its level times its block's power of
+ * two, which bf16 holds exactly. (D, R) = (512, 64) or (256, 32).
+ */
+
+/*
+ * Stores n rows at slots loc[i]: y = latent R_eff in FP32 (rotation_t = R_eff^T,
+ * bf16 [D, D] row-major) or, with rotation_t null, y = latent. Per 32 elements the
+ * scale is the least power of two (from 2^-64) under which the largest magnitude
+ * is below 7; codes are rounded to nearest even, up to 6, so no element is off by more than
+ * half a step. A block that is not finite or would need a scale above 2^32 is
+ * stored as NaN. latent: bf16 [n, D], row stride latent_stride; k_pe: bf16, any
+ * strides. A slot outside the cache is skipped; slots of one call must differ,
+ * except for padding slots that nobody reads. One launch, no window.
+ */
+int rolaq_mx4_write_rows(const void* latent, int64_t latent_stride, const void* k_pe, int64_t pe_stride0,
+                         int64_t pe_stride1, const void* rotation_t, const int64_t* loc, int64_t n, int D, int R,
+                         uint8_t* codes, uint8_t* scales, void* rope_buf, int64_t num_slots, void* stream);
+
+/*
+ * Row i of out (bf16, stride out_stride) = [latent | rope] of slot slots[i]; with
+ * rotation (R_eff, bf16 [D, D] row-major) the latent is multiplied by R_eff^T in
+ * FP32 and rounded to bf16, without it the stored values are returned exactly. A
+ * slot outside the cache reads as NaN.
+ */
+int rolaq_mx4_read_rows(const int64_t* slots, int64_t n, const uint8_t* codes, const uint8_t* scales,
+                        const void* rope_buf, int64_t num_slots, const void* rotation, int D, int R, void* out,
+                        int64_t out_stride, void* stream);
+
+/* Bytes of rolaq_mx4_attend_fwd's workspace at width D on the current device, the
+ * same for every batch. Host only. */
+int rolaq_mx4_attend_workspace(int D, int64_t* bytes);
+
+/*
+ * Absorbed MLA attention over the MX4 cache. Request b has the queries
+ * qo_indptr[b] .. qo_indptr[b + 1] - 1 (null: query b alone), at most max_q_len,
+ * and kv_lens[b] cached positions, the queries' own included; its i-th query of n
+ * sees positions 0 .. kv_lens[b] - n + i. Position t lies in slot
+ * kv_indices[kv_indptr[b] + t / page_size] * page_size + t % page_size.
+ *   s_t = sm_scale (q_lat . x_t + q_rope . rope_t),  out = softmax(s) x,
+ * x_t the stored latent row. out: bf16 [T, H, D], in the frame of the cached rows; lse
+ * (or null): FP32 [T, H], the natural log of the sum of exp(s). A query that
+ * sees no position gets 0 and -inf; queries past qo_indptr[B], and past max_q_len
+ * of a request, are left as they were. A length that its page list does not
+ * reach is cut there, an index outside the cache reads its last slots: no read
+ * goes past the buffers that are described here. q: bf16 [T, H, D + R],
+ * 16-byte aligned, strides multiples of 8; out 8-byte aligned, strides multiples
+ * of 4. 1 <= H <= 128, page_size a power of two.
+ * workspace: rolaq_mx4_attend_workspace bytes, 256-byte aligned, its contents
+ * unspecified before and after; calls that overlap on a device need one each.
+ * A request's tiles are cut over the compute units by all requests' lengths: its
+ * low-order bits depend on the batch; the same call repeats bit for bit. No
+ * allocation, no synchronisation.
+ */
+int rolaq_mx4_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* codes,
+                         const uint8_t* scales, const void* rope_buf, int64_t num_slots, const int32_t* qo_indptr,
+                         const int32_t* kv_indptr, const int32_t* kv_indices, int64_t n_indices, int page_size,
+                         const int64_t* kv_lens, int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale,
+                         void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

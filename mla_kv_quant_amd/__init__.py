@@ -10,6 +10,9 @@ Hand-written HIP kernels for gfx950 behind a C ABI (``include/rolaq_mla.h``,
   MLA decode over the packed cache with split-K and LSE merge;
 * ``extend.packed_mla_extend_fwd`` -- causal chunked-prefill attention over the
   packed prefix plus the chunk;
+* ``mx4`` -- a 4-bit latent cache beside the INT2 one: ``MX4MLAPool``,
+  ``write_rows``, ``read_rows`` and ``attend_fwd`` (decode, verification of drafted
+  tokens, chunked prefill);
 * ``artifacts`` -- RoLaQ artifact loading and read-rotation folding.
 
 The library is loaded lazily on first use and there is no CPU fallback.
@@ -17,5 +20,6 @@ The library is loaded lazily on first use and there is no CPU fallback.
 
 from . import artifacts, kernels, synth  # noqa: F401
 from .pool import PackedMLAPool  # noqa: F401
+from .mx4 import MX4MLAPool  # noqa: F401
 
-__all__ = ["artifacts", "kernels", "synth", "PackedMLAPool"]
+__all__ = ["artifacts", "kernels", "synth", "PackedMLAPool", "MX4MLAPool"]

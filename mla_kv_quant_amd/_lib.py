@@ -50,6 +50,14 @@ SIGNATURES = {
     "rolaq_extend_scratch_rows": [c_int, c_int, c_int, c_int, c_int, c_int64, c_void_p],
     "rolaq_assemble_rows": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_int, c_int, c_void_p, c_int64, c_void_p],
+    "rolaq_mx4_write_rows": [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int,
+                             c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p],
+    "rolaq_mx4_read_rows": [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_int,
+                            c_void_p, c_int64, c_void_p],
+    "rolaq_mx4_attend_workspace": [c_int, c_void_p],
+    "rolaq_mx4_attend_fwd": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                             c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_float,
+                             c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
 }
 
 _LIB: ctypes.CDLL | None = None

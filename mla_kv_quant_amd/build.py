@@ -19,7 +19,8 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 ROOT = HERE.parent
 LIB = HERE / "librolaq_mla.so"
-SOURCES = ["api.cpp", "pack.hip", "writer.hip", "decode.hip", "extend.hip", "assemble.hip"]
+SOURCES = ["api.cpp", "pack.hip", "writer.hip", "decode.hip", "extend.hip", "assemble.hip",
+           "mx4_rows.hip", "mx4_attend.hip"]
 ARCH = "gfx950"
 
 

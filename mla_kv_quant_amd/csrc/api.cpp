@@ -11,6 +11,7 @@
 #include "../../include/rolaq_mla.h"
 
 #include "rolaq_args.h"
+#include "mx4_args.h"
 
 namespace {
 
@@ -531,4 +532,179 @@ int rolaq_assemble_rows(const int64_t* slots, int64_t n, const uint8_t* codes, c
 
 }  // extern "C"
 
+// ---- the 4-bit (MX4) latent cache --------------------------------------------------
 
+namespace {
+
+// The cache arguments that every MX4 entry point takes.
+int check_mx4_cache(const char* fn, const uint8_t* codes, const uint8_t* scales, const void* rope_buf,
+                    int64_t num_slots, int D, int R) {
+  if (!((D == 512 && R == 64) || (D == 256 && R == 32)))
+    return fail(ROLAQ_ERR_INVALID, "%s: (D, R) must be (512, 64) or (256, 32), got (%d, %d)", fn, D, R);
+  if (!codes || !scales || !rope_buf) return fail(ROLAQ_ERR_INVALID, "%s: null cache pointer", fn);
+  if (!aligned(codes, 16) || !aligned(scales, 16) || !aligned(rope_buf, 16))
+    return fail(ROLAQ_ERR_INVALID, "%s: cache buffers must be 16-byte aligned", fn);
+  if (num_slots < 1 || num_slots > INT32_MAX)
+    return fail(ROLAQ_ERR_INVALID, "%s: num_slots must be between 1 and 2^31 - 1", fn);
+  return ROLAQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rolaq_mx4_write_rows(const void* latent, int64_t latent_stride, const void* k_pe, int64_t pe_stride0,
+                         int64_t pe_stride1, const void* rotation_t, const int64_t* loc, int64_t n, int D, int R,
+                         uint8_t* codes, uint8_t* scales, void* rope_buf, int64_t num_slots, void* stream) {
+  const char* const fn = "mx4_write_rows";
+  if (n < 0) return fail(ROLAQ_ERR_INVALID, "%s: n < 0", fn);
+  if (n == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  const int rc = check_mx4_cache(fn, codes, scales, rope_buf, num_slots, D, R);
+  if (rc != ROLAQ_OK) return rc;
+  if (!latent || !k_pe || !loc) return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  if (n > (int64_t(1) << 31)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^31 rows", fn);
+  if (latent_stride < D || latent_stride % 8 || latent_stride >= (1 << 24) || !aligned(latent, 16))
+    return fail(ROLAQ_ERR_INVALID,
+                "%s: latent must be 16-byte aligned with a row stride >= D, multiple of 8, below 2^24", fn);
+  if (!aligned(k_pe, 2)) return fail(ROLAQ_ERR_INVALID, "%s: misaligned k_pe", fn);
+  if (rotation_t && !aligned(rotation_t, 16)) return fail(ROLAQ_ERR_INVALID, "%s: rotation must be 16-byte aligned", fn);
+  if (!rotation_t) {
+    rolaq::Mx4RowsArgs a{};
+    a.slots = loc;
+    a.n = n;
+    a.num_slots = num_slots;
+    a.x = static_cast<const uint16_t*>(latent);
+    a.xs = latent_stride;
+    a.k_pe = static_cast<const uint16_t*>(k_pe);
+    a.pe_s0 = pe_stride0;
+    a.pe_s1 = pe_stride1;
+    a.codes = codes;
+    a.scales = scales;
+    a.rope = static_cast<uint16_t*>(rope_buf);
+    return hip_status(rolaq_launch_mx4_write_plain(a, D, static_cast<hipStream_t>(stream)), "mx4_write_rows launch");
+  }
+  rolaq::WriterArgs a{};
+  a.x = static_cast<const uint16_t*>(latent);
+  a.xs = latent_stride;
+  a.rt = static_cast<const uint16_t*>(rotation_t);
+  a.loc = loc;
+  a.n = n;
+  a.codes = codes;
+  a.scales = scales;
+  a.num_slots = num_slots;
+  a.k_pe = static_cast<const uint16_t*>(k_pe);
+  a.pe_s0 = pe_stride0;
+  a.pe_s1 = pe_stride1;
+  a.R = R;
+  a.rope = static_cast<uint16_t*>(rope_buf);
+  return hip_status(rolaq_launch_writer(a, D, cu_count(), static_cast<hipStream_t>(stream)), "mx4_write_rows launch");
+}
+
+int rolaq_mx4_read_rows(const int64_t* slots, int64_t n, const uint8_t* codes, const uint8_t* scales,
+                        const void* rope_buf, int64_t num_slots, const void* rotation, int D, int R, void* out,
+                        int64_t out_stride, void* stream) {
+  const char* const fn = "mx4_read_rows";
+  if (n < 0) return fail(ROLAQ_ERR_INVALID, "%s: n < 0", fn);
+  if (n == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  const int rc = check_mx4_cache(fn, codes, scales, rope_buf, num_slots, D, R);
+  if (rc != ROLAQ_OK) return rc;
+  if (!slots || !out) return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  if (n > (int64_t(1) << 31)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^31 rows", fn);
+  if (!aligned(out, 16) || out_stride < D + R || out_stride % 8)
+    return fail(ROLAQ_ERR_INVALID, "%s: out must be 16-byte aligned with a row stride >= D + R, multiple of 8", fn);
+  if (rotation && !aligned(rotation, 16)) return fail(ROLAQ_ERR_INVALID, "%s: rotation must be 16-byte aligned", fn);
+  if (rotation) {
+    rolaq::AssembleArgs a{};
+    a.slots = slots;
+    a.n = n;
+    a.codes = codes;
+    a.scales = scales;
+    a.num_slots = num_slots;
+    a.rope = static_cast<const uint16_t*>(rope_buf);
+    a.rot = static_cast<const uint16_t*>(rotation);
+    a.R = R;
+    a.out = static_cast<uint16_t*>(out);
+    a.out_st = out_stride;
+    return hip_status(rolaq_launch_assemble(a, D, static_cast<hipStream_t>(stream)), "mx4_read_rows launch");
+  }
+  rolaq::Mx4RowsArgs a{};
+  a.slots = slots;
+  a.n = n;
+  a.num_slots = num_slots;
+  a.codes = const_cast<uint8_t*>(codes);
+  a.scales = const_cast<uint8_t*>(scales);
+  a.rope = const_cast<uint16_t*>(static_cast<const uint16_t*>(rope_buf));
+  a.out = static_cast<uint16_t*>(out);
+  a.out_st = out_stride;
+  return hip_status(rolaq_launch_mx4_read(a, D, static_cast<hipStream_t>(stream)), "mx4_read_rows launch");
+}
+
+int rolaq_mx4_attend_workspace(int D, int64_t* bytes) {
+  if ((D != 512 && D != 256) || !bytes)
+    return fail(ROLAQ_ERR_INVALID, "mx4_attend_workspace: D must be 256 or 512, bytes not null");
+  *bytes = rolaq_mx4_attend_ws_bytes(D, cu_count());
+  g_err[0] = '\0';
+  return ROLAQ_OK;
+}
+
+int rolaq_mx4_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* codes,
+                         const uint8_t* scales, const void* rope_buf, int64_t num_slots, const int32_t* qo_indptr,
+                         const int32_t* kv_indptr, const int32_t* kv_indices, int64_t n_indices, int page_size,
+                         const int64_t* kv_lens, int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale,
+                         void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  const char* const fn = "mx4_attend_fwd";
+  if (T < 0 || B < 0 || max_q_len < 0) return fail(ROLAQ_ERR_INVALID, "%s: negative T, B or max_q_len", fn);
+  if (H < 1 || H > kMaxHeads) return fail(ROLAQ_ERR_INVALID, "%s: H must be between 1 and %d, got %d", fn, kMaxHeads, H);
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(ROLAQ_ERR_INVALID, "%s: invalid sm_scale", fn);
+  if (page_size < 1 || (page_size & (page_size - 1)))
+    return fail(ROLAQ_ERR_INVALID, "%s: page_size must be a power of two, got %d", fn, page_size);
+  if (T == 0 || B == 0 || max_q_len == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  const int rc = check_mx4_cache(fn, codes, scales, rope_buf, num_slots, D, R);
+  if (rc != ROLAQ_OK) return rc;
+  if (!q || !kv_indptr || !kv_lens || !out || !workspace || (!kv_indices && n_indices > 0))
+    return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  if (n_indices < 0 || n_indices > INT32_MAX) return fail(ROLAQ_ERR_INVALID, "%s: n_indices out of range", fn);
+  if (T > (1 << 24)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries", fn);
+  if (!qo_indptr && (max_q_len != 1 || T < B))
+    return fail(ROLAQ_ERR_INVALID, "%s: without qo_indptr each request has one query (max_q_len 1, T >= B)", fn);
+  // (a longer maximum than there are queries sizes the grid for nothing)
+  const int most = int(std::min<int64_t>(max_q_len, T));
+  const int64_t row_blocks = (int64_t(most) * H + 63) / 64;
+  if (row_blocks * B > (int64_t(1) << 30))
+    return fail(ROLAQ_ERR_INVALID, "%s: B * max_q_len * H is too large for one launch", fn);
+  if (!aligned(q, 16) || q_stride_t % 8 || q_stride_h % 8 || q_stride_h < D + R || q_stride_t < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: q must be 16-byte aligned with strides multiple of 8 and q_stride_h >= D + R", fn);
+  if (!aligned(out, 8) || out_stride_t % 4 || out_stride_h % 4 || out_stride_h < D || out_stride_t < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: out must be 8-byte aligned with strides multiple of 4 and out_stride_h >= D", fn);
+  if (!aligned(workspace, 256) || workspace_bytes < rolaq_mx4_attend_ws_bytes(D, cu_count()))
+    return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 256-byte aligned and hold %lld bytes", fn,
+                (long long)rolaq_mx4_attend_ws_bytes(D, cu_count()));
+  rolaq::Mx4AttendArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.codes = codes;
+  a.scales = scales;
+  a.rope = static_cast<const uint16_t*>(rope_buf);
+  a.num_slots = num_slots;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.n_indices = n_indices;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.kv_lens = kv_lens;
+  a.T = int(T);
+  a.B = B;
+  a.H = H;
+  a.max_q_len = most;
+  a.sm_scale = sm_scale;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_st = out_stride_t;
+  a.o_sh = out_stride_h;
+  a.lse = lse;
+  a.ws = static_cast<uint8_t*>(workspace);
+  return hip_status(rolaq_launch_mx4_attend(a, D, cu_count(), static_cast<hipStream_t>(stream)), "mx4_attend_fwd launch");
+}
+
+}  // extern "C"

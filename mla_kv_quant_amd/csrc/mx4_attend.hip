@@ -1,0 +1,720 @@
+// Absorbed MLA attention over the 4-bit (MX4) latent cache (gfx950): decode,
+// verification of a few drafted tokens and chunked prefill with one kernel.
+//
+// For a query row (token i of n, head) over the positions t <= len - n + i:
+//   s_t = sm_scale (q_lat . x_t + q_pe . r_t),  O = sum_t softmax(s)_t x_t,
+// x_t the stored latent row (4-bit codes times 2^e for each 32 of them), r_t the
+// bf16 rope row.
+//
+// A block of four waves walks 64-position tiles for 16 G query rows (G = 1, 2, 4
+// groups of 16). Tiles are copied by asynchronous loads straight into an LDS ring
+// as they lie in the cache: 4-bit codes stay 4-bit up to the matrix core.
+// * Scores: wave w takes group w % G and the positions 16 G (w / G) .. of a tile.
+//   The codes are the A operand of v_mfma_scale_f32_16x16x128_f8f6f4 as they
+//   are, with the block scales as its A scales, so nothing is expanded. The bf16
+//   query is split into two e4m3 parts, hi + lo / 16, with one power of two for
+//   a row: eight significant bits are two times four, so the split is exact
+//   for values down to 2^-13 of the row's largest and off by less than 2^-21 of
+//   it below. Rope terms are bf16 MFMAs into the same FP32 accumulators.
+// * Softmax in FP32, log2 domain, against a whole-number reference for each
+//   row: a tile's largest score rounded up, moved only when a later score passes
+//   it by more than 2^30 (bf16 probabilities have FP32's range). A reference
+//   then moves by whole powers of two, exact in the accumulators as in P.
+// * Output: wave w takes the features D/4 w .. of all G groups. The codes come
+//   out of LDS transposed (ds_read_b64_tr_b4: 16 positions of one feature), become
+//   bf16 pairs by v_cvt_scalef32_pk_bf16_fp4 (one instruction for two values) and
+//   meet P in bf16 MFMAs. A position's block scale is applied to P instead of
+//   to the 32 values: an integer subtraction in P's exponents, P 2^(s - 159),
+//   saturating at zero (v_pk_sub_u16 with clamp), which is exact; O is multiplied
+//   by 2^32 at the end. Masked positions have P = 0 and finite codes, so what they
+//   hold does not reach O.
+// One barrier a tile: the scores of tile i + 1 and the output of tile i lie between
+// two barriers.
+//
+// Work: the tiles of all (request, row block) pairs lie on one line that is cut
+// into equal parts, a part for each block; a pair cut by a border leaves partials
+// that mx4_merge_kernel joins. With many row blocks each has a block of its own.
+#include "rolaq_common.h"
+#include "mx4_args.h"
+
+#include <algorithm>
+#include <utility>
+
+namespace rolaq {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+constexpr int kMx4Tile = 64;           // positions in a tile
+constexpr int kMx4Idx = 4;             // tiles whose page numbers are held (ring slots - 1 at least)
+constexpr float kMx4NoRef = -268435456.f;  // reference of a row that has seen no score
+constexpr float kMx4Slack = 30.f;      // log2 by which a score may pass its row's reference
+
+// D = A(16x128, E2M1) * B(128x16, E4M3) + C. Lane l holds A[l%16][32(l/16)+i] (nibble
+// i of four dwords) with the scale of those 32 in byte SA of sa, and
+// B[16(l/16)+i][l%16], B[64+16(l/16)+i][l%16] (bytes i and 16+i) with the scale of
+// B[32(l/16)..+31] in byte SB of sb.
+template <int SA, int SB>
+__device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
+  const i32x8 aa = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aa, b, c, 4, 0, SA, (int)sa, SB, (int)sb);
+}
+
+// Asynchronous copies into LDS, 16 or 4 bytes for each lane, lane l's to
+// lds + 16 l (4 l). In assembly because the compiler, which tracks such copies,
+// would wait for all of them before any LDS read; the kernel waits by count.
+__device__ __forceinline__ void copy16(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const void* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Packed saturating subtraction of two 16-bit fields.
+__device__ __forceinline__ uint32_t sub_sat(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
+// Eight 4-bit codes -> eight bf16 values, in order.
+__device__ __forceinline__ u32x4 fp4x8_to_bf16(uint32_t v) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 0)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 1)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 2)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 3))};
+}
+
+template <typename F, int... I>
+__device__ __forceinline__ void for_each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F&& f) {
+  for_each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+template <int D, int R, int G>
+struct Mx4Geo {
+  static constexpr int ROWS = 16 * G;
+  static constexpr int NB = D / 32;   // scale blocks of a row
+  static constexpr int KS = D / 128;  // K-steps of the latent scores; also blocks per lane group
+  static constexpr int CB = D / 2;    // code bytes of a row
+  static constexpr int FW = D / 4;    // features of a wave
+  static constexpr int FT = FW / 16;  // its output tiles
+  static constexpr int TW = 4 / G;    // waves that share a group's positions
+  static constexpr int CODES = kMx4Tile * CB, ROPE = kMx4Tile * 2 * R, SCALES = 1024;
+  static constexpr int TILE = CODES + ROPE + SCALES;  // a ring slot
+  static constexpr int S = D == 512 ? 5 : 4;          // ring slots
+  static constexpr int OCC = D == 512 ? 1 : 2;        // blocks on a CU
+  static constexpr int LOADS = CODES / 4096 + ROPE / 4096 + 1;  // a wave's copies for a tile
+  // LDS offsets
+  static constexpr int P = S * TILE;                        // [2][ROWS][64] bf16, 16-byte chunks swizzled
+  static constexpr int ES = P + 2 * ROWS * 128;             // [2][NB][64] exponent fields of the scales
+  static constexpr int IDX = ES + 2 * NB * 128;             // [kMx4Idx][4][64] page numbers
+  static constexpr int FLAG = IDX + kMx4Idx * 1024;         // [2][4]
+  static constexpr int WREF = FLAG + 32;                    // [2][4][16]
+  static constexpr int LSUM = WREF + 512;                   // [4][16]
+  static constexpr int FIND = LSUM + 256;                   // [8]: wave sums, the first unit's request
+  static constexpr int PREF = FIND + 64;                    // [kMx4Requests + 1]
+  static constexpr int LDS = PREF + 4 * (kMx4Requests + 4);
+  static_assert(LDS * OCC <= 160 * 1024, "LDS of a CU");
+  static_assert(S - 1 <= kMx4Idx, "page numbers in flight");
+  static constexpr int SLOT = ROWS * (D + 2) * 4;  // bytes of a partial: O, then (reference, sum) by row
+};
+
+constexpr int kMx4WsHead = 4 * (kMx4Requests + 64);  // the tile counts at the start of the workspace
+
+// A request's part of the batch.
+struct Mx4Request {
+  int q0, nq;        // first query, queries
+  int len;           // cached positions
+  int list, pages;   // first entry of its page list, and how many
+};
+
+__device__ __forceinline__ Mx4Request mx4_request(const Mx4AttendArgs& a, int b) {
+  Mx4Request r;
+  r.q0 = a.qo_indptr ? a.qo_indptr[b] : b;
+  const int q1 = a.qo_indptr ? a.qo_indptr[b + 1] : b + 1;
+  r.q0 = min(max(r.q0, 0), a.T);
+  r.nq = min(max(min(q1, a.T) - r.q0, 0), a.max_q_len);
+  r.list = a.kv_indptr[b];
+  const int end = a.kv_indptr[b + 1];
+  r.list = max(r.list, 0);
+  r.pages = (int)min((int64_t)max(end - r.list, 0), max(a.n_indices - r.list, (int64_t)0));
+  const int64_t most = (int64_t)r.pages << a.page_shift;  // positions that the list reaches
+  r.len = (int)max(min(min(a.kv_lens[b], most), (int64_t)0x3fffffff), (int64_t)0);
+  return r;
+}
+
+__device__ __forceinline__ int mx4_row_blocks(const Mx4Request& r, int H, int rows) { return (r.nq * H + rows - 1) / rows; }
+__device__ __forceinline__ int mx4_tiles(const Mx4Request& r) { return max((r.len + kMx4Tile - 1) / kMx4Tile, 1); }
+
+// Unit range of block j of n over `units`: [units j / n, units (j + 1) / n).
+__device__ __forceinline__ uint32_t mx4_first_unit(uint32_t units, uint32_t j, uint32_t n) {
+  return (uint32_t)((uint64_t)units * j / n);
+}
+// The block that has unit u.
+__device__ __forceinline__ uint32_t mx4_block_of(uint32_t u, uint32_t units, uint32_t n) {
+  return (uint32_t)((((uint64_t)u + 1) * n - 1) / units);
+}
+
+template <int D, int R, int G>
+__global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel(Mx4AttendArgs a) {
+  using Ge = Mx4Geo<D, R, G>;
+  constexpr int NB = Ge::NB, KS = Ge::KS, CB = Ge::CB, FT = Ge::FT, TW = Ge::TW, S = Ge::S;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)smem;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int la = lane & 15, gq = lane >> 4;
+  const int gw = wave % G, tw = wave / G;  // this wave's group and its share of a tile's positions
+
+  // ---- which units are this block's --------------------------------------------
+  uint32_t u = 0, u_end = 1, nblk = 1;
+  int b = 0, rb_only = 0;
+  uint32_t* const pref = reinterpret_cast<uint32_t*>(smem + Ge::PREF);
+  if (a.blocks > 0) {
+    // tiles of all requests, summed: four requests a thread
+    uint32_t* const find = reinterpret_cast<uint32_t*>(smem + Ge::FIND);
+    uint32_t n[4], s = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = 4 * tid + k;
+      n[k] = 0;
+      if (i < a.B) {
+        const Mx4Request r = mx4_request(a, i);
+        n[k] = (uint32_t)mx4_row_blocks(r, a.H, Ge::ROWS) * (uint32_t)mx4_tiles(r);
+      }
+      s += n[k];
+    }
+    uint32_t incl = s;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t v = __shfl_up(incl, d);
+      if (lane >= d) incl += v;
+    }
+    if (lane == 63) find[wave] = incl;
+    __syncthreads();
+    uint32_t base = incl - s, units = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t v = find[w];
+      if (w < wave) base += v;
+      units += v;
+    }
+    nblk = min((uint32_t)a.blocks, units);
+    if (blockIdx.x == 0) {  // for the merge
+      uint32_t* const g = reinterpret_cast<uint32_t*>(a.ws);
+      uint32_t at = base;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (4 * tid + k < a.B) g[4 * tid + k] = at;
+        at += n[k];
+      }
+      if (tid == 0) g[a.B] = units;
+    }
+    if (units == 0) return;
+    // consecutive parts on one XCD (blocks go round the XCDs in turn): they share pages
+    const uint32_t per = gridDim.x / 8;
+    const uint32_t j = gridDim.x % 8 == 0 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
+    if (j >= nblk) return;
+    u = mx4_first_unit(units, j, nblk);
+    u_end = mx4_first_unit(units, j + 1, nblk);
+    uint32_t at = base;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      pref[4 * tid + k] = at;
+      if (at <= u && u < at + n[k]) find[4] = 4 * tid + k;
+      at += n[k];
+    }
+    if (tid == 255) pref[kMx4Requests] = units;
+    __syncthreads();
+    b = find[4];
+    a.blocks = (int)j;  // (from here on: this block's number)
+  } else {
+    // a block for each (row block, request), the later row blocks of a request,
+    // which see most positions, first
+    b = blockIdx.x % a.B;
+    rb_only = a.row_blocks - 1 - blockIdx.x / a.B;
+  }
+  const bool shared = a.ws != nullptr;
+
+  const uint32_t max_page = (uint32_t)((a.num_slots - 1) >> a.page_shift), max_slot = (uint32_t)(a.num_slots - 1);
+  const uint32_t page_mask = (1u << a.page_shift) - 1;
+  const float c2 = a.sm_scale * kLog2e;
+  int nth = 0;  // segments done
+
+  while (u < u_end) {
+    // ---- the next segment: tiles [t0, t1) of a row block of request b ---------------
+    int rb, t0, t1, ntiles;
+    Mx4Request rq = mx4_request(a, b);
+    if (shared) {
+      const uint32_t p0 = pref[b], p1 = pref[b + 1];
+      if (u >= p1) {  // (also requests without queries)
+        ++b;
+        continue;
+      }
+      ntiles = mx4_tiles(rq);
+      rb = (u - p0) / ntiles;
+      t0 = (u - p0) - rb * ntiles;
+      t1 = (int)min((uint32_t)ntiles, t0 + (u_end - u));
+      u += t1 - t0;
+    } else {
+      u = u_end;
+      rb = rb_only;
+      if (rb >= mx4_row_blocks(rq, a.H, Ge::ROWS)) return;
+      ntiles = mx4_tiles(rq);
+      t0 = 0;
+      t1 = ntiles;
+    }
+    const bool whole = t0 == 0 && t1 == ntiles;
+    const int rows = rq.nq * a.H, row0 = rb * Ge::ROWS;
+    // positions that a row sees: its causal limit; rows past the last see none
+    const int last_row = min(row0 + Ge::ROWS, rows) - 1;
+    const int vis_all = rq.len - rq.nq + row0 / a.H + 1;          // seen by every row of the block
+    const int vis_most = rq.len - rq.nq + last_row / a.H + 1;     // by any
+    const int my_row = row0 + 16 * gw + la;
+    const int vis = my_row < rows ? rq.len - rq.nq + my_row / a.H + 1 : 0;
+    const bool full_rows = row0 + Ge::ROWS <= rows;
+    const int t_end = min(t1, (vis_most + kMx4Tile - 1) / kMx4Tile);
+    const int nt = max(t_end - t0, 0);  // tiles to walk
+    const int pos_last = max(rq.len - 1, 0);
+
+    __syncthreads();  // the last segment's LDS reads are done
+
+    // ---- page numbers and tiles, asynchronously ---------------------------------------
+    auto copy_idx = [&](int k) {
+      const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + la, pos_last);
+      copy4(a.kv_indices + rq.list + (pos >> a.page_shift),
+            lds0 + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256);
+    };
+    auto slot_of = [&](int k, int x) {  // cache slot of position x of this wave's 16
+      const uint32_t page =
+          *reinterpret_cast<const uint32_t*>(smem + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256 + 4 * x);
+      const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + x, pos_last);
+      return min((min(page, max_page) << a.page_shift) + ((uint32_t)pos & page_mask), max_slot);
+    };
+    auto copy_tile = [&](int k) {
+      const uint32_t dst = lds0 + (uint32_t)(k % S) * Ge::TILE;
+      constexpr int RC = 1024 / CB, LC = 64 / RC;  // rows of a copy, lanes of a row
+#pragma unroll
+      for (int j = 0; j < 16 / RC; ++j) {
+        const int x = RC * j + lane / LC, t = 16 * wave + x;
+        const int c = (lane % LC) ^ (D == 512 ? t & 15 : (t >> 1) & 7);
+        copy16(a.codes + (uint64_t)slot_of(k, x) * CB + 16 * c, dst + 16 * wave * CB + 1024 * j);
+      }
+      constexpr int RR = 1024 / (2 * R), LR = 64 / RR;
+#pragma unroll
+      for (int j = 0; j < 16 / RR; ++j) {
+        const int x = RR * j + lane / LR, t = 16 * wave + x;
+        const int c = (lane % LR) ^ (R == 64 ? (t >> 1) & 7 : (t >> 2) & 3);
+        copy16(a.rope + (uint64_t)slot_of(k, x) * R + 8 * c, dst + Ge::CODES + 16 * wave * 2 * R + 1024 * j);
+      }
+      constexpr int LS = NB / 4;  // lanes of a row's scales
+      const int x = (lane / LS) & 15;
+      copy4(a.scales + (uint64_t)slot_of(k, x) * NB + 4 * (lane % LS), dst + Ge::CODES + Ge::ROPE + 256 * wave);
+    };
+
+    // ---- the query rows of this wave's group: e4m3 hi and lo parts, rope ---------------
+    i32x8 qhi[KS], qlo[KS];
+    u32x4 qpe[R / 32];
+    uint32_t qscale;
+    {
+      const int r = min(my_row, max(rows - 1, 0));
+      const int tok = min(rq.q0 + r / a.H, a.T - 1);
+      const uint16_t* q = a.q + (int64_t)tok * a.q_st + (int64_t)(r % a.H) * a.q_sh;
+      u32x4 v[KS][2][2];
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // K index 64 h + 16 gq + i of step s is feature 32 (KS kb + s) + 16 (gq & 1) + i, kb = 2 h + gq / 2
+          const uint16_t* p = q + 32 * (KS * (2 * h + (gq >> 1)) + s) + 16 * (gq & 1);
+          v[s][h][0] = gload<u32x4>(p);
+          v[s][h][1] = gload<u32x4>(p + 8);
+        }
+#pragma unroll
+      for (int k = 0; k < R / 32; ++k) qpe[k] = gload<u32x4>(q + D + 32 * k + 8 * gq);
+      // largest magnitude of the row, as bits (NaN above infinity)
+      uint32_t big = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w = v[s][h][e][i] & 0x7fff7fffu;
+              big = max(big, max(w & 0xffffu, w >> 16));
+            }
+      big = max(big, (uint32_t)__shfl_xor((int)big, 16));
+      big = max(big, (uint32_t)__shfl_xor((int)big, 32));
+      const int e = max((int)(big >> 7), 16);  // biased exponent
+      // scaled so that the largest lies in [2^7, 2^8); lo is 2^4 finer
+      const float up = __uint_as_float((uint32_t)(min(max(127 + 127 + 7 - e, 1), 254)) << 23);
+      qscale = e >= 255 ? 0xffffu : (uint32_t)(e - 7) | (uint32_t)(e - 11) << 8;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {  // dword d: values 4 d .. 4 d + 3 of 16
+            const uint32_t w0 = v[s][h][d >> 1][2 * (d & 1)], w1 = v[s][h][d >> 1][2 * (d & 1) + 1];
+            const float f0 = bf16_lo(w0) * up, f1 = bf16_hi(w0) * up, f2 = bf16_lo(w1) * up, f3 = bf16_hi(w1) * up;
+            int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f0, f1, 0, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(f2, f3, hi, true);
+            const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+            int lo = __builtin_amdgcn_cvt_pk_fp8_f32((f0 - b0.x) * 16.f, (f1 - b0.y) * 16.f, 0, false);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32((f2 - b1.x) * 16.f, (f3 - b1.y) * 16.f, lo, true);
+            qhi[s][4 * h + d] = hi;
+            qlo[s][4 * h + d] = lo;
+          }
+    }
+
+    f32x4 o[G][FT];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int j = 0; j < FT; ++j) o[g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float ref[G];  // reference of row la of each group, the same in every wave
+#pragma unroll
+    for (int g = 0; g < G; ++g) ref[g] = kMx4NoRef;
+    float lsum = 0.f, ltile = 0.f, wref = kMx4NoRef;  // this lane's sums (its positions of row la of group gw)
+
+    // Scores and probabilities of tile k: P, the scales' exponent fields and the
+    // wave's flag go to LDS buffer k & 1.
+    auto scores = [&](int k) {
+      const uint8_t* const slot = smem + (k % S) * Ge::TILE;
+      const int buf = k & 1;
+      f32x4 acc[G];
+#pragma unroll
+      for (int m = 0; m < G; ++m) {
+        const int t = 16 * (tw * G + m) + la;
+        const uint8_t* const row = slot + t * CB;
+        const int f = D == 512 ? t & 15 : (t >> 1) & 7;
+        const uint8_t* const sp = slot + Ge::CODES + Ge::ROPE + 256 * (tw * G + m) + la * NB + gq * KS;
+        const uint32_t sa = KS == 4 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp);
+        f32x4 c = {0.f, 0.f, 0.f, 0.f}, d = {0.f, 0.f, 0.f, 0.f};
+        static_for<KS>([&](auto s) {
+          const u32x4 kc = *reinterpret_cast<const u32x4*>(row + 16 * ((gq * KS + s) ^ f));
+          c = mfma_fp4_fp8<s, 0>(kc, qhi[s], c, sa, qscale);
+          d = mfma_fp4_fp8<s, 1>(kc, qlo[s], d, sa, qscale);
+        });
+        const uint8_t* const pe = slot + Ge::CODES + t * 2 * R;
+        const int fr = R == 64 ? (t >> 1) & 7 : (t >> 2) & 3;
+#pragma unroll
+        for (int j = 0; j < R / 32; ++j)
+          d = mfma16x16x32(*reinterpret_cast<const u32x4*>(pe + 16 * ((4 * j + gq) ^ fr)), qpe[j], d);
+        acc[m] = c + d;
+      }
+      // exponent fields of the scales of this wave's 16 copied positions: (159 - s) << 7
+      {
+        constexpr int LS = NB / 4;
+        if (LS == 4 || lane < 16 * LS) {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(slot + Ge::CODES + Ge::ROPE + 256 * wave + 4 * lane);
+          uint16_t* const es = reinterpret_cast<uint16_t*>(smem + Ge::ES + buf * NB * 128) + 4 * (lane % LS) * 64 +
+                               16 * wave + lane / LS;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) es[64 * i] = (uint16_t)(max(kMx4High - (int)((w >> (8 * i)) & 255u), 0) << 7);
+        }
+      }
+      const int p0 = kMx4Tile * (t0 + k);
+      const bool masked = !full_rows || p0 + kMx4Tile > vis_all;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int m = 0; m < G; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[m][i] *= c2;
+          if (masked && p0 + 16 * (tw * G + m) + 4 * gq + i >= vis) acc[m][i] = -INFINITY;
+          mx = fmaxf(mx, acc[m][i]);
+        }
+      float r = ref[gw];
+      const bool moved = __builtin_amdgcn_ballot_w64(mx > r + kMx4Slack) != 0;
+      if (__builtin_expect(moved, 0)) {
+        const float top = wave_max_over_groups(mx);
+        if (top > r + kMx4Slack) r = ceilf(top);
+        if (gq == 0) *reinterpret_cast<float*>(smem + Ge::WREF + 256 * buf + 64 * wave + 4 * la) = r;
+      }
+      if (lane == 0) *reinterpret_cast<uint32_t*>(smem + Ge::FLAG + 16 * buf + 4 * wave) = moved;
+      wref = r;
+      ltile = 0.f;
+#pragma unroll
+      for (int m = 0; m < G; ++m) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(acc[m][i] - r);
+          ltile += p[i];
+        }
+        // chunk (8 positions) c of a row at c ^ (row & 7)
+        const int c = 2 * (tw * G + m) + (gq >> 1);
+        *reinterpret_cast<u32x2*>(smem + Ge::P + buf * Ge::ROWS * 128 + (16 * gw + la) * 128 + 16 * (c ^ (la & 7)) +
+                                  8 * (gq & 1)) = u32x2{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
+      }
+    };
+
+    // Output of tile k: O^T += X^T P^T over this wave's features.
+    auto output = [&](int k) {
+      const uint8_t* const slot = smem + (k % S) * Ge::TILE;
+      const int buf = k & 1;
+      const u32x4 fl = *reinterpret_cast<const u32x4*>(smem + Ge::FLAG + 16 * buf);
+      u32x4 p[G][2];  // row la: positions 16 gq .. 16 gq + 15
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          p[g][h] = *reinterpret_cast<const u32x4*>(smem + Ge::P + buf * Ge::ROWS * 128 + (16 * g + la) * 128 +
+                                                    16 * ((2 * gq + h) ^ (la & 7)));
+      if (__builtin_expect(__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w) != 0, 0)) {
+        // some wave moved a reference: all go to the largest, and what was
+        // computed against smaller ones is scaled down by powers of two
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          float mine[TW], top = ref[g];
+#pragma unroll
+          for (int w = 0; w < TW; ++w) {
+            const int wv = w * G + g;
+            const float r = *reinterpret_cast<const float*>(smem + Ge::WREF + 256 * buf + 64 * wv + 4 * la);
+            mine[w] = fl[wv] ? r : ref[g];
+            top = fmaxf(top, mine[w]);
+          }
+          const float f = __builtin_amdgcn_exp2f(ref[g] - top);
+#pragma unroll
+          for (int j = 0; j < FT; ++j) o[g][j] *= f;
+          float r = mine[0];  // of the wave that made this lane's 16 positions
+#pragma unroll
+          for (int w = 1; w < TW; ++w) r = gq / G == w ? mine[w] : r;
+          const uint32_t down = (uint32_t)fminf(top - r, 511.f) << 7;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[g][h][i] = sub_sat(p[g][h][i], down | down << 16);
+          if (g == gw) {
+            lsum = lsum * f;
+            ltile = ltile * __builtin_amdgcn_exp2f(wref - top);
+          }
+          ref[g] = top;
+        }
+      }
+      lsum += ltile;
+#pragma unroll
+      for (int bb = 0; bb < FT / 2; ++bb) {
+        const int nb = wave * (FT / 2) + bb;  // scale block: features 32 nb ..
+        const u32x4* const es = reinterpret_cast<const u32x4*>(smem + Ge::ES + buf * NB * 128 + nb * 128 + 32 * gq);
+        const u32x4 e0 = es[0], e1 = es[1];
+        const int t = 16 * gq + la;
+        const int ch = nb ^ (D == 512 ? t & 15 : (t >> 1) & 7);
+        u32x4 x[2][2];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)(slot + t * CB + 16 * ch + 8 * f));
+          x[f][0] = fp4x8_to_bf16((uint32_t)v.x);
+          x[f][1] = fp4x8_to_bf16((uint32_t)v.y);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          u32x4 ps[2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            ps[0][i] = sub_sat(p[g][0][i], e0[i]);
+            ps[1][i] = sub_sat(p[g][1][i], e1[i]);
+          }
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) o[g][2 * bb + f] = mfma16x16x32(x[f][h], ps[h], o[g][2 * bb + f]);
+        }
+      }
+    };
+
+    // ---- the tile loop -------------------------------------------------------------
+    // Copies in order: before the loop tiles 0 .. S - 3, in turn k (after barrier k)
+    // tile k + S - 1, each behind the page numbers of the tile S - 2 later. Barrier
+    // k waits until tile k + 1 is in; then tiles k + 2 .. k + S - 2 may be on their
+    // way. Turn k = -1 has no output, turn nt - 1 no scores.
+    if (nt > 0) {
+#pragma unroll 1
+      for (int k = 0; k < S - 2; ++k) copy_idx(k);
+      wait_loads<0>();
+#pragma unroll 1
+      for (int k = 0; k < S - 2; ++k) {
+        copy_idx(k + S - 2);
+        if (k < nt) copy_tile(k);
+      }
+#pragma unroll 1
+      for (int k = -1; k < nt; ++k) {
+        const int out_there = min(nt - 2 - k, S - 3);  // tiles past k + 1 already asked for
+        if (out_there >= 2) {
+          wait_loads<(S - 3) + 2 * Ge::LOADS>();
+        } else if (out_there == 1) {
+          wait_loads<(S - 3) + Ge::LOADS>();
+        } else {
+          wait_loads<S - 3>();
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        copy_idx(k + 2 * S - 3);
+        if (k + S - 1 < nt) copy_tile(k + S - 1);
+        if (k >= 0) output(k);
+        if (k + 1 < nt) scores(k + 1);
+      }
+    }
+    wait_loads<0>();  // (page numbers asked for past the end)
+
+    // ---- the rows' sums, then the output or a partial --------------------------------
+    lsum = wave_sum_over_groups(lsum);
+    if (gq == 0) *reinterpret_cast<float*>(smem + Ge::LSUM + 64 * wave + 4 * la) = lsum;
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float l = 0.f;
+#pragma unroll
+      for (int w = 0; w < TW; ++w) l += *reinterpret_cast<const float*>(smem + Ge::LSUM + 64 * (w * G + g) + 4 * la);
+      const int r = row0 + 16 * g + la;
+      if (r >= rows) continue;
+      const int tok = rq.q0 + r / a.H, head = r % a.H;
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 4294967296.f / l;
+        uint16_t* const out = a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + Ge::FW * wave + 4 * gq;
+#pragma unroll
+        for (int j = 0; j < FT; ++j) {
+          const f32x4 v = o[g][j] * inv;
+          *reinterpret_cast<u32x2*>(out + 16 * j) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        }
+        if (a.lse && wave == 0 && gq == 0)
+          a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (ref[g] + log2f(l)) * kLn2;
+      } else {
+        uint8_t* const part = a.ws + kMx4WsHead + ((int64_t)2 * a.blocks + (nth > 0)) * Ge::SLOT;
+        float* const po = reinterpret_cast<float*>(part) + (16 * g + la) * D + Ge::FW * wave + 4 * gq;
+#pragma unroll
+        for (int j = 0; j < FT; ++j) *reinterpret_cast<f32x4*>(po + 16 * j) = o[g][j];
+        if (wave == 0 && gq == 0)
+          reinterpret_cast<f32x2*>(part + Ge::ROWS * D * 4)[16 * g + la] = f32x2{ref[g], l};
+      }
+    }
+    ++nth;
+  }
+}
+
+// Joins the partials of the row blocks that were cut: a block for ROWS_M rows of
+// one row block, D / 4 threads a row. Rows of row blocks that one block walked are
+// left as that block wrote them.
+template <int D>
+__global__ __launch_bounds__(256) void mx4_merge_kernel(Mx4AttendArgs a, int rows_per_block) {
+  constexpr int RM = 256 / (D / 4);
+  const int b = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
+  const Mx4Request rq = mx4_request(a, b);
+  const int nrb = mx4_row_blocks(rq, a.H, rows_per_block);
+  if (rb >= nrb) return;
+  const uint32_t* const pref = reinterpret_cast<const uint32_t*>(a.ws);
+  const uint32_t units = pref[a.B], tiles = mx4_tiles(rq), u0 = pref[b] + rb * tiles;
+  const uint32_t nblk = min((uint32_t)a.blocks, units);
+  const uint32_t j0 = mx4_block_of(u0, units, nblk), j1 = mx4_block_of(u0 + tiles - 1, units, nblk);
+  if (j0 == j1) return;
+  const int rl = blockIdx.y * RM + threadIdx.x / (D / 4), r = rb * rows_per_block + rl;
+  if (r >= rq.nq * a.H) return;
+  const int c = threadIdx.x % (D / 4);
+  const int64_t slot = (int64_t)rows_per_block * (D + 2) * 4;
+  // block j's part of this pair is its second segment if it starts before the pair, else its first
+  const int first = mx4_first_unit(units, j0, nblk) < u0;
+  const uint8_t* const parts = a.ws + kMx4WsHead;
+  float m = kMx4NoRef, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int N = 8;
+  for (uint32_t j = j0; j <= j1; j += N) {
+    f32x2 ml[N];
+    f32x4 v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t jj = min(j + i, j1);
+      const uint8_t* const p = parts + ((int64_t)2 * jj + (jj == j0 ? first : 0)) * slot;
+      ml[i] = reinterpret_cast<const f32x2*>(p + (int64_t)rows_per_block * D * 4)[rl];
+      v[i] = *reinterpret_cast<const f32x4*>(p + ((int64_t)rl * D + 4 * c) * 4);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, ml[i].x);
+    const float f = __builtin_amdgcn_exp2f(m - top);
+    l *= f;
+    o *= f;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float w = j + i <= j1 ? __builtin_amdgcn_exp2f(ml[i].x - top) : 0.f;
+      if (j + i <= j1) {
+        l = fmaf(w, ml[i].y, l);
+        o += v[i] * w;
+      }
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 4294967296.f / l;
+  o *= inv;
+  const int tok = rq.q0 + r / a.H, head = r % a.H;
+  *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * c) =
+      u32x2{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
+  if (a.lse && c == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <int D, int R, int G>
+hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
+  using Ge = Mx4Geo<D, R, G>;
+  const int64_t rows = (int64_t)a.max_q_len * a.H;
+  a.row_blocks = (int)((rows + Ge::ROWS - 1) / Ge::ROWS);
+  // Shared out while there are few row blocks for each CU; past that, or with more
+  // requests than a block's sums hold, each row block has a block.
+  const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
+  const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus;
+  const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G>,
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);
+  if (e != hipSuccess) return e;
+  if (!shared) {
+    a.ws = nullptr;
+    a.blocks = 0;
+    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G>), dim3((unsigned)((int64_t)a.row_blocks * a.B)), dim3(256), Ge::LDS,
+                       stream, a);
+    return hipGetLastError();
+  }
+  a.blocks = num_cus * Ge::OCC;
+  hipLaunchKernelGGL((mx4_attend_kernel<D, R, G>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
+  hipError_t rc = hipGetLastError();
+  if (rc != hipSuccess) return rc;
+  constexpr int RM = 256 / (D / 4);
+  hipLaunchKernelGGL((mx4_merge_kernel<D>), dim3((unsigned)(a.row_blocks * a.B), Ge::ROWS / RM), dim3(256), 0, stream, a,
+                     Ge::ROWS);
+  return hipGetLastError();
+}
+
+}  // namespace rolaq
+
+int64_t rolaq_mx4_attend_ws_bytes(int D, int num_cus) {
+  using namespace rolaq;
+  // two partials of 64 rows a block
+  return kMx4WsHead + (D == 512 ? (int64_t)2 * num_cus * Mx4Geo<512, 64, 4>::OCC * Mx4Geo<512, 64, 4>::SLOT
+                                : (int64_t)2 * num_cus * Mx4Geo<256, 32, 4>::OCC * Mx4Geo<256, 32, 4>::SLOT);
+}
+
+hipError_t rolaq_launch_mx4_attend(const rolaq::Mx4AttendArgs& a, int D, int num_cus, hipStream_t stream) {
+  using namespace rolaq;
+  const int64_t rows = (int64_t)a.max_q_len * a.H;
+#define ROLAQ_MX4(DD, RR)                                                    \
+  if (D == DD) {                                                             \
+    if (rows <= 16) return launch_attend<DD, RR, 1>(a, num_cus, stream);     \
+    if (rows <= 32) return launch_attend<DD, RR, 2>(a, num_cus, stream);     \
+    return launch_attend<DD, RR, 4>(a, num_cus, stream);                     \
+  }
+  ROLAQ_MX4(512, 64)
+  ROLAQ_MX4(256, 32)
+#undef ROLAQ_MX4
+  return hipErrorInvalidValue;
+}

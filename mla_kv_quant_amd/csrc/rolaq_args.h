@@ -74,6 +74,10 @@ struct WriterArgs {
   float eps;
   uint16_t* y;
   int64_t ys;
+  // MX4 rows instead of INT2 ones (codes then holds 4-bit codes, and the
+  // quantizer, the window and its maps are unused): scale bytes, or null
+  uint8_t* scales;
+  int64_t num_slots;
 };
 
 struct ExtendArgs {
@@ -120,6 +124,10 @@ struct AssembleArgs {
   int R;
   uint16_t* out;              // [n, out_st] bf16: latent (D) then rope (R)
   int64_t out_st;
+  // MX4 rows instead of INT2 ones (codes then holds 4-bit codes, and params,
+  // hp and the maps are unused): scale bytes, or null
+  const uint8_t* scales;
+  int64_t num_slots;
 };
 
 }  // namespace rolaq

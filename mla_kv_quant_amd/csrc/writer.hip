@@ -18,6 +18,7 @@
 // permuted so that each lane ends up with whole packed words of one row.
 #include "rolaq_common.h"
 #include "rolaq_args.h"
+#include "mx4_codec.h"
 
 #include <algorithm>
 #include <cstddef>
@@ -211,6 +212,33 @@ __device__ __forceinline__ void store_row(const WriterArgs& a, Acc acc, int64_t 
   }
 }
 
+// The same row as MX4: lane gq's 32 columns are one block, so its scale and codes
+// need no other lane (the INT2 codec's statistics take two sums over four).
+template <int D, typename Acc>
+__device__ __forceinline__ void store_row_mx4(const WriterArgs& a, Acc acc, int64_t row, int64_t sl, u32x2 pe, int g,
+                                              int gq, int gr) {
+  float big = 0.f;
+#pragma unroll
+  for (int mb = 0; mb < 8; ++mb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(acc(mb)[i]));
+  // (a row with a value that is not finite rotates to rows of NaN and infinities,
+  // and the maximum of nothing but NaN is 0 here: the sum tells)
+  const float any = acc(0)[0] - acc(0)[0];
+  const uint32_t s = mx4_scale(any == any ? __float_as_uint(big) : 0x7fc00000u);
+  const float f = mx4_pow2(s);
+  if (row < a.n && sl >= 0 && sl < a.num_slots) {
+    *reinterpret_cast<u32x4*>(a.codes + sl * (D / 2) + 16 * (4 * g + gq)) =
+        u32x4{mx4_codes8(acc(0), acc(1), f), mx4_codes8(acc(2), acc(3), f), mx4_codes8(acc(4), acc(5), f),
+              mx4_codes8(acc(6), acc(7), f)};
+    a.scales[sl * (D / 32) + 4 * g + gq] = (uint8_t)s;
+    if (a.pe_vec)
+      *reinterpret_cast<u32x2*>(a.rope + sl * a.R + 16 * g + 4 * gr) = pe;
+    else if (g == 0)
+      for (int r = gq; r < a.R; r += 4) a.rope[sl * a.R + r] = a.k_pe[row * a.pe_s0 + r * a.pe_s1];
+  }
+}
+
 // Block = one quantization group g x a stripe of 64-row tiles. The block's
 // R_g^T slice stays in LDS; its eight waves each own whole tiles and never
 // synchronise after staging. Blocks of the NG groups of one stripe get the same
@@ -222,7 +250,8 @@ __device__ __forceinline__ void store_row(const WriterArgs& a, Acc acc, int64_t 
 // of a row each sum 8 columns per K-step, then a quad sum), and every K-step
 // chunk is normalized in registers before it becomes an MFMA operand; each
 // group's block also stores a quarter (1/NG) of the normalized rows' columns to y.
-template <int D, bool NORM>
+// MX4: the rows are stored as 4-bit blocks (store_row_mx4).
+template <int D, bool NORM, bool MX4>
 __global__ __launch_bounds__(64 * kWriterWaves, 1) void writer_kernel(WriterArgs a) {
   using G = WriterGeo<D>;
   constexpr int NG = G::NG, KS = G::KS, STR = G::STRIDE;
@@ -442,6 +471,23 @@ __global__ __launch_bounds__(64 * kWriterWaves, 1) void writer_kernel(WriterArgs
     int lane_now;
     asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane_now));
     const int lr = lane_now & 15, gr = lane_now >> 4;
+    if constexpr (MX4) {
+      int64_t slot[4];
+      u32x2 pes[4];
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) {
+        const int64_t r = min(row0 + 16 * nb + lr, a.n - 1);
+        pes[nb] = a.pe_vec ? *reinterpret_cast<const u32x2*>(a.k_pe + r * a.pe_s0 + 16 * g + 4 * gr) : u32x2{0u, 0u};
+        slot[nb] = a.loc[r];
+      }
+#pragma unroll
+      for (int nb = 0; nb < 4; ++nb) {
+        __builtin_amdgcn_sched_barrier(0);
+        store_row_mx4<D>(a, [&](int mb) -> f32x4& { return acc[mb][nb]; }, row0 + 16 * nb + lr, slot[nb], pes[nb], g, gq,
+                         gr);
+      }
+      continue;
+    }
     const CodeTests t3 = code_tests(a.thr);
     int64_t slot[4];
     int32_t seq[4], pos[4], req[4];
@@ -481,7 +527,7 @@ __global__ __launch_bounds__(64 * kWriterWaves, 1) void writer_kernel(WriterArgs
 // D = 512: 1 row 13.2 -> 7.4, 1024 rows 14.3 -> 8.1; with the norm 21.6 -> 8.0 and
 // 22.9 -> 8.8; D = 256, 1 row: 10.1 -> 5.3, with the norm 14.3 -> 5.7.
 // ---------------------------------------------------------------------------
-template <int D, bool NORM>
+template <int D, bool NORM, bool MX4>
 __global__ __launch_bounds__(64 * kWriterWaves, 1) void writer_few_kernel(WriterArgs a) {
   constexpr int NG = D / 128, KS = D / 32, KW = KS / kWriterWaves;  // K-steps, and those that a wave loads
   static_assert(KS % kWriterWaves == 0, "each wave loads whole K-steps");
@@ -530,11 +576,13 @@ __global__ __launch_bounds__(64 * kWriterWaves, 1) void writer_few_kernel(Writer
     if (wave == 0) {
       if (a.pe_vec) pe = *reinterpret_cast<const u32x2*>(a.k_pe + rc * a.pe_s0 + 16 * g + 4 * gq);
       slot = a.loc[rc];
-      seq = seq32[2 * rc];
-      pos = pos32[2 * rc] + pos_adj;
-      // a request index that does not fit 32 bits is outside [0, max_reqs)
-      const int32_t rlo = req32[2 * rc], rhi = req32[2 * rc + 1];
-      req = rhi == (rlo >> 31) ? rlo : -1;
+      if constexpr (!MX4) {
+        seq = seq32[2 * rc];
+        pos = pos32[2 * rc] + pos_adj;
+        // a request index that does not fit 32 bits is outside [0, max_reqs)
+        const int32_t rlo = req32[2 * rc], rhi = req32[2 * rc + 1];
+        req = rhi == (rlo >> 31) ? rlo : -1;
+      }
     }
     if constexpr (NORM) {
       // the row's sum of squares: eight columns per K-step and lane, the
@@ -571,16 +619,19 @@ __global__ __launch_bounds__(64 * kWriterWaves, 1) void writer_few_kernel(Writer
       f32x4 acc[kWriterWaves];
 #pragma unroll
       for (int mb = 0; mb < kWriterWaves; ++mb) acc[mb] = s_c[mb * 64 + lane];
-      store_row<D>(a, [&](int mb) -> f32x4& { return acc[mb]; }, row, slot, pos, seq, req, pe, g, gq, gq, t3);
+      if constexpr (MX4)
+        store_row_mx4<D>(a, [&](int mb) -> f32x4& { return acc[mb]; }, row, slot, pe, g, gq, gq);
+      else
+        store_row<D>(a, [&](int mb) -> f32x4& { return acc[mb]; }, row, slot, pos, seq, req, pe, g, gq, gq, t3);
     }
   }
 }
 
 // kernarg_field: WriterArgs must stay writer_kernel's one explicit argument
-static_assert(std::is_same<decltype(&writer_kernel<512, false>), void (*)(WriterArgs)>::value &&
-                  std::is_same<decltype(&writer_kernel<256, true>), void (*)(WriterArgs)>::value,
+static_assert(std::is_same<decltype(&writer_kernel<512, false, false>), void (*)(WriterArgs)>::value &&
+                  std::is_same<decltype(&writer_kernel<256, true, false>), void (*)(WriterArgs)>::value,
               "writer_kernel's only argument must be WriterArgs (read at kernel-argument offset 0)");
-static_assert(std::is_same<decltype(&writer_few_kernel<512, false>), void (*)(WriterArgs)>::value,
+static_assert(std::is_same<decltype(&writer_few_kernel<512, false, false>), void (*)(WriterArgs)>::value,
               "writer_few_kernel's only argument must be WriterArgs (read at kernel-argument offset 0)");
 
 }  // namespace rolaq
@@ -620,31 +671,35 @@ hipError_t rolaq_launch_writer(const rolaq::WriterArgs& args_in, int D, int num_
   if (tiles16 <= few_stripes * (a.gamma ? 5 : 3)) {
     a.nstripes = (int)std::min(tiles16, few_stripes);
     const dim3 few((unsigned)(a.nstripes * NG));
-#define ROLAQ_FEW(DD, NORM)                                                                    \
-    if (D == DD && (a.gamma != nullptr) == NORM) {                                             \
-      hipLaunchKernelGGL((writer_few_kernel<DD, NORM>), few, dim3(64 * kWriterWaves), 0, stream, a); \
+#define ROLAQ_FEW(DD, NORM, MX4)                                                               \
+    if (D == DD && (a.gamma != nullptr) == NORM && (a.scales != nullptr) == MX4) {             \
+      hipLaunchKernelGGL((writer_few_kernel<DD, NORM, MX4>), few, dim3(64 * kWriterWaves), 0, stream, a); \
       return hipGetLastError();                                                                \
     }
-    ROLAQ_FEW(512, false)
-    ROLAQ_FEW(256, false)
-    ROLAQ_FEW(512, true)
-    ROLAQ_FEW(256, true)
+    ROLAQ_FEW(512, false, false)
+    ROLAQ_FEW(256, false, false)
+    ROLAQ_FEW(512, true, false)
+    ROLAQ_FEW(256, true, false)
+    ROLAQ_FEW(512, false, true)
+    ROLAQ_FEW(256, false, true)
 #undef ROLAQ_FEW
   }
   const dim3 grid((unsigned)(stripes * NG)), block(64 * kWriterWaves);
-#define ROLAQ_WRITER(DD, NORM, LDS)                                                                         \
-  if (D == DD && (a.gamma != nullptr) == NORM) {                                                           \
+#define ROLAQ_WRITER(DD, NORM, MX4, LDS)                                                                    \
+  if (D == DD && (a.gamma != nullptr) == NORM && (a.scales != nullptr) == MX4) {                           \
     const int lds = WriterGeo<DD>::LDS;                                                                    \
-    const hipError_t e = hipFuncSetAttribute((const void*)writer_kernel<DD, NORM>,                         \
+    const hipError_t e = hipFuncSetAttribute((const void*)writer_kernel<DD, NORM, MX4>,                         \
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);             \
     if (e != hipSuccess) return e;                                                                         \
-    hipLaunchKernelGGL((writer_kernel<DD, NORM>), grid, block, lds, stream, a);                            \
+    hipLaunchKernelGGL((writer_kernel<DD, NORM, MX4>), grid, block, lds, stream, a);                            \
     return hipGetLastError();                                                                              \
   }
-  ROLAQ_WRITER(512, false, LDS_BYTES)
-  ROLAQ_WRITER(256, false, LDS_BYTES)
-  ROLAQ_WRITER(512, true, LDS_NORM_BYTES)
-  ROLAQ_WRITER(256, true, LDS_NORM_BYTES)
+  ROLAQ_WRITER(512, false, false, LDS_BYTES)
+  ROLAQ_WRITER(256, false, false, LDS_BYTES)
+  ROLAQ_WRITER(512, true, false, LDS_NORM_BYTES)
+  ROLAQ_WRITER(256, true, false, LDS_NORM_BYTES)
+  ROLAQ_WRITER(512, false, true, LDS_BYTES)
+  ROLAQ_WRITER(256, false, true, LDS_BYTES)
 #undef ROLAQ_WRITER
   return hipErrorInvalidValue;
 }

@@ -33,6 +33,24 @@ def _stream(t: torch.Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+class _on:
+    """``dev`` as the current device for the calls inside: a launch goes to a
+    stream of its tensors' device. Nothing where it is current already."""
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index if dev.type == "cuda" else None
+
+    def __enter__(self):
+        self.before = None
+        if self.index is not None and self.index != torch.cuda.current_device():
+            self.before = torch.cuda.current_device()
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.before is not None:
+            torch.cuda.set_device(self.before)
+
+
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, ndim: int | None = None):
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor")
@@ -420,4 +438,105 @@ def assemble_rows(slots: torch.Tensor, codes: torch.Tensor, params: torch.Tensor
     _lib.check(_lib.load().rolaq_assemble_rows(
         _p(slots), slots.numel(), _p(codes), _p(params), _p(rope_buf), _p(hp_c), _p(row_of_slot),
         _p(owner_of_row), _p(rotation), D, R, _p(out), out.stride(0), _stream(codes)))
+    return out
+
+
+# ---- the 4-bit (MX4) latent cache ------------------------------------------------
+MX4_BLOCK = 32
+
+
+def _mx4_cache(codes, scales, rope_buf, dev):
+    """(slots, D, R) of a layer's MX4 buffers."""
+    _need_all(dev, ((codes, "codes", torch.uint8, 2), (scales, "scales", torch.uint8, 2),
+                    (rope_buf, "rope_buf", torch.bfloat16, 2)))
+    slots, D = codes.shape[0], codes.shape[1] * 2
+    if scales.shape != (slots, D // MX4_BLOCK) or rope_buf.shape[0] != slots:
+        raise ValueError("cache buffers do not match")
+    return slots, D, rope_buf.shape[1]
+
+
+def mx4_write_rows(latent: torch.Tensor, k_pe: torch.Tensor, rotation_t: torch.Tensor | None, loc: torch.Tensor,
+                   codes: torch.Tensor, scales: torch.Tensor, rope_buf: torch.Tensor) -> None:
+    """Rotate (``rotation_t`` = ``R_eff^T``, or None) + quantize + store ``n`` rows at slots ``loc``."""
+    dev = codes.device
+    slots, D, R = _mx4_cache(codes, scales, rope_buf, dev)
+    _need(latent, "latent", torch.bfloat16, dev, 2)
+    _need(k_pe, "k_pe", torch.bfloat16, dev, 2)
+    _need_all(dev, ((loc, "loc", torch.int64, 1),))
+    n = loc.shape[0]
+    if latent.shape != (n, D) or k_pe.shape != (n, R):
+        raise ValueError(f"latent must be [{n}, {D}] and k_pe [{n}, {R}]")
+    if n and latent.stride(1) != 1:
+        raise ValueError("latent rows must be contiguous")
+    if rotation_t is not None:
+        _need_all(dev, ((rotation_t, "rotation_t", torch.bfloat16, 2),))
+        if rotation_t.shape != (D, D):
+            raise ValueError("rotation_t must be [D, D]")
+    with _on(dev):
+        _lib.check(_lib.load().rolaq_mx4_write_rows(
+            _p(latent), latent.stride(0), _p(k_pe), k_pe.stride(0), k_pe.stride(1), _p(rotation_t), _p(loc), n, D, R,
+            _p(codes), _p(scales), _p(rope_buf), slots, _stream(codes)))
+
+
+def mx4_read_rows(slots: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, rope_buf: torch.Tensor,
+                  rotation: torch.Tensor | None, out: torch.Tensor) -> torch.Tensor:
+    """Rows at ``slots`` as bf16 ``[n, D + R]`` (the latent times ``rotation^T`` where there is one)."""
+    dev = codes.device
+    num, D, R = _mx4_cache(codes, scales, rope_buf, dev)
+    _need_all(dev, ((slots, "slots", torch.int64, 1),))
+    n = slots.shape[0]
+    if rotation is not None:
+        _need_all(dev, ((rotation, "rotation", torch.bfloat16, 2),))
+        if rotation.shape != (D, D):
+            raise ValueError("rotation must be [D, D]")
+    _need(out, "out", torch.bfloat16, dev, 2)
+    if out.shape[0] < n or out.shape[1] < D + R or (n and out.stride(1) != 1):
+        raise ValueError("out must be [n, >= D + R] with a contiguous last dim")
+    with _on(dev):
+        _lib.check(_lib.load().rolaq_mx4_read_rows(
+            _p(slots), n, _p(codes), _p(scales), _p(rope_buf), num, _p(rotation), D, R, _p(out), out.stride(0),
+            _stream(codes)))
+    return out
+
+
+def mx4_attend_workspace_bytes(D: int, device) -> int:
+    """Bytes of :func:`mx4_attend_fwd`'s workspace at width ``D`` on ``device``, whatever the batch."""
+    n = ctypes.c_int64(0)
+    with _on(torch.device(device)):
+        _lib.check(_lib.load().rolaq_mx4_attend_workspace(int(D), ctypes.byref(n)))
+    return n.value
+
+
+def mx4_attend_fwd(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, rope_buf: torch.Tensor,
+                   qo_indptr: torch.Tensor | None, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
+                   kv_lens: torch.Tensor, max_q_len: int, out: torch.Tensor, sm_scale: float, workspace: torch.Tensor,
+                   page_size: int = 1, lse: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ``q [T, H, D + R]`` over the MX4 cache -> ``out [T, H, D]`` (and ``lse [T, H]``)."""
+    dev = q.device
+    _need(q, "q", torch.bfloat16, dev, 3)
+    slots, D, R = _mx4_cache(codes, scales, rope_buf, dev)
+    T, H, DR = q.shape
+    if DR != D + R or (q.numel() and q.stride(2) != 1):
+        raise ValueError("q must be [T, H, D + R] with a contiguous last dim")
+    i32 = torch.int32
+    _need_all(dev, ((kv_indptr, "kv_indptr", i32, 1), (kv_indices, "kv_indices", i32, 1),
+                    (kv_lens, "kv_lens", torch.int64, 1), (workspace, "workspace", torch.uint8, 1)))
+    if qo_indptr is not None:
+        _need_all(dev, ((qo_indptr, "qo_indptr", i32, 1),))
+    B = T if qo_indptr is None else qo_indptr.shape[0] - 1
+    if B < 0 or kv_indptr.shape[0] < B + 1 or kv_lens.shape[0] < B:
+        raise ValueError("index tensors are shorter than the batch")
+    _need(out, "out", torch.bfloat16, dev, 3)
+    if out.shape[0] < T or out.shape[1] != H or out.shape[2] != D or (out.numel() and out.stride(2) != 1):
+        raise ValueError("out must be [>= T, H, D] with a contiguous last dim")
+    if lse is not None:
+        _need_all(dev, ((lse, "lse", torch.float32, 2),))
+        if lse.shape[0] < T or lse.shape[1] != H:
+            raise ValueError("lse must be [>= T, H]")
+    with _on(dev):
+        _lib.check(_lib.load().rolaq_mx4_attend_fwd(
+            _p(q), q.stride(0), q.stride(1), _p(codes), _p(scales), _p(rope_buf), slots, _p(qo_indptr), _p(kv_indptr),
+            _p(kv_indices), kv_indices.shape[0], int(page_size), _p(kv_lens), T, B, H, D, R, int(max_q_len),
+            float(sm_scale), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace), workspace.shape[0],
+            _stream(q)))
     return out

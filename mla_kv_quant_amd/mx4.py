@@ -1,0 +1,124 @@
+"""The 4-bit latent cache (MX4): pool, writer, read-back and attention.
+
+For layers, or models, that do not stand INT2: a cached latent row is D 4-bit
+floats (E2M1) with one power-of-two scale for 32 of them, beside the bf16 rope
+key -- 400 bytes a token and layer at (512, 64), 200 at (256, 32), against
+1152 and 576 in bf16 -- with no BF16 window and no quantizer parameters. The
+matrix cores of gfx950 take the codes as they are stored. Rows may be rotated
+by a layer's ``R_eff``, as in the INT2 cache; queries and outputs are then in the
+rotated frame (``artifacts.fold_read_rotation``).
+
+Every call launches on the current stream of its tensors' device, allocates
+nothing but an output that was not given (and the attention's workspace, once
+for a pool) and makes no synchronisation, so it can be captured in a HIP graph.
+The reference has no 4-bit cache.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import kernels
+from .writer import SUPPORTED_DIMS, _as_int64, _rows, _write_rotation
+
+
+class MX4MLAPool:
+    """Per-layer 4-bit cache buffers (layouts: ``include/rolaq_mla.h``).
+
+    ``size`` token slots besides slot 0, which is for graph padding.
+    ``rotations``: per-layer ``[D, D]`` rotations (or None), held in bf16
+    (``R_eff = fp32(bf16(R))``). The functions of this module take any object
+    with these attributes.
+    """
+
+    def __init__(self, size: int, layer_num: int, kv_lora_rank: int = 512, qk_rope_head_dim: int = 64, device="cuda",
+                 rotations=None, start_layer: int = 0):
+        if (kv_lora_rank, qk_rope_head_dim) not in SUPPORTED_DIMS:
+            raise ValueError(f"(kv_lora_rank, qk_rope_head_dim) must be one of {sorted(SUPPORTED_DIMS)}")
+        self.size = int(size)
+        self.layer_num = int(layer_num)
+        self.start_layer = int(start_layer)
+        self.kv_lora_rank = D = int(kv_lora_rank)
+        self.qk_rope_head_dim = int(qk_rope_head_dim)
+        self.device = torch.device(device)
+        slots, dev = self.size + 1, self.device
+
+        def buf(width, dtype):
+            return [torch.zeros(slots, width, dtype=dtype, device=dev) for _ in range(self.layer_num)]
+
+        self.c_codes = buf(D // 2, torch.uint8)
+        self.c_scales = buf(D // kernels.MX4_BLOCK, torch.uint8)
+        self.rope_buf = buf(self.qk_rope_head_dim, torch.bfloat16)
+        rotations = rotations or [None] * self.layer_num
+        self.rotations = [None if r is None else r.to(device=dev, dtype=torch.bfloat16) for r in rotations]
+
+    def latent_rotation(self, layer_id: int, local: bool = True):
+        return self.rotations[layer_id - self.start_layer if local else layer_id]
+
+    def get_kv_size_bytes(self) -> int:
+        D = self.kv_lora_rank
+        return (self.size + 1) * self.layer_num * (D // 2 + D // kernels.MX4_BLOCK + 2 * self.qk_rope_head_dim)
+
+
+def attend_workspace(pool) -> torch.Tensor:
+    """The attention's workspace of ``pool``, allocated once (67 MB at width 512):
+    every layer and batch uses it. Calls that may overlap on the GPU (two streams,
+    two graphs replayed side by side) need one each, passed as ``workspace``."""
+    ws = getattr(pool, "_mx4_workspace", None)
+    if ws is None:
+        dev = pool.c_codes[0].device
+        ws = torch.empty(kernels.mx4_attend_workspace_bytes(pool.kv_lora_rank, dev), dtype=torch.uint8, device=dev)
+        pool._mx4_workspace = ws
+    return ws
+
+
+def write_rows(pool, layer_id, loc, c_kv, k_pe) -> None:
+    """Store rows of layer ``layer_id`` at slots ``loc``: a decode step's or a prefill chunk's.
+
+    ``c_kv``: bf16 latents ``[n, D]`` (after ``kv_a_layernorm``; any shape with
+    ``n * D`` elements), ``k_pe``: bf16 rope keys. One launch rotates (on a
+    layer with a rotation), quantizes, packs and stores. Slots of one call must
+    differ, except for the padding slot; one outside the cache is skipped.
+    """
+    li = layer_id - pool.start_layer
+    rt = _write_rotation(pool, layer_id, pool.latent_rotation(layer_id, local=True))
+    kernels.mx4_write_rows(_rows(c_kv, pool.kv_lora_rank), _rows(k_pe, pool.qk_rope_head_dim), rt, _as_int64(loc),
+                           pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li])
+
+
+def read_rows(pool, layer_id, slots, out=None, unrotate: bool = True):
+    """Rows at ``slots`` of layer ``layer_id``: bf16 ``[n, D + R]`` (latent | rope).
+
+    With ``unrotate``, the latent of a rotated layer is multiplied back by
+    ``R_eff^T`` (FP32 sums, one rounding); else it is returned as it is stored,
+    exactly. A slot outside the cache reads as NaN.
+    """
+    li = layer_id - pool.start_layer
+    s = _as_int64(slots)
+    if out is None:
+        out = torch.empty(s.shape[0], pool.kv_lora_rank + pool.qk_rope_head_dim, dtype=torch.bfloat16,
+                          device=pool.c_codes[li].device)
+    rot = pool.latent_rotation(layer_id, local=True) if unrotate else None
+    if rot is not None:
+        rot = rot.to(torch.bfloat16).contiguous()
+    return kernels.mx4_read_rows(s, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], rot, out)
+
+
+def attend_fwd(q, o, pool, layer_id, kv_indptr, kv_indices, kv_lens, sm_scale, qo_indptr=None, max_q_len: int = 1,
+               page_size: int = 1, lse=None, workspace=None):
+    """Absorbed MLA attention over layer ``layer_id`` of ``pool``: decode, token verification, chunked prefill.
+
+    ``q``: bf16 ``[T, H, D + R]`` (absorbed latent query | rope query), ``o``: bf16
+    ``[T, H, D]``. ``kv_indptr``/``kv_indices``: int32 page (or token) lists;
+    ``kv_lens``: ``[B]`` cached positions, those of the queries' own rows (written
+    before) included. ``qo_indptr``: int32 ``[B + 1]`` query offsets, None for
+    one query each; query ``i`` of ``n`` sees the positions up to
+    ``kv_lens[b] - n + i``. ``max_q_len``: the most queries of a request (later
+    ones are left out). ``lse``: FP32 ``[T, H]``, receives the natural log of the
+    sum of exponentials. A query that sees nothing gets 0 (and -inf).
+    ``workspace``: of ``attend_workspace``'s size, the pool's own if not given.
+    """
+    li = layer_id - pool.start_layer
+    return kernels.mx4_attend_fwd(q, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], qo_indptr, kv_indptr,
+                                  kv_indices, _as_int64(kv_lens), max_q_len, o, sm_scale,
+                                  attend_workspace(pool) if workspace is None else workspace, page_size, lse)

@@ -1,0 +1,455 @@
+"""The MX4 cache on the GPU against the float64 oracle (oracle/mx4.py).
+
+Tolerances, from the arithmetic of the kernels:
+
+* rows without a rotation and stored rows: none, the bytes are exact;
+* rotated rows: an FP32 sum of D exact products is off by at most D 2^-24 of the
+  sum of their magnitudes (``err``); a stored value is then a level whose
+  distance from the exact value is at most the nearest level's plus 2 err;
+* rows rotated back: that error plus half a bf16 step (2^-8 of the value);
+* attention: each probability is rounded to bf16 (2^-8 of itself), scores are
+  FP32 sums (``ds`` = (D + R) 2^-23 sum |q k| sm_scale, the query's split off by at
+  most 2^-21 of its largest element more), and the output is rounded once:
+  |do| <= (2^-8 + 2 ds + 2^-16) sum softmax |x| + 2^-8 |o|. The LSE has the scores' error and
+  2^-20 for the FP32 sum, its logarithm and the final product with ln 2.
+"""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from mla_kv_quant_amd import MX4MLAPool, kernels, mx4, synth
+from oracle import mx4 as oracle
+from tests.helpers import alloc_slots
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def dims(D):
+    return D, D // 8
+
+
+def fill(pool, slots, x, pe):
+    """Write fp32 rows into layer 0 with the oracle's codec."""
+    code, s = oracle.encode(x)
+    at = torch.as_tensor(slots)
+    pool.c_codes[0][at.to(DEV)] = oracle.pack(code).to(DEV)
+    pool.c_scales[0][at.to(DEV)] = s.to(DEV)
+    pool.rope_buf[0][at.to(DEV)] = pe.to(DEV)
+
+
+class Batch:
+    """A cache with requests of the given lengths and query counts, and its oracle results."""
+
+    def __init__(self, D, H, lens, qlens, page, seed=0, spread=1.0, q_std=None, grow=0.0):
+        D, R = dims(D)
+        self.D, self.R, self.H, self.page, self.lens, self.qlens = D, R, H, page, lens, qlens
+        self.slots, pages, num = alloc_slots(lens, page, seed)
+        self.pool = MX4MLAPool(num - 1, 1, D, R, device=DEV)
+        # what nobody sees: NaN blocks and infinite rope rows
+        self.pool.c_scales[0].fill_(255)
+        self.pool.c_codes[0].random_(0, 256)
+        self.pool.rope_buf[0].fill_(float("inf"))
+        g = torch.Generator().manual_seed(seed + 5)
+        self.sm = 1 / math.sqrt(1.5 * D / 4)
+        self.T = sum(qlens)
+        std = q_std if q_std is not None else 2.0 / (self.sm * math.sqrt(D + R) * spread)
+        self.q = (torch.randn(self.T, H, D + R, generator=g) * std).to(torch.bfloat16)
+        self.x, self.pe = [], []
+        for b, n in enumerate(lens):
+            x = torch.randn(n, D, generator=g) * spread
+            if grow:  # later rows lie more and more along the first query
+                x += torch.linspace(0, grow, n)[:, None] * self.q[0, 0, :D].float()
+            pe = torch.randn(n, R, generator=g).to(torch.bfloat16)
+            if n:
+                fill(self.pool, self.slots[b], x, pe)
+            code, s = oracle.encode(x)
+            self.x.append(oracle.decode(oracle.pack(code), s))
+            self.pe.append(pe)
+        self.qo = torch.tensor(np.concatenate(([0], np.cumsum(qlens))), dtype=torch.int32, device=DEV)
+        self.kv_indptr = torch.tensor(np.concatenate(([0], np.cumsum([len(p) for p in pages]))), dtype=torch.int32,
+                                      device=DEV)
+        self.kv_indices = torch.tensor(np.concatenate([p for p in pages] + [np.zeros(0)]), dtype=torch.int32, device=DEV)
+        self.kv_lens = torch.tensor(lens, dtype=torch.int64, device=DEV)
+
+    def run(self, q=None, o=None, lse=None, decode=False, **kw):
+        q = self.q.to(DEV) if q is None else q
+        o = torch.full((self.T, self.H, self.D), 7.0, dtype=torch.bfloat16, device=DEV) if o is None else o
+        mx4.attend_fwd(q, o, self.pool, 0, self.kv_indptr, self.kv_indices, self.kv_lens, self.sm,
+                       qo_indptr=None if decode else self.qo, max_q_len=max(self.qlens), page_size=self.page, lse=lse,
+                       **kw)
+        return o
+
+    def check(self, o, lse=None, requests=None):
+        o = o.double().cpu()
+        t = 0
+        for b, (n, m) in enumerate(zip(self.lens, self.qlens)):
+            if requests is not None and b not in requests:
+                t += m
+                continue
+            q = self.q[t:t + m]
+            vis = [n - m + i + 1 for i in range(m)]
+            want, wl, w = oracle.attend(q, self.x[b], self.pe[b], vis, self.sm)
+            if n:
+                k = torch.cat((self.x[b], self.pe[b].double()), -1).abs()
+                big = q[..., :self.D].double().abs().amax(-1, keepdim=True)
+                ds = self.sm * ((self.D + self.R) * 2.0 ** -23 * (q.double().abs() @ k.t()).amax(-1)
+                                + (2.0 ** -21 * big * self.x[b].abs().sum(-1).amax())[..., 0])
+            else:
+                ds = torch.zeros(m, self.H, dtype=torch.float64)
+            tol = (2.0 ** -8 + 2 * ds[..., None] + 2.0 ** -16) * w + 2.0 ** -8 * want.abs()
+            bad = (o[t:t + m] - want).abs() > tol
+            assert not bad.any(), (b, n, m, bad.sum().item(), ((o[t:t + m] - want).abs() / (tol + 1e-300)).max().item())
+            if lse is not None:
+                got = lse[t:t + m].double().cpu()
+                seen = torch.isfinite(wl)
+                assert torch.equal(seen, torch.isfinite(got)) and (got[~seen] == float("-inf")).all()
+                off = (got - wl).abs()[seen]
+                assert (off <= (ds + 2.0 ** -20 * (1 + wl.abs()))[seen]).all(), off.max().item()
+            t += m
+
+
+# ---- rows ------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("n", [1, 3, 64, 257])
+def test_plain_rows_are_exact(D, n):
+    D, R = dims(D)
+    pool = MX4MLAPool(600, 2, D, R, device=DEV, start_layer=3)
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn(n, D, generator=g) * torch.exp2(torch.rand(n, D // 32, generator=g) * 90 - 60).repeat_interleave(32, 1)
+    x[0, :32] = 0
+    x = x.to(torch.bfloat16)
+    pe = torch.randn(n, R, generator=g).to(torch.bfloat16)
+    loc = torch.randperm(600, generator=g)[:n] + 1
+    mx4.write_rows(pool, 4, loc.to(DEV), x.to(DEV), pe.to(DEV))
+    code, s = oracle.encode(x.float())
+    assert torch.equal(pool.c_codes[1][loc.to(DEV)].cpu(), oracle.pack(code))
+    assert torch.equal(pool.c_scales[1][loc.to(DEV)].cpu(), s)
+    assert torch.equal(pool.rope_buf[1][loc.to(DEV)].cpu(), pe)
+    other = torch.ones(601, dtype=torch.bool)
+    other[loc] = False
+    assert (pool.c_codes[1][other.to(DEV)] == 0).all() and (pool.rope_buf[1][other.to(DEV)] == 0).all()
+    assert (pool.c_codes[0] == 0).all()
+    back = mx4.read_rows(pool, 4, loc.to(DEV)).cpu()
+    assert torch.equal(back[:, :D].double(), oracle.decode(oracle.pack(code), s)) and torch.equal(back[:, D:], pe)
+
+
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("n", [1, 15, 17, 100, 1000, 9000])
+def test_rotated_rows(D, n):
+    D, R = dims(D)
+    rot = synth.make_rotation(D, 3)
+    pool = MX4MLAPool(n + 20, 1, D, R, device=DEV, rotations=[rot])
+    x = synth.make_latent(n, D, 5, seed=n, factor=8.0)
+    pe = synth.make_normal((n, R), n + 1)
+    loc = torch.randperm(n + 20, generator=torch.Generator().manual_seed(n))[:n] + 1
+    mx4.write_rows(pool, 0, loc.to(DEV), x.to(DEV), pe.to(DEV))
+    r = rot.to(torch.bfloat16).double()
+    y = x.double() @ r
+    err = D * 2.0 ** -24 * (x.double().abs() @ r.abs())
+    s = pool.c_scales[0][loc.to(DEV)].cpu()
+    v = oracle.decode(pool.c_codes[0][loc.to(DEV)].cpu(), s)
+    # scales: those of the exact rows, moved by the error at most
+    eb = err.unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(-1, -1, 32).flatten(-2)
+    lo = oracle.scale_bytes(torch.sign(y) * (y.abs() - eb).clamp(min=0))
+    hi = oracle.scale_bytes(y + torch.sign(y) * eb)
+    assert ((s >= lo) & (s <= hi)).all()
+    f = torch.ldexp(torch.ones(s.shape, dtype=torch.float64), s.long() - 127).repeat_interleave(32, -1)
+    near = torch.full_like(y, float("inf"))
+    for level in oracle.LEVELS:
+        near = torch.minimum(near, (y.abs() - level * f).abs())
+    assert ((v - y).abs() <= near + 2 * err).all()
+    assert torch.equal(pool.rope_buf[0][loc.to(DEV)].cpu(), pe)
+    # as stored, and rotated back
+    assert torch.equal(mx4.read_rows(pool, 0, loc.to(DEV), unrotate=False).cpu()[:, :D].double(), v)
+    back = mx4.read_rows(pool, 0, loc.to(DEV)).cpu()
+    want = v @ r.t()
+    tol = 2.0 ** -8 * want.abs() + 1.01 * D * 2.0 ** -24 * (v.abs() @ r.abs().t())
+    assert ((back[:, :D].double() - want).abs() <= tol).all() and torch.equal(back[:, D:], pe)
+
+
+def test_rotated_rows_do_not_depend_on_the_launch_size():
+    D, R, n = 512, 64, 9000
+    rot = synth.make_rotation(D, 3)
+    x, pe = synth.make_latent(n, D, 5, seed=1).to(DEV), synth.make_normal((n, R), 2).to(DEV)
+    a = MX4MLAPool(n, 1, D, R, device=DEV, rotations=[rot])
+    b = MX4MLAPool(n, 1, D, R, device=DEV, rotations=[rot])
+    loc = torch.arange(1, n + 1, device=DEV)
+    mx4.write_rows(a, 0, loc, x, pe)
+    for i in range(0, n, 1500):
+        mx4.write_rows(b, 0, loc[i:i + 1500], x[i:i + 1500], pe[i:i + 1500])
+    assert torch.equal(a.c_codes[0], b.c_codes[0]) and torch.equal(a.c_scales[0], b.c_scales[0])
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+def test_rows_that_are_not_finite(rotated):
+    D, R = 512, 64
+    pool = MX4MLAPool(16, 1, D, R, device=DEV, rotations=[synth.make_rotation(D, 1)] if rotated else None)
+    x = torch.randn(6, D, generator=torch.Generator().manual_seed(1))
+    x[0, 7], x[1, 40], x[2, 100], x[3, 500], x[4] = float("nan"), float("inf"), -float("inf"), 3e38, 0
+    x = x.to(torch.bfloat16)
+    loc = torch.arange(1, 7, device=DEV)
+    mx4.write_rows(pool, 0, loc, x.to(DEV), torch.zeros(6, R, dtype=torch.bfloat16, device=DEV))
+    s = pool.c_scales[0][loc].cpu()
+    v = mx4.read_rows(pool, 0, loc, unrotate=False)[:, :D].float().cpu()
+    if rotated:
+        assert (s[:4] == 255).all() and torch.isnan(v[:4]).all()
+        assert torch.isnan(mx4.read_rows(pool, 0, loc)[:4, :D]).all()
+    else:
+        assert torch.equal(s, oracle.scale_bytes(x.float()))
+        assert [(s[i] == 255).nonzero().tolist() for i in range(4)] == [[[0]], [[1]], [[3]], [[15]]]
+    assert (v[4] == 0).all() and torch.isfinite(v[5]).all()
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+@pytest.mark.parametrize("D", [512, 256])
+def test_strided_inputs_and_slots_outside_the_cache(rotated, D):
+    D, R = dims(D)
+    rot = [synth.make_rotation(D, 1)] if rotated else None
+    n = 40
+    x = synth.make_latent(n, D, 3, 1).to(DEV)
+    pe = synth.make_normal((n, R), 2).to(DEV)
+    loc = torch.arange(1, n + 1, device=DEV)
+    want = MX4MLAPool(n, 1, D, R, device=DEV, rotations=rot)
+    mx4.write_rows(want, 0, loc, x, pe)
+    pool = MX4MLAPool(n, 1, D, R, device=DEV, rotations=rot)
+    wide = torch.zeros(n, D + R + 8, dtype=torch.bfloat16, device=DEV)
+    wide[:, :D] = x
+    pe_t = pe.t().contiguous().t()  # columns apart
+    bad = loc.clone()
+    bad[3], bad[5], bad[7] = -1, n + 1, 1 << 40
+    mx4.write_rows(pool, 0, bad, wide[:, :D], pe_t)
+    keep = torch.ones(n + 1, dtype=torch.bool, device=DEV)
+    keep[[4, 6, 8]] = False
+    for a, b in ((pool.c_codes, want.c_codes), (pool.c_scales, want.c_scales), (pool.rope_buf, want.rope_buf)):
+        assert torch.equal(a[0][keep], b[0][keep]) and (a[0][~keep] == 0).all()
+    out = torch.full((n + 2, D + R + 16), 3.0, dtype=torch.bfloat16, device=DEV)
+    mx4.read_rows(want, 0, bad, out=out)
+    assert torch.isnan(out[[3, 5, 7], :D + R]).all()
+    assert (out[n:] == 3).all() and (out[:, D + R:] == 3).all()
+    ok = [i for i in range(n) if i not in (3, 5, 7)]
+    assert torch.equal(out[ok, :D + R], mx4.read_rows(want, 0, loc)[ok])
+
+
+def test_no_rows():
+    pool = MX4MLAPool(16, 1, device=DEV)
+    none = torch.zeros(0, dtype=torch.int64, device=DEV)
+    mx4.write_rows(pool, 0, none, torch.zeros(0, 512, dtype=torch.bfloat16, device=DEV),
+                   torch.zeros(0, 64, dtype=torch.bfloat16, device=DEV))
+    assert mx4.read_rows(pool, 0, none).shape == (0, 576)
+    q = torch.zeros(0, 16, 576, dtype=torch.bfloat16, device=DEV)
+    i32 = torch.zeros(1, dtype=torch.int32, device=DEV)
+    mx4.attend_fwd(q, q[..., :512].contiguous(), pool, 0, i32, i32, none, 0.1)
+
+
+# ---- attention -----------------------------------------------------------------------
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("H", [1, 8, 16, 17, 32, 40, 128])
+@pytest.mark.parametrize("page", [1, 64])
+def test_decode(D, H, page):
+    b = Batch(D, H, [1, 63, 0, 64, 65, 300, 1025], [1] * 7, page, seed=H)
+    lse = torch.empty(b.T, H, device=DEV)
+    o = b.run(lse=lse, decode=True)
+    b.check(o, lse)
+    assert torch.equal(o, b.run())  # the same batch by query offsets, bit for bit
+
+
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("H,qlens", [(16, [3, 1, 4, 2, 0, 4]), (40, [2, 9, 1, 0, 5, 3]), (5, [7, 1, 20, 2, 9, 33])])
+@pytest.mark.parametrize("page", [16, 128])
+def test_a_few_queries(D, H, qlens, page):
+    # the third request has fewer positions than queries: its first see nothing
+    b = Batch(D, H, [3, 500, 2, 64, 10, 700], qlens, page, seed=3)
+    lse = torch.empty(b.T, H, device=DEV)
+    b.check(b.run(lse=lse), lse)
+
+
+@pytest.mark.parametrize("D,H,lens,qlens", [
+    (512, 16, [130, 900, 257], [130, 200, 1]),
+    (256, 40, [200, 513], [199, 77]),
+    (256, 3, [1000], [1000]),
+])
+def test_prefill(D, H, lens, qlens):
+    b = Batch(D, H, lens, qlens, 32, seed=9)
+    lse = torch.empty(b.T, H, device=DEV)
+    b.check(b.run(lse=lse), lse)
+
+
+@pytest.mark.parametrize("D,H", [(512, 16), (256, 40)])
+def test_many_row_blocks(D, H):
+    # more row blocks than are shared out: a block each
+    n = 8200 if H == 16 else 3300
+    b = Batch(D, H, [n, 70], [n - 50, 66], 64, seed=2)
+    o = b.run()
+    rows = [0, 1, 63, 64, 1000, n - 51]
+    want, _, w = oracle.attend(b.q[rows], b.x[0], b.pe[0], [51 + i for i in rows], b.sm)
+    tol = (2.0 ** -8 + 2.0 ** -10) * w + 2.0 ** -8 * want.abs()  # (scores off by far less than 2^-11)
+    assert ((o[rows].double().cpu() - want).abs() <= tol).all()
+    b.check(o, requests=[1])
+
+
+def test_many_requests():
+    # more requests than a block's sums hold
+    lens = [(37 * i) % 130 for i in range(1100)]
+    b = Batch(256, 4, lens, [1] * 1100, 16, seed=4)
+    o = b.run(decode=True)
+    b.check(o, requests=range(0, 1100, 7))
+    few = Batch(256, 4, lens[:1000], [1] * 1000, 16, seed=4)
+    few.check(few.run(decode=True), requests=range(0, 1000, 11))
+
+
+@pytest.mark.parametrize("H", [16, 30, 64])
+def test_scores_that_outgrow_the_reference(H):
+    """Row references have to move by far more than the slack, at tiles of every wave."""
+    b = Batch(512, H, [1500, 200], [1, 1], 64, seed=6, q_std=1.0, grow=6.0)
+    lse = torch.empty(b.T, H, device=DEV)
+    b.check(b.run(lse=lse), lse)
+    assert lse.max().item() > 60
+
+
+def test_latents_of_small_and_large_magnitude():
+    for spread in (1e-4, 3e3):
+        b = Batch(512, 16, [400, 100], [1, 2], 16, seed=8, spread=spread)
+        b.check(b.run())
+
+
+def test_long_context_beside_short_ones():
+    b = Batch(256, 16, [70001, 5, 3000], [1, 1, 1], 64, seed=12)
+    lse = torch.empty(b.T, 16, device=DEV)
+    b.check(b.run(lse=lse), lse)
+
+
+def test_rows_that_are_not_finite_stay_where_they_are():
+    b = Batch(512, 16, [200, 200, 200], [1, 1, 1], 64, seed=1)
+    q = b.q.clone()
+    q[0, 3, 17] = float("nan")
+    q[1, 5, 530] = float("inf")
+    o = b.run(q=q.to(DEV)).float().cpu()
+    assert torch.isnan(o[0, 3]).all() and torch.isnan(o[1, 5]).all()
+    o[0, 3], o[1, 5] = 0, 0
+    assert torch.isfinite(o).all()
+    # a NaN row that is seen makes its request NaN, and no other
+    b.pool.c_scales[0][int(b.slots[1][150])] = 255
+    o = b.run().float().cpu()
+    assert torch.isnan(o[1]).all() and torch.isfinite(o[0]).all() and torch.isfinite(o[2]).all()
+
+
+def test_strides_and_rows_behind_the_last_sequence():
+    b = Batch(512, 16, [100, 300], [2, 3], 32, seed=7)
+    q = torch.zeros(b.T + 4, 20, b.D + b.R + 16, dtype=torch.bfloat16, device=DEV)
+    q[:b.T, 2:18, 8:8 + b.D + b.R] = b.q.to(DEV)
+    o = torch.full((b.T + 4, 18, b.D + 8), 5.0, dtype=torch.bfloat16, device=DEV)
+    mx4.attend_fwd(q[:, 2:18, 8:8 + b.D + b.R], o[:, 1:17, 4:4 + b.D], b.pool, 0, b.kv_indptr, b.kv_indices, b.kv_lens,
+                   b.sm, qo_indptr=b.qo, max_q_len=3, page_size=32)
+    b.check(o[:b.T, 1:17, 4:4 + b.D])
+    assert (o[b.T:] == 5).all() and (o[:, 0] == 5).all() and (o[:, 17] == 5).all()
+    assert (o[..., :4] == 5).all() and (o[..., 4 + b.D:] == 5).all()
+
+
+def test_bad_pages_read_inside_the_cache():
+    b = Batch(256, 16, [300, 300], [1, 1], 64, seed=7)
+    bad = b.kv_indices.clone()
+    bad[0], bad[1], bad[2] = 1 << 30, -5, 0x7fffffff
+    o = torch.zeros(2, 16, 256, dtype=torch.bfloat16, device=DEV)
+    mx4.attend_fwd(b.q.to(DEV), o, b.pool, 0, b.kv_indptr, bad, b.kv_lens, b.sm, page_size=64)
+    b.check(o, requests=[1])
+    # a list that ends early cuts the length
+    short = b.kv_indptr.clone()
+    lens = b.kv_lens.clone()
+    lens[1] = 1 << 40
+    mx4.attend_fwd(b.q.to(DEV), o, b.pool, 0, short, b.kv_indices[:-1], lens, b.sm, page_size=64)
+    want, _, w = oracle.attend(b.q[1:], b.x[1][:256], b.pe[1][:256], [256], b.sm)
+    assert ((o[1:].double().cpu() - want).abs() <= (2.0 ** -8 + 2.0 ** -10) * w + 2.0 ** -8 * want.abs()).all()
+
+
+def test_same_call_repeats_bit_for_bit_and_layout_does_not_matter():
+    a = Batch(512, 16, [700, 40, 2000], [1, 1, 1], 64, seed=11)
+    first = a.run()
+    mx4.attend_workspace(a.pool).fill_(255)
+    assert torch.equal(first, a.run())
+    ws = torch.zeros(kernels.mx4_attend_workspace_bytes(512, DEV), dtype=torch.uint8, device=DEV)
+    assert torch.equal(first, a.run(workspace=ws))
+
+
+def test_captured_step_is_replayed():
+    """Write and attend captured together; every replay against the eager result, with eager work between."""
+    D, R, H, n = 512, 64, 16, 3
+    rot = synth.make_rotation(D, 5)
+    lens = [129, 700, 64]
+    b = Batch(D, H, lens, [1] * n, 64, seed=13)
+    b.pool.rotations = [rot.to(DEV, torch.bfloat16)]
+    loc = torch.tensor([int(s[-1]) for s in b.slots], device=DEV)
+    x, pe = torch.zeros(n, D, dtype=torch.bfloat16, device=DEV), torch.zeros(n, R, dtype=torch.bfloat16, device=DEV)
+    q = b.q.to(DEV)
+    o = torch.zeros(n, H, D, dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        mx4.write_rows(b.pool, 0, loc, x, pe)
+        mx4.attend_fwd(q, o, b.pool, 0, b.kv_indptr, b.kv_indices, b.kv_lens, b.sm, page_size=64)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        x.copy_(synth.make_latent(n, D, 5, seed=i))
+        pe.copy_(synth.make_normal((n, R), i))
+        o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = o.clone()
+        o.zero_()
+        step()
+        torch.cuda.synchronize()
+        assert torch.equal(got, o)
+        assert got.abs().max() > 0
+
+
+def test_another_stream():
+    b = Batch(512, 16, [500, 900], [1, 1], 64, seed=14)
+    want = b.run()
+    q = b.q.to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = b.run(q=q)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_prefill_then_decode_as_a_server_does():
+    """Prefill in two chunks, each written and then attended over, then decode steps, on a rotated layer."""
+    D, R, H, page = 512, 64, 16, 64
+    rot = synth.make_rotation(D, 21)
+    slots, pages, num = alloc_slots([330, 210], page, 5)
+    pool = MX4MLAPool(num - 1, 1, D, R, device=DEV, rotations=[rot])
+    sm = 1 / math.sqrt(192)
+    xs = [synth.make_latent(len(s), D, 5, seed=40 + i, factor=8.0) for i, s in enumerate(slots)]
+    pes = [synth.make_normal((len(s), R), 50 + i) for i, s in enumerate(slots)]
+    kv_indptr = torch.tensor([0, len(pages[0]), len(pages[0]) + len(pages[1])], dtype=torch.int32, device=DEV)
+    kv_indices = torch.tensor(np.concatenate(pages), dtype=torch.int32, device=DEV)
+    done = [0, 0]
+    for step, m in enumerate([(128, 200), (200, 8), (1, 1), (1, 1)]):
+        loc = np.concatenate([slots[i][done[i]:done[i] + m[i]] for i in range(2)])
+        x = torch.cat([xs[i][done[i]:done[i] + m[i]] for i in range(2)])
+        pe = torch.cat([pes[i][done[i]:done[i] + m[i]] for i in range(2)])
+        mx4.write_rows(pool, 0, torch.from_numpy(loc).to(DEV), x.to(DEV), pe.to(DEV))
+        done = [done[i] + m[i] for i in range(2)]
+        T = sum(m)
+        q = synth.make_normal((T, H, D + R), 60 + step, std=0.5)
+        o = torch.empty(T, H, D, dtype=torch.bfloat16, device=DEV)
+        mx4.attend_fwd(q.to(DEV), o, pool, 0, kv_indptr, kv_indices, torch.tensor(done, device=DEV), sm,
+                       qo_indptr=torch.tensor([0, m[0], T], dtype=torch.int32, device=DEV), max_q_len=max(m),
+                       page_size=page)
+        t = 0
+        for i in range(2):
+            at = torch.from_numpy(slots[i][:done[i]]).to(DEV)
+            v = oracle.decode(pool.c_codes[0][at].cpu(), pool.c_scales[0][at].cpu())
+            want, _, w = oracle.attend(q[t:t + m[i]], v, pes[i][:done[i]], [done[i] - m[i] + j + 1 for j in range(m[i])], sm)
+            off = (o[t:t + m[i]].double().cpu() - want).abs()
+            assert (off <= (2.0 ** -8 + 2.0 ** -10) * w + 2.0 ** -8 * want.abs()).all()
+            t += m[i]
