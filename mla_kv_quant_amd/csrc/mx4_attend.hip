@@ -72,6 +72,16 @@ __device__ __forceinline__ void copy4(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
 }
 
+// The same from a scalar base and a 32-bit offset for each lane.
+__device__ __forceinline__ void copy16(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -81,6 +91,31 @@ __device__ __forceinline__ void wait_loads() {
 __device__ __forceinline__ uint32_t sub_sat(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t,
                             __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
+// One group's output accumulators times f where need is not 0, in
+// place in AGPRs (the branch is inside, so the compiler sees no join and adds no
+// copies of them; the waits cover the MFMAs before and behind).
+__device__ __forceinline__ void scale_acc8(f32x4 (&o)[8], float f, uint32_t need) {
+  float t0, t1, t2, t3;
+  asm volatile(
+      "s_cmp_lg_u32 %13, 0\n\t"
+      "s_cbranch_scc0 1f\n\t"
+      "s_nop 7\n\ts_nop 7\n\t"
+      "ROLAQ_ACC_SCALE %0, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %1, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %2, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %3, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %4, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %5, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %6, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "ROLAQ_ACC_SCALE %7, %8, %9, %10, %11, %12, %12, %12, %12\n\t"
+      "s_nop 7\n"
+      "1:"
+      : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]),
+        "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+      : "v"(f), "s"(need)
+      : "scc");
 }
 
 // Eight 4-bit codes -> eight bf16 values, in order.
@@ -113,6 +148,7 @@ struct Mx4Geo {
   static constexpr int TILE = CODES + ROPE + SCALES;  // a ring slot
   static constexpr int S = D == 512 ? 5 : 4;          // ring slots
   static constexpr int OCC = D == 512 ? 1 : 2;        // blocks on a CU
+  static constexpr bool ACC = D == 512 && G >= 2;     // over 256 registers: O in AGPRs
   static constexpr int LOADS = CODES / 4096 + ROPE / 4096 + 1;  // a wave's copies for a tile
   // LDS offsets
   static constexpr int P = S * TILE;                        // [2][ROWS][64] bf16, 16-byte chunks swizzled
@@ -165,10 +201,14 @@ __device__ __forceinline__ uint32_t mx4_block_of(uint32_t u, uint32_t units, uin
   return (uint32_t)((((uint64_t)u + 1) * n - 1) / units);
 }
 
-template <int D, int R, int G>
-__global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel(Mx4AttendArgs a) {
+// PAGED: pages of 16 positions or more. A wave copies 16 positions, which then lie
+// in one page: its number is a scalar, and the copies' offsets are the same for
+// every tile. Otherwise the page numbers of 16 positions come through LDS.
+template <int D, int R, int G, bool PAGED>
+__global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_attend_kernel(Mx4AttendArgs a) {
   using Ge = Mx4Geo<D, R, G>;
   constexpr int NB = Ge::NB, KS = Ge::KS, CB = Ge::CB, FT = Ge::FT, TW = Ge::TW, S = Ge::S;
+  if constexpr (Ge::ACC) define_acc_macros();
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)smem;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -250,6 +290,21 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
   const uint32_t page_mask = (1u << a.page_shift) - 1;
   const float c2 = a.sm_scale * kLog2e;
   int nth = 0;  // segments done
+  // A wave's copies of 16 positions: RC (RR) rows of codes (rope) at a time, LC (LR)
+  // lanes a row; chunk c of row t goes to chunk c ^ f(t), so that 16 lanes that read
+  // one chunk of 16 rows, or 16 rows' parts of one block, meet all banks.
+  constexpr int RC = 1024 / CB, LC = 64 / RC, RR = 1024 / (2 * R), LR = 64 / RR, LS = NB / 4;
+  auto code_swz = [](int t) { return D == 512 ? t & 15 : (t >> 1) & 7; };
+  auto rope_swz = [](int t) { return R == 64 ? (t >> 1) & 7 : (t >> 2) & 3; };
+  auto code_off = [&](int j) {  // byte of copy j's piece within the 16 rows
+    const int t = RC * j + lane / LC;
+    return t * CB + 16 * ((lane % LC) ^ code_swz(t));
+  };
+  auto rope_off = [&](int j) {
+    const int t = RR * j + lane / LR;
+    return t * 2 * R + 16 * ((lane % LR) ^ rope_swz(t));
+  };
+  const int scale_off = ((lane / LS) & 15) * NB + 4 * (lane % LS);
 
   while (u < u_end) {
     // ---- the next segment: tiles [t0, t1) of a row block of request b ---------------
@@ -290,47 +345,69 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
     __syncthreads();  // the last segment's LDS reads are done
 
     // ---- page numbers and tiles, asynchronously ---------------------------------------
+    const int list_last = pos_last & ~15;  // (PAGED) first of the last 16 positions
+    auto page_of = [&](int k) -> uint32_t {  // PAGED: page of this wave's 16 positions of tile k
+      const int pos = min(kMx4Tile * (t0 + k) + 16 * wave, list_last);
+      return *(const __attribute__((address_space(4))) uint32_t*)(a.kv_indices + rq.list + (pos >> a.page_shift));
+    };
     auto copy_idx = [&](int k) {
       const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + la, pos_last);
       copy4(a.kv_indices + rq.list + (pos >> a.page_shift),
             lds0 + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256);
     };
-    auto slot_of = [&](int k, int x) {  // cache slot of position x of this wave's 16
-      const uint32_t page =
-          *reinterpret_cast<const uint32_t*>(smem + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256 + 4 * x);
-      const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + x, pos_last);
-      return min((min(page, max_page) << a.page_shift) + ((uint32_t)pos & page_mask), max_slot);
+    // Copies of tile k to the ring slot at byte `at`; `slot(x)`: cache slot of position x of this wave's 16.
+    auto copy_slots = [&](uint32_t at, auto&& slot) {
+      uint32_t sl[16 / RC + 16 / RR + 1];
+#pragma unroll
+      for (int j = 0; j < 16 / RC; ++j) sl[j] = slot(RC * j + lane / LC);
+#pragma unroll
+      for (int j = 0; j < 16 / RR; ++j) sl[16 / RC + j] = slot(RR * j + lane / LR);
+      sl[16 / RC + 16 / RR] = slot((lane / LS) & 15);
+#pragma unroll
+      for (int j = 0; j < 16 / RC; ++j)
+        copy16(a.codes + (uint64_t)sl[j] * CB + code_off(j) % CB, at + 16 * wave * CB + 1024 * j);
+#pragma unroll
+      for (int j = 0; j < 16 / RR; ++j)
+        copy16(reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)sl[16 / RC + j] * (2 * R) + rope_off(j) % (2 * R),
+               at + Ge::CODES + 16 * wave * 2 * R + 1024 * j);
+      copy4(a.scales + (uint64_t)sl[16 / RC + 16 / RR] * NB + 4 * (lane % LS), at + Ge::CODES + Ge::ROPE + 256 * wave);
     };
-    auto copy_tile = [&](int k) {
-      const uint32_t dst = lds0 + (uint32_t)(k % S) * Ge::TILE;
-      constexpr int RC = 1024 / CB, LC = 64 / RC;  // rows of a copy, lanes of a row
+    auto copy_tile = [&](int k, uint32_t at, uint32_t page) {
+      at += lds0;
+      if constexpr (PAGED) {
+        const int pos = min(kMx4Tile * (t0 + k) + 16 * wave, list_last);
+        const uint32_t s0 = (min(page, max_page) << a.page_shift) + ((uint32_t)pos & page_mask);
+        if (__builtin_expect(s0 + 15 <= max_slot, 1)) {
+          const uint8_t* const c = a.codes + (uint64_t)s0 * CB;
+          const uint8_t* const r = reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)s0 * (2 * R);
 #pragma unroll
-      for (int j = 0; j < 16 / RC; ++j) {
-        const int x = RC * j + lane / LC, t = 16 * wave + x;
-        const int c = (lane % LC) ^ (D == 512 ? t & 15 : (t >> 1) & 7);
-        copy16(a.codes + (uint64_t)slot_of(k, x) * CB + 16 * c, dst + 16 * wave * CB + 1024 * j);
-      }
-      constexpr int RR = 1024 / (2 * R), LR = 64 / RR;
+          for (int j = 0; j < 16 / RC; ++j) copy16(c, (uint32_t)code_off(j), at + 16 * wave * CB + 1024 * j);
 #pragma unroll
-      for (int j = 0; j < 16 / RR; ++j) {
-        const int x = RR * j + lane / LR, t = 16 * wave + x;
-        const int c = (lane % LR) ^ (R == 64 ? (t >> 1) & 7 : (t >> 2) & 3);
-        copy16(a.rope + (uint64_t)slot_of(k, x) * R + 8 * c, dst + Ge::CODES + 16 * wave * 2 * R + 1024 * j);
+          for (int j = 0; j < 16 / RR; ++j)
+            copy16(r, (uint32_t)rope_off(j), at + Ge::CODES + 16 * wave * 2 * R + 1024 * j);
+          copy4(a.scales + (uint64_t)s0 * NB, (uint32_t)scale_off, at + Ge::CODES + Ge::ROPE + 256 * wave);
+        } else {  // the cache ends inside the page
+          copy_slots(at, [&](int x) { return min(s0 + (uint32_t)x, max_slot); });
+        }
+      } else {
+        const uint8_t* const idx = smem + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256;
+        copy_slots(at, [&](int x) {
+          const uint32_t p = *reinterpret_cast<const uint32_t*>(idx + 4 * x);
+          const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + x, pos_last);
+          return min((min(p, max_page) << a.page_shift) + ((uint32_t)pos & page_mask), max_slot);
+        });
       }
-      constexpr int LS = NB / 4;  // lanes of a row's scales
-      const int x = (lane / LS) & 15;
-      copy4(a.scales + (uint64_t)slot_of(k, x) * NB + 4 * (lane % LS), dst + Ge::CODES + Ge::ROPE + 256 * wave);
     };
 
     // ---- the query rows of this wave's group: e4m3 hi and lo parts, rope ---------------
     i32x8 qhi[KS], qlo[KS];
     u32x4 qpe[R / 32];
     uint32_t qscale;
+    u32x4 v[KS][2][2];
     {
       const int r = min(my_row, max(rows - 1, 0));
       const int tok = min(rq.q0 + r / a.H, a.T - 1);
       const uint16_t* q = a.q + (int64_t)tok * a.q_st + (int64_t)(r % a.H) * a.q_sh;
-      u32x4 v[KS][2][2];
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -342,6 +419,42 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
         }
 #pragma unroll
       for (int k = 0; k < R / 32; ++k) qpe[k] = gload<u32x4>(q + D + 32 * k + 8 * gq);
+    }
+    // The first tiles are asked for behind the query's loads; those are waited for here,
+    // with the page numbers, so that no wait for them is left behind the tiles.
+    uint32_t page = 0;  // PAGED: of the next tile to ask for
+    if (nt > 0) {
+      if constexpr (PAGED) {
+        page = page_of(0);
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < S - 2; ++k) copy_idx(k);
+      }
+    }
+    wait_loads<0>();
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+      asm volatile("" : "+v"(v[s][0][0]), "+v"(v[s][0][1]), "+v"(v[s][1][0]), "+v"(v[s][1][1]));
+#pragma unroll
+    for (int k = 0; k < R / 32; ++k) asm volatile("" : "+v"(qpe[k]));
+    uint32_t ask = 0;  // ring slot of the next tile to ask for
+    auto next = [](uint32_t at) { return at + Ge::TILE == S * Ge::TILE ? 0u : at + Ge::TILE; };
+    auto ask_tile = [&](int k) {
+      if (k < nt) {
+        const uint32_t p = page;
+        if constexpr (PAGED) page = page_of(k + 1);
+        copy_tile(k, ask, p);
+        ask = next(ask);
+      }
+    };
+    if (nt > 0) {
+#pragma unroll 1
+      for (int k = 0; k < S - 2; ++k) {
+        if constexpr (!PAGED) copy_idx(k + S - 2);
+        ask_tile(k);
+      }
+    }
+    {
       // largest magnitude of the row, as bits (NaN above infinity)
       uint32_t big = 0;
 #pragma unroll
@@ -391,15 +504,15 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
 
     // Scores and probabilities of tile k: P, the scales' exponent fields and the
     // wave's flag go to LDS buffer k & 1.
-    auto scores = [&](int k) {
-      const uint8_t* const slot = smem + (k % S) * Ge::TILE;
+    auto scores = [&](int k, uint32_t at) {
+      const uint8_t* const slot = smem + at;
       const int buf = k & 1;
       f32x4 acc[G];
 #pragma unroll
       for (int m = 0; m < G; ++m) {
         const int t = 16 * (tw * G + m) + la;
         const uint8_t* const row = slot + t * CB;
-        const int f = D == 512 ? t & 15 : (t >> 1) & 7;
+        const int f = code_swz(t);
         const uint8_t* const sp = slot + Ge::CODES + Ge::ROPE + 256 * (tw * G + m) + la * NB + gq * KS;
         const uint32_t sa = KS == 4 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp);
         f32x4 c = {0.f, 0.f, 0.f, 0.f}, d = {0.f, 0.f, 0.f, 0.f};
@@ -409,7 +522,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
           d = mfma_fp4_fp8<s, 1>(kc, qlo[s], d, sa, qscale);
         });
         const uint8_t* const pe = slot + Ge::CODES + t * 2 * R;
-        const int fr = R == 64 ? (t >> 1) & 7 : (t >> 2) & 3;
+        const int fr = rope_swz(t);
 #pragma unroll
         for (int j = 0; j < R / 32; ++j)
           d = mfma16x16x32(*reinterpret_cast<const u32x4*>(pe + 16 * ((4 * j + gq) ^ fr)), qpe[j], d);
@@ -417,7 +530,6 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
       }
       // exponent fields of the scales of this wave's 16 copied positions: (159 - s) << 7
       {
-        constexpr int LS = NB / 4;
         if (LS == 4 || lane < 16 * LS) {
           const uint32_t w = *reinterpret_cast<const uint32_t*>(slot + Ge::CODES + Ge::ROPE + 256 * wave + 4 * lane);
           uint16_t* const es = reinterpret_cast<uint16_t*>(smem + Ge::ES + buf * NB * 128) + 4 * (lane % LS) * 64 +
@@ -463,8 +575,8 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
     };
 
     // Output of tile k: O^T += X^T P^T over this wave's features.
-    auto output = [&](int k) {
-      const uint8_t* const slot = smem + (k % S) * Ge::TILE;
+    auto output = [&](int k, uint32_t at) {
+      const uint8_t* const slot = smem + at;
       const int buf = k & 1;
       const u32x4 fl = *reinterpret_cast<const u32x4*>(smem + Ge::FLAG + 16 * buf);
       u32x4 p[G][2];  // row la: positions 16 gq .. 16 gq + 15
@@ -474,7 +586,11 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
         for (int h = 0; h < 2; ++h)
           p[g][h] = *reinterpret_cast<const u32x4*>(smem + Ge::P + buf * Ge::ROWS * 128 + (16 * g + la) * 128 +
                                                     16 * ((2 * gq + h) ^ (la & 7)));
-      if (__builtin_expect(__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w) != 0, 0)) {
+      float fall[G];  // factor by which a group's earlier sums fall
+#pragma unroll
+      for (int g = 0; g < G; ++g) fall[g] = 1.f;
+      const uint32_t moved = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
+      if (__builtin_expect(moved != 0, 0)) {
         // some wave moved a reference: all go to the largest, and what was
         // computed against smaller ones is scaled down by powers of two
 #pragma unroll
@@ -487,9 +603,11 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
             mine[w] = fl[wv] ? r : ref[g];
             top = fmaxf(top, mine[w]);
           }
-          const float f = __builtin_amdgcn_exp2f(ref[g] - top);
+          fall[g] = __builtin_amdgcn_exp2f(ref[g] - top);
+          if constexpr (!Ge::ACC) {
 #pragma unroll
-          for (int j = 0; j < FT; ++j) o[g][j] *= f;
+            for (int j = 0; j < FT; ++j) o[g][j] *= fall[g];
+          }
           float r = mine[0];  // of the wave that made this lane's 16 positions
 #pragma unroll
           for (int w = 1; w < TW; ++w) r = gq / G == w ? mine[w] : r;
@@ -499,11 +617,15 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[g][h][i] = sub_sat(p[g][h][i], down | down << 16);
           if (g == gw) {
-            lsum = lsum * f;
+            lsum = lsum * fall[g];
             ltile = ltile * __builtin_amdgcn_exp2f(wref - top);
           }
           ref[g] = top;
         }
+      }
+      if constexpr (Ge::ACC) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) scale_acc8(o[g], fall[g], moved);
       }
       lsum += ltile;
 #pragma unroll
@@ -512,7 +634,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
         const u32x4* const es = reinterpret_cast<const u32x4*>(smem + Ge::ES + buf * NB * 128 + nb * 128 + 32 * gq);
         const u32x4 e0 = es[0], e1 = es[1];
         const int t = 16 * gq + la;
-        const int ch = nb ^ (D == 512 ? t & 15 : (t >> 1) & 7);
+        const int ch = nb ^ code_swz(t);
         u32x4 x[2][2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
@@ -539,38 +661,41 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::OCC)) void mx4_attend_kernel
 
     // ---- the tile loop -------------------------------------------------------------
     // Copies in order: before the loop tiles 0 .. S - 3, in turn k (after barrier k)
-    // tile k + S - 1, each behind the page numbers of the tile S - 2 later. Barrier
-    // k waits until tile k + 1 is in; then tiles k + 2 .. k + S - 2 may be on their
-    // way. Turn k = -1 has no output, turn nt - 1 no scores.
+    // tile k + S - 1, each (without PAGED) behind the page numbers of the tile S - 2
+    // later. Barrier k waits until tile k + 1 is in; then tiles k + 2 .. k + S - 2 may
+    // be on their way. Turn k = -1 has no output, turn nt - 1 no scores.
+    constexpr int IC = PAGED ? 0 : S - 3;  // page number copies behind tile k + 1
+    uint32_t here = 0, ahead = 0;          // ring slots of tiles k and k + 1
+    auto meet = [&](int k) {
+      const int there = nt - 2 - k;  // tiles past k + 1
+      if (there >= S - 3) {
+        wait_loads<IC + (S - 3) * Ge::LOADS>();
+      } else if (S > 4 && there == 1) {
+        wait_loads<IC + Ge::LOADS>();
+      } else {
+        wait_loads<IC>();
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if constexpr (!PAGED) copy_idx(k + 2 * S - 3);
+      ask_tile(k + S - 1);
+    };
     if (nt > 0) {
+      meet(-1);
+      scores(0, 0);
 #pragma unroll 1
-      for (int k = 0; k < S - 2; ++k) copy_idx(k);
-      wait_loads<0>();
-#pragma unroll 1
-      for (int k = 0; k < S - 2; ++k) {
-        copy_idx(k + S - 2);
-        if (k < nt) copy_tile(k);
+      for (int k = 0; k < nt - 1; ++k) {
+        here = ahead;
+        ahead = next(ahead);
+        meet(k);
+        output(k, here);
+        scores(k + 1, ahead);
       }
-#pragma unroll 1
-      for (int k = -1; k < nt; ++k) {
-        const int out_there = min(nt - 2 - k, S - 3);  // tiles past k + 1 already asked for
-        if (out_there >= 2) {
-          wait_loads<(S - 3) + 2 * Ge::LOADS>();
-        } else if (out_there == 1) {
-          wait_loads<(S - 3) + Ge::LOADS>();
-        } else {
-          wait_loads<S - 3>();
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        copy_idx(k + 2 * S - 3);
-        if (k + S - 1 < nt) copy_tile(k + S - 1);
-        if (k >= 0) output(k);
-        if (k + 1 < nt) scores(k + 1);
-      }
+      meet(nt - 1);
+      output(nt - 1, ahead);
     }
-    wait_loads<0>();  // (page numbers asked for past the end)
+    if constexpr (!PAGED) wait_loads<0>();  // (page numbers asked for past the end)
 
     // ---- the rows' sums, then the output or a partial --------------------------------
     lsum = wave_sum_over_groups(lsum);
@@ -666,7 +791,7 @@ __global__ __launch_bounds__(256) void mx4_merge_kernel(Mx4AttendArgs a, int row
   if (a.lse && c == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-template <int D, int R, int G>
+template <int D, int R, int G, bool PAGED>
 hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   using Ge = Mx4Geo<D, R, G>;
   const int64_t rows = (int64_t)a.max_q_len * a.H;
@@ -675,24 +800,30 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   // requests than a block's sums hold, each row block has a block.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
   const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus;
-  const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G>,
+  const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);
   if (e != hipSuccess) return e;
   if (!shared) {
     a.ws = nullptr;
     a.blocks = 0;
-    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G>), dim3((unsigned)((int64_t)a.row_blocks * a.B)), dim3(256), Ge::LDS,
+    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3((unsigned)((int64_t)a.row_blocks * a.B)), dim3(256), Ge::LDS,
                        stream, a);
     return hipGetLastError();
   }
   a.blocks = num_cus * Ge::OCC;
-  hipLaunchKernelGGL((mx4_attend_kernel<D, R, G>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
+  hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   constexpr int RM = 256 / (D / 4);
   hipLaunchKernelGGL((mx4_merge_kernel<D>), dim3((unsigned)(a.row_blocks * a.B), Ge::ROWS / RM), dim3(256), 0, stream, a,
                      Ge::ROWS);
   return hipGetLastError();
+}
+
+template <int D, int R, int G>
+hipError_t launch_paged(const Mx4AttendArgs& a, int num_cus, hipStream_t stream) {
+  return a.page_shift >= 4 ? launch_attend<D, R, G, true>(a, num_cus, stream)
+                           : launch_attend<D, R, G, false>(a, num_cus, stream);
 }
 
 }  // namespace rolaq
@@ -709,9 +840,9 @@ hipError_t rolaq_launch_mx4_attend(const rolaq::Mx4AttendArgs& a, int D, int num
   const int64_t rows = (int64_t)a.max_q_len * a.H;
 #define ROLAQ_MX4(DD, RR)                                                    \
   if (D == DD) {                                                             \
-    if (rows <= 16) return launch_attend<DD, RR, 1>(a, num_cus, stream);     \
-    if (rows <= 32) return launch_attend<DD, RR, 2>(a, num_cus, stream);     \
-    return launch_attend<DD, RR, 4>(a, num_cus, stream);                     \
+    if (rows <= 16) return launch_paged<DD, RR, 1>(a, num_cus, stream);      \
+    if (rows <= 32) return launch_paged<DD, RR, 2>(a, num_cus, stream);      \
+    return launch_paged<DD, RR, 4>(a, num_cus, stream);                      \
   }
   ROLAQ_MX4(512, 64)
   ROLAQ_MX4(256, 32)
