@@ -30,10 +30,12 @@ struct Mx4AttendArgs {
   uint16_t* out;  // [T, H, D] bf16, strides (o_st, o_sh)
   int64_t o_st, o_sh;
   float* lse;   // [T, H] or null
-  uint8_t* ws;  // workspace: tile counts and partials
+  uint8_t* ws;  // workspace: the merge's jobs and the partials
   // set by the launcher
   int blocks;      // > 0: the batch's tiles shared out over so many blocks; 0: a block for each row block
   int row_blocks;  // row blocks of a request of max_q_len queries
+  int h_inv;       // 65536 / H rounded up
+  int by_pair;     // the merge's jobs are numbered by (request, row block), not by block
 };
 
 struct Mx4RowsArgs {

@@ -157,21 +157,30 @@ struct Mx4Geo {
   static constexpr int FLAG = IDX + kMx4Idx * 1024;         // [2][4]
   static constexpr int WREF = FLAG + 32;                    // [2][4][16]
   static constexpr int LSUM = WREF + 512;                   // [4][16]
-  static constexpr int FIND = LSUM + 256;                   // [8]: wave sums, the first unit's request
-  static constexpr int PREF = FIND + 64;                    // [kMx4Requests + 1]
-  static constexpr int LDS = PREF + 4 * (kMx4Requests + 4);
+  static constexpr int LDS = LSUM + 256;
   static_assert(LDS * OCC <= 160 * 1024, "LDS of a CU");
   static_assert(S - 1 <= kMx4Idx, "page numbers in flight");
   static constexpr int SLOT = ROWS * (D + 2) * 4;  // bytes of a partial: O, then (reference, sum) by row
 };
 
-constexpr int kMx4WsHead = 4 * (kMx4Requests + 64);  // the tile counts at the start of the workspace
+// What the attend kernel leaves for the merge at the start of the workspace, by pair
+// (request and row block), or by block where there are more pairs than kMx4Jobs.
+struct Mx4Job {
+  int parts;       // blocks that hold partials of the pair, from block `first` on; 0: nothing to join
+  int first;
+  int second;      // block `first`'s is its second segment (else its first, as all others')
+  int row0, rows;  // first row of the pair, rows of the request
+  int q0;          // first query of the request
+  int pad[2];
+};
+constexpr int kMx4Jobs = 4096;
+constexpr int kMx4WsHead = kMx4Jobs * sizeof(Mx4Job);
 
 // A request's part of the batch.
 struct Mx4Request {
   int q0, nq;        // first query, queries
   int len;           // cached positions
-  int list, pages;   // first entry of its page list, and how many
+  int list;          // first entry of its page list
 };
 
 __device__ __forceinline__ Mx4Request mx4_request(const Mx4AttendArgs& a, int b) {
@@ -183,14 +192,26 @@ __device__ __forceinline__ Mx4Request mx4_request(const Mx4AttendArgs& a, int b)
   r.list = a.kv_indptr[b];
   const int end = a.kv_indptr[b + 1];
   r.list = max(r.list, 0);
-  r.pages = (int)min((int64_t)max(end - r.list, 0), max(a.n_indices - r.list, (int64_t)0));
-  const int64_t most = (int64_t)r.pages << a.page_shift;  // positions that the list reaches
+  const int64_t pages = min((int64_t)max(end - r.list, 0), max(a.n_indices - r.list, (int64_t)0));
+  const int64_t most = pages << a.page_shift;  // positions that the list reaches
   r.len = (int)max(min(min(a.kv_lens[b], most), (int64_t)0x3fffffff), (int64_t)0);
   return r;
 }
 
 __device__ __forceinline__ int mx4_row_blocks(const Mx4Request& r, int H, int rows) { return (r.nq * H + rows - 1) / rows; }
 __device__ __forceinline__ int mx4_tiles(const Mx4Request& r) { return max((r.len + kMx4Tile - 1) / kMx4Tile, 1); }
+
+// Inclusive sum over the lanes up to this one (DPP: shifts within rows of 16, then
+// the rows' last lanes to the rows behind).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15, rows 1 and 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31, rows 2 and 3
+  return v;
+}
 
 // Unit range of block j of n over `units`: [units j / n, units (j + 1) / n).
 __device__ __forceinline__ uint32_t mx4_first_unit(uint32_t units, uint32_t j, uint32_t n) {
@@ -217,72 +238,73 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
   const int gw = wave % G, tw = wave / G;  // this wave's group and its share of a tile's positions
 
   // ---- which units are this block's --------------------------------------------
-  uint32_t u = 0, u_end = 1, nblk = 1;
+  uint32_t u = 0, u_end = 1;
+  uint32_t u_req = 0;  // first unit of request b
+  uint32_t all_units = 0, all_blocks = 0;
+  Mx4Job* jobs = nullptr;
   int b = 0, rb_only = 0;
-  uint32_t* const pref = reinterpret_cast<uint32_t*>(smem + Ge::PREF);
+  Mx4Request rq;
   if (a.blocks > 0) {
-    // tiles of all requests, summed: four requests a thread
-    uint32_t* const find = reinterpret_cast<uint32_t*>(smem + Ge::FIND);
-    uint32_t n[4], s = 0;
+    // Tiles of all requests, summed by every wave for itself (a request a lane, 256
+    // requests' loads in one round trip), then the request that has the first unit.
+    const auto units_of = [&](const Mx4Request& r, int i) {
+      return i < a.B ? (uint32_t)mx4_row_blocks(r, a.H, Ge::ROWS) * (uint32_t)mx4_tiles(r) : 0u;
+    };
+    Mx4Request r4[4];
+    uint32_t n4[4], at4[4], units = 0;
+    const auto load4 = [&](int c) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = 4 * tid + k;
-      n[k] = 0;
-      if (i < a.B) {
-        const Mx4Request r = mx4_request(a, i);
-        n[k] = (uint32_t)mx4_row_blocks(r, a.H, Ge::ROWS) * (uint32_t)mx4_tiles(r);
-      }
-      s += n[k];
-    }
-    uint32_t incl = s;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t v = __shfl_up(incl, d);
-      if (lane >= d) incl += v;
-    }
-    if (lane == 63) find[wave] = incl;
-    __syncthreads();
-    uint32_t base = incl - s, units = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t v = find[w];
-      if (w < wave) base += v;
-      units += v;
-    }
-    nblk = min((uint32_t)a.blocks, units);
-    if (blockIdx.x == 0) {  // for the merge
-      uint32_t* const g = reinterpret_cast<uint32_t*>(a.ws);
-      uint32_t at = base;
+      for (int k = 0; k < 4; ++k)
+        if (k == 0 || c + 64 * k < a.B) r4[k] = mx4_request(a, min(c + 64 * k + lane, a.B - 1));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        if (4 * tid + k < a.B) g[4 * tid + k] = at;
-        at += n[k];
+        n4[k] = at4[k] = 0;
+        if (k > 0 && c + 64 * k >= a.B) continue;
+        n4[k] = units_of(r4[k], c + 64 * k + lane);
+        const uint32_t incl = wave_scan(n4[k]);
+        at4[k] = units + incl - n4[k];
+        units += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
       }
-      if (tid == 0) g[a.B] = units;
-    }
-    if (units == 0) return;
+    };
+    for (int c = 0; c < a.B; c += 256) load4(c);
+    const uint32_t nblk = min((uint32_t)a.blocks, units);
     // consecutive parts on one XCD (blocks go round the XCDs in turn): they share pages
     const uint32_t per = gridDim.x / 8;
     const uint32_t j = gridDim.x % 8 == 0 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
-    if (j >= nblk) return;
+    jobs = reinterpret_cast<Mx4Job*>(a.ws);
+    if (j >= nblk) {  // (also without any unit)
+      if (!a.by_pair && tid == 0) jobs[j].parts = 0;
+      return;
+    }
     u = mx4_first_unit(units, j, nblk);
     u_end = mx4_first_unit(units, j + 1, nblk);
-    uint32_t at = base;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      pref[4 * tid + k] = at;
-      if (at <= u && u < at + n[k]) find[4] = 4 * tid + k;
-      at += n[k];
-    }
-    if (tid == 255) pref[kMx4Requests] = units;
-    __syncthreads();
-    b = find[4];
     a.blocks = (int)j;  // (from here on: this block's number)
+    all_units = units;
+    all_blocks = nblk;
+    const bool again = a.B > 256;  // only the last 256 requests' sums are held
+    if (again) units = 0;
+    for (int c = 0; c < a.B; c += 256) {
+      if (again) load4(c);  // (its running sum starts again)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(at4[k] <= u && u < at4[k] + n4[k]);
+        if (hit) {
+          const int l = __builtin_ctzll(hit);
+          b = c + 64 * k + l;
+          u_req = (uint32_t)__builtin_amdgcn_readlane((int)at4[k], l);
+          rq.q0 = __builtin_amdgcn_readlane(r4[k].q0, l);
+          rq.nq = __builtin_amdgcn_readlane(r4[k].nq, l);
+          rq.len = __builtin_amdgcn_readlane(r4[k].len, l);
+          rq.list = __builtin_amdgcn_readlane(r4[k].list, l);
+        }
+      }
+    }
   } else {
     // a block for each (row block, request), the later row blocks of a request,
     // which see most positions, first
     b = blockIdx.x % a.B;
     rb_only = a.row_blocks - 1 - blockIdx.x / a.B;
+    rq = mx4_request(a, b);
   }
   const bool shared = a.ws != nullptr;
 
@@ -308,35 +330,47 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
 
   while (u < u_end) {
     // ---- the next segment: tiles [t0, t1) of a row block of request b ---------------
-    int rb, t0, t1, ntiles;
-    Mx4Request rq = mx4_request(a, b);
+    int rb, t0, t1, ntiles = mx4_tiles(rq);
     if (shared) {
-      const uint32_t p0 = pref[b], p1 = pref[b + 1];
-      if (u >= p1) {  // (also requests without queries)
-        ++b;
+      const uint32_t done = u - u_req;
+      rb = done / ntiles;
+      if (rb >= mx4_row_blocks(rq, a.H, Ge::ROWS)) {  // on to the next request (one without queries has no units)
+        u_req = u;
+        rq = mx4_request(a, ++b);
         continue;
       }
-      ntiles = mx4_tiles(rq);
-      rb = (u - p0) / ntiles;
-      t0 = (u - p0) - rb * ntiles;
+      t0 = done - rb * ntiles;
+      // The merge's job for this pair: by the block that begins it, or (by block) by the
+      // one that takes it over from there.
+      if (tid == 0 && (a.by_pair ? t0 == 0 : nth == 0)) {
+        const uint32_t u0 = u - t0, j1 = mx4_block_of(u0 + ntiles - 1, all_units, all_blocks);
+        const uint32_t j0 = a.by_pair ? (uint32_t)a.blocks : mx4_block_of(u0, all_units, all_blocks);
+        const bool cut = a.by_pair ? j1 > j0 : t0 > 0 && (int)j0 + 1 == a.blocks;
+        jobs[a.by_pair ? b * a.row_blocks + rb : a.blocks] =
+            Mx4Job{cut ? (int)(j1 - j0 + 1) : 0, (int)j0, mx4_first_unit(all_units, j0, all_blocks) < u0, rb * Ge::ROWS,
+                   rq.nq * a.H, rq.q0, {0, 0}};
+      }
       t1 = (int)min((uint32_t)ntiles, t0 + (u_end - u));
       u += t1 - t0;
     } else {
       u = u_end;
       rb = rb_only;
       if (rb >= mx4_row_blocks(rq, a.H, Ge::ROWS)) return;
-      ntiles = mx4_tiles(rq);
       t0 = 0;
       t1 = ntiles;
     }
     const bool whole = t0 == 0 && t1 == ntiles;
     const int rows = rq.nq * a.H, row0 = rb * Ge::ROWS;
+    // queries and heads of rows row0 + x, x < 64: one division, then exact products (row0 % H + x < 192)
+    const int tok0 = row0 / a.H, head0 = row0 - tok0 * a.H;
+    auto tok_of = [&](int x) { return tok0 + (((head0 + x) * a.h_inv) >> 16); };
     // positions that a row sees: its causal limit; rows past the last see none
     const int last_row = min(row0 + Ge::ROWS, rows) - 1;
-    const int vis_all = rq.len - rq.nq + row0 / a.H + 1;          // seen by every row of the block
-    const int vis_most = rq.len - rq.nq + last_row / a.H + 1;     // by any
+    const int vis_all = rq.len - rq.nq + tok0 + 1;                // seen by every row of the block
+    const int vis_most = rq.len - rq.nq + tok_of(last_row - row0) + 1;  // by any
     const int my_row = row0 + 16 * gw + la;
-    const int vis = my_row < rows ? rq.len - rq.nq + my_row / a.H + 1 : 0;
+    const int my_tok = tok_of(16 * gw + la);
+    const int vis = my_row < rows ? rq.len - rq.nq + my_tok + 1 : 0;
     const bool full_rows = row0 + Ge::ROWS <= rows;
     const int t_end = min(t1, (vis_most + kMx4Tile - 1) / kMx4Tile);
     const int nt = max(t_end - t0, 0);  // tiles to walk
@@ -405,9 +439,9 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     uint32_t qscale;
     u32x4 v[KS][2][2];
     {
-      const int r = min(my_row, max(rows - 1, 0));
-      const int tok = min(rq.q0 + r / a.H, a.T - 1);
-      const uint16_t* q = a.q + (int64_t)tok * a.q_st + (int64_t)(r % a.H) * a.q_sh;
+      const bool mine = my_row < rows;  // (rows past the last: the pair's first row)
+      const int tok = mine ? my_tok : tok0, head = mine ? head0 + 16 * gw + la - (my_tok - tok0) * a.H : head0;
+      const uint16_t* q = a.q + (int64_t)(rq.q0 + tok) * a.q_st + (int64_t)head * a.q_sh;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -708,7 +742,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       for (int w = 0; w < TW; ++w) l += *reinterpret_cast<const float*>(smem + Ge::LSUM + 64 * (w * G + g) + 4 * la);
       const int r = row0 + 16 * g + la;
       if (r >= rows) continue;
-      const int tok = rq.q0 + r / a.H, head = r % a.H;
+      const int tq = tok_of(16 * g + la), tok = rq.q0 + tq, head = head0 + 16 * g + la - (tq - tok0) * a.H;
       if (whole) {
         const float inv = l == 0.f ? 0.f : 4294967296.f / l;
         uint16_t* const out = a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + Ge::FW * wave + 4 * gq;
@@ -732,40 +766,37 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
   }
 }
 
-// Joins the partials of the row blocks that were cut: a block for ROWS_M rows of
-// one row block, D / 4 threads a row. Rows of row blocks that one block walked are
-// left as that block wrote them.
-template <int D>
-__global__ __launch_bounds__(256) void mx4_merge_kernel(Mx4AttendArgs a, int rows_per_block) {
-  constexpr int RM = 256 / (D / 4);
-  const int b = blockIdx.x / a.row_blocks, rb = blockIdx.x % a.row_blocks;
-  const Mx4Request rq = mx4_request(a, b);
-  const int nrb = mx4_row_blocks(rq, a.H, rows_per_block);
-  if (rb >= nrb) return;
-  const uint32_t* const pref = reinterpret_cast<const uint32_t*>(a.ws);
-  const uint32_t units = pref[a.B], tiles = mx4_tiles(rq), u0 = pref[b] + rb * tiles;
-  const uint32_t nblk = min((uint32_t)a.blocks, units);
-  const uint32_t j0 = mx4_block_of(u0, units, nblk), j1 = mx4_block_of(u0 + tiles - 1, units, nblk);
-  if (j0 == j1) return;
-  const int rl = blockIdx.y * RM + threadIdx.x / (D / 4), r = rb * rows_per_block + rl;
-  if (r >= rq.nq * a.H) return;
-  const int c = threadIdx.x % (D / 4);
+// Joins the partials of the pairs that were cut: a block for a job and THREADS / (D / 4
+// PARTS) rows, D / 4 threads for each of PARTS shares of a row's partials, four of
+// them in flight for each. What bounds it is latency (the job, then the partials), so
+// blocks are small enough to be on the card all at once.
+template <int D, int PARTS, int THREADS>
+__global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int rows_per_block) {
+  constexpr int C = D / 4, N = 4, RM = THREADS / C / PARTS;
+  __shared__ f32x4 s_o[PARTS][C];
+  __shared__ f32x2 s_ml[PARTS];
+  const Mx4Job job = reinterpret_cast<const Mx4Job*>(a.ws)[blockIdx.x];
+  if (a.by_pair) {  // (pairs that there are not: their jobs are not written)
+    const int b = blockIdx.x / a.row_blocks;
+    const Mx4Request rq = mx4_request(a, b);
+    if ((int)(blockIdx.x % a.row_blocks) >= mx4_row_blocks(rq, a.H, rows_per_block)) return;
+  }
+  const int c = threadIdx.x % C, unit = __builtin_amdgcn_readfirstlane(threadIdx.x / C);
+  const int part = unit % PARTS, rl = blockIdx.y * RM + unit / PARTS, r = job.row0 + rl;
+  if (job.parts == 0 || r >= job.rows || rl >= rows_per_block) return;
   const int64_t slot = (int64_t)rows_per_block * (D + 2) * 4;
-  // block j's part of this pair is its second segment if it starts before the pair, else its first
-  const int first = mx4_first_unit(units, j0, nblk) < u0;
-  const uint8_t* const parts = a.ws + kMx4WsHead;
+  const uint8_t* const parts = a.ws + kMx4WsHead + 2 * job.first * slot;
   float m = kMx4NoRef, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  constexpr int N = 8;
-  for (uint32_t j = j0; j <= j1; j += N) {
+  for (int j = part; j < job.parts; j += N * PARTS) {
     f32x2 ml[N];
     f32x4 v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const uint32_t jj = min(j + i, j1);
-      const uint8_t* const p = parts + ((int64_t)2 * jj + (jj == j0 ? first : 0)) * slot;
-      ml[i] = reinterpret_cast<const f32x2*>(p + (int64_t)rows_per_block * D * 4)[rl];
-      v[i] = *reinterpret_cast<const f32x4*>(p + ((int64_t)rl * D + 4 * c) * 4);
+      const int jj = min(j + i * PARTS, job.parts - 1);
+      const uint8_t* const p = parts + (2 * jj + (jj == 0 ? job.second : 0)) * slot;
+      ml[i] = gload<f32x2>(p + (int64_t)rows_per_block * D * 4 + 8 * rl);
+      v[i] = gload<f32x4>(p + ((int64_t)rl * D + 4 * c) * 4);
     }
     float top = m;
 #pragma unroll
@@ -776,16 +807,35 @@ __global__ __launch_bounds__(256) void mx4_merge_kernel(Mx4AttendArgs a, int row
     m = top;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float w = j + i <= j1 ? __builtin_amdgcn_exp2f(ml[i].x - top) : 0.f;
-      if (j + i <= j1) {
+      if (j + i * PARTS < job.parts) {
+        const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
         l = fmaf(w, ml[i].y, l);
         o += v[i] * w;
       }
     }
   }
+  if constexpr (PARTS > 1) {
+    s_o[part][c] = o;
+    if (c == 0) s_ml[part] = f32x2{m, l};
+    __syncthreads();
+    if (part) return;
+    float top = m;
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) top = fmaxf(top, s_ml[i].x);
+    const float f = __builtin_amdgcn_exp2f(m - top);
+    l *= f;
+    o *= f;
+    m = top;
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) {
+      const float w = __builtin_amdgcn_exp2f(s_ml[i].x - top);
+      l = fmaf(w, s_ml[i].y, l);
+      o += s_o[i][c] * w;
+    }
+  }
   const float inv = l == 0.f ? 0.f : 4294967296.f / l;
   o *= inv;
-  const int tok = rq.q0 + r / a.H, head = r % a.H;
+  const int tok = job.q0 + r / a.H, head = r % a.H;
   *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * c) =
       u32x2{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
   if (a.lse && c == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
@@ -796,6 +846,7 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   using Ge = Mx4Geo<D, R, G>;
   const int64_t rows = (int64_t)a.max_q_len * a.H;
   a.row_blocks = (int)((rows + Ge::ROWS - 1) / Ge::ROWS);
+  a.h_inv = (65536 + a.H - 1) / a.H;
   // Shared out while there are few row blocks for each CU; past that, or with more
   // requests than a block's sums hold, each row block has a block.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
@@ -810,13 +861,20 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
                        stream, a);
     return hipGetLastError();
   }
-  a.blocks = num_cus * Ge::OCC;
+  a.blocks = std::min(num_cus * Ge::OCC, kMx4Jobs);
+  const int64_t pairs = (int64_t)a.B * a.row_blocks;
+  a.by_pair = pairs <= a.blocks;
   hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  constexpr int RM = 256 / (D / 4);
-  hipLaunchKernelGGL((mx4_merge_kernel<D>), dim3((unsigned)(a.row_blocks * a.B), Ge::ROWS / RM), dim3(256), 0, stream, a,
-                     Ge::ROWS);
+  // Many partials of a row (a small batch): a block for a row, its threads share them.
+  const int64_t there = std::min<int64_t>(rows, Ge::ROWS), jobs = a.by_pair ? pairs : a.blocks;
+  constexpr int U = 512 / (D / 4), RM = 256 / (D / 4);
+  if (pairs * 16 <= a.blocks)
+    hipLaunchKernelGGL((mx4_merge_kernel<D, U, 512>), dim3(jobs, there), dim3(512), 0, stream, a, Ge::ROWS);
+  else
+    hipLaunchKernelGGL((mx4_merge_kernel<D, 1, 256>), dim3(jobs, (there + RM - 1) / RM), dim3(256), 0, stream, a,
+                       Ge::ROWS);
   return hipGetLastError();
 }
 
