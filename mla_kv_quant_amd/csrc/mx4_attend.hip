@@ -18,18 +18,23 @@
 //   it below. Rope terms are bf16 MFMAs into the same FP32 accumulators.
 // * Softmax in FP32, log2 domain, against a whole-number reference for each
 //   row: a tile's largest score rounded up, moved only when a later score passes
-//   it by more than 2^30 (bf16 probabilities have FP32's range). A reference
+//   it by more than 2^8 (bf16 probabilities have FP32's range). A reference
 //   then moves by whole powers of two, exact in the accumulators as in P.
 // * Output: wave w takes the features D/4 w .. of all G groups. The codes come
 //   out of LDS transposed (ds_read_b64_tr_b4: 16 positions of one feature), become
 //   bf16 pairs by v_cvt_scalef32_pk_bf16_fp4 (one instruction for two values) and
-//   meet P in bf16 MFMAs. A position's block scale is applied to P instead of
-//   to the 32 values: an integer subtraction in P's exponents, P 2^(s - 159),
-//   saturating at zero (v_pk_sub_u16 with clamp), which is exact; O is multiplied
-//   by 2^32 at the end. Masked positions have P = 0 and finite codes, so what they
-//   hold does not reach O.
+//   meet P in bf16 MFMAs. The block scales go into exponents, two at a time and
+//   exactly. With one group (few rows) they are taken from P's: P 2^(s - 159)
+//   (v_pk_sub_u16, saturating at zero), O 2^-32 of its value. With more they are
+//   added to the values', once for all groups: x 2^(s - 63) (v_pk_add_u16; a zero
+//   becomes 2^(s - 190), 2^-126 of the smallest level), O 2^64 times its value.
+//   Masked positions have P = 0 and finite values (a scale byte that is none counts
+//   as one), so what they hold does not reach O.
 // One barrier a tile: the scores of tile i + 1 and the output of tile i lie between
-// two barriers.
+// two barriers, so that matrix, vector and LDS work of both can overlap. With one
+// group the loop waits for HBM (5.8 TB/s in it); with four at 512 features a turn is
+// 2200 cycles of matrix instructions in 5100, and the rest is LDS reads (every wave
+// reads the whole tile's keys for its group) and what they wait for.
 //
 // Work: the tiles of all (request, row block) pairs lie on one line that is cut
 // into equal parts, a part for each block; a pair cut by a border leaves partials
@@ -50,7 +55,8 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 constexpr int kMx4Tile = 64;           // positions in a tile
 constexpr int kMx4Idx = 4;             // tiles whose page numbers are held (ring slots - 1 at least)
 constexpr float kMx4NoRef = -268435456.f;  // reference of a row that has seen no score
-constexpr float kMx4Slack = 30.f;      // log2 by which a score may pass its row's reference
+constexpr float kMx4Slack = 8.f;       // log2 by which a score may pass its row's reference: sums of
+                                       // 2^21 such P times 6 2^96, the largest value held, stay below 2^128
 
 // D = A(16x128, E2M1) * B(128x16, E4M3) + C. Lane l holds A[l%16][32(l/16)+i] (nibble
 // i of four dwords) with the scale of those 32 in byte SA of sa, and
@@ -118,6 +124,11 @@ __device__ __forceinline__ void scale_acc8(f32x4 (&o)[8], float f, uint32_t need
       : "scc");
 }
 
+// Sum of two 16-bit fields each (no carry between them).
+__device__ __forceinline__ uint32_t add16(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, a) + __builtin_bit_cast(u16x2, b));
+}
+
 // Eight 4-bit codes -> eight bf16 values, in order.
 __device__ __forceinline__ u32x4 fp4x8_to_bf16(uint32_t v) {
   return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 0)),
@@ -137,29 +148,46 @@ __device__ __forceinline__ void static_for(F&& f) {
 
 template <int D, int R, int G>
 struct Mx4Geo {
+  static constexpr int W = 4;         // waves
   static constexpr int ROWS = 16 * G;
   static constexpr int NB = D / 32;   // scale blocks of a row
   static constexpr int KS = D / 128;  // K-steps of the latent scores; also blocks per lane group
   static constexpr int CB = D / 2;    // code bytes of a row
-  static constexpr int FW = D / 4;    // features of a wave
+  static constexpr int FW = D / W;    // features of a wave
   static constexpr int FT = FW / 16;  // its output tiles
-  static constexpr int TW = 4 / G;    // waves that share a group's positions
-  static constexpr int CODES = kMx4Tile * CB, ROPE = kMx4Tile * 2 * R, SCALES = 1024;
+  static constexpr int TW = W / G;    // waves that share a group's positions
+  static constexpr int MT = 4 / TW;   // 16-position sub-tiles of a wave's scores
+  static constexpr int CT = kMx4Tile / W;  // positions that a wave copies
+  static constexpr int CODES = kMx4Tile * CB, ROPE = kMx4Tile * 2 * R, SCALES = 256 * W;
   static constexpr int TILE = CODES + ROPE + SCALES;  // a ring slot
   static constexpr int S = D == 512 ? 5 : 4;          // ring slots
   static constexpr int OCC = D == 512 ? 1 : 2;        // blocks on a CU
   static constexpr bool ACC = D == 512 && G >= 2;     // over 256 registers: O in AGPRs
-  static constexpr int LOADS = CODES / 4096 + ROPE / 4096 + 1;  // a wave's copies for a tile
+  // A turn in two parts, tile k + 1's products beside tile k's expansion, then tile k's
+  // output beside tile k + 1's softmax: it holds the whole expanded tile, for which 256
+  // features and four groups have no registers (two blocks on a CU). Per step of 24
+  // requests with 128 heads, 512 features: 86 us, 94 without; of 64 x 16384 positions with
+  // 40 heads, 256 features: 100 us, 89 without.
+  static constexpr bool MIX = D == 512 && G >= 2;
+  // Halves of P that the other turn holds at a time: with four groups one, 92 us for two
+  // at the latter step's 96; with fewer both, 54.9 us for 55.8 (32 x 16384, 16 heads, 512).
+  static constexpr int PH = G == 4 ? 1 : 2;
+  // Block scales to V's exponents, not to P's: 16 additions for 32 features against 8 G. At
+  // G = 1 the other way round takes 56.4 us for 55.8.
+  static constexpr bool VSIDE = G >= 2;
+  static constexpr float UNIT = VSIDE ? 0x1p-64f : 0x1p32f;  // of O
+  static constexpr int LOADS = (CODES + ROPE) / (1024 * W) + 1;  // a wave's copies for a tile
   // LDS offsets
   static constexpr int P = S * TILE;                        // [2][ROWS][64] bf16, 16-byte chunks swizzled
   static constexpr int ES = P + 2 * ROWS * 128;             // [2][NB][64] exponent fields of the scales
-  static constexpr int IDX = ES + 2 * NB * 128;             // [kMx4Idx][4][64] page numbers
-  static constexpr int FLAG = IDX + kMx4Idx * 1024;         // [2][4]
-  static constexpr int WREF = FLAG + 32;                    // [2][4][16]
-  static constexpr int LSUM = WREF + 512;                   // [4][16]
-  static constexpr int LDS = LSUM + 256;
+  static constexpr int IDX = ES + 2 * NB * 128;             // [kMx4Idx][W][64] page numbers
+  static constexpr int FLAG = IDX + kMx4Idx * 256 * W;      // [2][W]
+  static constexpr int WREF = FLAG + 8 * W;                 // [2][W][16]
+  static constexpr int LSUM = WREF + 128 * W;               // [W][16]
+  static constexpr int LDS = LSUM + 64 * W;
   static_assert(LDS * OCC <= 160 * 1024, "LDS of a CU");
   static_assert(S - 1 <= kMx4Idx, "page numbers in flight");
+  static_assert(TW >= 1 && TW <= 4 && FT % 2 == 0, "a wave's scores and features");
   static constexpr int SLOT = ROWS * (D + 2) * 4;  // bytes of a partial: O, then (reference, sum) by row
 };
 
@@ -201,6 +229,19 @@ __device__ __forceinline__ Mx4Request mx4_request(const Mx4AttendArgs& a, int b)
 __device__ __forceinline__ int mx4_row_blocks(const Mx4Request& r, int H, int rows) { return (r.nq * H + rows - 1) / rows; }
 __device__ __forceinline__ int mx4_tiles(const Mx4Request& r) { return max((r.len + kMx4Tile - 1) / kMx4Tile, 1); }
 
+// Outputs v times f (one over the row's sum) as bf16. What is below 2^-94 is 0: there P with
+// a scale taken from its exponents saturates at zero, and zeros with a scale added to
+// theirs have gone into v as at most 2^-95.
+template <bool FLUSH>
+__device__ __forceinline__ u32x2 finish(f32x4 v, float f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] *= f;
+    if (FLUSH && fabsf(v[i]) < 0x1p-94f) v[i] = 0.f;
+  }
+  return u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+}
+
 // Inclusive sum over the lanes up to this one (DPP: shifts within rows of 16, then
 // the rows' last lanes to the rows behind).
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
@@ -222,14 +263,15 @@ __device__ __forceinline__ uint32_t mx4_block_of(uint32_t u, uint32_t units, uin
   return (uint32_t)((((uint64_t)u + 1) * n - 1) / units);
 }
 
-// PAGED: pages of 16 positions or more. A wave copies 16 positions, which then lie
-// in one page: its number is a scalar, and the copies' offsets are the same for
-// every tile. Otherwise the page numbers of 16 positions come through LDS.
+// PAGED: pages of 16 positions or more. A wave copies CT = 64 / W positions, 16 or 8,
+// which then lie in one page: its number is a scalar, and the copies' offsets are the
+// same for every tile. Otherwise the positions' page numbers come through LDS.
 template <int D, int R, int G, bool PAGED>
 __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_attend_kernel(Mx4AttendArgs a) {
   using Ge = Mx4Geo<D, R, G>;
-  constexpr int NB = Ge::NB, KS = Ge::KS, CB = Ge::CB, FT = Ge::FT, TW = Ge::TW, S = Ge::S;
   if constexpr (Ge::ACC) define_acc_macros();
+  constexpr int W = Ge::W;
+  constexpr int NB = Ge::NB, KS = Ge::KS, CB = Ge::CB, FT = Ge::FT, TW = Ge::TW, MT = Ge::MT, CT = Ge::CT, S = Ge::S;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_u8*)smem;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -312,21 +354,21 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
   const uint32_t page_mask = (1u << a.page_shift) - 1;
   const float c2 = a.sm_scale * kLog2e;
   int nth = 0;  // segments done
-  // A wave's copies of 16 positions: RC (RR) rows of codes (rope) at a time, LC (LR)
+  // A wave's copies of CT positions: RC (RR) rows of codes (rope) at a time, LC (LR)
   // lanes a row; chunk c of row t goes to chunk c ^ f(t), so that 16 lanes that read
   // one chunk of 16 rows, or 16 rows' parts of one block, meet all banks.
   constexpr int RC = 1024 / CB, LC = 64 / RC, RR = 1024 / (2 * R), LR = 64 / RR, LS = NB / 4;
   auto code_swz = [](int t) { return D == 512 ? t & 15 : (t >> 1) & 7; };
   auto rope_swz = [](int t) { return R == 64 ? (t >> 1) & 7 : (t >> 2) & 3; };
-  auto code_off = [&](int j) {  // byte of copy j's piece within the 16 rows
+  auto code_off = [&](int j) {  // byte of copy j's piece within the CT rows
     const int t = RC * j + lane / LC;
-    return t * CB + 16 * ((lane % LC) ^ code_swz(t));
+    return t * CB + 16 * ((lane % LC) ^ code_swz(CT * wave + t));
   };
   auto rope_off = [&](int j) {
     const int t = RR * j + lane / LR;
-    return t * 2 * R + 16 * ((lane % LR) ^ rope_swz(t));
+    return t * 2 * R + 16 * ((lane % LR) ^ rope_swz(CT * wave + t));
   };
-  const int scale_off = ((lane / LS) & 15) * NB + 4 * (lane % LS);
+  const int scale_off = ((lane / LS) % CT) * NB + 4 * (lane % LS);
 
   while (u < u_end) {
     // ---- the next segment: tiles [t0, t1) of a row block of request b ---------------
@@ -379,55 +421,55 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     __syncthreads();  // the last segment's LDS reads are done
 
     // ---- page numbers and tiles, asynchronously ---------------------------------------
-    const int list_last = pos_last & ~15;  // (PAGED) first of the last 16 positions
-    auto page_of = [&](int k) -> uint32_t {  // PAGED: page of this wave's 16 positions of tile k
-      const int pos = min(kMx4Tile * (t0 + k) + 16 * wave, list_last);
+    const int list_last = pos_last & ~(CT - 1);  // (PAGED) first of the last CT positions
+    auto page_of = [&](int k) -> uint32_t {  // PAGED: page of this wave's CT positions of tile k
+      const int pos = min(kMx4Tile * (t0 + k) + CT * wave, list_last);
       return *(const __attribute__((address_space(4))) uint32_t*)(a.kv_indices + rq.list + (pos >> a.page_shift));
     };
     auto copy_idx = [&](int k) {
-      const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + la, pos_last);
+      const int pos = min(kMx4Tile * (t0 + k) + CT * wave + la % CT, pos_last);
       copy4(a.kv_indices + rq.list + (pos >> a.page_shift),
-            lds0 + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256);
+            lds0 + Ge::IDX + ((k & (kMx4Idx - 1)) * W + wave) * 256);
     };
-    // Copies of tile k to the ring slot at byte `at`; `slot(x)`: cache slot of position x of this wave's 16.
+    // Copies of tile k to the ring slot at byte `at`; `slot(x)`: cache slot of position x of this wave's CT.
     auto copy_slots = [&](uint32_t at, auto&& slot) {
-      uint32_t sl[16 / RC + 16 / RR + 1];
+      uint32_t sl[CT / RC + CT / RR + 1];
 #pragma unroll
-      for (int j = 0; j < 16 / RC; ++j) sl[j] = slot(RC * j + lane / LC);
+      for (int j = 0; j < CT / RC; ++j) sl[j] = slot(RC * j + lane / LC);
 #pragma unroll
-      for (int j = 0; j < 16 / RR; ++j) sl[16 / RC + j] = slot(RR * j + lane / LR);
-      sl[16 / RC + 16 / RR] = slot((lane / LS) & 15);
+      for (int j = 0; j < CT / RR; ++j) sl[CT / RC + j] = slot(RR * j + lane / LR);
+      sl[CT / RC + CT / RR] = slot((lane / LS) % CT);
 #pragma unroll
-      for (int j = 0; j < 16 / RC; ++j)
-        copy16(a.codes + (uint64_t)sl[j] * CB + code_off(j) % CB, at + 16 * wave * CB + 1024 * j);
+      for (int j = 0; j < CT / RC; ++j)
+        copy16(a.codes + (uint64_t)sl[j] * CB + code_off(j) % CB, at + CT * wave * CB + 1024 * j);
 #pragma unroll
-      for (int j = 0; j < 16 / RR; ++j)
-        copy16(reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)sl[16 / RC + j] * (2 * R) + rope_off(j) % (2 * R),
-               at + Ge::CODES + 16 * wave * 2 * R + 1024 * j);
-      copy4(a.scales + (uint64_t)sl[16 / RC + 16 / RR] * NB + 4 * (lane % LS), at + Ge::CODES + Ge::ROPE + 256 * wave);
+      for (int j = 0; j < CT / RR; ++j)
+        copy16(reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)sl[CT / RC + j] * (2 * R) + rope_off(j) % (2 * R),
+               at + Ge::CODES + CT * wave * 2 * R + 1024 * j);
+      copy4(a.scales + (uint64_t)sl[CT / RC + CT / RR] * NB + 4 * (lane % LS), at + Ge::CODES + Ge::ROPE + 256 * wave);
     };
     auto copy_tile = [&](int k, uint32_t at, uint32_t page) {
       at += lds0;
       if constexpr (PAGED) {
-        const int pos = min(kMx4Tile * (t0 + k) + 16 * wave, list_last);
+        const int pos = min(kMx4Tile * (t0 + k) + CT * wave, list_last);
         const uint32_t s0 = (min(page, max_page) << a.page_shift) + ((uint32_t)pos & page_mask);
-        if (__builtin_expect(s0 + 15 <= max_slot, 1)) {
+        if (__builtin_expect(s0 + CT - 1 <= max_slot, 1)) {
           const uint8_t* const c = a.codes + (uint64_t)s0 * CB;
           const uint8_t* const r = reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)s0 * (2 * R);
 #pragma unroll
-          for (int j = 0; j < 16 / RC; ++j) copy16(c, (uint32_t)code_off(j), at + 16 * wave * CB + 1024 * j);
+          for (int j = 0; j < CT / RC; ++j) copy16(c, (uint32_t)code_off(j), at + CT * wave * CB + 1024 * j);
 #pragma unroll
-          for (int j = 0; j < 16 / RR; ++j)
-            copy16(r, (uint32_t)rope_off(j), at + Ge::CODES + 16 * wave * 2 * R + 1024 * j);
+          for (int j = 0; j < CT / RR; ++j)
+            copy16(r, (uint32_t)rope_off(j), at + Ge::CODES + CT * wave * 2 * R + 1024 * j);
           copy4(a.scales + (uint64_t)s0 * NB, (uint32_t)scale_off, at + Ge::CODES + Ge::ROPE + 256 * wave);
         } else {  // the cache ends inside the page
           copy_slots(at, [&](int x) { return min(s0 + (uint32_t)x, max_slot); });
         }
       } else {
-        const uint8_t* const idx = smem + Ge::IDX + ((k & (kMx4Idx - 1)) * 4 + wave) * 256;
+        const uint8_t* const idx = smem + Ge::IDX + ((k & (kMx4Idx - 1)) * W + wave) * 256;
         copy_slots(at, [&](int x) {
           const uint32_t p = *reinterpret_cast<const uint32_t*>(idx + 4 * x);
-          const int pos = min(kMx4Tile * (t0 + k) + 16 * wave + x, pos_last);
+          const int pos = min(kMx4Tile * (t0 + k) + CT * wave + x, pos_last);
           return min((min(p, max_page) << a.page_shift) + ((uint32_t)pos & page_mask), max_slot);
         });
       }
@@ -471,14 +513,14 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       asm volatile("" : "+v"(v[s][0][0]), "+v"(v[s][0][1]), "+v"(v[s][1][0]), "+v"(v[s][1][1]));
 #pragma unroll
     for (int k = 0; k < R / 32; ++k) asm volatile("" : "+v"(qpe[k]));
-    uint32_t ask = 0;  // ring slot of the next tile to ask for
+    uint32_t ask_at = 0;  // ring slot of the next tile to ask for
     auto next = [](uint32_t at) { return at + Ge::TILE == S * Ge::TILE ? 0u : at + Ge::TILE; };
     auto ask_tile = [&](int k) {
       if (k < nt) {
         const uint32_t p = page;
         if constexpr (PAGED) page = page_of(k + 1);
-        copy_tile(k, ask, p);
-        ask = next(ask);
+        copy_tile(k, ask_at, p);
+        ask_at = next(ask_at);
       }
     };
     if (nt > 0) {
@@ -536,105 +578,135 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     for (int g = 0; g < G; ++g) ref[g] = kMx4NoRef;
     float lsum = 0.f, ltile = 0.f, wref = kMx4NoRef;  // this lane's sums (its positions of row la of group gw)
 
-    // Scores and probabilities of tile k: P, the scales' exponent fields and the
-    // wave's flag go to LDS buffer k & 1.
-    auto scores = [&](int k, uint32_t at) {
+    // The operands of 16 positions' scores (sub-tile m of this wave's MT) from the ring slot `at`.
+    struct Keys {
+      u32x4 code[KS], pe[R / 32];
+      uint32_t scale;
+    };
+    auto read_keys = [&](uint32_t at, int m) {
       const uint8_t* const slot = smem + at;
-      const int buf = k & 1;
-      f32x4 acc[G];
+      const int t = 16 * (tw * MT + m) + la;
+      Keys kv;
 #pragma unroll
-      for (int m = 0; m < G; ++m) {
-        const int t = 16 * (tw * G + m) + la;
-        const uint8_t* const row = slot + t * CB;
-        const int f = code_swz(t);
-        const uint8_t* const sp = slot + Ge::CODES + Ge::ROPE + 256 * (tw * G + m) + la * NB + gq * KS;
-        const uint32_t sa = KS == 4 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp);
-        f32x4 c = {0.f, 0.f, 0.f, 0.f}, d = {0.f, 0.f, 0.f, 0.f};
-        static_for<KS>([&](auto s) {
-          const u32x4 kc = *reinterpret_cast<const u32x4*>(row + 16 * ((gq * KS + s) ^ f));
-          c = mfma_fp4_fp8<s, 0>(kc, qhi[s], c, sa, qscale);
-          d = mfma_fp4_fp8<s, 1>(kc, qlo[s], d, sa, qscale);
-        });
-        const uint8_t* const pe = slot + Ge::CODES + t * 2 * R;
-        const int fr = rope_swz(t);
+      for (int s = 0; s < KS; ++s)
+        kv.code[s] = *reinterpret_cast<const u32x4*>(slot + t * CB + 16 * ((gq * KS + s) ^ code_swz(t)));
+      const uint8_t* const sp = slot + Ge::CODES + Ge::ROPE + 256 * (t / CT) + t % CT * NB + gq * KS;
+      kv.scale = KS == 4 ? *reinterpret_cast<const uint32_t*>(sp) : *reinterpret_cast<const uint16_t*>(sp);
 #pragma unroll
-        for (int j = 0; j < R / 32; ++j)
-          d = mfma16x16x32(*reinterpret_cast<const u32x4*>(pe + 16 * ((4 * j + gq) ^ fr)), qpe[j], d);
-        acc[m] = c + d;
-      }
-      // exponent fields of the scales of this wave's 16 copied positions: (159 - s) << 7
-      {
-        if (LS == 4 || lane < 16 * LS) {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(slot + Ge::CODES + Ge::ROPE + 256 * wave + 4 * lane);
-          uint16_t* const es = reinterpret_cast<uint16_t*>(smem + Ge::ES + buf * NB * 128) + 4 * (lane % LS) * 64 +
-                               16 * wave + lane / LS;
+      for (int j = 0; j < R / 32; ++j)
+        kv.pe[j] = *reinterpret_cast<const u32x4*>(slot + Ge::CODES + t * 2 * R + 16 * ((4 * j + gq) ^ rope_swz(t)));
+      return kv;
+    };
+    // Their products with the query rows of this wave's group: the latent ones on e4m3
+    // hi and lo, the rope ones on bf16. With a single sub-tile two chains take turns.
+    auto products = [&](const Keys& kv) {
+      f32x4 c = {0.f, 0.f, 0.f, 0.f}, d2 = {0.f, 0.f, 0.f, 0.f};
+      f32x4& d = MT == 1 ? d2 : c;
+      static_for<KS>([&](auto s) {
+        c = mfma_fp4_fp8<s, 0>(kv.code[s], qhi[s], c, kv.scale, qscale);
+        d = mfma_fp4_fp8<s, 1>(kv.code[s], qlo[s], d, kv.scale, qscale);
+      });
 #pragma unroll
-          for (int i = 0; i < 4; ++i) es[64 * i] = (uint16_t)(max(kMx4High - (int)((w >> (8 * i)) & 255u), 0) << 7);
-        }
-      }
-      const int p0 = kMx4Tile * (t0 + k);
-      const bool masked = !full_rows || p0 + kMx4Tile > vis_all;
-      float mx = -INFINITY;
-#pragma unroll
-      for (int m = 0; m < G; ++m)
+      for (int j = 0; j < R / 32; ++j) d = mfma16x16x32(kv.pe[j], qpe[j], d);
+      return MT == 1 ? c + d : c;
+    };
+    // Exponent fields of the scales of this wave's CT copied positions, (s - 63) << 7 or
+    // (159 - s) << 7, to LDS buffer k & 1.
+    auto scale_fields = [&](int k, uint32_t at) {
+      if (CT * LS == 64 || lane < CT * LS) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + at + Ge::CODES + Ge::ROPE + 256 * wave + 4 * lane);
+        uint16_t* const es =
+            reinterpret_cast<uint16_t*>(smem + Ge::ES + (k & 1) * NB * 128) + 4 * (lane % LS) * 64 + CT * wave + lane / LS;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          acc[m][i] *= c2;
-          if (masked && p0 + 16 * (tw * G + m) + 4 * gq + i >= vis) acc[m][i] = -INFINITY;
-          mx = fmaxf(mx, acc[m][i]);
+          const int c = (int)((w >> (8 * i)) & 255u);
+          es[64 * i] = (uint16_t)((Ge::VSIDE ? min(max(c - kMx4Low, 0), kMx4High - kMx4Low) : max(kMx4High - c, 0)) << 7);
         }
-      float r = ref[gw];
-      const bool moved = __builtin_amdgcn_ballot_w64(mx > r + kMx4Slack) != 0;
+      }
+    };
+    // What is rare about tile k's scores: positions that not every row sees, and a
+    // score that passes its row's reference by more than the slack. The wave's flag
+    // and its reference go to LDS buffer k & 1.
+    auto look = [&](int k, f32x4 (&acc)[MT]) {
+      const int p0 = kMx4Tile * (t0 + k), buf = k & 1;
+      if (__builtin_expect(!full_rows || p0 + kMx4Tile > vis_all, 0)) {
+        asm volatile("");  // (a branch: most tiles have nothing to mask)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (p0 + 16 * (tw * MT + m) + 4 * gq + i >= vis) acc[m][i] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, acc[m][i]);
+      mx *= c2;
+      wref = ref[gw];
+      const bool moved = __builtin_amdgcn_ballot_w64(mx > wref + kMx4Slack) != 0;
       if (__builtin_expect(moved, 0)) {
         const float top = wave_max_over_groups(mx);
-        if (top > r + kMx4Slack) r = ceilf(top);
-        if (gq == 0) *reinterpret_cast<float*>(smem + Ge::WREF + 256 * buf + 64 * wave + 4 * la) = r;
+        if (top > wref + kMx4Slack) wref = ceilf(top);
+        if (gq == 0) *reinterpret_cast<float*>(smem + Ge::WREF + 64 * W * buf + 64 * wave + 4 * la) = wref;
       }
-      if (lane == 0) *reinterpret_cast<uint32_t*>(smem + Ge::FLAG + 16 * buf + 4 * wave) = moved;
-      wref = r;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(smem + Ge::FLAG + 4 * W * buf + 4 * wave) = moved;
+    };
+    // Probabilities of tile k, to LDS buffer k & 1.
+    auto softmax = [&](int k, const f32x4 (&acc)[MT]) {
       ltile = 0.f;
 #pragma unroll
-      for (int m = 0; m < G; ++m) {
+      for (int m = 0; m < MT; ++m) {
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(acc[m][i] - r);
+          p[i] = __builtin_amdgcn_exp2f(fmaf(acc[m][i], c2, -wref));
           ltile += p[i];
         }
         // chunk (8 positions) c of a row at c ^ (row & 7)
-        const int c = 2 * (tw * G + m) + (gq >> 1);
-        *reinterpret_cast<u32x2*>(smem + Ge::P + buf * Ge::ROWS * 128 + (16 * gw + la) * 128 + 16 * (c ^ (la & 7)) +
+        const int c = 2 * (tw * MT + m) + (gq >> 1);
+        *reinterpret_cast<u32x2*>(smem + Ge::P + (k & 1) * Ge::ROWS * 128 + (16 * gw + la) * 128 + 16 * (c ^ (la & 7)) +
                                   8 * (gq & 1)) = u32x2{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
       }
     };
-
-    // Output of tile k: O^T += X^T P^T over this wave's features.
-    auto output = [&](int k, uint32_t at) {
-      const uint8_t* const slot = smem + at;
+    // P of tile k: row la of group g, positions 16 gq + 8 h .. + 7.
+    auto read_p = [&](int k, int g, int h) {
+      return *reinterpret_cast<const u32x4*>(smem + Ge::P + (k & 1) * Ge::ROWS * 128 + (16 * g + la) * 128 +
+                                             16 * ((2 * gq + h) ^ (la & 7)));
+    };
+    struct Flags {
+      uint32_t of[W];
+    };
+    auto read_flags = [&](int k) {
+      Flags f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) f.of[w] = reinterpret_cast<const uint32_t*>(smem + Ge::FLAG + 4 * W * (k & 1))[w];
+      return f;
+    };
+    // The common references of tile k: where a wave has moved one (not 0 returned), all
+    // go to the largest, and what was computed against smaller ones is scaled down
+    // by powers of two, earlier sums here, P by `lower` with `down`.
+    uint32_t down[G];  // by how many powers of two a group's P of this lane's positions falls
+    auto agree = [&](int k, const Flags& fl) {
       const int buf = k & 1;
-      const u32x4 fl = *reinterpret_cast<const u32x4*>(smem + Ge::FLAG + 16 * buf);
-      u32x4 p[G][2];  // row la: positions 16 gq .. 16 gq + 15
+      uint32_t any = 0;
 #pragma unroll
-      for (int g = 0; g < G; ++g)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          p[g][h] = *reinterpret_cast<const u32x4*>(smem + Ge::P + buf * Ge::ROWS * 128 + (16 * g + la) * 128 +
-                                                    16 * ((2 * gq + h) ^ (la & 7)));
+      for (int w = 0; w < W; ++w) any |= fl.of[w];
+      const uint32_t moved = __builtin_amdgcn_readfirstlane(any);
       float fall[G];  // factor by which a group's earlier sums fall
 #pragma unroll
       for (int g = 0; g < G; ++g) fall[g] = 1.f;
-      const uint32_t moved = __builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w);
+#pragma unroll
+      for (int g = 0; g < G; ++g) down[g] = 0;
       if (__builtin_expect(moved != 0, 0)) {
-        // some wave moved a reference: all go to the largest, and what was
-        // computed against smaller ones is scaled down by powers of two
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           float mine[TW], top = ref[g];
 #pragma unroll
           for (int w = 0; w < TW; ++w) {
             const int wv = w * G + g;
-            const float r = *reinterpret_cast<const float*>(smem + Ge::WREF + 256 * buf + 64 * wv + 4 * la);
-            mine[w] = fl[wv] ? r : ref[g];
+            const float r = *reinterpret_cast<const float*>(smem + Ge::WREF + 64 * W * buf + 64 * wv + 4 * la);
+            mine[w] = fl.of[wv] ? r : ref[g];
             top = fmaxf(top, mine[w]);
           }
           fall[g] = __builtin_amdgcn_exp2f(ref[g] - top);
@@ -644,12 +716,9 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
           }
           float r = mine[0];  // of the wave that made this lane's 16 positions
 #pragma unroll
-          for (int w = 1; w < TW; ++w) r = gq / G == w ? mine[w] : r;
-          const uint32_t down = (uint32_t)fminf(top - r, 511.f) << 7;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[g][h][i] = sub_sat(p[g][h][i], down | down << 16);
+          for (int w = 1; w < TW; ++w) r = gq * TW / 4 == w ? mine[w] : r;
+          const uint32_t d = (uint32_t)fminf(top - r, 511.f) << 7;
+          down[g] = d | d << 16;
           if (g == gw) {
             lsum = lsum * fall[g];
             ltile = ltile * __builtin_amdgcn_exp2f(wref - top);
@@ -662,33 +731,107 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
         for (int g = 0; g < G; ++g) scale_acc8(o[g], fall[g], moved);
       }
       lsum += ltile;
+      return moved;
+    };
+    auto lower = [&](u32x4& p, uint32_t d) {
 #pragma unroll
-      for (int bb = 0; bb < FT / 2; ++bb) {
-        const int nb = wave * (FT / 2) + bb;  // scale block: features 32 nb ..
-        const u32x4* const es = reinterpret_cast<const u32x4*>(smem + Ge::ES + buf * NB * 128 + nb * 128 + 32 * gq);
-        const u32x4 e0 = es[0], e1 = es[1];
-        const int t = 16 * gq + la;
-        const int ch = nb ^ code_swz(t);
-        u32x4 x[2][2];
+      for (int i = 0; i < 4; ++i) p[i] = sub_sat(p[i], d);
+    };
+    // (MIX) 32 of this wave's features of tile k (scale block bb of its FT / 2), as they lie in the
+    // ring slot `at`, and as bf16 with the scales in their exponents: positions 16 gq .. + 15
+    // (two halves) of feature la of two output tiles.
+    struct Raw {
+      u32x4 e[2];
+      i32x2 v[2];
+    };
+    auto read_raw = [&](int k, uint32_t at, int bb) {
+      const int t = 16 * gq + la, nb = wave * (FT / 2) + bb;
+      const u32x4* const es = reinterpret_cast<const u32x4*>(smem + Ge::ES + (k & 1) * NB * 128 + nb * 128 + 32 * gq);
+      Raw r;
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-              (__attribute__((address_space(3))) i32x2*)(slot + t * CB + 16 * ch + 8 * f));
-          x[f][0] = fp4x8_to_bf16((uint32_t)v.x);
-          x[f][1] = fp4x8_to_bf16((uint32_t)v.y);
+      for (int f = 0; f < 2; ++f) {
+        r.e[f] = es[f];
+        r.v[f] = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)(smem + at + t * CB + 16 * (nb ^ code_swz(t)) + 8 * f));
+      }
+      return r;
+    };
+    auto expand = [&](const Raw& r, u32x4 (&x0)[2], u32x4 (&x1)[2]) {
+      x0[0] = fp4x8_to_bf16((uint32_t)r.v[0].x);
+      x0[1] = fp4x8_to_bf16((uint32_t)r.v[0].y);
+      x1[0] = fp4x8_to_bf16((uint32_t)r.v[1].x);
+      x1[1] = fp4x8_to_bf16((uint32_t)r.v[1].y);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x0[h][i] = add16(x0[h][i], r.e[h][i]);
+          x1[h][i] = add16(x1[h][i], r.e[h][i]);
+        }
+    };
+    // O^T += X^T P^T of tile k, with N halves (8 of a lane's 16 positions) of P at a time.
+    auto outputs = [&](int k, uint32_t at) {
+      constexpr int N = Ge::PH;
+      u32x4 p[G][N];
+      auto read_ps = [&](int h0) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int h = 0; h < N; ++h) p[g][h] = read_p(k, g, h0 + h);
+      };
+      const Flags fl = read_flags(k);
+      read_ps(0);
+      const uint32_t moved = agree(k, fl);
+      const int t = 16 * gq + la;
+      u32x2 x[FT];  // 16 positions of feature la of each output tile
+      auto read_x = [&](int j) {
+        x[j] = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)(smem + at + t * CB + 16 * ((wave * (FT / 2) + j / 2) ^ code_swz(t)) +
+                                                       8 * (j % 2))));
+      };
+      if constexpr (N == 1) {
+#pragma unroll
+        for (int j = 0; j < FT; ++j) read_x(j);
+      }
+#pragma unroll
+      for (int h0 = 0; h0 < 2; h0 += N) {
+        if (h0) read_ps(h0);
+        if (__builtin_expect(moved != 0, 0)) {
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int h = 0; h < N; ++h) lower(p[g][h], down[g]);
         }
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          u32x4 ps[2];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ps[0][i] = sub_sat(p[g][0][i], e0[i]);
-            ps[1][i] = sub_sat(p[g][1][i], e1[i]);
+        for (int bb = 0; bb < FT / 2; ++bb) {
+          if constexpr (N == 2) {
+            read_x(2 * bb);
+            read_x(2 * bb + 1);
           }
+          const uint8_t* const es = smem + Ge::ES + (k & 1) * NB * 128 + (wave * (FT / 2) + bb) * 128 + 32 * gq + 16 * h0;
 #pragma unroll
-          for (int f = 0; f < 2; ++f)
+          for (int h = 0; h < N; ++h) {
+            const u32x4 e = *reinterpret_cast<const u32x4*>(es + 16 * h);
+            const uint32_t w0 = x[2 * bb][h0 + h], w1 = x[2 * bb + 1][h0 + h];
+            u32x4 x0 = fp4x8_to_bf16(w0), x1 = fp4x8_to_bf16(w1);
+            if constexpr (Ge::VSIDE) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) o[g][2 * bb + f] = mfma16x16x32(x[f][h], ps[h], o[g][2 * bb + f]);
+              for (int i = 0; i < 4; ++i) {
+                x0[i] = add16(x0[i], e[i]);
+                x1[i] = add16(x1[i], e[i]);
+              }
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              u32x4 q = p[g][h];
+              if constexpr (!Ge::VSIDE) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[i] = sub_sat(q[i], e[i]);
+              }
+              o[g][2 * bb] = mfma16x16x32(x0, q, o[g][2 * bb]);
+              o[g][2 * bb + 1] = mfma16x16x32(x1, q, o[g][2 * bb + 1]);
+            }
+          }
         }
       }
     };
@@ -697,7 +840,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     // Copies in order: before the loop tiles 0 .. S - 3, in turn k (after barrier k)
     // tile k + S - 1, each (without PAGED) behind the page numbers of the tile S - 2
     // later. Barrier k waits until tile k + 1 is in; then tiles k + 2 .. k + S - 2 may
-    // be on their way. Turn k = -1 has no output, turn nt - 1 no scores.
+    // be on their way. Turn k has tile k's output and tile k + 1's scores.
     constexpr int IC = PAGED ? 0 : S - 3;  // page number copies behind tile k + 1
     uint32_t here = 0, ahead = 0;          // ring slots of tiles k and k + 1
     auto meet = [&](int k) {
@@ -712,22 +855,77 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
+    };
+    auto ask = [&](int k) {
       if constexpr (!PAGED) copy_idx(k + 2 * S - 3);
       ask_tile(k + S - 1);
     };
     if (nt > 0) {
+      f32x4 acc[MT];
       meet(-1);
-      scores(0, 0);
+      ask(-1);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] = products(read_keys(0, m));
+      scale_fields(0, 0);
+      look(0, acc);
+      softmax(0, acc);
 #pragma unroll 1
       for (int k = 0; k < nt - 1; ++k) {
         here = ahead;
         ahead = next(ahead);
         meet(k);
-        output(k, here);
-        scores(k + 1, ahead);
+        if constexpr (Ge::MIX) {
+          constexpr int STEPS = MT > FT / 2 ? MT : FT / 2;
+          u32x4 p[G][2], x[FT][2];
+          // first part: the LDS reads of a step go out a step ahead of it
+          const Flags fl = read_flags(k);
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) p[g][h] = read_p(k, g, h);
+          Keys keys = read_keys(ahead, 0);
+          Raw raw = read_raw(k, here, 0);
+          ask(k);
+          if (__builtin_expect(agree(k, fl) != 0, 0)) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) lower(p[g][h], down[g]);
+          }
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            Keys keys2;
+            Raw raw2;
+            if (i + 1 < MT) keys2 = read_keys(ahead, i + 1);
+            if (i + 1 < FT / 2) raw2 = read_raw(k, here, i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i < MT) acc[i] = products(keys);
+            if (i < FT / 2) expand(raw, x[2 * i], x[2 * i + 1]);
+            if (i + 1 == STEPS) scale_fields(k + 1, ahead);
+            if (i + 1 < MT) keys = keys2;
+            if (i + 1 < FT / 2) raw = raw2;
+          }
+          // second part
+          look(k + 1, acc);
+#pragma unroll
+          for (int j = 0; j < FT; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int g = 0; g < G; ++g) o[g][j] = mfma16x16x32(x[j][h], p[g][h], o[g][j]);
+          softmax(k + 1, acc);
+        } else {
+          ask(k);
+          outputs(k, here);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[m] = products(read_keys(ahead, m));
+          scale_fields(k + 1, ahead);
+          look(k + 1, acc);
+          softmax(k + 1, acc);
+        }
       }
       meet(nt - 1);
-      output(nt - 1, ahead);
+      outputs(nt - 1, ahead);
     }
     if constexpr (!PAGED) wait_loads<0>();  // (page numbers asked for past the end)
 
@@ -744,12 +942,11 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       if (r >= rows) continue;
       const int tq = tok_of(16 * g + la), tok = rq.q0 + tq, head = head0 + 16 * g + la - (tq - tok0) * a.H;
       if (whole) {
-        const float inv = l == 0.f ? 0.f : 4294967296.f / l;
+        const float inv = l == 0.f ? 0.f : Ge::UNIT / l;
         uint16_t* const out = a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + Ge::FW * wave + 4 * gq;
 #pragma unroll
         for (int j = 0; j < FT; ++j) {
-          const f32x4 v = o[g][j] * inv;
-          *reinterpret_cast<u32x2*>(out + 16 * j) = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+          *reinterpret_cast<u32x2*>(out + 16 * j) = finish<Ge::VSIDE>(o[g][j], inv);
         }
         if (a.lse && wave == 0 && gq == 0)
           a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (ref[g] + log2f(l)) * kLn2;
@@ -757,7 +954,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
         uint8_t* const part = a.ws + kMx4WsHead + ((int64_t)2 * a.blocks + (nth > 0)) * Ge::SLOT;
         float* const po = reinterpret_cast<float*>(part) + (16 * g + la) * D + Ge::FW * wave + 4 * gq;
 #pragma unroll
-        for (int j = 0; j < FT; ++j) *reinterpret_cast<f32x4*>(po + 16 * j) = o[g][j];
+        for (int j = 0; j < FT; ++j) *reinterpret_cast<f32x4*>(po + 16 * j) = o[g][j] * Ge::UNIT;
         if (wave == 0 && gq == 0)
           reinterpret_cast<f32x2*>(part + Ge::ROWS * D * 4)[16 * g + la] = f32x2{ref[g], l};
       }
@@ -833,11 +1030,9 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
       o += s_o[i][c] * w;
     }
   }
-  const float inv = l == 0.f ? 0.f : 4294967296.f / l;
-  o *= inv;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = job.q0 + r / a.H, head = r % a.H;
-  *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * c) =
-      u32x2{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
+  *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * c) = finish<true>(o, inv);
   if (a.lse && c == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
