@@ -20,7 +20,7 @@ CSRC = HERE / "csrc"
 ROOT = HERE.parent
 LIB = HERE / "librolaq_mla.so"
 SOURCES = ["api.cpp", "pack.hip", "writer.hip", "decode.hip", "extend.hip", "assemble.hip",
-           "mx4_rows.hip", "mx4_attend.hip"]
+           "mx4_rows.hip", "mx4_unrotate.hip", "mx4_attend.hip"]
 ARCH = "gfx950"
 
 

@@ -613,20 +613,6 @@ int rolaq_mx4_read_rows(const int64_t* slots, int64_t n, const uint8_t* codes, c
   if (!aligned(out, 16) || out_stride < D + R || out_stride % 8)
     return fail(ROLAQ_ERR_INVALID, "%s: out must be 16-byte aligned with a row stride >= D + R, multiple of 8", fn);
   if (rotation && !aligned(rotation, 16)) return fail(ROLAQ_ERR_INVALID, "%s: rotation must be 16-byte aligned", fn);
-  if (rotation) {
-    rolaq::AssembleArgs a{};
-    a.slots = slots;
-    a.n = n;
-    a.codes = codes;
-    a.scales = scales;
-    a.num_slots = num_slots;
-    a.rope = static_cast<const uint16_t*>(rope_buf);
-    a.rot = static_cast<const uint16_t*>(rotation);
-    a.R = R;
-    a.out = static_cast<uint16_t*>(out);
-    a.out_st = out_stride;
-    return hip_status(rolaq_launch_assemble(a, D, static_cast<hipStream_t>(stream)), "mx4_read_rows launch");
-  }
   rolaq::Mx4RowsArgs a{};
   a.slots = slots;
   a.n = n;
@@ -636,6 +622,9 @@ int rolaq_mx4_read_rows(const int64_t* slots, int64_t n, const uint8_t* codes, c
   a.rope = const_cast<uint16_t*>(static_cast<const uint16_t*>(rope_buf));
   a.out = static_cast<uint16_t*>(out);
   a.out_st = out_stride;
+  a.rot = static_cast<const uint16_t*>(rotation);
+  if (rotation)
+    return hip_status(rolaq_launch_mx4_unrotate(a, D, cu_count(), static_cast<hipStream_t>(stream)), "mx4_read_rows launch");
   return hip_status(rolaq_launch_mx4_read(a, D, static_cast<hipStream_t>(stream)), "mx4_read_rows launch");
 }
 

@@ -13,7 +13,6 @@
 // the cast order of rotate_quantize (quantizer.py:121-122).
 #include "rolaq_common.h"
 #include "rolaq_args.h"
-#include "mx4_codec.h"
 
 namespace rolaq {
 
@@ -79,9 +78,7 @@ struct AsmRotGeo {
   static constexpr int LDS = kAsmRotRows * STR;
 };
 
-// MX4: the rows are 4-bit ones (codes and scale bytes; a slot outside the cache
-// reads as NaN), and only the gather differs.
-template <int D, bool MX4>
+template <int D>
 __global__ __launch_bounds__(64 * kAsmRotWaves, 1) void assemble_rot_kernel(AssembleArgs a) {
   constexpr int NG = D / 128, STR = AsmRotGeo<D>::STR, KS = D / 32;
   constexpr int CW = D / kAsmRotWaves, MB = CW / 16, NB = kAsmRotRows / 16;
@@ -119,12 +116,8 @@ __global__ __launch_bounds__(64 * kAsmRotWaves, 1) void assemble_rot_kernel(Asse
     int32_t hr = -1;
     if (row < a.n) {
       slot = a.slots[row];
-      if constexpr (MX4) {
-        hr = slot >= 0 && slot < a.num_slots ? 0 : 1;  // 1: no such slot
-      } else {
-        const int32_t r = a.row_of_slot[slot];
-        if (r >= 0 && a.owner_of_row[r] == (int32_t)slot) hr = r;
-      }
+      const int32_t r = a.row_of_slot[slot];
+      if (r >= 0 && a.owner_of_row[r] == (int32_t)slot) hr = r;
     }
     s_slot[tid] = slot;
     s_hr[tid] = hr;
@@ -136,22 +129,7 @@ __global__ __launch_bounds__(64 * kAsmRotWaves, 1) void assemble_rot_kernel(Asse
   // 16-byte LDS chunks. Few, wide loads per thread keep many
   // in flight.
   constexpr int CCH = D / 64;  // 16-byte code chunks per row
-  if constexpr (MX4) {
-    // one item = row r and block j of 32 columns: 16 bytes of codes
-    for (int c = tid; c < kAsmRotRows * (D / 32); c += NT) {
-      const int r = c / (D / 32), j = c % (D / 32);
-      const int64_t slot = s_slot[r];
-      u32x4 w = {0u, 0u, 0u, 0u};
-      uint32_t s = row0 + r < a.n ? kMx4NaN : kMx4Low;
-      if (row0 + r < a.n && s_hr[r] == 0) {
-        w = *reinterpret_cast<const u32x4*>(a.codes + slot * (D / 2) + 16 * j);
-        s = a.scales[slot * (D / 32) + j];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4*>(s_x + r * STR + 64 * j + 16 * i) = mx4_values8(w[i], s);
-    }
-  }
-  for (int c = tid; !MX4 && c < kAsmRotRows * CCH; c += NT) {
+  for (int c = tid; c < kAsmRotRows * CCH; c += NT) {
     const int r = c / CCH, j = c % CCH;
     const int64_t slot = s_slot[r];
     const int32_t hr = s_hr[r];
@@ -193,10 +171,7 @@ __global__ __launch_bounds__(64 * kAsmRotWaves, 1) void assemble_rot_kernel(Asse
   for (int c = tid; c < kAsmRotRows * (a.R / 8); c += NT) {
     const int r = c / (a.R / 8), ch = c % (a.R / 8);
     const int64_t slot = s_slot[r];
-    if (MX4 && row0 + r < a.n && s_hr[r] != 0)
-      *reinterpret_cast<u32x4*>(a.out + (row0 + r) * a.out_st + D + 8 * ch) =
-          u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
-    else if (slot >= 0)
+    if (slot >= 0)
       *reinterpret_cast<u32x4*>(a.out + (row0 + r) * a.out_st + D + 8 * ch) =
           *reinterpret_cast<const u32x4*>(a.rope + slot * a.R + 8 * ch);
   }
@@ -254,18 +229,16 @@ hipError_t rolaq_launch_assemble(const rolaq::AssembleArgs& a, int D, hipStream_
   using namespace rolaq;
   if (a.rot) {
     const dim3 grid((unsigned)((a.n + kAsmRotRows - 1) / kAsmRotRows)), block(64 * kAsmRotWaves);
-#define ROLAQ_ASM_ROT(DD, MX4)                                                                            \
-    if (D == DD && (a.scales != nullptr) == MX4) {                                                        \
-      const hipError_t e = hipFuncSetAttribute((const void*)assemble_rot_kernel<DD, MX4>,                 \
+#define ROLAQ_ASM_ROT(DD)                                                                                 \
+    if (D == DD) {                                                                                        \
+      const hipError_t e = hipFuncSetAttribute((const void*)assemble_rot_kernel<DD>,                      \
                                                hipFuncAttributeMaxDynamicSharedMemorySize, AsmRotGeo<DD>::LDS); \
       if (e != hipSuccess) return e;                                                                      \
-      hipLaunchKernelGGL((assemble_rot_kernel<DD, MX4>), grid, block, AsmRotGeo<DD>::LDS, stream, a);     \
+      hipLaunchKernelGGL((assemble_rot_kernel<DD>), grid, block, AsmRotGeo<DD>::LDS, stream, a);          \
       return hipGetLastError();                                                                           \
     }
-    ROLAQ_ASM_ROT(512, false)
-    ROLAQ_ASM_ROT(256, false)
-    ROLAQ_ASM_ROT(512, true)
-    ROLAQ_ASM_ROT(256, true)
+    ROLAQ_ASM_ROT(512)
+    ROLAQ_ASM_ROT(256)
 #undef ROLAQ_ASM_ROT
     return hipErrorInvalidValue;
   }

@@ -50,7 +50,7 @@ struct Mx4RowsArgs {
   uint16_t* rope;
   uint16_t* out;  // reader: [n, out_st] bf16, latent (D) then rope (R)
   int64_t out_st;
-  const uint16_t* rot;  // reader: R_eff [D, D] row-major, or null
+  const uint16_t* rot;  // reader of rotated rows: R_eff [D, D] row-major, 16-byte aligned
 };
 
 }  // namespace rolaq
@@ -60,3 +60,4 @@ hipError_t rolaq_launch_mx4_attend(const rolaq::Mx4AttendArgs& a, int D, int num
 int64_t rolaq_mx4_attend_ws_bytes(int D, int num_cus);
 hipError_t rolaq_launch_mx4_write_plain(const rolaq::Mx4RowsArgs& a, int D, hipStream_t stream);
 hipError_t rolaq_launch_mx4_read(const rolaq::Mx4RowsArgs& a, int D, hipStream_t stream);
+hipError_t rolaq_launch_mx4_unrotate(const rolaq::Mx4RowsArgs& a, int D, int num_cus, hipStream_t stream);

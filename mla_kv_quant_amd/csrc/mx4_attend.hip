@@ -41,13 +41,12 @@
 // that mx4_merge_kernel joins. With many row blocks each has a block of its own.
 #include "rolaq_common.h"
 #include "mx4_args.h"
+#include "mx4_tile.h"
 
 #include <algorithm>
-#include <utility>
 
 namespace rolaq {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
@@ -57,41 +56,6 @@ constexpr int kMx4Idx = 4;             // tiles whose page numbers are held (rin
 constexpr float kMx4NoRef = -268435456.f;  // reference of a row that has seen no score
 constexpr float kMx4Slack = 8.f;       // log2 by which a score may pass its row's reference: sums of
                                        // 2^21 such P times 6 2^96, the largest value held, stay below 2^128
-
-// D = A(16x128, E2M1) * B(128x16, E4M3) + C. Lane l holds A[l%16][32(l/16)+i] (nibble
-// i of four dwords) with the scale of those 32 in byte SA of sa, and
-// B[16(l/16)+i][l%16], B[64+16(l/16)+i][l%16] (bytes i and 16+i) with the scale of
-// B[32(l/16)..+31] in byte SB of sb.
-template <int SA, int SB>
-__device__ __forceinline__ f32x4 mfma_fp4_fp8(u32x4 a, i32x8 b, f32x4 c, uint32_t sa, uint32_t sb) {
-  const i32x8 aa = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(aa, b, c, 4, 0, SA, (int)sa, SB, (int)sb);
-}
-
-// Asynchronous copies into LDS, 16 or 4 bytes for each lane, lane l's to
-// lds + 16 l (4 l). In assembly because the compiler, which tracks such copies,
-// would wait for all of them before any LDS read; the kernel waits by count.
-__device__ __forceinline__ void copy16(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
-}
-__device__ __forceinline__ void copy4(const void* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
-}
-
-// The same from a scalar base and a 32-bit offset for each lane.
-__device__ __forceinline__ void copy16(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
-}
-__device__ __forceinline__ void copy4(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
-}
-
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 // Packed saturating subtraction of two 16-bit fields.
 __device__ __forceinline__ uint32_t sub_sat(uint32_t a, uint32_t b) {
@@ -135,15 +99,6 @@ __device__ __forceinline__ u32x4 fp4x8_to_bf16(uint32_t v) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 1)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 2)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, 1.0f, 3))};
-}
-
-template <typename F, int... I>
-__device__ __forceinline__ void for_each_of(F&& f, std::integer_sequence<int, I...>) {
-  (f(std::integral_constant<int, I>{}), ...);
-}
-template <int N, typename F>
-__device__ __forceinline__ void static_for(F&& f) {
-  for_each_of(f, std::make_integer_sequence<int, N>{});
 }
 
 template <int D, int R, int G>
@@ -530,43 +485,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
         ask_tile(k);
       }
     }
-    {
-      // largest magnitude of the row, as bits (NaN above infinity)
-      uint32_t big = 0;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t w = v[s][h][e][i] & 0x7fff7fffu;
-              big = max(big, max(w & 0xffffu, w >> 16));
-            }
-      big = max(big, (uint32_t)__shfl_xor((int)big, 16));
-      big = max(big, (uint32_t)__shfl_xor((int)big, 32));
-      const int e = max((int)(big >> 7), 16);  // biased exponent
-      // scaled so that the largest lies in [2^7, 2^8); lo is 2^4 finer
-      const float up = __uint_as_float((uint32_t)(min(max(127 + 127 + 7 - e, 1), 254)) << 23);
-      qscale = e >= 255 ? 0xffffu : (uint32_t)(e - 7) | (uint32_t)(e - 11) << 8;
-#pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {  // dword d: values 4 d .. 4 d + 3 of 16
-            const uint32_t w0 = v[s][h][d >> 1][2 * (d & 1)], w1 = v[s][h][d >> 1][2 * (d & 1) + 1];
-            const float f0 = bf16_lo(w0) * up, f1 = bf16_hi(w0) * up, f2 = bf16_lo(w1) * up, f3 = bf16_hi(w1) * up;
-            int hi = __builtin_amdgcn_cvt_pk_fp8_f32(f0, f1, 0, false);
-            hi = __builtin_amdgcn_cvt_pk_fp8_f32(f2, f3, hi, true);
-            const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-            int lo = __builtin_amdgcn_cvt_pk_fp8_f32((f0 - b0.x) * 16.f, (f1 - b0.y) * 16.f, 0, false);
-            lo = __builtin_amdgcn_cvt_pk_fp8_f32((f2 - b1.x) * 16.f, (f3 - b1.y) * 16.f, lo, true);
-            qhi[s][4 * h + d] = hi;
-            qlo[s][4 * h + d] = lo;
-          }
-    }
+    qscale = mx4_split<KS>(v, qhi, qlo);
 
     f32x4 o[G][FT];
 #pragma unroll

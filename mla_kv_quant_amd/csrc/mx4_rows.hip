@@ -1,7 +1,7 @@
 // MX4 latent cache rows without a rotation (gfx950): the writer of un-rotated
 // layers and the read-back of rows as they are stored. Both move bytes: a row
 // is 2 (D + R) bytes of bf16 against D / 2 + D / 32 + 2 R in the cache. Rows of
-// rotated layers are written by writer_kernel and read by assemble_rot_kernel.
+// rotated layers are written by writer_kernel and read by mx4_unrotate_kernel.
 #include "mx4_codec.h"
 
 namespace rolaq {

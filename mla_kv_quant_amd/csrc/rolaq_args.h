@@ -124,10 +124,6 @@ struct AssembleArgs {
   int R;
   uint16_t* out;              // [n, out_st] bf16: latent (D) then rope (R)
   int64_t out_st;
-  // MX4 rows instead of INT2 ones (codes then holds 4-bit codes, and params,
-  // hp and the maps are unused): scale bytes, or null
-  const uint8_t* scales;
-  int64_t num_slots;
 };
 
 }  // namespace rolaq
