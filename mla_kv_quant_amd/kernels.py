@@ -33,22 +33,13 @@ def _stream(t: torch.Tensor):
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-class _on:
-    """``dev`` as the current device for the calls inside: a launch goes to a
-    stream of its tensors' device. Nothing where it is current already."""
-
-    def __init__(self, dev: torch.device):
-        self.index = dev.index if dev.type == "cuda" else None
-
-    def __enter__(self):
-        self.before = None
-        if self.index is not None and self.index != torch.cuda.current_device():
-            self.before = torch.cuda.current_device()
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+def _call(dev: torch.device, fn, *args):
+    """``fn(*args)`` with ``dev`` as the current device: a launch goes to a stream of its tensors' device."""
+    if dev.type != "cuda" or dev.index == torch.cuda.current_device():
+        _lib.check(fn(*args))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args))
 
 
 def _need(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, ndim: int | None = None):
@@ -472,10 +463,8 @@ def mx4_write_rows(latent: torch.Tensor, k_pe: torch.Tensor, rotation_t: torch.T
         _need_all(dev, ((rotation_t, "rotation_t", torch.bfloat16, 2),))
         if rotation_t.shape != (D, D):
             raise ValueError("rotation_t must be [D, D]")
-    with _on(dev):
-        _lib.check(_lib.load().rolaq_mx4_write_rows(
-            _p(latent), latent.stride(0), _p(k_pe), k_pe.stride(0), k_pe.stride(1), _p(rotation_t), _p(loc), n, D, R,
-            _p(codes), _p(scales), _p(rope_buf), slots, _stream(codes)))
+    _call(dev, _lib.load().rolaq_mx4_write_rows, _p(latent), latent.stride(0), _p(k_pe), k_pe.stride(0),
+          k_pe.stride(1), _p(rotation_t), _p(loc), n, D, R, _p(codes), _p(scales), _p(rope_buf), slots, _stream(codes))
 
 
 def mx4_read_rows(slots: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, rope_buf: torch.Tensor,
@@ -492,18 +481,15 @@ def mx4_read_rows(slots: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor
     _need(out, "out", torch.bfloat16, dev, 2)
     if out.shape[0] < n or out.shape[1] < D + R or (n and out.stride(1) != 1):
         raise ValueError("out must be [n, >= D + R] with a contiguous last dim")
-    with _on(dev):
-        _lib.check(_lib.load().rolaq_mx4_read_rows(
-            _p(slots), n, _p(codes), _p(scales), _p(rope_buf), num, _p(rotation), D, R, _p(out), out.stride(0),
-            _stream(codes)))
+    _call(dev, _lib.load().rolaq_mx4_read_rows, _p(slots), n, _p(codes), _p(scales), _p(rope_buf), num, _p(rotation),
+          D, R, _p(out), out.stride(0), _stream(codes))
     return out
 
 
 def mx4_attend_workspace_bytes(D: int, device) -> int:
     """Bytes of :func:`mx4_attend_fwd`'s workspace at width ``D`` on ``device``, whatever the batch."""
     n = ctypes.c_int64(0)
-    with _on(torch.device(device)):
-        _lib.check(_lib.load().rolaq_mx4_attend_workspace(int(D), ctypes.byref(n)))
+    _call(torch.device(device), _lib.load().rolaq_mx4_attend_workspace, int(D), ctypes.byref(n))
     return n.value
 
 
@@ -533,10 +519,8 @@ def mx4_attend_fwd(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, r
         _need_all(dev, ((lse, "lse", torch.float32, 2),))
         if lse.shape[0] < T or lse.shape[1] != H:
             raise ValueError("lse must be [>= T, H]")
-    with _on(dev):
-        _lib.check(_lib.load().rolaq_mx4_attend_fwd(
-            _p(q), q.stride(0), q.stride(1), _p(codes), _p(scales), _p(rope_buf), slots, _p(qo_indptr), _p(kv_indptr),
-            _p(kv_indices), kv_indices.shape[0], int(page_size), _p(kv_lens), T, B, H, D, R, int(max_q_len),
-            float(sm_scale), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace), workspace.shape[0],
-            _stream(q)))
+    _call(dev, _lib.load().rolaq_mx4_attend_fwd, _p(q), q.stride(0), q.stride(1), _p(codes), _p(scales), _p(rope_buf),
+          slots, _p(qo_indptr), _p(kv_indptr), _p(kv_indices), kv_indices.shape[0], int(page_size), _p(kv_lens), T, B, H,
+          D, R, int(max_q_len), float(sm_scale), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace),
+          workspace.shape[0], _stream(q))
     return out

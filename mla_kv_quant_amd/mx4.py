@@ -99,7 +99,7 @@ def read_rows(pool, layer_id, slots, out=None, unrotate: bool = True):
         out = torch.empty(s.shape[0], pool.kv_lora_rank + pool.qk_rope_head_dim, dtype=torch.bfloat16,
                           device=pool.c_codes[li].device)
     rot = pool.latent_rotation(layer_id, local=True) if unrotate else None
-    if rot is not None:
+    if rot is not None and not (rot.dtype == torch.bfloat16 and rot.is_contiguous()):
         rot = rot.to(torch.bfloat16).contiguous()
     return kernels.mx4_read_rows(s, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], rot, out)
 
