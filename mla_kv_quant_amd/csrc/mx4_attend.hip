@@ -53,7 +53,7 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr int kMx4Tile = 64;           // positions in a tile
 constexpr int kMx4Idx = 4;             // tiles whose page numbers are held (ring slots - 1 at least)
-constexpr float kMx4NoRef = -268435456.f;  // reference of a row that has seen no score
+constexpr float kMx4NoRef = -0x1.fffffep127f;  // reference of a row that has seen no score
 constexpr float kMx4Slack = 8.f;       // log2 by which a score may pass its row's reference: sums of
                                        // 2^21 such P times 6 2^96, the largest value held, stay below 2^128
 
@@ -161,7 +161,8 @@ constexpr int kMx4WsHead = kMx4Jobs * sizeof(Mx4Job);
 
 // A request's part of the batch.
 struct Mx4Request {
-  int q0, nq;        // first query, queries
+  int q0, nq;        // first query, queries (max_q_len at most)
+  int past;          // positions before the first query's own (negative: the first ones see nothing)
   int len;           // cached positions
   int list;          // first entry of its page list
 };
@@ -171,13 +172,15 @@ __device__ __forceinline__ Mx4Request mx4_request(const Mx4AttendArgs& a, int b)
   r.q0 = a.qo_indptr ? a.qo_indptr[b] : b;
   const int q1 = a.qo_indptr ? a.qo_indptr[b + 1] : b + 1;
   r.q0 = min(max(r.q0, 0), a.T);
-  r.nq = min(max(min(q1, a.T) - r.q0, 0), a.max_q_len);
+  const int nq = max(min(q1, a.T) - r.q0, 0);
+  r.nq = min(nq, a.max_q_len);
   r.list = a.kv_indptr[b];
   const int end = a.kv_indptr[b + 1];
   r.list = max(r.list, 0);
   const int64_t pages = min((int64_t)max(end - r.list, 0), max(a.n_indices - r.list, (int64_t)0));
   const int64_t most = pages << a.page_shift;  // positions that the list reaches
   r.len = (int)max(min(min(a.kv_lens[b], most), (int64_t)0x3fffffff), (int64_t)0);
+  r.past = r.len - nq;
   return r;
 }
 
@@ -240,7 +243,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
   uint32_t all_units = 0, all_blocks = 0;
   Mx4Job* jobs = nullptr;
   int b = 0, rb_only = 0;
-  Mx4Request rq;
+  Mx4Request rq = {};
   if (a.blocks > 0) {
     // Tiles of all requests, summed by every wave for itself (a request a lane, 256
     // requests' loads in one round trip), then the request that has the first unit.
@@ -291,6 +294,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
           u_req = (uint32_t)__builtin_amdgcn_readlane((int)at4[k], l);
           rq.q0 = __builtin_amdgcn_readlane(r4[k].q0, l);
           rq.nq = __builtin_amdgcn_readlane(r4[k].nq, l);
+          rq.past = __builtin_amdgcn_readlane(r4[k].past, l);
           rq.len = __builtin_amdgcn_readlane(r4[k].len, l);
           rq.list = __builtin_amdgcn_readlane(r4[k].list, l);
         }
@@ -332,8 +336,9 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       const uint32_t done = u - u_req;
       rb = done / ntiles;
       if (rb >= mx4_row_blocks(rq, a.H, Ge::ROWS)) {  // on to the next request (one without queries has no units)
+        if (++b >= a.B) break;
         u_req = u;
-        rq = mx4_request(a, ++b);
+        rq = mx4_request(a, b);
         continue;
       }
       t0 = done - rb * ntiles;
@@ -363,11 +368,11 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     auto tok_of = [&](int x) { return tok0 + (((head0 + x) * a.h_inv) >> 16); };
     // positions that a row sees: its causal limit; rows past the last see none
     const int last_row = min(row0 + Ge::ROWS, rows) - 1;
-    const int vis_all = rq.len - rq.nq + tok0 + 1;                // seen by every row of the block
-    const int vis_most = rq.len - rq.nq + tok_of(last_row - row0) + 1;  // by any
+    const int vis_all = rq.past + tok0 + 1;                // seen by every row of the block
+    const int vis_most = rq.past + tok_of(last_row - row0) + 1;  // by any
     const int my_row = row0 + 16 * gw + la;
     const int my_tok = tok_of(16 * gw + la);
-    const int vis = my_row < rows ? rq.len - rq.nq + my_tok + 1 : 0;
+    const int vis = my_row < rows ? rq.past + my_tok + 1 : 0;
     const bool full_rows = row0 + Ge::ROWS <= rows;
     const int t_end = min(t1, (vis_most + kMx4Tile - 1) / kMx4Tile);
     const int nt = max(t_end - t0, 0);  // tiles to walk
@@ -573,13 +578,16 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     };
     // Probabilities of tile k, to LDS buffer k & 1.
     auto softmax = [&](int k, const f32x4 (&acc)[MT]) {
+      // (the score rounded before the difference, as in the reference: fused, one of
+      // 2^31 and more could pass its own maximum by 2^7)
+#pragma clang fp contract(off)
       ltile = 0.f;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[i] = __builtin_amdgcn_exp2f(fmaf(acc[m][i], c2, -wref));
+          p[i] = __builtin_amdgcn_exp2f(acc[m][i] * c2 - wref);
           ltile += p[i];
         }
         // chunk (8 positions) c of a row at c ^ (row & 7)
@@ -882,13 +890,14 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
   }
 }
 
-// Joins the partials of the pairs that were cut: a block for a job and THREADS / (D / 4
-// PARTS) rows, D / 4 threads for each of PARTS shares of a row's partials, four of
-// them in flight for each. What bounds it is latency (the job, then the partials), so
+// Joins the partials of the pairs that were cut: a block for a job, 4 C columns and
+// THREADS / (C PARTS) rows, C threads for each of PARTS shares of a row's partials, four
+// of them in flight for each. What bounds it is latency (the job, then the partials), so
 // blocks are small enough to be on the card all at once.
-template <int D, int PARTS, int THREADS>
+template <int D, int C, int PARTS, int THREADS>
 __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int rows_per_block) {
-  constexpr int C = D / 4, N = 4, RM = THREADS / C / PARTS;
+  constexpr int N = 4, RM = THREADS / C / PARTS;
+  static_assert(PARTS == 1 || RM == 1, "blocks with several shares leave as one");
   __shared__ f32x4 s_o[PARTS][C];
   __shared__ f32x2 s_ml[PARTS];
   const Mx4Job job = reinterpret_cast<const Mx4Job*>(a.ws)[blockIdx.x];
@@ -897,7 +906,8 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
     const Mx4Request rq = mx4_request(a, b);
     if ((int)(blockIdx.x % a.row_blocks) >= mx4_row_blocks(rq, a.H, rows_per_block)) return;
   }
-  const int c = threadIdx.x % C, unit = __builtin_amdgcn_readfirstlane(threadIdx.x / C);
+  const int c = threadIdx.x % C, col = 4 * (C * blockIdx.z + c);
+  const int unit = C % 64 == 0 ? __builtin_amdgcn_readfirstlane(threadIdx.x / C) : threadIdx.x / C;
   const int part = unit % PARTS, rl = blockIdx.y * RM + unit / PARTS, r = job.row0 + rl;
   if (job.parts == 0 || r >= job.rows || rl >= rows_per_block) return;
   const int64_t slot = (int64_t)rows_per_block * (D + 2) * 4;
@@ -912,7 +922,7 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
       const int jj = min(j + i * PARTS, job.parts - 1);
       const uint8_t* const p = parts + (2 * jj + (jj == 0 ? job.second : 0)) * slot;
       ml[i] = gload<f32x2>(p + (int64_t)rows_per_block * D * 4 + 8 * rl);
-      v[i] = gload<f32x4>(p + ((int64_t)rl * D + 4 * c) * 4);
+      v[i] = gload<f32x4>(p + ((int64_t)rl * D + col) * 4);
     }
     float top = m;
 #pragma unroll
@@ -951,8 +961,8 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = job.q0 + r / a.H, head = r % a.H;
-  *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + 4 * c) = finish<true>(o, inv);
-  if (a.lse && c == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + col) = finish<true>(o, inv);
+  if (a.lse && col == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 template <int D, int R, int G, bool PAGED>
@@ -961,10 +971,15 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_q_len * a.H;
   a.row_blocks = (int)((rows + Ge::ROWS - 1) / Ge::ROWS);
   a.h_inv = (65536 + a.H - 1) / a.H;
-  // Shared out while there are few row blocks for each CU; past that, or with more
-  // requests than a block's sums hold, each row block has a block.
+  // Shared out while there are few row blocks for each CU; past that, with more
+  // requests than a block's sums hold, or with more tiles than 32 bits count, each row
+  // block has a block. us, shared out / a block each: decode 32 x 4096 with 16 heads 24.5 / 78.7;
+  // ragged chunks with 6 row blocks a CU, D = 512: 873 to 1106 / 1109 to 1301; chunks of one
+  // length, D = 512, 4 row blocks a CU 577 / 523, 8 1141 / 1040; D = 256, 9 a CU, ragged 850 / 905, of one
+  // length 670 / 583.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
-  const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus;
+  const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + a.B;
+  const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
   const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);
   if (e != hipSuccess) return e;
@@ -981,13 +996,19 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
-  // Many partials of a row (a small batch): a block for a row, its threads share them.
+  // Partials of a row: 16 and more in U shares of whole rows, 16 U and more (a few pairs) in 16
+  // shares of 128 columns, fewer in one. Both kernels at D = 512, 16 heads, 8192 positions, by the last two: 1
+  // request 21.5 us for 40.8, 8 20.3 for 24.7, 16 24.4 for 26.1, 32 34.8 for 35.1, and 32 with 128
+  // heads 99.7 for 93.2; by the first two: 1 request 16.9 for 21.2 (of 16384 positions 19.5
+  // for 29.3), 4 17.3 for 18.7, 8 20.3 for 20.2, 16 25.2 for 24.2.
   const int64_t there = std::min<int64_t>(rows, Ge::ROWS), jobs = a.by_pair ? pairs : a.blocks;
-  constexpr int U = 512 / (D / 4), RM = 256 / (D / 4);
-  if (pairs * 16 <= a.blocks)
-    hipLaunchKernelGGL((mx4_merge_kernel<D, U, 512>), dim3(jobs, there), dim3(512), 0, stream, a, Ge::ROWS);
+  constexpr int RM = 256 / (D / 4), U = 512 / (D / 4);
+  if (pairs * 16 * U <= a.blocks)
+    hipLaunchKernelGGL((mx4_merge_kernel<D, 32, 16, 512>), dim3(jobs, there, D / 128), dim3(512), 0, stream, a, Ge::ROWS);
+  else if (pairs * 16 <= a.blocks)
+    hipLaunchKernelGGL((mx4_merge_kernel<D, D / 4, U, 512>), dim3(jobs, there), dim3(512), 0, stream, a, Ge::ROWS);
   else
-    hipLaunchKernelGGL((mx4_merge_kernel<D, 1, 256>), dim3(jobs, (there + RM - 1) / RM), dim3(256), 0, stream, a,
+    hipLaunchKernelGGL((mx4_merge_kernel<D, D / 4, 1, 256>), dim3(jobs, (there + RM - 1) / RM), dim3(256), 0, stream, a,
                        Ge::ROWS);
   return hipGetLastError();
 }
@@ -1010,6 +1031,8 @@ int64_t rolaq_mx4_attend_ws_bytes(int D, int num_cus) {
 hipError_t rolaq_launch_mx4_attend(const rolaq::Mx4AttendArgs& a, int D, int num_cus, hipStream_t stream) {
   using namespace rolaq;
   const int64_t rows = (int64_t)a.max_q_len * a.H;
+  // As few groups as hold a request's rows. us, of 32 x 4096 positions, for four groups' kernel:
+  // 16 rows at D = 512 24.5 / 36.3, at 256 17.5 / 22.8; 32 rows 31.7 / 39.4 and 22.4 / 25.5.
 #define ROLAQ_MX4(DD, RR)                                                    \
   if (D == DD) {                                                             \
     if (rows <= 16) return launch_paged<DD, RR, 1>(a, num_cus, stream);      \

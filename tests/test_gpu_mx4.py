@@ -310,6 +310,40 @@ def test_scores_that_outgrow_the_reference(H):
     assert lse.max().item() > 60
 
 
+@pytest.mark.parametrize("H,longest", [(16, 2), (40, 1), (4, 7)])
+def test_queries_past_the_longest_are_left_out(H, longest):
+    b = Batch(512, H, [200, 90, 300], [5, 1, 9], 64, seed=3)
+    o = torch.full((b.T, H, 512), 7.0, dtype=torch.bfloat16, device=DEV)
+    mx4.attend_fwd(b.q.to(DEV), o, b.pool, 0, b.kv_indptr, b.kv_indices, b.kv_lens, b.sm, qo_indptr=b.qo,
+                   max_q_len=longest, page_size=64)
+    o = o.cpu()
+    t = 0
+    for i, (n, m) in enumerate(zip(b.lens, b.qlens)):
+        k = min(m, longest)  # these see what they see beside the ones left out
+        want, _, w = oracle.attend(b.q[t:t + k], b.x[i], b.pe[i], [n - m + j + 1 for j in range(k)], b.sm)
+        tol = (2.0 ** -8 + 2.0 ** -10) * w + 2.0 ** -8 * want.abs()  # (scores off by far less than 2^-11)
+        assert ((o[t:t + k].double() - want).abs() <= tol).all()
+        assert (o[t + k:t + m] == 7).all()
+        t += m
+
+
+@pytest.mark.parametrize("H", [16, 48])
+def test_scores_far_below_any_mask(H):
+    """Equal rows under a query that scores each at -7e11: their mean is the row itself, exactly."""
+    b = Batch(512, H, [300, 64], [1, 1], 64, seed=3)
+    for i, s in enumerate(b.slots):
+        x = torch.full((len(s), 512), 1.0 + i)
+        x[:, 1::2] = 3.0
+        fill(b.pool, s, x, torch.zeros(len(s), 64, dtype=torch.bfloat16))
+    q = torch.full((2, H, 576), -float(1 << 20), dtype=torch.bfloat16, device=DEV)
+    o, lse = torch.empty(2, H, 512, dtype=torch.bfloat16, device=DEV), torch.empty(2, H, device=DEV)
+    mx4.attend_fwd(q, o, b.pool, 0, b.kv_indptr, b.kv_indices, b.kv_lens, 640.0, page_size=64, lse=lse)
+    for i in range(2):
+        assert (o[i, :, 0::2] == 1.0 + i).all() and (o[i, :, 1::2] == 3.0).all()
+        score = -640.0 * (1 << 20) * 256 * (4.0 + i)
+        assert torch.isfinite(lse[i]).all() and ((lse[i].double().cpu() / score - 1).abs() < 2.0 ** -20).all()
+
+
 def test_latents_of_small_and_large_magnitude():
     for spread in (1e-4, 3e3):
         b = Batch(512, 16, [400, 100], [1, 2], 16, seed=8, spread=spread)
