@@ -29,6 +29,9 @@ Pinning (what checks each function, see ``tests/test_oracle_*.py``):
 * ``attention`` -- float64 brute force on tiny inputs, exact-softmax
   invariants (split-K LSE merge equals the unsplit result, empty splits are
   neutral) and rotation invariance of the absorbed form.
+* ``mx4`` -- the 4-bit latent cache, which the reference does not have: the format's
+  levels, scale rule and packing by hand-written vectors and brute force over
+  all levels, attention in float64.
 """
 
 from . import codec, layout, window, attention  # noqa: F401

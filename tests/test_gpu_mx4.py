@@ -234,6 +234,80 @@ def test_strided_inputs_and_slots_outside_the_cache(rotated, D):
     assert torch.equal(out[ok, :D + R], mx4.read_rows(want, 0, loc)[ok])
 
 
+@pytest.mark.parametrize("D", [512, 256])
+def test_rows_back_do_not_depend_on_the_launch_size(D):
+    """Many rows and few take different kernels: the same sums, row by row, wherever the rows lie and go."""
+    D, R = dims(D)
+    n = 20001 if D == 256 else 9001
+    pool = MX4MLAPool(n + 7, 1, D, R, device=DEV, rotations=[synth.make_rotation(D, 6)])
+    g = torch.Generator().manual_seed(5)
+    loc = (torch.randperm(n + 7, generator=g)[:n] + 1).to(DEV)
+    mx4.write_rows(pool, 0, loc, synth.make_latent(n, D, 5, seed=8).to(DEV), synth.make_normal((n, R), 9).to(DEV))
+    at = loc.clone()
+    at[[0, 63, 64, 5000, n - 1]] = torch.tensor([-1, n + 8, 1 << 40, -(1 << 50), n + 8], device=DEV)
+    at[100] = at[101] = at[7000]  # (a slot more than once)
+    out = torch.full((n + 3, D + R + 24), 5.0, dtype=torch.bfloat16, device=DEV)
+    mx4.read_rows(pool, 0, at, out=out)
+    few = torch.cat([mx4.read_rows(pool, 0, at[i:i + 900]) for i in range(0, n, 900)])
+    dead = torch.zeros(n, dtype=torch.bool, device=DEV)
+    dead[[0, 63, 64, 5000, n - 1]] = True
+    assert torch.equal(out[:n][~dead, :D + R], few[~dead])
+    assert torch.isnan(out[:n][dead, :D + R]).all() and torch.isnan(few[dead]).all()
+    assert (out[n:] == 5).all() and (out[:, D + R:] == 5).all()
+    assert torch.isfinite(few[~dead]).all()
+
+
+def test_a_rotation_with_values_far_apart():
+    """Rows of R_eff whose values span more than the split's exact range: off by 2^-21 of the largest for each product."""
+    D, R, n = 512, 64, 300
+    rot = synth.make_rotation(D, 2).float()
+    rot[3] *= torch.exp2(torch.linspace(0, -40, D))
+    rot[7], rot[9] = 0, 1e-30
+    pool = MX4MLAPool(n, 1, D, R, device=DEV)
+    loc = torch.arange(1, n + 1, device=DEV)
+    mx4.write_rows(pool, 0, loc, synth.make_latent(n, D, 5, seed=8).to(DEV), synth.make_normal((n, R), 9).to(DEV))
+    v = mx4.read_rows(pool, 0, loc)[:, :D].double().cpu()
+    pool.rotations = [rot.to(DEV, torch.bfloat16)]
+    back = mx4.read_rows(pool, 0, loc)[:, :D].double().cpu()
+    r = rot.to(torch.bfloat16).double()
+    want = v @ r.t()
+    tol = 2.0 ** -8 * want.abs() + 1.01 * D * 2.0 ** -24 * (v.abs() @ r.abs().t()) \
+        + 2.0 ** -21 * v.abs().sum(-1, keepdim=True) * r.abs().amax(-1)
+    assert ((back - want).abs() <= tol).all() and (back[:, 7] == 0).all()
+
+
+def test_rows_back_captured_and_on_another_stream():
+    D, R, n = 512, 64, 5000
+    pool = MX4MLAPool(n, 1, D, R, device=DEV, rotations=[synth.make_rotation(D, 6)])
+    loc = torch.arange(1, n + 1, device=DEV)
+    pe = synth.make_normal((n, R), 9).to(DEV)
+    out = torch.empty(n, D + R, dtype=torch.bfloat16, device=DEV)
+    side = torch.cuda.Stream()
+    x = synth.make_latent(n, D, 5, seed=0).to(DEV)
+
+    def step():
+        mx4.write_rows(pool, 0, loc, x, pe)
+        mx4.read_rows(pool, 0, loc, out=out)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(3):
+        x.copy_(synth.make_latent(n, D, 5, seed=i + 1))
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        out.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        side.synchronize()
+        assert torch.equal(got, out) and got.abs().max() > 0
+
+
 def test_no_rows():
     pool = MX4MLAPool(16, 1, device=DEV)
     none = torch.zeros(0, dtype=torch.int64, device=DEV)
