@@ -654,7 +654,8 @@ int rolaq_mx4_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   if (!q || !kv_indptr || !kv_lens || !out || !workspace || (!kv_indices && n_indices > 0))
     return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
   if (n_indices < 0 || n_indices > INT32_MAX) return fail(ROLAQ_ERR_INVALID, "%s: n_indices out of range", fn);
-  if (T > (1 << 24)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries", fn);
+  if (T > (1 << 24) || T * H > (1 << 30))
+    return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries, or 2^30 query rows", fn);
   if (!qo_indptr && (max_q_len != 1 || T < B))
     return fail(ROLAQ_ERR_INVALID, "%s: without qo_indptr each request has one query (max_q_len 1, T >= B)", fn);
   // (a longer maximum than there are queries sizes the grid for nothing)

@@ -128,8 +128,8 @@ struct Mx4Geo {
   // requests with 128 heads, 512 features: 86 us, 94 without; of 64 x 16384 positions with
   // 40 heads, 256 features: 100 us, 89 without.
   static constexpr bool MIX = D == 512 && G >= 2;
-  // Halves of P that the other turn holds at a time: with four groups one, 92 us for two
-  // at the latter step's 96; with fewer both, 54.9 us for 55.8 (32 x 16384, 16 heads, 512).
+  // Halves of P that the other turn holds at a time: with four groups one, 92 us for
+  // both at the latter step's 96; with fewer both, 56.4 us for one's 57.4 (32 x 16384, 16 heads, 512).
   static constexpr int PH = G == 4 ? 1 : 2;
   // Block scales to V's exponents, not to P's: 16 additions for 32 features against 8 G. At
   // G = 1 the other way round takes 56.4 us for 55.8.

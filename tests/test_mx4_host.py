@@ -79,6 +79,7 @@ def test_attend_arguments():
     refused(fn, changed(ok, i6=0), "num_slots")
     refused(fn, changed(ok, i10=-1), "n_indices")
     refused(fn, changed(ok, i13=(1 << 24) + 1), "queries")
+    refused(fn, changed(ok, i13=1 << 24, i15=128), "query rows")
     refused(fn, changed(ok, i7=None), "qo_indptr")            # two queries each need offsets
     refused(fn, changed(ok, i7=None, i18=1, i13=3), "qo_indptr")  # fewer queries than requests
     refused(fn, changed(ok, i14=1 << 30, i13=1 << 24, i18=1 << 20), "too large")
