@@ -37,12 +37,13 @@
 // reads the whole tile's keys for its group) and what they wait for.
 //
 // Measured, kernel alone: 32 x 16384 positions, 16 heads, D = 512: 49 us (4.3 TB/s); 24 ragged
-// requests with 128 heads: 82 us (590 TFLOP/s); 64 x 16384, 40 heads, D = 256: 89 us; chunks of 4 x
+// requests with 128 heads: 71 us (690 TFLOP/s); 64 x 16384, 40 heads, D = 256: 89 us; chunks of 4 x
 // 2048 behind 14336, 40 heads, D = 256: 4.6 ms (1.18 PFLOP/s).
 //
-// Work: the tiles of all (request, row block) pairs lie on one line that is cut
-// into equal parts, a part for each block; a pair cut by a border leaves partials
-// that mx4_merge_kernel joins. With many row blocks each has a block of its own.
+// Work: the tiles of all (request, row block) pairs, each behind an allowance for its
+// start and end, lie on one line that is cut into equal parts, a part for each block;
+// a pair cut by a border leaves partials that mx4_merge_kernel joins. With many row
+// blocks each has a block of its own.
 #include "rolaq_common.h"
 #include "mx4_args.h"
 #include "mx4_tile.h"
@@ -135,6 +136,12 @@ struct Mx4Geo {
   // G = 1 the other way round takes 56.4 us for 55.8.
   static constexpr bool VSIDE = G >= 2;
   static constexpr float UNIT = VSIDE ? 0x1p-64f : 0x1p32f;  // of O
+  // A pair's start (query, first tiles) and end (output or partial) count as so many tiles
+  // where the work is cut, so that a block with two of them has fewer. us, 0 / 3 / 6 / 10: 24 ragged
+  // requests with 128 heads 86.7 / 81.2 / 76.5 / 77.1; 16 with 2 .. 4 queries 54.9 / 49.0 / 45.2 / 44.9; 400 short
+  // ones, 16 heads, 100.8 / 83.8 / 79.3 / 80.7; ragged chunks 882 / 866 / 847 / 854; D = 256, 64 ragged requests,
+  // 16 heads 29.4 / 27.0 / 25.5 / 25.8, ragged chunks 376 / 373 / 379 / 377.
+  static constexpr int PRE = 6;
   static constexpr int LOADS = (CODES + ROPE) / (1024 * W) + 1;  // a wave's copies for a tile
   // LDS offsets
   static constexpr int P = S * TILE;                        // [2][ROWS][64] bf16, 16-byte chunks swizzled
@@ -247,12 +254,13 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
   uint32_t all_units = 0, all_blocks = 0;
   Mx4Job* jobs = nullptr;
   int b = 0, rb_only = 0;
+  uint32_t pre = Ge::PRE;  // units before a pair's tiles, for its start and end
   Mx4Request rq = {};
   if (a.blocks > 0) {
     // Tiles of all requests, summed by every wave for itself (a request a lane, 256
     // requests' loads in one round trip), then the request that has the first unit.
     const auto units_of = [&](const Mx4Request& r, int i) {
-      return i < a.B ? (uint32_t)mx4_row_blocks(r, a.H, Ge::ROWS) * (uint32_t)mx4_tiles(r) : 0u;
+      return i < a.B ? (uint32_t)mx4_row_blocks(r, a.H, Ge::ROWS) * ((uint32_t)mx4_tiles(r) + pre) : 0u;
     };
     Mx4Request r4[4];
     uint32_t n4[4], at4[4], units = 0;
@@ -260,6 +268,20 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (k == 0 || c + 64 * k < a.B) r4[k] = mx4_request(a, min(c + 64 * k + lane, a.B - 1));
+      if (a.B <= 256) {
+        // pairs of one size that fill whole blocks, or blocks that fill whole pairs, stay so
+        const uint32_t rb0 = __builtin_amdgcn_readfirstlane(mx4_row_blocks(r4[0], a.H, Ge::ROWS));
+        const uint32_t nt0 = __builtin_amdgcn_readfirstlane(mx4_tiles(r4[0]));
+        uint64_t other = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k == 0 || 64 * k < a.B)
+            other |= __builtin_amdgcn_ballot_w64(64 * k + lane < a.B &&
+                                                 ((uint32_t)mx4_row_blocks(r4[k], a.H, Ge::ROWS) != rb0 ||
+                                                  (uint32_t)mx4_tiles(r4[k]) != nt0));
+        const uint32_t pairs = a.B * rb0, n = min((uint32_t)a.blocks, pairs * nt0);
+        if (other == 0 && pairs > 0 && (n % pairs == 0 || pairs % n == 0)) pre = 0;
+      }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         n4[k] = at4[k] = 0;
@@ -337,27 +359,29 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     // ---- the next segment: tiles [t0, t1) of a row block of request b ---------------
     int rb, t0, t1, ntiles = mx4_tiles(rq);
     if (shared) {
-      const uint32_t done = u - u_req;
-      rb = done / ntiles;
+      const uint32_t done = u - u_req, span = ntiles + pre;
+      rb = done / span;
       if (rb >= mx4_row_blocks(rq, a.H, Ge::ROWS)) {  // on to the next request (one without queries has no units)
         if (++b >= a.B) break;
         u_req = u;
         rq = mx4_request(a, b);
         continue;
       }
-      t0 = done - rb * ntiles;
+      const uint32_t at = done - rb * span, n = min(span - at, u_end - u), u0 = u - at + pre;  // u0: its first tile
+      u += n;
+      t0 = max((int)(at - pre), 0);
+      t1 = (int)(at + n - pre);
+      if (t1 <= 0) continue;  // its tiles begin in the next block
       // The merge's job for this pair: by the block that begins it, or (by block) by the
       // one that takes it over from there.
       if (tid == 0 && (a.by_pair ? t0 == 0 : nth == 0)) {
-        const uint32_t u0 = u - t0, j1 = mx4_block_of(u0 + ntiles - 1, all_units, all_blocks);
+        const uint32_t j1 = mx4_block_of(u0 + ntiles - 1, all_units, all_blocks);
         const uint32_t j0 = a.by_pair ? (uint32_t)a.blocks : mx4_block_of(u0, all_units, all_blocks);
         const bool cut = a.by_pair ? j1 > j0 : t0 > 0 && (int)j0 + 1 == a.blocks;
         jobs[a.by_pair ? b * a.row_blocks + rb : a.blocks] =
-            Mx4Job{cut ? (int)(j1 - j0 + 1) : 0, (int)j0, mx4_first_unit(all_units, j0, all_blocks) < u0, rb * Ge::ROWS,
+            Mx4Job{cut ? (int)(j1 - j0 + 1) : 0, (int)j0, mx4_first_unit(all_units, j0, all_blocks) < u0 - pre, rb * Ge::ROWS,
                    rq.nq * a.H, rq.q0, {0, 0}};
       }
-      t1 = (int)min((uint32_t)ntiles, t0 + (u_end - u));
-      u += t1 - t0;
     } else {
       u = u_end;
       rb = rb_only;
@@ -892,6 +916,7 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     }
     ++nth;
   }
+  if (shared && !a.by_pair && nth == 0 && tid == 0) jobs[a.blocks].parts = 0;
 }
 
 // Joins the partials of the pairs that were cut: a block for a job, 4 C columns and
@@ -982,7 +1007,7 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   // length, D = 512, 4 row blocks a CU 577 / 523, 8 1141 / 1040; D = 256, 9 a CU, ragged 850 / 905, of one
   // length 670 / 583.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
-  const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + a.B;
+  const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + (int64_t)(1 + Ge::PRE) * a.B;
   const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
   const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);

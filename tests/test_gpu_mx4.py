@@ -384,6 +384,29 @@ def test_scores_that_outgrow_the_reference(H):
     assert lse.max().item() > 60
 
 
+def test_a_few_requests_with_queries_among_many_without():
+    """Blocks whose part of the work holds no tile, and what an earlier call left in the workspace."""
+    before = Batch(512, 40, [5000, 3, 2600, 70] * 9, [1, 30, 2, 9] * 9, 64, seed=6)
+    lens, qlens = [60 + 7 * i for i in range(302)], [20] + [0] * 300 + [3]
+    b = Batch(512, 40, lens, qlens, 64, seed=5)
+    ws = torch.empty(kernels.mx4_attend_workspace_bytes(512, DEV), dtype=torch.uint8, device=DEV)
+    before.run(workspace=ws)
+    lse = torch.empty(b.T, 40, device=DEV)
+    o = b.run(workspace=ws, lse=lse)
+    b.check(o, lse, requests=[0, 301])
+    assert torch.equal(o, b.run(workspace=torch.zeros_like(ws)))
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 8, 64, 256, 300])
+@pytest.mark.parametrize("D,H", [(512, 16), (256, 40)])
+def test_requests_of_one_length(D, H, n):
+    """Pairs that fill whole blocks, blocks that fill whole pairs, and neither."""
+    for tiles in (1, 4, 5):
+        b = Batch(D, H, [64 * tiles - 3] * n, [1] * n, 64, seed=n + tiles)
+        some = range(0, n, max(1, n // 16))
+        b.check(b.run(decode=True), requests=some)
+
+
 @pytest.mark.parametrize("H,longest", [(16, 2), (40, 1), (4, 7)])
 def test_queries_past_the_longest_are_left_out(H, longest):
     b = Batch(512, H, [200, 90, 300], [5, 1, 9], 64, seed=3)
