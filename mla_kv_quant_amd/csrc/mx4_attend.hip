@@ -327,10 +327,12 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       }
     }
   } else {
-    // a block for each (row block, request), the later row blocks of a request,
-    // which see most positions, first
-    b = blockIdx.x % a.B;
-    rb_only = a.row_blocks - 1 - blockIdx.x / a.B;
+    // a block for each (request, row block), the later row blocks of a request,
+    // which see most positions, first; request by request, so that each is
+    // spread over the XCDs (blocks go round them in turn; requests in turn, in a multiple
+    // of 8, would each lie on one: 32 ragged chunks, 40 heads, D = 256 8.9 ms for 3.9)
+    b = blockIdx.x / a.row_blocks;
+    rb_only = a.row_blocks - 1 - blockIdx.x % a.row_blocks;
     rq = mx4_request(a, b);
   }
   const bool shared = a.ws != nullptr;
@@ -1003,9 +1005,8 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   // Shared out while there are few row blocks for each CU; past that, with more
   // requests than a block's sums hold, or with more tiles than 32 bits count, each row
   // block has a block. us, shared out / a block each: decode 32 x 4096 with 16 heads 24.5 / 78.7;
-  // ragged chunks with 6 row blocks a CU, D = 512: 873 to 1106 / 1109 to 1301; chunks of one
-  // length, D = 512, 4 row blocks a CU 577 / 523, 8 1141 / 1040; D = 256, 9 a CU, ragged 850 / 905, of one
-  // length 670 / 583.
+  // ragged chunks, D = 512, 5 row blocks a CU 742 / 854 and 1014 / 974, 7 a CU 1252 / 1232 and 1090 / 1115; D = 256,
+  // 15 a CU 1549 / 1387; chunks of one length, 2 a CU 292 / 283, 16 a CU 2271 / 2064.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
   const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + (int64_t)(1 + Ge::PRE) * a.B;
   const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
