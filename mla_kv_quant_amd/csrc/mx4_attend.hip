@@ -362,14 +362,16 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     int rb, t0, t1, ntiles = mx4_tiles(rq);
     if (shared) {
       const uint32_t done = u - u_req, span = ntiles + pre;
-      rb = done / span;
-      if (rb >= mx4_row_blocks(rq, a.H, Ge::ROWS)) {  // on to the next request (one without queries has no units)
+      const int nrb = mx4_row_blocks(rq, a.H, Ge::ROWS), i = done / span;
+      if (i >= nrb) {  // on to the next request (one without queries has no units)
         if (++b >= a.B) break;
         u_req = u;
         rq = mx4_request(a, b);
         continue;
       }
-      const uint32_t at = done - rb * span, n = min(span - at, u_end - u), u0 = u - at + pre;  // u0: its first tile
+      // first and last row blocks in turns: the later ones see more positions
+      rb = i & 1 ? nrb - 1 - (i >> 1) : i >> 1;
+      const uint32_t at = done - i * span, n = min(span - at, u_end - u), u0 = u - at + pre;  // u0: its first tile
       u += n;
       t0 = max((int)(at - pre), 0);
       t1 = (int)(at + n - pre);
@@ -1002,14 +1004,15 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_q_len * a.H;
   a.row_blocks = (int)((rows + Ge::ROWS - 1) / Ge::ROWS);
   a.h_inv = (65536 + a.H - 1) / a.H;
-  // Shared out while there are few row blocks for each CU; past that, with more
-  // requests than a block's sums hold, or with more tiles than 32 bits count, each row
-  // block has a block. us, shared out / a block each: decode 32 x 4096 with 16 heads 24.5 / 78.7;
-  // ragged chunks, D = 512, 5 row blocks a CU 742 / 854 and 1014 / 974, 7 a CU 1252 / 1232 and 1090 / 1115; D = 256,
-  // 15 a CU 1549 / 1387; chunks of one length, 2 a CU 292 / 283, 16 a CU 2271 / 2064.
+  // Shared out, but for more requests than a block's sums hold, more tiles than 32 bits
+  // count, and, where two blocks run on a CU, more than 6 row blocks for each CU: those
+  // have a block each. us, shared out / a block each: decode 32 x 4096 with 16 heads, D = 512, 24.5 / 78.7;
+  // chunks of one length, D = 512, 2 row blocks a CU 279 / 284, 8 1027 / 1040, 16 2035 / 2066; ragged ones, 5 a CU
+  // 732 / 852, 18 2754 / 2784; 400 requests of 1 .. 8 queries, 128 heads 1377 / 2358; D = 256, ragged chunks, 3 a CU 442
+  // / 480, 5 389 / 347 and 222 / 288, 8 512 / 577 and 869 / 769, 15 1185 / 1116; of one length, 5 352 / 333, 20 4993 / 4661.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
   const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + (int64_t)(1 + Ge::PRE) * a.B;
-  const bool shared = a.B <= kMx4Requests && items <= 6 * (int64_t)num_cus && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
+  const bool shared = a.B <= kMx4Requests && (Ge::OCC == 1 || items <= 6 * (int64_t)num_cus) && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
   const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);
   if (e != hipSuccess) return e;

@@ -384,6 +384,13 @@ def test_scores_that_outgrow_the_reference(H):
     assert lse.max().item() > 60
 
 
+@pytest.mark.parametrize("H,qlens", [(16, [1] * 1100), (40, [1 + i % 3 for i in range(1100)])])
+def test_many_requests_of_the_large_width(H, qlens):
+    lens = [(41 * i) % 200 for i in range(1100)]
+    b = Batch(512, H, lens, qlens, 32, seed=4)
+    b.check(b.run(), requests=range(0, 1100, 37))
+
+
 def test_a_few_requests_with_queries_among_many_without():
     """Blocks whose part of the work holds no tile, and what an earlier call left in the workspace."""
     before = Batch(512, 40, [5000, 3, 2600, 70] * 9, [1, 30, 2, 9] * 9, 64, seed=6)
