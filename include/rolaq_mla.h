@@ -333,8 +333,9 @@ int rolaq_mx4_write_rows(const void* latent, int64_t latent_stride, const void* 
 /*
  * Row i of out (bf16, stride out_stride) = [latent | rope] of slot slots[i]; with
  * rotation (R_eff, bf16 [D, D] row-major) the latent is multiplied by R_eff^T in
- * FP32 and rounded to bf16, without it the stored values are returned exactly. A
- * slot outside the cache reads as NaN.
+ * FP32 and rounded to bf16 (values of R_eff below 2^-13 of the largest in their row
+ * enter to 2^-21 of it, larger ones exactly; a row with a NaN block is NaN), without
+ * it the stored values are returned exactly. A slot outside the cache reads as NaN.
  */
 int rolaq_mx4_read_rows(const int64_t* slots, int64_t n, const uint8_t* codes, const uint8_t* scales,
                         const void* rope_buf, int64_t num_slots, const void* rotation, int D, int R, void* out,
@@ -351,7 +352,7 @@ int rolaq_mx4_attend_workspace(int D, int64_t* bytes);
  * sees positions 0 .. kv_lens[b] - n + i. Position t lies in slot
  * kv_indices[kv_indptr[b] + t / page_size] * page_size + t % page_size.
  *   s_t = sm_scale (q_lat . x_t + q_rope . rope_t),  out = softmax(s) x,
- * x_t the stored latent row. out: bf16 [T, H, D], in the frame of the cached rows; lse
+ * x_t the stored latent row (q_lat enters as R_eff does above). out: bf16 [T, H, D], in the frame of the cached rows; lse
  * (or null): FP32 [T, H], the natural log of the sum of exp(s). A query that
  * sees no position gets 0 and -inf; queries past qo_indptr[B], and past max_q_len
  * of a request, are left as they were. A length that its page list does not
