@@ -131,9 +131,12 @@ __global__ __launch_bounds__(64 * WV) void mx4_unrotate_kernel(Mx4RowsArgs a, in
     }
   };
   auto turn = [&](int k, auto first) __attribute__((always_inline)) {
-    // tile k is in, and all reads of the other buffer are done; the last turn's
-    // stores, all of them issued (only a part's last tile can end early) and
-    // the newest, may be on their way
+    // Tile k is in, and all reads of the other buffer are done. In flight here, the oldest
+    // first, are tile k's copies (two or one of codes, one of scales), its rope if it is
+    // stored here, the next slots; and behind them, from a block's third turn on, the
+    // stores of the turn before, all STORES of them (only a part's last tile can
+    // end early): these may go on. The first two turns have none behind their copies: the
+    // first waits for everything here, the second where the loop begins.
     wait_loads<first ? 0 : STORES>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -169,6 +172,7 @@ __global__ __launch_bounds__(64 * WV) void mx4_unrotate_kernel(Mx4RowsArgs a, in
     }
   };
   turn(k0, std::true_type{});
+  wait_loads<0>();  // (tile k0 + 1's copies, with no stores behind them to count)
 #pragma unroll 1
   for (int k = k0 + 1; k < k1; ++k) turn(k, std::false_type{});
   store(k1 - 1, true);
