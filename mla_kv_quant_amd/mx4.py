@@ -10,8 +10,9 @@ rotated frame (``artifacts.fold_read_rotation``).
 
 Every call launches on the current stream of its tensors' device, allocates
 nothing but an output that was not given (and the attention's workspace, once
-for a pool) and makes no synchronisation, so it can be captured in a HIP graph.
-The reference has no 4-bit cache.
+for a pool) and makes no synchronisation, so it can be captured in a HIP graph;
+the one exception is a write that finds its layer's rotation new or changed
+(``write_rows``). The reference has no 4-bit cache.
 """
 
 from __future__ import annotations
@@ -19,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import kernels
-from .writer import SUPPORTED_DIMS, _as_int64, _rows, _write_rotation
+from .writer import SUPPORTED_DIMS, _as_int64, _rows
 
 
 class MX4MLAPool:
@@ -72,6 +73,50 @@ def attend_workspace(pool) -> torch.Tensor:
     return ws
 
 
+def _rotation_t(pool, layer_id):
+    """bf16 R_eff^T of a layer as the writer takes it (None: no rotation).
+
+    Kept for the pool with the tensor that it was laid out from, and laid out again,
+    in the same buffer, when that is another tensor or torch has counted a change of
+    it. Any stream may use what is kept: the layout waits for all that may still
+    read the buffer, and is complete when this returns. During a capture, where nothing can be
+    waited for, and for tensors that count no changes it is part of the call instead.
+    """
+    r = pool.latent_rotation(layer_id, local=True)
+    if r is None:
+        return None
+    kept = getattr(pool, "_mx4_rotations_t", None)
+    if kept is None:
+        kept = pool._mx4_rotations_t = {}
+    entry = kept.get(layer_id)
+    try:
+        version = r._version
+    except RuntimeError:  # an inference tensor
+        version = None
+    if entry is not None and entry[0] is r and entry[1] == version and version is not None:
+        return entry[2]
+    if r.is_cuda:
+        with torch.cuda.device(r.device):
+            if version is None or torch.cuda.is_current_stream_capturing():
+                return r.to(torch.bfloat16).t().contiguous()
+            torch.cuda.synchronize()
+            rt = _lay_out(r, entry)
+            torch.cuda.current_stream().synchronize()
+    elif version is None:
+        return r.to(torch.bfloat16).t().contiguous()
+    else:
+        rt = _lay_out(r, entry)
+    kept[layer_id] = (r, version, rt)
+    return rt
+
+
+def _lay_out(r, entry):
+    t = r.to(torch.bfloat16).t()
+    if entry is None or entry[2].device != t.device or entry[2].shape != t.shape:
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return entry[2].copy_(t)
+
+
 def write_rows(pool, layer_id, loc, c_kv, k_pe) -> None:
     """Store rows of layer ``layer_id`` at slots ``loc``: a decode step's or a prefill chunk's.
 
@@ -79,9 +124,16 @@ def write_rows(pool, layer_id, loc, c_kv, k_pe) -> None:
     ``n * D`` elements), ``k_pe``: bf16 rope keys. One launch rotates (on a
     layer with a rotation), quantizes, packs and stores. Slots of one call must
     differ, except for the padding slot; one outside the cache is skipped.
+
+    The kernel reads ``R_eff^T``, which the first write of a layer lays out and the pool
+    keeps. The first write after the rotation has changed (another tensor, or the
+    same one changed by a torch operation on it; a change through ``.data`` is not
+    seen) lays it out again and, like the first, waits for the device; calls
+    captured before follow from there on. A write that is captured before its layer has been laid
+    out does it in the graph at each replay.
     """
     li = layer_id - pool.start_layer
-    rt = _write_rotation(pool, layer_id, pool.latent_rotation(layer_id, local=True))
+    rt = _rotation_t(pool, layer_id)
     kernels.mx4_write_rows(_rows(c_kv, pool.kv_lora_rank), _rows(k_pe, pool.qk_rope_head_dim), rt, _as_int64(loc),
                            pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li])
 

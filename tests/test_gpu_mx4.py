@@ -591,3 +591,72 @@ def test_prefill_then_decode_as_a_server_does():
             off = (o[t:t + m[i]].double().cpu() - want).abs()
             assert (off <= (2.0 ** -8 + 2.0 ** -10) * w + 2.0 ** -8 * want.abs()).all()
             t += m[i]
+
+
+# ---- a layer's rotation, as it is when a row is written ---------------------------------
+def written_codes(rot, x, pe, loc):
+    """Cached rows of a pool that has never had another rotation."""
+    pool = MX4MLAPool(loc.numel() + 8, 1, x.shape[1], pe.shape[1], device=DEV, rotations=[rot])
+    mx4.write_rows(pool, 0, loc, x, pe)
+    return pool.c_codes[0], pool.c_scales[0]
+
+
+@pytest.mark.parametrize("D", [512, 256])
+def test_rows_take_the_rotation_as_it_is(D):
+    D, R = dims(D)
+    n = 70
+    loc = torch.arange(1, n + 1, device=DEV)
+    x, pe = synth.make_latent(n, D, 5, seed=1).to(DEV), synth.make_normal((n, R), 2).to(DEV)
+    rots = [synth.make_rotation(D, s).to(DEV, torch.bfloat16) for s in range(4)]
+    want = [written_codes(r.clone(), x, pe, loc) for r in rots]
+    pool = MX4MLAPool(n + 8, 1, D, R, device=DEV, rotations=[rots[0].clone()])
+
+    def check(i):
+        assert torch.equal(pool.c_codes[0], want[i][0]) and torch.equal(pool.c_scales[0], want[i][1])
+
+    mx4.write_rows(pool, 0, loc, x, pe)
+    check(0)
+    pool.rotations[0].copy_(rots[1])  # in place
+    mx4.write_rows(pool, 0, loc, x, pe)
+    check(1)
+    pool.rotations[0] = rots[2].clone()  # another tensor
+    mx4.write_rows(pool, 0, loc, x, pe)
+    check(2)
+    # a first write (after a change) on one stream, the next at once on another
+    side = torch.cuda.Stream()
+    pool.rotations[0].copy_(rots[3])
+    torch.cuda.synchronize()
+    mx4.write_rows(pool, 0, loc[:1], x[:1], pe[:1])
+    with torch.cuda.stream(side):
+        mx4.write_rows(pool, 0, loc, x, pe)
+    torch.cuda.synchronize()
+    check(3)
+
+
+@pytest.mark.parametrize("warm", [False, True])
+def test_captured_writes_and_a_rotation_that_changes(warm):
+    """A write whose layer has not been laid out yet when it is captured, and one whose has."""
+    D, R, n = 256, 32, 30
+    loc = torch.arange(1, n + 1, device=DEV)
+    x, pe = synth.make_latent(n, D, 5, seed=1).to(DEV), synth.make_normal((n, R), 2).to(DEV)
+    rots = [synth.make_rotation(D, s).to(DEV, torch.bfloat16) for s in range(2)]
+    want = [written_codes(r.clone(), x, pe, loc) for r in rots]
+    pool = MX4MLAPool(n + 8, 1, D, R, device=DEV, rotations=[rots[0].clone()])
+    mx4.write_rows(MX4MLAPool(n, 1, D, R, device=DEV, rotations=[rots[1]]), 0, loc, x, pe)
+    if warm:
+        mx4.write_rows(pool, 0, loc, x, pe)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mx4.write_rows(pool, 0, loc, x, pe)
+    for i in (0, 0, 1, 1, 0):
+        pool.rotations[0].copy_(rots[i])
+        if warm:  # (captured calls follow with the next call outside a capture)
+            mx4.write_rows(pool, 0, loc, x, pe)
+        pool.c_codes[0].zero_()
+        pool.c_scales[0].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(pool.c_codes[0], want[i][0]) and torch.equal(pool.c_scales[0], want[i][1])
+        mx4.write_rows(pool, 0, loc, x, pe)
+        assert torch.equal(pool.c_codes[0], want[i][0])

@@ -150,3 +150,61 @@ def test_attend_tensors():
                dict(qo_indptr=torch.zeros(0, dtype=torch.int32))):
         with pytest.raises(ValueError):
             call(**kw)
+
+
+# ---- the rotation that a write takes: the layer's as it is now ------------------------
+def written(monkeypatch, pool, layer=0):
+    """R_eff^T that a write of one row hands to the kernel."""
+    got = []
+    monkeypatch.setattr(mx4.kernels, "mx4_write_rows", lambda x, pe, rt, *rest: got.append(rt))
+    D, R = pool.kv_lora_rank, pool.qk_rope_head_dim
+    mx4.write_rows(pool, layer, torch.ones(1, dtype=torch.int64), torch.zeros(1, D, dtype=BF), torch.zeros(1, R, dtype=BF))
+    return got[0]
+
+
+def rotation(seed):
+    return torch.randn(256, 256, generator=torch.Generator().manual_seed(seed))
+
+
+def laid_out(r):
+    return r.to(BF).t().contiguous()
+
+
+def test_a_rotation_that_changes_is_laid_out_again(monkeypatch):
+    pool = MX4MLAPool(32, 2, 256, 32, device="cpu", rotations=[rotation(1), rotation(2)], start_layer=3)
+    first = written(monkeypatch, pool, 3)
+    assert torch.equal(first, laid_out(rotation(1))) and written(monkeypatch, pool, 3) is first  # laid out once
+    assert torch.equal(written(monkeypatch, pool, 4), laid_out(rotation(2)))
+    # weights loaded into the tensor that is there
+    pool.rotations[0].copy_(rotation(3))
+    assert torch.equal(written(monkeypatch, pool, 3), laid_out(rotation(3)))
+    # another tensor in its place, and what it replaces gone (another may get its id)
+    for seed in range(4, 12):
+        pool.rotations[0] = rotation(seed).to(BF)
+        assert torch.equal(written(monkeypatch, pool, 3), laid_out(rotation(seed)))
+    # all of this in one buffer, which captured calls hold
+    assert written(monkeypatch, pool, 3) is first
+    # none, and one again
+    pool.rotations[0] = None
+    assert written(monkeypatch, pool, 3) is None
+    pool.rotations[0] = rotation(12)
+    assert torch.equal(written(monkeypatch, pool, 3), laid_out(rotation(12)))
+    assert torch.equal(written(monkeypatch, pool, 4), laid_out(rotation(2)))
+
+
+def test_a_pool_that_builds_its_rotation_at_each_call(monkeypatch):
+    pool = MX4MLAPool(32, 1, 256, 32, device="cpu")
+    seeds = iter(range(20))
+    pool.latent_rotation = lambda layer_id, local=True: rotation(next(seeds))
+    for seed in range(20):
+        assert torch.equal(written(monkeypatch, pool), laid_out(rotation(seed)))
+
+
+def test_a_rotation_without_a_version(monkeypatch):
+    """Inference tensors do not count their changes: laid out at each call."""
+    with torch.inference_mode():
+        r = rotation(1).to(BF)
+        pool = MX4MLAPool(32, 1, 256, 32, device="cpu", rotations=[r])
+        assert torch.equal(written(monkeypatch, pool), laid_out(rotation(1)))
+        r.copy_(rotation(2))
+        assert torch.equal(written(monkeypatch, pool), laid_out(rotation(2)))
