@@ -217,15 +217,12 @@ __device__ __forceinline__ void store_row(const WriterArgs& a, Acc acc, int64_t 
 template <int D, typename Acc>
 __device__ __forceinline__ void store_row_mx4(const WriterArgs& a, Acc acc, int64_t row, int64_t sl, u32x2 pe, int g,
                                               int gq, int gr) {
-  float big = 0.f;
+  uint32_t big = 0;  // largest magnitude, as bits: NaN lies above infinity, wherever in the block it is
 #pragma unroll
   for (int mb = 0; mb < 8; ++mb)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) big = fmaxf(big, fabsf(acc(mb)[i]));
-  // (a row with a value that is not finite rotates to rows of NaN and infinities,
-  // and the maximum of nothing but NaN is 0 here: the sum tells)
-  const float any = acc(0)[0] - acc(0)[0];
-  const uint32_t s = mx4_scale(any == any ? __float_as_uint(big) : 0x7fc00000u);
+    for (int i = 0; i < 4; ++i) big = max(big, __float_as_uint(acc(mb)[i]) & 0x7fffffffu);
+  const uint32_t s = mx4_scale(big);
   const float f = mx4_pow2(s);
   if (row < a.n && sl >= 0 && sl < a.num_slots) {
     *reinterpret_cast<u32x4*>(a.codes + sl * (D / 2) + 16 * (4 * g + gq)) =

@@ -660,3 +660,24 @@ def test_captured_writes_and_a_rotation_that_changes(warm):
         assert torch.equal(pool.c_codes[0], want[i][0]) and torch.equal(pool.c_scales[0], want[i][1])
         mx4.write_rows(pool, 0, loc, x, pe)
         assert torch.equal(pool.c_codes[0], want[i][0])
+
+
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("n", [5, 9000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_one_value_of_a_rotated_block_that_is_not_finite(D, n, bad):
+    """Any column of a block, each in blocks of its own: R_eff is not finite there, the rest of the row is."""
+    D, R = dims(D)
+    rot = synth.make_rotation(D, 4)
+    loc = torch.arange(1, n + 1, device=DEV)
+    x, pe = synth.make_latent(n, D, 5, seed=1).to(DEV), synth.make_normal((n, R), 2).to(DEV)
+    x[x == 0] = 1.0  # (so that the products with infinities are infinities)
+    clean_codes, clean_scales = written_codes(rot.to(DEV), x, pe, loc)
+    for first in range(0, 32, 8):  # columns first .. first + 7 of the blocks 0 .. 7
+        at = [32 * i + first + i for i in range(8)]
+        r = rot.clone()
+        r[0, at] = bad
+        codes, scales = written_codes(r.to(DEV), x, pe, loc)
+        assert (scales[loc][:, :8] == 255).all(), first
+        assert torch.equal(scales[loc][:, 8:], clean_scales[loc][:, 8:])
+        assert torch.equal(codes[loc][:, 128:], clean_codes[loc][:, 128:])
