@@ -10,7 +10,7 @@ rotated frame (``artifacts.fold_read_rotation``).
 
 Every call launches on the current stream of its tensors' device, allocates
 nothing but an output that was not given (and the attention's workspace, once
-for a pool) and makes no synchronisation, so it can be captured in a HIP graph;
+for a stream) and makes no synchronisation, so it can be captured in a HIP graph;
 the one exception is a write that finds its layer's rotation new or changed
 (``write_rows``). The reference has no 4-bit cache.
 """
@@ -62,14 +62,28 @@ class MX4MLAPool:
 
 
 def attend_workspace(pool) -> torch.Tensor:
-    """The attention's workspace of ``pool``, allocated once (67 MB at width 512):
-    every layer and batch uses it. Calls that may overlap on the GPU (two streams,
-    two graphs replayed side by side) need one each, passed as ``workspace``."""
-    ws = getattr(pool, "_mx4_workspace", None)
+    """The attention's workspace of ``pool`` for calls on the current stream (67 MB at width 512).
+
+    One for each stream, allocated by its first call and used by every layer and batch
+    on it: calls of two streams may overlap. During a capture it is a new tensor
+    of the graph's memory, so graphs that do not share their memory may be replayed
+    side by side, and beside other calls.
+    """
+    like = pool.c_codes[0]
+    if like.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(like.device):
+            return attend_workspace(pool)
+    kept = getattr(pool, "_mx4_workspaces", None)
+    if kept is None:
+        kept = pool._mx4_workspaces = {}
+    capturing = torch.cuda.is_current_stream_capturing()
+    stream = kernels._stream(like)
+    ws = None if capturing else kept.get(stream)
     if ws is None:
-        dev = pool.c_codes[0].device
-        ws = torch.empty(kernels.mx4_attend_workspace_bytes(pool.kv_lora_rank, dev), dtype=torch.uint8, device=dev)
-        pool._mx4_workspace = ws
+        n = kernels.mx4_attend_workspace_bytes(pool.kv_lora_rank, like.device)
+        ws = torch.empty(n, dtype=torch.uint8, device=like.device)
+        if not capturing:
+            kept[stream] = ws
     return ws
 
 
@@ -168,7 +182,8 @@ def attend_fwd(q, o, pool, layer_id, kv_indptr, kv_indices, kv_lens, sm_scale, q
     ``kv_lens[b] - n + i``. ``max_q_len``: the most queries of a request (later
     ones are left out). ``lse``: FP32 ``[T, H]``, receives the natural log of the
     sum of exponentials. A query that sees nothing gets 0 (and -inf).
-    ``workspace``: of ``attend_workspace``'s size, the pool's own if not given.
+    ``workspace``: a tensor of ``attend_workspace``'s size that no call uses at the same
+    time; that function's if not given.
     """
     li = layer_id - pool.start_layer
     return kernels.mx4_attend_fwd(q, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], qo_indptr, kv_indptr,

@@ -681,3 +681,85 @@ def test_one_value_of_a_rotated_block_that_is_not_finite(D, n, bad):
         assert (scales[loc][:, :8] == 255).all(), first
         assert torch.equal(scales[loc][:, 8:], clean_scales[loc][:, 8:])
         assert torch.equal(codes[loc][:, 128:], clean_codes[loc][:, 128:])
+
+
+# ---- the attention's workspace: calls that overlap do not meet in it -----------------------
+def test_streams_and_captures_have_workspaces_of_their_own():
+    pool = MX4MLAPool(64, 1, 256, 32, device=DEV)
+    size = kernels.mx4_attend_workspace_bytes(256, DEV)
+    here = mx4.attend_workspace(pool)
+    assert here.numel() == size and mx4.attend_workspace(pool) is here
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        there = mx4.attend_workspace(pool)
+        assert there.data_ptr() != here.data_ptr() and mx4.attend_workspace(pool) is there
+    captured, graphs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):  # (a stream that has one already)
+            ws = mx4.attend_workspace(pool)
+            ws[:8].zero_()
+            captured.append(ws.data_ptr())
+        graphs.append(graph)
+        del ws
+    assert len({here.data_ptr(), there.data_ptr(), *captured}) == 4
+    assert mx4.attend_workspace(pool) is here
+    with torch.cuda.stream(side):
+        assert mx4.attend_workspace(pool) is there
+
+
+def two_batches():
+    """A prefill and a decode batch over one pool, whose pairs are cut into many parts."""
+    a = Batch(512, 40, [3000, 2500, 700], [300, 200, 90], 64, seed=21)
+    b = Batch(512, 16, [9000, 4000], [1, 1], 64, seed=22)
+    for name in ("c_codes", "c_scales", "rope_buf"):  # one pool: b's slots behind a's
+        rows = getattr(a.pool, name)[0].shape[0]
+        both = torch.cat((getattr(a.pool, name)[0], getattr(b.pool, name)[0]))
+        getattr(a.pool, name)[0] = both
+    b.kv_indices = b.kv_indices + rows // 64
+    assert rows % 64 == 0
+    b.pool = a.pool
+    return a, b
+
+
+def test_calls_on_two_streams_overlap():
+    a, b = two_batches()
+    want_a, want_b = a.run(), b.run()
+    qa, qb = a.q.to(DEV), b.q.to(DEV)
+    out_a = [torch.empty_like(want_a) for _ in range(12)]
+    out_b = [torch.empty_like(want_b) for _ in range(60)]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for i in range(12):
+        with torch.cuda.stream(streams[0]):
+            a.run(q=qa, o=out_a[i])
+        with torch.cuda.stream(streams[1]):
+            for o in out_b[5 * i:5 * i + 5]:
+                b.run(q=qb, o=o)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want_a) for o in out_a) and all(torch.equal(o, want_b) for o in out_b)
+
+
+def test_graphs_replayed_side_by_side():
+    a, b = two_batches()
+    want_a, want_b = a.run(), b.run()
+    qa, qb = a.q.to(DEV), b.q.to(DEV)
+    outs = [torch.empty_like(want_a), torch.empty_like(want_b), torch.empty_like(want_b)]
+    graphs, streams = [], [torch.cuda.Stream() for _ in outs]
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(4):
+                a.run(q=qa, o=outs[0]) if i == 0 else b.run(q=qb, o=outs[1])
+        graphs.append(graph)
+    for _ in range(4):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        with torch.cuda.stream(streams[2]):
+            b.run(q=qb, o=outs[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want_a) and torch.equal(outs[1], want_b) and torch.equal(outs[2], want_b)
