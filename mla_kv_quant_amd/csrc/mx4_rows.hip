@@ -5,9 +5,21 @@
 // rotated layers are written by writer_kernel and read by mx4_unrotate_kernel.
 #include "mx4_codec.h"
 
+#include <algorithm>
+
 namespace rolaq {
 
 constexpr int kMx4RowThreads = 256;
+
+// A launch's blocks lie in two dimensions: one holds less than 2^32 threads, which
+// 2^31 rows of up to 72 pass.
+__device__ __forceinline__ int64_t mx4_row_thread() {
+  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kMx4RowThreads + threadIdx.x;
+}
+dim3 mx4_row_grid(int64_t threads) {
+  const int64_t blocks = (threads + kMx4RowThreads - 1) / kMx4RowThreads, x = std::min<int64_t>(blocks, 1 << 23);
+  return dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
 
 // A thread takes eight latent values (16 bytes in, a dword of codes out): four
 // lanes make a block of 32, whose largest magnitude is a quad maximum on integer
@@ -16,7 +28,7 @@ constexpr int kMx4RowThreads = 256;
 template <int D, int R>
 __global__ __launch_bounds__(kMx4RowThreads) void mx4_write_kernel(Mx4RowsArgs a, int pe_vec) {
   constexpr int LAT = D / 8, PER = LAT + R / 8;  // threads of a row
-  const int64_t i = (int64_t)blockIdx.x * kMx4RowThreads + threadIdx.x;
+  const int64_t i = mx4_row_thread();
   const int64_t nlat = a.n * LAT;
   // all latent pieces first, so that the lanes of a block lie together
   const bool lat = i < nlat;
@@ -68,7 +80,7 @@ __global__ __launch_bounds__(kMx4RowThreads) void mx4_write_kernel(Mx4RowsArgs a
 template <int D, int R>
 __global__ __launch_bounds__(kMx4RowThreads) void mx4_read_kernel(Mx4RowsArgs a) {
   constexpr int PER = (D + R) / 8;
-  const int64_t i = (int64_t)blockIdx.x * kMx4RowThreads + threadIdx.x;
+  const int64_t i = mx4_row_thread();
   const int64_t row = i / PER;
   const int c = (int)(i % PER);
   if (row >= a.n) return;
@@ -89,8 +101,7 @@ __global__ __launch_bounds__(kMx4RowThreads) void mx4_read_kernel(Mx4RowsArgs a)
 hipError_t rolaq_launch_mx4_write_plain(const rolaq::Mx4RowsArgs& a, int D, hipStream_t stream) {
   using namespace rolaq;
   const int R = D / 8;
-  const int64_t threads = a.n * ((D + R) / 8);
-  const dim3 grid((unsigned)((threads + kMx4RowThreads - 1) / kMx4RowThreads)), block(kMx4RowThreads);
+  const dim3 grid = mx4_row_grid(a.n * ((D + R) / 8)), block(kMx4RowThreads);
   const int pe_vec = a.pe_s1 == 1 && a.pe_s0 % 8 == 0 && reinterpret_cast<uintptr_t>(a.k_pe) % 16 == 0;
   if (D == 512)
     hipLaunchKernelGGL((mx4_write_kernel<512, 64>), grid, block, 0, stream, a, pe_vec);
@@ -102,8 +113,7 @@ hipError_t rolaq_launch_mx4_write_plain(const rolaq::Mx4RowsArgs& a, int D, hipS
 hipError_t rolaq_launch_mx4_read(const rolaq::Mx4RowsArgs& a, int D, hipStream_t stream) {
   using namespace rolaq;
   const int R = D / 8;
-  const int64_t threads = a.n * ((D + R) / 8);
-  const dim3 grid((unsigned)((threads + kMx4RowThreads - 1) / kMx4RowThreads)), block(kMx4RowThreads);
+  const dim3 grid = mx4_row_grid(a.n * ((D + R) / 8)), block(kMx4RowThreads);
   if (D == 512)
     hipLaunchKernelGGL((mx4_read_kernel<512, 64>), grid, block, 0, stream, a);
   else

@@ -763,3 +763,32 @@ def test_graphs_replayed_side_by_side():
             b.run(q=qb, o=outs[2])
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want_a) and torch.equal(outs[1], want_b) and torch.equal(outs[2], want_b)
+
+
+# ---- launches of more threads or blocks than one dimension of a grid holds -----------------
+def test_rows_of_more_than_2_32_threads():
+    """59.7 million rows of 72 threads each, without a rotation: read, and written (nearly all outside the cache)."""
+    D, R, n = 512, 64, (1 << 32) // 72 + 1000
+    pool = MX4MLAPool(99, 1, D, R, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(100, D, device=DEV, generator=g).bfloat16()
+    pe = torch.randn(100, R, device=DEV, generator=g).bfloat16()
+    mx4.write_rows(pool, 0, torch.arange(100, device=DEV), x, pe)
+    table = mx4.read_rows(pool, 0, torch.arange(100, device=DEV))
+    big = torch.empty(n, D + R, dtype=torch.bfloat16, device=DEV)  # 69 GB
+    try:
+        slots = torch.randint(0, 100, (n,), device=DEV, generator=g)
+        mx4.read_rows(pool, 0, slots, out=big)
+        for at in (0, 1 << 25, n - 100000):
+            assert torch.equal(big[at:at + 100000], table[slots[at:at + 100000]]), at
+        slots.fill_(-1)
+        at = torch.cat((torch.arange(50, device=DEV), torch.arange(n - 50, n, device=DEV)))
+        slots[at] = torch.arange(100, device=DEV)
+        big[at, :D] = x.flip(0)
+        mx4.write_rows(pool, 0, slots, big[:, :D], pe[:1].expand(n, R))
+        code, s = oracle.encode(x.flip(0).float().cpu())
+        assert torch.equal(pool.c_codes[0].cpu(), oracle.pack(code)) and torch.equal(pool.c_scales[0].cpu(), s)
+        assert torch.equal(pool.rope_buf[0], pe[:1].expand(100, R))
+    finally:
+        del big
+        torch.cuda.empty_cache()
