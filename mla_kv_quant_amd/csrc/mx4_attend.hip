@@ -331,8 +331,10 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     // which see most positions, first; request by request, so that each is
     // spread over the XCDs (blocks go round them in turn; requests in turn, in a multiple
     // of 8, would each lie on one: 32 ragged chunks, 40 heads, D = 256 8.9 ms for 3.9)
-    b = blockIdx.x / a.row_blocks;
-    rb_only = a.row_blocks - 1 - blockIdx.x % a.row_blocks;
+    const uint32_t j = blockIdx.y * gridDim.x + blockIdx.x;
+    b = j / (uint32_t)a.row_blocks;
+    if (b >= a.B) return;
+    rb_only = a.row_blocks - 1 - (int)(j % (uint32_t)a.row_blocks);
     rq = mx4_request(a, b);
   }
   const bool shared = a.ws != nullptr;
@@ -1019,8 +1021,10 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   if (!shared) {
     a.ws = nullptr;
     a.blocks = 0;
-    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3((unsigned)((int64_t)a.row_blocks * a.B)), dim3(256), Ge::LDS,
-                       stream, a);
+    // (in two dimensions: 2^24 blocks of 256 threads are too many for one)
+    const int64_t blocks = (int64_t)a.row_blocks * a.B, x = std::min<int64_t>(blocks, 1 << 22);
+    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), dim3(256),
+                       Ge::LDS, stream, a);
     return hipGetLastError();
   }
   a.blocks = std::min(num_cus * Ge::OCC, kMx4Jobs);

@@ -792,3 +792,19 @@ def test_rows_of_more_than_2_32_threads():
     finally:
         del big
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("D", [512, 256])
+def test_attention_of_2_24_blocks(D):
+    """2048 requests with a stated longest chunk of 4096 queries of 128 heads: the bits that the true length gives."""
+    n = 2048
+    b = Batch(D, 128, [2 + (7 * i) % 90 for i in range(n)], [2] * n, 16, seed=4)
+    q = b.q.to(DEV)
+    outs = []
+    for longest in (2, 8192):
+        o = torch.full((b.T, 128, D), 7.0, dtype=torch.bfloat16, device=DEV)
+        mx4.attend_fwd(q, o, b.pool, 0, b.kv_indptr, b.kv_indices, b.kv_lens, b.sm, qo_indptr=b.qo, max_q_len=longest,
+                       page_size=16)
+        outs.append(o)
+    assert torch.equal(outs[0], outs[1])
+    b.check(outs[1], requests=[0, 5, 1024, n - 1])
