@@ -19,7 +19,11 @@
 // * Softmax in FP32, log2 domain, against a whole-number reference for each
 //   row: a tile's largest score rounded up, moved only when a later score passes
 //   it by more than 2^8 (bf16 probabilities have FP32's range). A reference
-//   then moves by whole powers of two, exact in the accumulators as in P.
+//   then moves by whole powers of two, exact in the accumulators as in P. P is
+//   rounded to bf16, into whose exponents the block scales go; O is divided by the sum of
+//   the rounded P (v_dot2_f32_bf16, a chain for each sub-tile), so that weights add up
+//   to one and a row that is seen alone comes back as it is. The LSE, where a
+//   call asks for it, takes the sum of the P before rounding.
 // * Output: wave w takes the features D/4 w .. of all G groups. The codes come
 //   out of LDS transposed (ds_read_b64_tr_b4: 16 positions of one feature), become
 //   bf16 pairs by v_cvt_scalef32_pk_bf16_fp4 (one instruction for two values) and
@@ -93,6 +97,12 @@ __device__ __forceinline__ void scale_acc8(f32x4 (&o)[8], float f, uint32_t need
       : "scc");
 }
 
+// acc + both values of a packed pair of bf16 (exact products by one).
+__device__ __forceinline__ float sum_bf16x2(uint32_t v, float acc) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, v), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc,
+                                         false);
+}
+
 // Sum of two 16-bit fields each (no carry between them).
 __device__ __forceinline__ uint32_t add16(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, a) + __builtin_bit_cast(u16x2, b));
@@ -149,12 +159,12 @@ struct Mx4Geo {
   static constexpr int IDX = ES + 2 * NB * 128;             // [kMx4Idx][W][64] page numbers
   static constexpr int FLAG = IDX + kMx4Idx * 256 * W;      // [2][W]
   static constexpr int WREF = FLAG + 8 * W;                 // [2][W][16]
-  static constexpr int LSUM = WREF + 128 * W;               // [W][16]
-  static constexpr int LDS = LSUM + 64 * W;
+  static constexpr int LSUM = WREF + 128 * W;               // [W][16] of two sums
+  static constexpr int LDS = LSUM + 128 * W;
   static_assert(LDS * OCC <= 160 * 1024, "LDS of a CU");
   static_assert(S - 1 <= kMx4Idx, "page numbers in flight");
   static_assert(TW >= 1 && TW <= 4 && FT % 2 == 0, "a wave's scores and features");
-  static constexpr int SLOT = ROWS * (D + 2) * 4;  // bytes of a partial: O, then (reference, sum) by row
+  static constexpr int SLOT = ROWS * (D + 3) * 4;  // bytes of a partial: O, (reference, sum of rounded P) by row, sum of P by row
 };
 
 // What the attend kernel leaves for the merge at the start of the workspace, by pair
@@ -235,7 +245,9 @@ __device__ __forceinline__ uint32_t mx4_block_of(uint32_t u, uint32_t units, uin
 // PAGED: pages of 16 positions or more. A wave copies CT = 64 / W positions, 16 or 8,
 // which then lie in one page: its number is a scalar, and the copies' offsets are the
 // same for every tile. Otherwise the positions' page numbers come through LDS.
-template <int D, int R, int G, bool PAGED>
+// LSE: for calls that ask for it, the sum of P before its rounding as well. In one
+// kernel for both the largest prefill takes 4875 us for 4768, ragged chunks 844 for 821.
+template <int D, int R, int G, bool PAGED, bool LSE>
 __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_attend_kernel(Mx4AttendArgs a) {
   using Ge = Mx4Geo<D, R, G>;
   if constexpr (Ge::ACC) define_acc_macros();
@@ -534,7 +546,8 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     float ref[G];  // reference of row la of each group, the same in every wave
 #pragma unroll
     for (int g = 0; g < G; ++g) ref[g] = kMx4NoRef;
-    float lsum = 0.f, ltile = 0.f, wref = kMx4NoRef;  // this lane's sums (its positions of row la of group gw)
+    // this lane's sums (its positions of row la of group gw): of P as it is rounded, and (LSE) of P
+    float psum = 0.f, ptile = 0.f, lsum = 0.f, ltile = 0.f, wref = kMx4NoRef;
 
     // The operands of 16 positions' scores (sub-tile m of this wave's MT) from the ring slot `at`.
     struct Keys {
@@ -615,19 +628,21 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
       // (the score rounded before the difference, as in the reference: fused, one of
       // 2^31 and more could pass its own maximum by 2^7)
 #pragma clang fp contract(off)
-      ltile = 0.f;
+      ltile = ptile = 0.f;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           p[i] = __builtin_amdgcn_exp2f(acc[m][i] * c2 - wref);
-          ltile += p[i];
+          if constexpr (LSE) ltile += p[i];
         }
+        const u32x2 w = {pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
+        ptile += sum_bf16x2(w.y, sum_bf16x2(w.x, 0.f));
         // chunk (8 positions) c of a row at c ^ (row & 7)
         const int c = 2 * (tw * MT + m) + (gq >> 1);
         *reinterpret_cast<u32x2*>(smem + Ge::P + (k & 1) * Ge::ROWS * 128 + (16 * gw + la) * 128 + 16 * (c ^ (la & 7)) +
-                                  8 * (gq & 1)) = u32x2{pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3])};
+                                  8 * (gq & 1)) = w;
       }
     };
     // P of tile k: row la of group g, positions 16 gq + 8 h .. + 7.
@@ -681,8 +696,13 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
           const uint32_t d = (uint32_t)fminf(top - r, 511.f) << 7;
           down[g] = d | d << 16;
           if (g == gw) {
-            lsum = lsum * fall[g];
-            ltile = ltile * __builtin_amdgcn_exp2f(wref - top);
+            const float f = __builtin_amdgcn_exp2f(wref - top);
+            psum *= fall[g];
+            ptile *= f;
+            if constexpr (LSE) {
+              lsum *= fall[g];
+              ltile *= f;
+            }
           }
           ref[g] = top;
         }
@@ -691,7 +711,8 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
 #pragma unroll
         for (int g = 0; g < G; ++g) scale_acc8(o[g], fall[g], moved);
       }
-      lsum += ltile;
+      if constexpr (LSE) lsum += ltile;
+      psum += ptile;
       return moved;
     };
     auto lower = [&](u32x4& p, uint32_t d) {
@@ -891,33 +912,39 @@ __global__ __launch_bounds__(256, (Mx4Geo<D, R, G>::ACC ? 1 : 2)) void mx4_atten
     if constexpr (!PAGED) wait_loads<0>();  // (page numbers asked for past the end)
 
     // ---- the rows' sums, then the output or a partial --------------------------------
-    lsum = wave_sum_over_groups(lsum);
-    if (gq == 0) *reinterpret_cast<float*>(smem + Ge::LSUM + 64 * wave + 4 * la) = lsum;
+    if constexpr (LSE) lsum = wave_sum_over_groups(lsum);
+    psum = wave_sum_over_groups(psum);
+    if (gq == 0) *reinterpret_cast<f32x2*>(smem + Ge::LSUM + 128 * wave + 8 * la) = f32x2{lsum, psum};
     __syncthreads();
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      float l = 0.f;
+      f32x2 l = {0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < TW; ++w) l += *reinterpret_cast<const float*>(smem + Ge::LSUM + 64 * (w * G + g) + 4 * la);
+      for (int w = 0; w < TW; ++w) {
+        const f32x2 v = *reinterpret_cast<const f32x2*>(smem + Ge::LSUM + 128 * (w * G + g) + 8 * la);
+        l = f32x2{l.x + v.x, l.y + v.y};
+      }
       const int r = row0 + 16 * g + la;
       if (r >= rows) continue;
       const int tq = tok_of(16 * g + la), tok = rq.q0 + tq, head = head0 + 16 * g + la - (tq - tok0) * a.H;
       if (whole) {
-        const float inv = l == 0.f ? 0.f : Ge::UNIT / l;
+        const float inv = l.y == 0.f ? 0.f : Ge::UNIT / l.y;
         uint16_t* const out = a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + Ge::FW * wave + 4 * gq;
 #pragma unroll
         for (int j = 0; j < FT; ++j) {
           *reinterpret_cast<u32x2*>(out + 16 * j) = finish<Ge::VSIDE>(o[g][j], inv);
         }
-        if (a.lse && wave == 0 && gq == 0)
-          a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (ref[g] + log2f(l)) * kLn2;
+        if (LSE && wave == 0 && gq == 0)
+          a.lse[(int64_t)tok * a.H + head] = l.x == 0.f ? -INFINITY : (ref[g] + log2f(l.x)) * kLn2;
       } else {
         uint8_t* const part = a.ws + kMx4WsHead + ((int64_t)2 * a.blocks + (nth > 0)) * Ge::SLOT;
         float* const po = reinterpret_cast<float*>(part) + (16 * g + la) * D + Ge::FW * wave + 4 * gq;
 #pragma unroll
         for (int j = 0; j < FT; ++j) *reinterpret_cast<f32x4*>(po + 16 * j) = o[g][j] * Ge::UNIT;
-        if (wave == 0 && gq == 0)
-          reinterpret_cast<f32x2*>(part + Ge::ROWS * D * 4)[16 * g + la] = f32x2{ref[g], l};
+        if (wave == 0 && gq == 0) {
+          reinterpret_cast<f32x2*>(part + Ge::ROWS * D * 4)[16 * g + la] = f32x2{ref[g], l.y};
+          if constexpr (LSE) reinterpret_cast<float*>(part + Ge::ROWS * (D + 2) * 4)[16 * g + la] = l.x;
+        }
       }
     }
     ++nth;
@@ -935,6 +962,7 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
   static_assert(PARTS == 1 || RM == 1, "blocks with several shares leave as one");
   __shared__ f32x4 s_o[PARTS][C];
   __shared__ f32x2 s_ml[PARTS];
+  __shared__ float s_ls[PARTS];
   const Mx4Job job = reinterpret_cast<const Mx4Job*>(a.ws)[blockIdx.x];
   if (a.by_pair) {  // (pairs that there are not: their jobs are not written)
     const int b = blockIdx.x / a.row_blocks;
@@ -945,18 +973,20 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
   const int unit = C % 64 == 0 ? __builtin_amdgcn_readfirstlane(threadIdx.x / C) : threadIdx.x / C;
   const int part = unit % PARTS, rl = blockIdx.y * RM + unit / PARTS, r = job.row0 + rl;
   if (job.parts == 0 || r >= job.rows || rl >= rows_per_block) return;
-  const int64_t slot = (int64_t)rows_per_block * (D + 2) * 4;
+  const int64_t slot = (int64_t)rows_per_block * (D + 3) * 4;
   const uint8_t* const parts = a.ws + kMx4WsHead + 2 * job.first * slot;
-  float m = kMx4NoRef, l = 0.f;
+  float m = kMx4NoRef, l = 0.f, lse = 0.f;  // reference, sums of P as it was rounded and (for an LSE) of P
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int j = part; j < job.parts; j += N * PARTS) {
     f32x2 ml[N];
+    float ls[N];
     f32x4 v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int jj = min(j + i * PARTS, job.parts - 1);
       const uint8_t* const p = parts + (2 * jj + (jj == 0 ? job.second : 0)) * slot;
       ml[i] = gload<f32x2>(p + (int64_t)rows_per_block * D * 4 + 8 * rl);
+      ls[i] = a.lse ? gload<float>(p + (int64_t)rows_per_block * (D + 2) * 4 + 4 * rl) : 0.f;
       v[i] = gload<f32x4>(p + ((int64_t)rl * D + col) * 4);
     }
     float top = m;
@@ -964,6 +994,7 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
     for (int i = 0; i < N; ++i) top = fmaxf(top, ml[i].x);
     const float f = __builtin_amdgcn_exp2f(m - top);
     l *= f;
+    lse *= f;
     o *= f;
     m = top;
 #pragma unroll
@@ -971,13 +1002,17 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
       if (j + i * PARTS < job.parts) {
         const float w = __builtin_amdgcn_exp2f(ml[i].x - top);
         l = fmaf(w, ml[i].y, l);
+        lse = fmaf(w, ls[i], lse);
         o += v[i] * w;
       }
     }
   }
   if constexpr (PARTS > 1) {
     s_o[part][c] = o;
-    if (c == 0) s_ml[part] = f32x2{m, l};
+    if (c == 0) {
+      s_ml[part] = f32x2{m, l};
+      s_ls[part] = lse;
+    }
     __syncthreads();
     if (part) return;
     float top = m;
@@ -985,22 +1020,24 @@ __global__ __launch_bounds__(THREADS) void mx4_merge_kernel(Mx4AttendArgs a, int
     for (int i = 1; i < PARTS; ++i) top = fmaxf(top, s_ml[i].x);
     const float f = __builtin_amdgcn_exp2f(m - top);
     l *= f;
+    lse *= f;
     o *= f;
     m = top;
 #pragma unroll
     for (int i = 1; i < PARTS; ++i) {
       const float w = __builtin_amdgcn_exp2f(s_ml[i].x - top);
       l = fmaf(w, s_ml[i].y, l);
+      lse = fmaf(w, s_ls[i], lse);
       o += s_o[i][c] * w;
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int tok = job.q0 + r / a.H, head = r % a.H;
   *reinterpret_cast<u32x2*>(a.out + (int64_t)tok * a.o_st + (int64_t)head * a.o_sh + col) = finish<true>(o, inv);
-  if (a.lse && col == 0) a.lse[(int64_t)tok * a.H + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (a.lse && col == 0) a.lse[(int64_t)tok * a.H + head] = lse == 0.f ? -INFINITY : (m + log2f(lse)) * kLn2;
 }
 
-template <int D, int R, int G, bool PAGED>
+template <int D, int R, int G, bool PAGED, bool LSE>
 hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   using Ge = Mx4Geo<D, R, G>;
   const int64_t rows = (int64_t)a.max_q_len * a.H;
@@ -1015,7 +1052,7 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
   const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + (int64_t)(1 + Ge::PRE) * a.B;
   const bool shared = a.B <= kMx4Requests && (Ge::OCC == 1 || items <= 6 * (int64_t)num_cus) && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
-  const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED>,
+  const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED, LSE>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);
   if (e != hipSuccess) return e;
   if (!shared) {
@@ -1023,14 +1060,14 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
     a.blocks = 0;
     // (in two dimensions: 2^24 blocks of 256 threads are too many for one)
     const int64_t blocks = (int64_t)a.row_blocks * a.B, x = std::min<int64_t>(blocks, 1 << 22);
-    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), dim3(256),
+    hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED, LSE>), dim3((unsigned)x, (unsigned)((blocks + x - 1) / x)), dim3(256),
                        Ge::LDS, stream, a);
     return hipGetLastError();
   }
   a.blocks = std::min(num_cus * Ge::OCC, kMx4Jobs);
   const int64_t pairs = (int64_t)a.B * a.row_blocks;
   a.by_pair = pairs <= a.blocks;
-  hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
+  hipLaunchKernelGGL((mx4_attend_kernel<D, R, G, PAGED, LSE>), dim3(a.blocks), dim3(256), Ge::LDS, stream, a);
   hipError_t rc = hipGetLastError();
   if (rc != hipSuccess) return rc;
   // Partials of a row: 16 and more in U shares of whole rows, 16 U and more (a few pairs) in 16
@@ -1052,8 +1089,11 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
 
 template <int D, int R, int G>
 hipError_t launch_paged(const Mx4AttendArgs& a, int num_cus, hipStream_t stream) {
-  return a.page_shift >= 4 ? launch_attend<D, R, G, true>(a, num_cus, stream)
-                           : launch_attend<D, R, G, false>(a, num_cus, stream);
+  if (a.lse)
+    return a.page_shift >= 4 ? launch_attend<D, R, G, true, true>(a, num_cus, stream)
+                             : launch_attend<D, R, G, false, true>(a, num_cus, stream);
+  return a.page_shift >= 4 ? launch_attend<D, R, G, true, false>(a, num_cus, stream)
+                           : launch_attend<D, R, G, false, false>(a, num_cus, stream);
 }
 
 }  // namespace rolaq

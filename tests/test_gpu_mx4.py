@@ -808,3 +808,31 @@ def test_attention_of_2_24_blocks(D):
         outs.append(o)
     assert torch.equal(outs[0], outs[1])
     b.check(outs[1], requests=[0, 5, 1024, n - 1])
+
+
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("H,qlens", [(16, [1, 1, 1, 1]), (5, [3, 1, 4, 4]), (40, [1, 2, 60, 3])])
+@pytest.mark.parametrize("page", [1, 64])
+def test_weights_add_up_to_one(D, H, qlens, page):
+    """Requests of equal rows, whatever each position's score (the rope parts differ): the row itself, exactly.
+
+    Weights that add up to 1 + e give the row times 1 + e; FP32 sums and the division leave
+    |e| < 2^-16, which no bf16 value of one or two significant bits (a level times a power of
+    two) is changed by in rounding. The first request's first queries see one position and two.
+    """
+    b = Batch(D, H, [qlens[0], 2, 700, 9001], qlens, page, seed=17)
+    g = torch.Generator().manual_seed(3)
+    rows = []
+    for i, s in enumerate(b.slots):
+        x = torch.randn(1, D, generator=g).expand(len(s), D)
+        fill(b.pool, s, x, b.pe[i])
+        code, sc = oracle.encode(x[:1])
+        rows.append(oracle.decode(oracle.pack(code), sc)[0])
+    lse = torch.empty(b.T, H, device=DEV)
+    o = b.run(lse=lse).double().cpu()
+    t = 0
+    for row, m, n in zip(rows, qlens, b.lens):
+        seen = [j for j in range(m) if n - m + j >= 0]
+        assert (o[[t + j for j in seen]] == row).all(), (n, m)
+        t += m
+    assert lse.std() > 0.1
