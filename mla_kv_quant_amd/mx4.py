@@ -17,10 +17,16 @@ the one exception is a write that finds its layer's rotation new or changed
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import kernels
 from .writer import SUPPORTED_DIMS, _as_int64, _rows
+
+# A call of the attention is two launches, the first of which leaves in the workspace what the
+# second joins: calls of several host threads on one stream must not get in between.
+_turns = threading.Lock()
 
 
 class MX4MLAPool:
@@ -65,7 +71,8 @@ def attend_workspace(pool) -> torch.Tensor:
     """The attention's workspace of ``pool`` for calls on the current stream (67 MB at width 512).
 
     One for each stream, allocated by its first call and used by every layer and batch
-    on it: calls of two streams may overlap. During a capture it is a new tensor
+    on it: calls of two streams may overlap, and ``attend_fwd`` keeps those of several
+    host threads on one stream apart. During a capture it is a new tensor
     of the graph's memory, so graphs that do not share their memory may be replayed
     side by side, and beside other calls.
     """
@@ -186,6 +193,9 @@ def attend_fwd(q, o, pool, layer_id, kv_indptr, kv_indices, kv_lens, sm_scale, q
     time; that function's if not given.
     """
     li = layer_id - pool.start_layer
-    return kernels.mx4_attend_fwd(q, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], qo_indptr, kv_indptr,
-                                  kv_indices, _as_int64(kv_lens), max_q_len, o, sm_scale,
-                                  attend_workspace(pool) if workspace is None else workspace, page_size, lse)
+    args = (q, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], qo_indptr, kv_indptr, kv_indices,
+            _as_int64(kv_lens), max_q_len, o, sm_scale)
+    if workspace is not None:
+        return kernels.mx4_attend_fwd(*args, workspace, page_size, lse)
+    with _turns:
+        return kernels.mx4_attend_fwd(*args, attend_workspace(pool), page_size, lse)

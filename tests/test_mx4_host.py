@@ -208,3 +208,31 @@ def test_a_rotation_without_a_version(monkeypatch):
         assert torch.equal(written(monkeypatch, pool), laid_out(rotation(1)))
         r.copy_(rotation(2))
         assert torch.equal(written(monkeypatch, pool), laid_out(rotation(2)))
+
+
+# ---- two host threads on one stream ----------------------------------------------------
+def test_calls_of_two_threads_take_turns_in_the_pool_s_workspace(monkeypatch):
+    """A call is two launches with the workspace between them: no other call's may come in between."""
+    import threading
+    import time
+
+    pool = small_pool()
+    inside, met = [], []
+
+    def launch(*args):
+        inside.append(1)
+        met.append(len(inside))
+        time.sleep(0.002)  # (as ctypes does, lets other threads run)
+        inside.pop()
+
+    monkeypatch.setattr(mx4.kernels, "mx4_attend_fwd", launch)
+    monkeypatch.setattr(mx4, "attend_workspace", lambda p: torch.zeros(16, dtype=torch.uint8))
+    q, o = torch.zeros(3, 16, 576, dtype=BF), torch.zeros(3, 16, 512, dtype=BF)
+    ptr, idx, lens = torch.zeros(4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.ones(3, dtype=torch.int64)
+    threads = [threading.Thread(target=lambda: [mx4.attend_fwd(q, o, pool, 0, ptr, idx, lens, 0.1) for _ in range(10)])
+               for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(met) == 40 and max(met) == 1
