@@ -190,15 +190,14 @@ struct Mx4Request {
 
 __device__ __forceinline__ Mx4Request mx4_request(const Mx4AttendArgs& a, int b) {
   Mx4Request r;
-  r.q0 = a.qo_indptr ? a.qo_indptr[b] : b;
-  const int q1 = a.qo_indptr ? a.qo_indptr[b + 1] : b + 1;
-  r.q0 = min(max(r.q0, 0), a.T);
-  const int nq = max(min(q1, a.T) - r.q0, 0);
+  // (every offset within its range before any difference, which could wrap)
+  const auto query = [&](int i) { return min(max(a.qo_indptr ? a.qo_indptr[i] : i, 0), a.T); };
+  r.q0 = query(b);
+  const int nq = max(query(b + 1) - r.q0, 0);
   r.nq = min(nq, a.max_q_len);
-  r.list = a.kv_indptr[b];
-  const int end = a.kv_indptr[b + 1];
-  r.list = max(r.list, 0);
-  const int64_t pages = min((int64_t)max(end - r.list, 0), max(a.n_indices - r.list, (int64_t)0));
+  r.list = max(a.kv_indptr[b], 0);
+  const int64_t end = min((int64_t)max(a.kv_indptr[b + 1], 0), a.n_indices);
+  const int64_t pages = max(end - r.list, (int64_t)0);
   const int64_t most = pages << a.page_shift;  // positions that the list reaches
   r.len = (int)max(min(min(a.kv_lens[b], most), (int64_t)0x3fffffff), (int64_t)0);
   r.past = r.len - nq;

@@ -836,3 +836,22 @@ def test_weights_add_up_to_one(D, H, qlens, page):
         assert (o[[t + j for j in seen]] == row).all(), (n, m)
         t += m
     assert lse.std() > 0.1
+
+
+@pytest.mark.parametrize("B", [3, 1100])
+def test_offsets_far_outside_read_and_write_nothing_there(B):
+    """Offsets whose differences do not fit 32 bits: such a request has no queries, or no positions; others are as they were."""
+    b = Batch(256, 16, [100] * B, [1] * B, 16, seed=7)
+    want = b.run()
+    room = torch.full((2 * B + 64, 16, 256), 7.0, dtype=torch.bfloat16, device=DEV)
+    low = -(1 << 31)
+    for at, value in ((2, low), (2, low + 1), (B, low), (1, (1 << 31) - 1)):
+        for which in ("qo_indptr", "kv_indptr"):
+            room.fill_(7.0)
+            off = {"qo_indptr": b.qo.clone(), "kv_indptr": b.kv_indptr.clone()}
+            off[which][at] = value
+            mx4.attend_fwd(b.q.to(DEV), room[:B], b.pool, 0, off["kv_indptr"], b.kv_indices, b.kv_lens, b.sm,
+                           qo_indptr=off["qo_indptr"], max_q_len=1, page_size=16)
+            assert (room[B:] == 7).all()
+            same = [i for i in range(1, B) if i not in (at - 1, at)]  # (a start cut to 0 is row 0's)
+            assert torch.equal(room[same], want[same]), (at, value, which)
