@@ -150,7 +150,7 @@ struct Mx4Geo {
   // where the work is cut, so that a block with two of them has fewer. us, 0 / 3 / 6 / 10: 24 ragged
   // requests with 128 heads 86.7 / 81.2 / 76.5 / 77.1; 16 with 2 .. 4 queries 54.9 / 49.0 / 45.2 / 44.9; 400 short
   // ones, 16 heads, 100.8 / 83.8 / 79.3 / 80.7; ragged chunks 882 / 866 / 847 / 854; D = 256, 64 ragged requests,
-  // 16 heads 29.4 / 27.0 / 25.5 / 25.8, ragged chunks 376 / 373 / 379 / 377.
+  // 16 heads 29.4 / 27.0 / 25.5 / 25.8; and ragged chunks, where nothing is gained, 376 / 373 / 379 / 377.
   static constexpr int PRE = 6;
   static constexpr int LOADS = (CODES + ROPE) / (1024 * W) + 1;  // a wave's copies for a tile
   // LDS offsets
@@ -1043,14 +1043,22 @@ hipError_t launch_attend(Mx4AttendArgs a, int num_cus, hipStream_t stream) {
   a.row_blocks = (int)((rows + Ge::ROWS - 1) / Ge::ROWS);
   a.h_inv = (65536 + a.H - 1) / a.H;
   // Shared out, but for more requests than a block's sums hold, more tiles than 32 bits
-  // count, and, where two blocks run on a CU, more than 6 row blocks for each CU: those
-  // have a block each. us, shared out / a block each: decode 32 x 4096 with 16 heads, D = 512, 24.5 / 78.7;
-  // chunks of one length, D = 512, 2 row blocks a CU 279 / 284, 8 1027 / 1040, 16 2035 / 2066; ragged ones, 5 a CU
-  // 732 / 852, 18 2754 / 2784; 400 requests of 1 .. 8 queries, 128 heads 1377 / 2358; D = 256, ragged chunks, 3 a CU 442
-  // / 480, 5 389 / 347 and 222 / 288, 8 512 / 577 and 869 / 769, 15 1185 / 1116; of one length, 5 352 / 333, 20 4993 / 4661.
+  // count, and, where two blocks run on a CU, more than 4 row blocks for each CU: those
+  // have a block each. What sharing costs is a block's sums, an even batch's cuts and, in
+  // chunks without a prefix, tiles that a row block does not see; what it brings is even
+  // work, the more the fewer row blocks there are to even it out, and lengths are not known here.
+  // us, shared out / a block each, by row blocks for a CU, 256 CUs. D = 256, 40 heads: ragged
+  // chunks behind prefixes 2.0 215 / 240, 2.5 266 / 328, 3.9 334 / 388, 7.6 653 / 675, 9.2
+  // 798 / 738, 21 2186 / 1982; of one length 2.0 185 / 182, 4.0 332 / 320, 8 592 / 567, 24
+  // 1916 / 1796; from their start 2.0 27.7 / 21.7, 4.0 43.6 / 41.6, 11 122 / 104; decode 1.3
+  // 132 / 154, 2.5 241 / 271; 16 heads, ragged 2.6 196 / 223, 3.7 337 / 341, 5.4 526 / 499,
+  // 16 1770 / 1578. D = 512: 128 heads, ragged 1.0 213 / 302, 2.9 471 / 539, 7.6 1237 / 1330,
+  // 16 2537 / 2600; of one length 1.0 180 / 172, 4.0 586 / 582, 12 1752 / 1764; from their
+  // start 1.0 28.5 / 19.9, 4.0 77 / 72, 8 147 / 149; decode 2.0 216 / 274, 8 791 / 871; 16
+  // heads, ragged 2.4 440 / 435, 6.9 1414 / 1473, 20 4005 / 3599.
   const int64_t items = ((int64_t)a.T * a.H + Ge::ROWS - 1) / Ge::ROWS;
   const int64_t most_tiles = (a.n_indices << a.page_shift) / kMx4Tile + (int64_t)(1 + Ge::PRE) * a.B;
-  const bool shared = a.B <= kMx4Requests && (Ge::OCC == 1 || items <= 6 * (int64_t)num_cus) && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
+  const bool shared = a.B <= kMx4Requests && (Ge::OCC == 1 || items <= 4 * (int64_t)num_cus) && most_tiles < ((int64_t)1 << 32) / a.row_blocks;
   const hipError_t e = hipFuncSetAttribute((const void*)mx4_attend_kernel<D, R, G, PAGED, LSE>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, Ge::LDS);
   if (e != hipSuccess) return e;
