@@ -855,3 +855,76 @@ def test_offsets_far_outside_read_and_write_nothing_there(B):
             assert (room[B:] == 7).all()
             same = [i for i in range(1, B) if i not in (at - 1, at)]  # (a start cut to 0 is row 0's)
             assert torch.equal(room[same], want[same]), (at, value, which)
+
+
+# ---- pages, caches and batches at their edges ----------------------------------------------
+@pytest.mark.parametrize("D,H", [(512, 16), (256, 40)])
+@pytest.mark.parametrize("page", [2, 8, 256])
+def test_other_page_sizes(D, H, page):
+    b = Batch(D, H, [1, 130, 77, 600], [1, 2, 3, 1], page, seed=page)
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("lens", [[0], [0, 0, 0], [1]])
+@pytest.mark.parametrize("H", [3, 40])
+def test_batches_that_see_next_to_nothing(lens, H):
+    b = Batch(512, H, lens, [2] * len(lens), 64, seed=1)
+    lse = torch.empty(b.T, H, device=DEV)
+    b.check(b.run(lse=lse), lse)
+
+
+@pytest.mark.parametrize("D", [512, 256])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("left", [1, 5, 15])
+def test_a_cache_that_ends_inside_its_last_page(D, page, left):
+    """The last page's slots past the cache's end are neither read nor needed."""
+    n = 3 * page + left
+    b = Batch(D, 16, [n, 100], [1, 2], page, seed=left)
+    num = (b.pool.c_codes[0].shape[0] // page + 4) * page + left  # the first request's pages become the last ones
+    pool = MX4MLAPool(num - 1, 1, D, D // 8, device=DEV)
+    first = num // page - 3
+    where = torch.arange(first * page, first * page + n)
+    assert where[-1] == num - 1
+    for name in ("c_codes", "c_scales", "rope_buf"):
+        old, new = getattr(b.pool, name)[0], getattr(pool, name)[0]
+        new[: old.shape[0]] = old
+        new[where.to(DEV)] = old[torch.as_tensor(b.slots[0]).to(DEV)]
+    b.kv_indices[:4] = torch.arange(first, first + 4, device=DEV)
+    b.pool = pool
+    b.check(b.run())
+
+
+@pytest.mark.parametrize("D", [512, 256])
+def test_rows_far_into_a_large_cache(D):
+    """Slots whose codes lie past 4 GB (and rope rows past 2 GB): written, read both ways and attended over."""
+    D, R = dims(D)
+    num = (1 << 33) // D + 4096  # D / 2 bytes a row: 4.3 GB of codes and more
+    rot = synth.make_rotation(D, 3)
+    n, page = 1000, 64
+    start = num // page * page - 16 * page
+    loc = torch.arange(start, start + n, device=DEV)
+    x, pe = synth.make_latent(n, D, 5, seed=1).to(DEV), synth.make_normal((n, R), 2).to(DEV)
+    big, small = (MX4MLAPool(k - 1, 1, D, R, device=DEV, rotations=[rot]) for k in (num, 16 * page))
+    here = loc - start
+    try:
+        for rotated in (True, False):
+            if not rotated:
+                big.rotations[0] = small.rotations[0] = None
+            mx4.write_rows(big, 0, loc, x, pe)
+            mx4.write_rows(small, 0, here, x, pe)
+            assert torch.equal(big.c_codes[0][loc], small.c_codes[0][here])
+            assert torch.equal(mx4.read_rows(big, 0, loc), mx4.read_rows(small, 0, here))
+        q = synth.make_normal((2, 16, D + R), 5, std=0.3).to(DEV)
+        for p in (page, 1):
+            outs = []
+            for pool, at in ((big, loc), (small, here)):
+                o = torch.empty(2, 16, D, dtype=torch.bfloat16, device=DEV)
+                idx = (at[::p] // p).to(torch.int32)
+                ptr = torch.tensor([0, idx.numel() // 2, idx.numel()], dtype=torch.int32, device=DEV)
+                lens = torch.tensor([500 // p * p, n - 500 // p * p - 7], device=DEV)
+                mx4.attend_fwd(q, o, pool, 0, ptr, idx, lens, 0.1, page_size=p)
+                outs.append(o)
+            assert torch.equal(*outs) and outs[0].abs().max() > 0
+    finally:
+        del big
+        torch.cuda.empty_cache()
