@@ -352,8 +352,9 @@ int rolaq_mx4_attend_workspace(int D, int64_t* bytes);
  * sees positions 0 .. kv_lens[b] - n + i. Position t lies in slot
  * kv_indices[kv_indptr[b] + t / page_size] * page_size + t % page_size.
  *   s_t = sm_scale (q_lat . x_t + q_rope . rope_t),  out = softmax(s) x,
- * x_t the stored latent row (q_lat enters as R_eff does above). out: bf16 [T, H, D], in the frame of the cached rows; lse
- * (or null): FP32 [T, H], the natural log of the sum of exp(s). A query that
+ * x_t the stored latent row (q_lat enters as R_eff does above). The weights are rounded
+ * to bf16 and out is divided by their sum as rounded. out: bf16 [T, H, D], in the frame of
+ * the cached rows; lse (or null): FP32 [T, H], the natural log of the sum of exp(s). A query that
  * sees no position gets 0 and -inf; queries past qo_indptr[B], and past max_q_len
  * of a request, are left as they were. A length that its page list does not
  * reach is cut there, an index outside the cache reads its last slots: no read

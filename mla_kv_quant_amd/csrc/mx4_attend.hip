@@ -36,13 +36,14 @@
 //   as one), so what they hold does not reach O.
 // One barrier a tile: the scores of tile i + 1 and the output of tile i lie between
 // two barriers, so that matrix, vector and LDS work of both can overlap. With one
-// group the loop waits for HBM (5.8 TB/s in it); with four at 512 features a turn is
-// 2200 cycles of matrix instructions in 5100, and the rest is LDS reads (every wave
-// reads the whole tile's keys for its group) and what they wait for.
+// group the loop waits for HBM (5.8 TB/s in it); with four at 512 features a turn takes
+// 5100 cycles, of which matrix instructions are 2200, vector ones some 1300 and LDS reads some
+// 1700 (every wave reads the whole tile's keys for its group): none of them is the bound, but
+// with one wave on a SIMD and a barrier a turn they follow each other.
 //
 // Measured, kernel alone: 32 x 16384 positions, 16 heads, D = 512: 49 us (4.3 TB/s); 24 ragged
 // requests with 128 heads: 71 us (690 TFLOP/s); 64 x 16384, 40 heads, D = 256: 89 us; chunks of 4 x
-// 2048 behind 14336, 40 heads, D = 256: 4.6 ms (1.18 PFLOP/s).
+// 2048 behind 14336, 40 heads, D = 256: 4.7 ms (1.16 PFLOP/s).
 //
 // Work: the tiles of all (request, row block) pairs, each behind an allowance for its
 // start and end, lie on one line that is cut into equal parts, a part for each block;

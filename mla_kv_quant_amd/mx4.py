@@ -68,7 +68,7 @@ class MX4MLAPool:
 
 
 def attend_workspace(pool) -> torch.Tensor:
-    """The attention's workspace of ``pool`` for calls on the current stream (67 MB at width 512).
+    """The attention's workspace of ``pool`` for calls on the current stream (68 MB at width 512).
 
     One for each stream, allocated by its first call and used by every layer and batch
     on it: calls of two streams may overlap, and ``attend_fwd`` keeps those of several
