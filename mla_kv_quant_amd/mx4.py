@@ -57,7 +57,9 @@ class MX4MLAPool:
         self.c_scales = buf(D // kernels.MX4_BLOCK, torch.uint8)
         self.rope_buf = buf(self.qk_rope_head_dim, torch.bfloat16)
         rotations = rotations or [None] * self.layer_num
-        self.rotations = [None if r is None else r.to(device=dev, dtype=torch.bfloat16) for r in rotations]
+        with torch.inference_mode(False):  # (a tensor of that mode does not count its changes: copied)
+            held = [None if r is None else r.to(device=dev, dtype=torch.bfloat16) for r in rotations]
+            self.rotations = [r.clone() if r is not None and r.is_inference() else r for r in held]
 
     def latent_rotation(self, layer_id: int, local: bool = True):
         return self.rotations[layer_id - self.start_layer if local else layer_id]
@@ -132,10 +134,11 @@ def _rotation_t(pool, layer_id):
 
 
 def _lay_out(r, entry):
-    t = r.to(torch.bfloat16).t()
-    if entry is None or entry[2].device != t.device or entry[2].shape != t.shape:
-        return t.contiguous() if not t.is_contiguous() else t.clone()
-    return entry[2].copy_(t)
+    with torch.inference_mode(False), torch.no_grad():  # (kept for calls of either mode)
+        t = r.to(torch.bfloat16).t()
+        if entry is None or entry[2].device != t.device or entry[2].shape != t.shape:
+            return t.clone(memory_format=torch.contiguous_format)
+        return entry[2].copy_(t)
 
 
 def write_rows(pool, layer_id, loc, c_kv, k_pe) -> None:

@@ -203,11 +203,36 @@ def test_a_pool_that_builds_its_rotation_at_each_call(monkeypatch):
 def test_a_rotation_without_a_version(monkeypatch):
     """Inference tensors do not count their changes: laid out at each call."""
     with torch.inference_mode():
-        r = rotation(1).to(BF)
-        pool = MX4MLAPool(32, 1, 256, 32, device="cpu", rotations=[r])
+        pool = MX4MLAPool(32, 1, 256, 32, device="cpu")
+        r = pool.rotations[0] = rotation(1).to(BF)
         assert torch.equal(written(monkeypatch, pool), laid_out(rotation(1)))
         r.copy_(rotation(2))
         assert torch.equal(written(monkeypatch, pool), laid_out(rotation(2)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_a_pool_made_in_inference_mode_lays_out_once(monkeypatch, dtype):
+    with torch.inference_mode():
+        pool = MX4MLAPool(32, 1, 256, 32, device="cpu", rotations=[rotation(1).to(dtype)])
+        first = written(monkeypatch, pool)
+        assert torch.equal(first, laid_out(rotation(1))) and written(monkeypatch, pool) is first
+        pool.rotations[0].copy_(rotation(2))
+        assert torch.equal(written(monkeypatch, pool), laid_out(rotation(2)))
+
+
+def test_a_rotation_in_and_out_of_inference_mode(monkeypatch):
+    """What is kept serves both, and a parameter's layout has no graph."""
+    pool = MX4MLAPool(32, 1, 256, 32, device="cpu", rotations=[rotation(1)])
+    with torch.inference_mode():
+        first = written(monkeypatch, pool)
+    pool.rotations[0].copy_(rotation(2))
+    assert torch.equal(written(monkeypatch, pool), laid_out(rotation(2)))
+    pool.rotations[0] = torch.nn.Parameter(rotation(3).to(BF))
+    for seed in (3, 4):
+        with torch.no_grad():
+            pool.rotations[0].copy_(rotation(seed))
+        rt = written(monkeypatch, pool)
+        assert rt is first and torch.equal(rt, laid_out(rotation(seed))) and not rt.requires_grad
 
 
 # ---- two host threads on one stream ----------------------------------------------------
