@@ -468,8 +468,9 @@ def run(st):
 
     kept, kept_lens, freed = evict.evict(st["acc"], st["kv_indptr"], st["kv_indices"], st["kv_lens"], case["budget"],
                                          sink=case["sink"], recent=case["recent"], page_size=case["page"],
-                                         req_pool_indices=st["reqs"], acc_out=st["acc_out"], kept=st["kept"],
-                                         kept_lens=st["kept_lens"], freed=st["freed"])
+                                         req_pool_indices=st["reqs"], max_kv_len=st["max_len"],
+                                         acc_out=st["acc_out"], kept=st["kept"], kept_lens=st["kept_lens"],
+                                         freed=st["freed"])
     return kept, kept_lens, freed, st["acc_out"]
 
 
