@@ -374,6 +374,93 @@ int rolaq_mx4_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
                          void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
+/*
+ * Rotary positions of the rope parts of queries (H heads) and keys (Hk heads), T
+ * tokens, one launch. A pair (a, b) of a head at position p becomes
+ *   (scale (a cos w - b sin w), scale (b cos w + a sin w)),  w = 2 pi p turns[i] / 2^64,
+ * pair i being elements (2 i, 2 i + 1) (interleaved) or (i, i + dim / 2) of the head's dim
+ * elements. FP32 arithmetic, one rounding; w is exact modulo a turn for positions of any size and sign.
+ * positions: int64 [T]; turns: [dim / 2] turns of a step of one position, modulo 1,
+ * times 2^64. type: 0 bf16, 1 fp16, 2 fp32, of all four tensors, which are [T, heads, dim]
+ * with element strides for the first two dims. An output is its input (same address and strides) or
+ * does not overlap it. H or Hk may be 0 (its pointers are not read). dim even, 2 to 512.
+ * 16-byte accesses where addresses and strides are multiples of 16 bytes and dim of 16 bytes' worth
+ * of pairs, else a pair at a time.
+ */
+int rolaq_rotary(const int64_t* positions, int64_t T, const uint64_t* turns, int dim, float scale, int interleaved,
+                 int type, const void* q, int64_t q_stride_t, int64_t q_stride_h, void* q_out, int64_t q_out_stride_t,
+                 int64_t q_out_stride_h, int H, const void* k, int64_t k_stride_t, int64_t k_stride_h, void* k_out,
+                 int64_t k_out_stride_t, int64_t k_out_stride_h, int Hk, void* stream);
+
+/* Bytes of rolaq_expanded_attend_fwd's workspace for a call of these sizes on the current
+ * device; 0 where it needs none (few query rows over long keys have their keys split). Host only. */
+int rolaq_expanded_attend_workspace(int64_t T, int64_t N, int B, int H, int nope, int max_q_len, int64_t* bytes);
+
+/*
+ * Attention over keys and values expanded from the latent (MHA-style prefill). Request b
+ * has the queries qo_indptr[b] .. qo_indptr[b + 1] - 1, at most max_q_len of which are
+ * computed, and the key rows kv_indptr[b] .. kv_indptr[b + 1] - 1, n of them for m queries. Query i
+ * sees its rows 0 .. n - m + i (causal) or all.
+ *   s_t = sm_scale (q_nope . k_nope_t,h + q_pe . k_pe_t),  out = softmax(s) v_h.
+ * q: bf16 [T, H, nope + rope]; kv: bf16 [N, H, nope + value] (k_nope | v), as kv_b_proj gives
+ * it; k_pe: bf16 [N, rope], shared by the heads; out: bf16 [T, H, value]; all 16-byte aligned
+ * with strides multiples of 8. lse (or null): FP32 [T, H], natural log of the sum of exp(s).
+ * (nope, rope, value) = (128, 64, 128) or (64, 32, 64). Weights are rounded to bf16 and out is divided
+ * by their sum as rounded; sums are FP32. A query that sees no key gets 0 and -inf (as does one whose scores are all -inf);
+ * queries of no request, and past max_q_len of one, are left as they were. Keys and values that a
+ * query does not see do not reach its output, whatever they hold. Offsets are brought into 0 .. T and 0 .. N.
+ * workspace: rolaq_expanded_attend_workspace bytes for these sizes, 16-byte aligned, contents
+ * unspecified before and after. No allocation, no synchronisation.
+ */
+int rolaq_expanded_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
+                              int64_t kv_stride_t, int64_t kv_stride_h, const void* k_pe, int64_t pe_stride_t,
+                              const int32_t* qo_indptr, const int32_t* kv_indptr, int64_t T, int64_t N, int B, int H,
+                              int nope, int rope, int value, int max_q_len, float sm_scale, int causal, void* out,
+                              int64_t out_stride_t, int64_t out_stride_h, float* lse, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/*
+ * Attention weight of every cached position of the MX4 cache, summed over a request's
+ * query rows:
+ *   acc[r, t] = (add ? acc[r, t] : 0) + sum over the queries i and heads h that see t of exp(s_t - lse[i, h]),
+ * s_t, who sees what, the cache, the index lists and their bounds as in rolaq_mx4_attend_fwd, whose
+ * lse ([T, H], contiguous) this takes; rows with lse = -inf count for nothing. r = req_idx[b] (null: b):
+ * a request whose r is outside 0 .. acc_rows - 1 is left out, positions from acc_cols on are not
+ * counted; rows r of one call must differ. acc: FP32, row stride acc_stride. A request's sums do not depend
+ * on the batch. No workspace, no allocation, no synchronisation.
+ */
+int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_stride_h, const float* lse,
+                                 const uint8_t* codes, const uint8_t* scales, const void* rope_buf, int64_t num_slots,
+                                 const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                 int64_t n_indices, int page_size, const int64_t* kv_lens, const int64_t* req_idx,
+                                 int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
+                                 int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* stream);
+
+/* Bytes of rolaq_evict's workspace for B requests of max_kv_len positions at most. Host only. */
+int rolaq_evict_workspace(int B, int64_t max_kv_len, int64_t* bytes);
+
+/*
+ * Which positions of each request stay in a cache. Request b has the positions
+ * 0 .. n - 1, n = kv_lens[b] cut to max_kv_len and to what its page list reaches (index lists as in
+ * rolaq_mx4_attend_fwd). With n <= budget all stay; else the first `sink`, the last `recent`,
+ * and the budget - sink - recent others of largest acc[r, t], the earlier of equal ones (a NaN is the largest,
+ * -0 equals 0). r = req_idx[b] (null: b); outside 0 .. acc_rows - 1 all weights count as 0 and acc_out is not written.
+ *   kept[b, j]    int32 [B, budget]: slot of the j-th position that stays, in order
+ *   kept_lens[b]  int64: how many (entries of kept past it are left as they were)
+ *   freed         int32 [freed_size]: slots of the others, in order, request after request (those past
+ *                 freed_size are dropped; there are sum over b of max(n - budget, 0))
+ *   acc_out[r, j] acc of the j-th position that stays, 0 from there to column n - 1, the others
+ *                 left as they were. May be acc itself (same address and stride), else must not overlap it.
+ * kept, with offsets b * budget, is a page list of pages of one slot. Rows r of one call must
+ * differ. acc and acc_out: FP32 [acc_rows, acc_cols]. workspace: rolaq_evict_workspace bytes,
+ * 16-byte aligned, not shared with a call that overlaps. No allocation, no synchronisation.
+ */
+int rolaq_evict(const float* acc, int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, float* acc_out,
+                int64_t acc_out_stride, const int64_t* req_idx, const int32_t* kv_indptr, const int32_t* kv_indices,
+                int64_t n_indices, int page_size, const int64_t* kv_lens, int B, int64_t max_kv_len, int budget, int sink,
+                int recent, int32_t* kept, int64_t* kept_lens, int32_t* freed, int64_t freed_size, void* workspace,
+                int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

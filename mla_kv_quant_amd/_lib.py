@@ -58,6 +58,20 @@ SIGNATURES = {
     "rolaq_mx4_attend_fwd": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
                              c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_float,
                              c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
+    "rolaq_rotary": [c_void_p, c_int64, c_void_p, c_int, c_float, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p,
+                     c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p],
+    "rolaq_expanded_attend_workspace": [c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p],
+    "rolaq_expanded_attend_fwd": [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                  c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int,
+                                  c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
+    "rolaq_mx4_accumulate_weights": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                     c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int,
+                                     c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_int64, c_int,
+                                     c_void_p],
+    "rolaq_evict_workspace": [c_int, c_int64, c_void_p],
+    "rolaq_evict": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int,
+                    c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,
+                    c_int64, c_void_p],
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -12,6 +12,7 @@
 
 #include "rolaq_args.h"
 #include "mx4_args.h"
+#include "serve_args.h"
 
 namespace {
 
@@ -695,6 +696,230 @@ int rolaq_mx4_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.lse = lse;
   a.ws = static_cast<uint8_t*>(workspace);
   return hip_status(rolaq_launch_mx4_attend(a, D, cu_count(), static_cast<hipStream_t>(stream)), "mx4_attend_fwd launch");
+}
+
+}  // extern "C"
+
+// ---- rotary positions, expanded attention, accumulated weights, eviction ---------------
+
+extern "C" {
+
+int rolaq_rotary(const int64_t* positions, int64_t T, const uint64_t* turns, int dim, float scale, int interleaved,
+                 int type, const void* q, int64_t q_stride_t, int64_t q_stride_h, void* q_out, int64_t q_out_stride_t,
+                 int64_t q_out_stride_h, int H, const void* k, int64_t k_stride_t, int64_t k_stride_h, void* k_out,
+                 int64_t k_out_stride_t, int64_t k_out_stride_h, int Hk, void* stream) {
+  const char* const fn = "rotary";
+  if (T < 0 || H < 0 || Hk < 0) return fail(ROLAQ_ERR_INVALID, "%s: negative T, H or Hk", fn);
+  if (dim < 2 || dim > 512 || dim % 2) return fail(ROLAQ_ERR_INVALID, "%s: dim must be even, 2 to 512, got %d", fn, dim);
+  if (type < 0 || type > 2) return fail(ROLAQ_ERR_INVALID, "%s: unknown type %d", fn, type);
+  if (!std::isfinite(scale)) return fail(ROLAQ_ERR_INVALID, "%s: scale must be finite", fn);
+  if (H > (1 << 20) || Hk > (1 << 20)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^20 heads", fn);
+  if (T == 0 || H + Hk == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  if (!positions || !turns || (H && (!q || !q_out)) || (Hk && (!k || !k_out)))
+    return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  const size_t size = type == 2 ? 4 : 2;
+  if (!aligned(q, size) || !aligned(q_out, size) || !aligned(k, size) || !aligned(k_out, size))
+    return fail(ROLAQ_ERR_INVALID, "%s: tensors must be aligned to their elements", fn);
+  rolaq::RotaryArgs a{};
+  a.positions = positions;
+  a.turns = turns;
+  a.scale = scale;
+  a.T = T;
+  a.dim = dim;
+  a.pairs = dim / 2;
+  a.H = H;
+  a.Hk = Hk;
+  a.x[0] = q, a.x[1] = k;
+  a.y[0] = q_out, a.y[1] = k_out;
+  a.x_st[0] = q_stride_t, a.x_sh[0] = q_stride_h, a.y_st[0] = q_out_stride_t, a.y_sh[0] = q_out_stride_h;
+  a.x_st[1] = k_stride_t, a.x_sh[1] = k_stride_h, a.y_st[1] = k_out_stride_t, a.y_sh[1] = k_out_stride_h;
+  return hip_status(rolaq_launch_rotary(a, type, interleaved != 0, cu_count(), static_cast<hipStream_t>(stream)),
+                    "rotary launch");
+}
+
+int rolaq_expanded_attend_workspace(int64_t T, int64_t N, int B, int H, int nope, int max_q_len, int64_t* bytes) {
+  if (T < 0 || N < 0 || B < 0 || H < 1 || H > kMaxHeads || max_q_len < 0 || (nope != 64 && nope != 128) || !bytes)
+    return fail(ROLAQ_ERR_INVALID, "expanded_attend_workspace: invalid sizes");
+  *bytes = T == 0 || B == 0 || max_q_len == 0
+               ? 0
+               : rolaq_expanded_ws_bytes(T, N, B, H, nope, int(std::min<int64_t>(max_q_len, T)), cu_count());
+  g_err[0] = '\0';
+  return ROLAQ_OK;
+}
+
+int rolaq_expanded_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* kv,
+                              int64_t kv_stride_t, int64_t kv_stride_h, const void* k_pe, int64_t pe_stride_t,
+                              const int32_t* qo_indptr, const int32_t* kv_indptr, int64_t T, int64_t N, int B, int H,
+                              int nope, int rope, int value, int max_q_len, float sm_scale, int causal, void* out,
+                              int64_t out_stride_t, int64_t out_stride_h, float* lse, void* workspace,
+                              int64_t workspace_bytes, void* stream) {
+  const char* const fn = "expanded_attend_fwd";
+  if (T < 0 || N < 0 || B < 0 || max_q_len < 0) return fail(ROLAQ_ERR_INVALID, "%s: negative T, N, B or max_q_len", fn);
+  if (H < 1 || H > kMaxHeads) return fail(ROLAQ_ERR_INVALID, "%s: H must be between 1 and %d, got %d", fn, kMaxHeads, H);
+  if (!((nope == 128 && rope == 64 && value == 128) || (nope == 64 && rope == 32 && value == 64)))
+    return fail(ROLAQ_ERR_INVALID, "%s: (nope, rope, value) must be (128, 64, 128) or (64, 32, 64), got (%d, %d, %d)", fn,
+                nope, rope, value);
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(ROLAQ_ERR_INVALID, "%s: invalid sm_scale", fn);
+  if (T == 0 || B == 0 || max_q_len == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  if (!q || !qo_indptr || !kv_indptr || !out || (N > 0 && (!kv || !k_pe)))
+    return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  if (T > (1 << 24) || N > (1 << 30)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries or 2^30 keys", fn);
+  if (!aligned(q, 16) || q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: q must be 16-byte aligned with strides multiple of 8", fn);
+  if (!aligned(kv, 16) || kv_stride_t % 8 || kv_stride_h % 8 || kv_stride_t < 0 || kv_stride_h < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: kv must be 16-byte aligned with strides multiple of 8", fn);
+  if (!aligned(k_pe, 16) || pe_stride_t % 8 || pe_stride_t < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: k_pe must be 16-byte aligned with a row stride multiple of 8", fn);
+  if (!aligned(out, 16) || out_stride_t % 8 || out_stride_h % 8 || out_stride_t < 0 || out_stride_h < value)
+    return fail(ROLAQ_ERR_INVALID, "%s: out must be 16-byte aligned with strides multiple of 8", fn);
+  const int most = int(std::min<int64_t>(max_q_len, T));
+  const int64_t ws = rolaq_expanded_ws_bytes(T, N, B, H, nope, most, cu_count());
+  if (ws > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < ws))
+    return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
+  if ((T / 32 + B) * H > (1 << 24))  // (2^32 threads and more are too many for one launch)
+    return fail(ROLAQ_ERR_INVALID, "%s: T * H is too large for one launch", fn);
+  rolaq::ExpandedArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.kv = static_cast<const uint16_t*>(kv);
+  a.kv_st = kv_stride_t;
+  a.kv_sh = kv_stride_h;
+  a.pe = static_cast<const uint16_t*>(k_pe);
+  a.pe_st = pe_stride_t;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.T = int(T);
+  a.N = int(N);
+  a.B = B;
+  a.H = H;
+  a.max_q_len = most;
+  a.sm_scale = sm_scale;
+  a.causal = causal != 0;
+  a.out = static_cast<uint16_t*>(out);
+  a.o_st = out_stride_t;
+  a.o_sh = out_stride_h;
+  a.lse = lse;
+  a.ws = static_cast<float*>(workspace);
+  return hip_status(rolaq_launch_expanded(a, nope, cu_count(), static_cast<hipStream_t>(stream)),
+                    "expanded_attend_fwd launch");
+}
+
+int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_stride_h, const float* lse,
+                                 const uint8_t* codes, const uint8_t* scales, const void* rope_buf, int64_t num_slots,
+                                 const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                 int64_t n_indices, int page_size, const int64_t* kv_lens, const int64_t* req_idx,
+                                 int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
+                                 int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* stream) {
+  const char* const fn = "mx4_accumulate_weights";
+  if (T < 0 || B < 0 || max_q_len < 0) return fail(ROLAQ_ERR_INVALID, "%s: negative T, B or max_q_len", fn);
+  if (H < 1 || H > kMaxHeads) return fail(ROLAQ_ERR_INVALID, "%s: H must be between 1 and %d, got %d", fn, kMaxHeads, H);
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return fail(ROLAQ_ERR_INVALID, "%s: invalid sm_scale", fn);
+  if (page_size < 1 || (page_size & (page_size - 1)))
+    return fail(ROLAQ_ERR_INVALID, "%s: page_size must be a power of two, got %d", fn, page_size);
+  if (acc_rows < 0 || acc_rows > INT32_MAX || acc_cols < 0 || acc_cols > INT32_MAX || acc_stride < acc_cols)
+    return fail(ROLAQ_ERR_INVALID, "%s: invalid sizes of acc", fn);
+  if (B == 0 || acc_rows == 0 || acc_cols == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  const int rc = check_mx4_cache(fn, codes, scales, rope_buf, num_slots, D, R);
+  if (rc != ROLAQ_OK) return rc;
+  if (!kv_indptr || !kv_lens || !acc || (!kv_indices && n_indices > 0) || (T > 0 && (!q || !lse)))
+    return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  if (n_indices < 0 || n_indices > INT32_MAX) return fail(ROLAQ_ERR_INVALID, "%s: n_indices out of range", fn);
+  if (!qo_indptr && (max_q_len != 1 || T < B))
+    return fail(ROLAQ_ERR_INVALID, "%s: without qo_indptr each request has one query (max_q_len 1, T >= B)", fn);
+  const int most = int(std::min<int64_t>(max_q_len, T));
+  if (T > (1 << 24) || T * H > (1 << 29) || int64_t(B) * most * H > (1 << 29))
+    return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries, or 2^29 query rows", fn);
+  if (!aligned(q, 16) || q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: q must be 16-byte aligned with strides multiple of 8", fn);
+  rolaq::Mx4WeightsArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_st = q_stride_t;
+  a.q_sh = q_stride_h;
+  a.codes = codes;
+  a.scales = scales;
+  a.rope = static_cast<const uint16_t*>(rope_buf);
+  a.num_slots = num_slots;
+  a.qo_indptr = qo_indptr;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.n_indices = n_indices;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.kv_lens = kv_lens;
+  a.T = int(T);
+  a.B = B;
+  a.H = H;
+  a.max_q_len = most;
+  a.sm_scale = sm_scale;
+  a.lse = lse;
+  a.req_idx = req_idx;
+  a.acc = acc;
+  a.acc_st = acc_stride;
+  a.acc_rows = int(acc_rows);
+  a.acc_cols = acc_cols;
+  a.add = add != 0;
+  return hip_status(rolaq_launch_mx4_weights(a, D, cu_count(), static_cast<hipStream_t>(stream)),
+                    "mx4_accumulate_weights launch");
+}
+
+int rolaq_evict_workspace(int B, int64_t max_kv_len, int64_t* bytes) {
+  if (B < 0 || max_kv_len < 0 || max_kv_len > (1 << 30) || !bytes)
+    return fail(ROLAQ_ERR_INVALID, "evict_workspace: invalid sizes");
+  *bytes = rolaq_evict_ws_bytes(B, max_kv_len);
+  g_err[0] = '\0';
+  return ROLAQ_OK;
+}
+
+int rolaq_evict(const float* acc, int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, float* acc_out,
+                int64_t acc_out_stride, const int64_t* req_idx, const int32_t* kv_indptr, const int32_t* kv_indices,
+                int64_t n_indices, int page_size, const int64_t* kv_lens, int B, int64_t max_kv_len, int budget, int sink,
+                int recent, int32_t* kept, int64_t* kept_lens, int32_t* freed, int64_t freed_size, void* workspace,
+                int64_t workspace_bytes, void* stream) {
+  const char* const fn = "evict";
+  if (B < 0 || acc_rows < 0 || acc_rows > INT32_MAX || acc_cols < 0 || acc_stride < acc_cols || acc_out_stride < acc_cols)
+    return fail(ROLAQ_ERR_INVALID, "%s: invalid B or sizes of acc", fn);
+  if (budget < 1 || sink < 0 || recent < 0 || int64_t(sink) + recent > budget)
+    return fail(ROLAQ_ERR_INVALID, "%s: budget must be positive and hold sink + recent, got %d, %d + %d", fn, budget, sink,
+                recent);
+  if (page_size < 1 || (page_size & (page_size - 1)))
+    return fail(ROLAQ_ERR_INVALID, "%s: page_size must be a power of two, got %d", fn, page_size);
+  if (max_kv_len < 0 || max_kv_len > acc_cols || max_kv_len > (1 << 30))
+    return fail(ROLAQ_ERR_INVALID, "%s: max_kv_len must be at most acc's columns and 2^30", fn);
+  if (n_indices < 0 || n_indices > INT32_MAX || freed_size < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: n_indices or freed_size out of range", fn);
+  if (B == 0) { g_err[0] = '\0'; return ROLAQ_OK; }
+  if (!kv_indptr || !kv_lens || !kept || !kept_lens || (!kv_indices && n_indices > 0) || (!freed && freed_size > 0) ||
+      ((!acc || !acc_out) && acc_rows > 0 && acc_cols > 0))
+    return fail(ROLAQ_ERR_INVALID, "%s: null pointer", fn);
+  const int64_t ws = rolaq_evict_ws_bytes(B, max_kv_len);
+  if (ws > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < ws))
+    return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
+  if (int64_t(B) * std::max<int64_t>(1, (max_kv_len + 16383) / 16384) > (1 << 21))
+    return fail(ROLAQ_ERR_INVALID, "%s: B * max_kv_len is too large for one launch", fn);
+  rolaq::EvictArgs a{};
+  a.acc = acc;
+  a.acc_out = acc_out;
+  a.acc_st = acc_stride;
+  a.acc_out_st = acc_out_stride;
+  a.acc_rows = int(acc_rows);
+  a.acc_cols = acc_cols;
+  a.req_idx = req_idx;
+  a.kv_indptr = kv_indptr;
+  a.kv_indices = kv_indices;
+  a.n_indices = n_indices;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.kv_lens = kv_lens;
+  a.B = B;
+  a.most = max_kv_len;
+  a.budget = budget;
+  a.sink = sink;
+  a.recent = recent;
+  a.kept = kept;
+  a.kept_lens = kept_lens;
+  a.freed = freed;
+  a.freed_size = freed_size;
+  a.ws = static_cast<uint8_t*>(workspace);
+  return hip_status(rolaq_launch_evict(a, static_cast<hipStream_t>(stream)), "evict launch");
 }
 
 }  // extern "C"

@@ -38,6 +38,30 @@ struct Mx4AttendArgs {
   int by_pair;     // the merge's jobs are numbered by (request, row block), not by block
 };
 
+struct Mx4WeightsArgs {
+  const uint16_t* q;  // as Mx4AttendArgs has them
+  int64_t q_st, q_sh;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const uint16_t* rope;
+  int64_t num_slots;
+  const int32_t* qo_indptr;
+  const int32_t* kv_indptr;
+  const int32_t* kv_indices;
+  int64_t n_indices;
+  int page_shift;
+  const int64_t* kv_lens;
+  int T, B, H, max_q_len;
+  float sm_scale;
+  const float* lse;        // [T, H]
+  const int64_t* req_idx;  // [B] or null
+  float* acc;              // [acc_rows, acc_cols], row stride acc_st
+  int64_t acc_st;
+  int acc_rows;
+  int64_t acc_cols;
+  int add;      // to what acc holds; else in its place
+};
+
 struct Mx4RowsArgs {
   const int64_t* slots;  // [n]
   int64_t n, num_slots;
@@ -56,6 +80,7 @@ struct Mx4RowsArgs {
 }  // namespace rolaq
 
 hipError_t rolaq_launch_mx4_attend(const rolaq::Mx4AttendArgs& a, int D, int num_cus, hipStream_t stream);
+hipError_t rolaq_launch_mx4_weights(const rolaq::Mx4WeightsArgs& a, int D, int num_cus, hipStream_t stream);
 // Bytes of workspace that attend asks for at width D, whatever the batch.
 int64_t rolaq_mx4_attend_ws_bytes(int D, int num_cus);
 hipError_t rolaq_launch_mx4_write_plain(const rolaq::Mx4RowsArgs& a, int D, hipStream_t stream);

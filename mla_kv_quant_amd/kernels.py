@@ -524,3 +524,168 @@ def mx4_attend_fwd(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, r
           D, R, int(max_q_len), float(sm_scale), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace),
           workspace.shape[0], _stream(q))
     return out
+
+
+# ---- rotary positions, expanded attention, accumulated weights, eviction -----------
+_ROTARY_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _rotary_heads(x, out, name, T, dim, dtype, dev):
+    """(heads, in strides, out strides) of a ``[T, heads, dim]`` or ``[T, dim]`` tensor and its output."""
+    for t, n in ((x, name), (out, name + "_out")):
+        _need(t, n, dtype, dev)
+        if t.ndim not in (2, 3) or t.shape != x.shape:
+            raise ValueError(f"{name} and its output must both be [T, heads, dim] or [T, dim]")
+        if t.shape[0] != T or t.shape[-1] != dim:
+            raise ValueError(f"{n} must be [{T}, (heads,) {dim}], got {tuple(t.shape)}")
+        if t.numel() and t.stride(-1) != 1:
+            raise ValueError(f"{n} must be contiguous in its last dim")
+    if any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"{name}_out must not repeat elements")
+    if x.ndim == 2:
+        return 1, (x.stride(0), 0), (out.stride(0), 0)
+    return x.shape[1], x.stride()[:2], out.stride()[:2]
+
+
+def rotary(positions: torch.Tensor, turns: torch.Tensor, scale: float, interleaved: bool, q: torch.Tensor,
+           q_out: torch.Tensor, k: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> None:
+    """``q`` (and ``k``), ``[T, heads, dim]`` or ``[T, dim]``, turned by ``positions [T]`` into their outputs."""
+    dev = q.device
+    if q.dtype not in _ROTARY_TYPES:
+        raise TypeError(f"q must be bf16, fp16 or fp32, got {q.dtype}")
+    _need_all(dev, ((positions, "positions", torch.int64, 1), (turns, "turns", torch.int64, 1)))
+    T, dim = positions.shape[0], 2 * turns.shape[0]
+    H, qs, qo = _rotary_heads(q, q_out, "q", T, dim, q.dtype, dev)
+    Hk, ks, ko = (0, (0, 0), (0, 0)) if k is None else _rotary_heads(k, k_out, "k", T, dim, q.dtype, dev)
+    _call(dev, _lib.load().rolaq_rotary, _p(positions), T, _p(turns), dim, float(scale), int(bool(interleaved)),
+          _ROTARY_TYPES[q.dtype], _p(q), qs[0], qs[1], _p(q_out), qo[0], qo[1], H, _p(k), ks[0], ks[1], _p(k_out),
+          ko[0], ko[1], Hk, _stream(q))
+
+
+def expanded_attend_workspace_bytes(T: int, N: int, B: int, H: int, nope: int, max_q_len: int, device) -> int:
+    """Bytes of :func:`expanded_attend_fwd`'s workspace for these sizes on ``device`` (0: none)."""
+    n = ctypes.c_int64(0)
+    _call(torch.device(device), _lib.load().rolaq_expanded_attend_workspace, int(T), int(N), int(B), int(H), int(nope),
+          int(max_q_len), ctypes.byref(n))
+    return n.value
+
+
+def expanded_attend_fwd(q: torch.Tensor, kv: torch.Tensor, k_pe: torch.Tensor, qo_indptr: torch.Tensor,
+                        kv_indptr: torch.Tensor, max_q_len: int, out: torch.Tensor, sm_scale: float,
+                        causal: bool = True, lse: torch.Tensor | None = None,
+                        workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of ``q [T, H, nope + rope]`` over ``kv [N, H, nope + value]`` and ``k_pe [N, rope]`` -> ``out [T, H, value]``.
+
+    ``workspace``: uint8, :func:`expanded_attend_workspace_bytes` long; allocated here when not given."""
+    dev = q.device
+    bf16 = torch.bfloat16
+    _need(q, "q", bf16, dev, 3)
+    _need(kv, "kv", bf16, dev, 3)
+    _need(k_pe, "k_pe", bf16, dev, 2)
+    _need(out, "out", bf16, dev, 3)
+    T, H, DK = q.shape
+    N, rope, value = k_pe.shape[0], k_pe.shape[1], out.shape[2]
+    nope = DK - rope
+    if kv.shape != (N, H, nope + value):
+        raise ValueError(f"kv must be [{N}, {H}, {nope + value}] to q's nope + rope, k_pe's rope and out's value, got "
+                         f"{tuple(kv.shape)}")
+    if out.shape[0] < T or out.shape[1] != H:
+        raise ValueError("out must be [>= T, H, value]")
+    if any(t.numel() and t.stride(-1) != 1 for t in (q, kv, k_pe, out)):
+        raise ValueError("q, kv, k_pe and out must be contiguous in their last dims")
+    i32 = torch.int32
+    _need_all(dev, ((qo_indptr, "qo_indptr", i32, 1), (kv_indptr, "kv_indptr", i32, 1)))
+    B = qo_indptr.shape[0] - 1
+    if B < 0 or kv_indptr.shape[0] < B + 1:
+        raise ValueError("index tensors are shorter than the batch")
+    if lse is not None:
+        _need_all(dev, ((lse, "lse", torch.float32, 2),))
+        if lse.shape[0] < T or lse.shape[1] != H:
+            raise ValueError("lse must be [>= T, H]")
+    if workspace is None:
+        # (a call that the library refuses is left to it)
+        taken = nope in (64, 128) and 1 <= H <= 128 and max_q_len >= 0
+        n = expanded_attend_workspace_bytes(T, N, B, H, nope, max_q_len, dev) if taken else 0
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    else:
+        _need_all(dev, ((workspace, "workspace", torch.uint8, 1),))
+    _call(dev, _lib.load().rolaq_expanded_attend_fwd, _p(q), q.stride(0), q.stride(1), _p(kv), kv.stride(0), kv.stride(1),
+          _p(k_pe), k_pe.stride(0), _p(qo_indptr), _p(kv_indptr), T, N, B, H, nope, rope, value, int(max_q_len),
+          float(sm_scale), int(bool(causal)), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace),
+          0 if workspace is None else workspace.shape[0], _stream(q))
+    return out
+
+
+def _acc_rows(acc, name, dev):
+    _need(acc, name, torch.float32, dev, 2)
+    if acc.numel() and (acc.stride(1) != 1 or (acc.shape[0] > 1 and acc.stride(0) < acc.shape[1])):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap")
+    return acc.stride(0) if acc.shape[0] > 1 else max(acc.shape[1], 1)
+
+
+def mx4_accumulate_weights(q: torch.Tensor, lse: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                           rope_buf: torch.Tensor, qo_indptr: torch.Tensor | None, kv_indptr: torch.Tensor,
+                           kv_indices: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int, acc: torch.Tensor,
+                           sm_scale: float, page_size: int = 1, req_idx: torch.Tensor | None = None,
+                           add: bool = True) -> torch.Tensor:
+    """Weights of the cached positions from ``q [T, H, D + R]`` with ``lse [T, H]``, summed into ``acc [rows, cols]``."""
+    dev = q.device
+    _need(q, "q", torch.bfloat16, dev, 3)
+    slots, D, R = _mx4_cache(codes, scales, rope_buf, dev)
+    T, H, DR = q.shape
+    if DR != D + R or (q.numel() and q.stride(2) != 1):
+        raise ValueError("q must be [T, H, D + R] with a contiguous last dim")
+    i32, i64 = torch.int32, torch.int64
+    _need_all(dev, ((lse, "lse", torch.float32, 2), (kv_indptr, "kv_indptr", i32, 1),
+                    (kv_indices, "kv_indices", i32, 1), (kv_lens, "kv_lens", i64, 1)))
+    if lse.shape[0] < T or lse.shape[1] != H:
+        raise ValueError("lse must be [>= T, H]")
+    if qo_indptr is not None:
+        _need_all(dev, ((qo_indptr, "qo_indptr", i32, 1),))
+    B = T if qo_indptr is None else qo_indptr.shape[0] - 1
+    if B < 0 or kv_indptr.shape[0] < B + 1 or kv_lens.shape[0] < B:
+        raise ValueError("index tensors are shorter than the batch")
+    if req_idx is not None:
+        _need_all(dev, ((req_idx, "req_idx", i64, 1),))
+        if req_idx.shape[0] < B:
+            raise ValueError("index tensors are shorter than the batch")
+    stride = _acc_rows(acc, "acc", dev)
+    _call(dev, _lib.load().rolaq_mx4_accumulate_weights, _p(q), q.stride(0), q.stride(1), _p(lse), _p(codes), _p(scales),
+          _p(rope_buf), slots, _p(qo_indptr), _p(kv_indptr), _p(kv_indices), kv_indices.shape[0], int(page_size),
+          _p(kv_lens), _p(req_idx), T, B, H, D, R, int(max_q_len), float(sm_scale), _p(acc), stride, acc.shape[0],
+          acc.shape[1], int(bool(add)), _stream(q))
+    return acc
+
+
+def evict(acc: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor, kv_lens: torch.Tensor, budget: int,
+          sink: int, recent: int, page_size: int, req_idx: torch.Tensor | None, max_kv_len: int, acc_out: torch.Tensor,
+          kept: torch.Tensor, kept_lens: torch.Tensor, freed: torch.Tensor,
+          workspace: torch.Tensor | None = None) -> None:
+    """The positions that stay of every request: slots in ``kept [B, budget]``, weights in ``acc_out``, the rest in ``freed``."""
+    dev = acc.device
+    i32, i64 = torch.int32, torch.int64
+    _need_all(dev, ((kv_indptr, "kv_indptr", i32, 1), (kv_indices, "kv_indices", i32, 1), (kv_lens, "kv_lens", i64, 1),
+                    (kept, "kept", i32, 2), (kept_lens, "kept_lens", i64, 1), (freed, "freed", i32, 1)))
+    B = kept.shape[0]
+    if kv_indptr.shape[0] < B + 1 or kv_lens.shape[0] < B or kept_lens.shape[0] < B:
+        raise ValueError("index tensors are shorter than the batch")
+    if kept.shape[1] != budget:
+        raise ValueError(f"kept must be [B, {budget}]")
+    if req_idx is not None:
+        _need_all(dev, ((req_idx, "req_idx", i64, 1),))
+        if req_idx.shape[0] < B:
+            raise ValueError("index tensors are shorter than the batch")
+    stride, out_stride = _acc_rows(acc, "acc", dev), _acc_rows(acc_out, "acc_out", dev)
+    if acc_out.shape != acc.shape:
+        raise ValueError("acc_out must have acc's shape")
+    if workspace is None:
+        n = ctypes.c_int64(0)
+        if 0 <= max_kv_len <= 1 << 30:  # (a call that the library refuses is left to it)
+            _call(dev, _lib.load().rolaq_evict_workspace, B, int(max_kv_len), ctypes.byref(n))
+        workspace = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+    else:
+        _need_all(dev, ((workspace, "workspace", torch.uint8, 1),))
+    _call(dev, _lib.load().rolaq_evict, _p(acc), stride, acc.shape[0], acc.shape[1], _p(acc_out), out_stride, _p(req_idx),
+          _p(kv_indptr), _p(kv_indices), kv_indices.shape[0], int(page_size), _p(kv_lens), B, int(max_kv_len), int(budget),
+          int(sink), int(recent), _p(kept), _p(kept_lens), _p(freed), freed.shape[0], _p(workspace),
+          0 if workspace is None else workspace.shape[0], _stream(acc))
