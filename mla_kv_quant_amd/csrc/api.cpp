@@ -766,10 +766,10 @@ int rolaq_expanded_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_strid
   if (T > (1 << 24) || N > (1 << 30)) return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries or 2^30 keys", fn);
   if (!aligned(q, 16) || q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
     return fail(ROLAQ_ERR_INVALID, "%s: q must be 16-byte aligned with strides multiple of 8", fn);
-  if (!aligned(kv, 16) || kv_stride_t % 8 || kv_stride_h % 8 || kv_stride_t < 0 || kv_stride_h < 0)
-    return fail(ROLAQ_ERR_INVALID, "%s: kv must be 16-byte aligned with strides multiple of 8", fn);
-  if (!aligned(k_pe, 16) || pe_stride_t % 8 || pe_stride_t < 0)
-    return fail(ROLAQ_ERR_INVALID, "%s: k_pe must be 16-byte aligned with a row stride multiple of 8", fn);
+  if (!aligned(kv, 16) || kv_stride_t % 8 || kv_stride_h % 8 || kv_stride_t < 0 || kv_stride_t >= (1 << 24) || kv_stride_h < 0)
+    return fail(ROLAQ_ERR_INVALID, "%s: kv must be 16-byte aligned with strides multiple of 8, the first below 2^24", fn);
+  if (!aligned(k_pe, 16) || pe_stride_t % 8 || pe_stride_t < 0 || pe_stride_t >= (1 << 24))
+    return fail(ROLAQ_ERR_INVALID, "%s: k_pe must be 16-byte aligned with a row stride multiple of 8, below 2^24", fn);
   if (!aligned(out, 16) || out_stride_t % 8 || out_stride_h % 8 || out_stride_t < 0 || out_stride_h < value)
     return fail(ROLAQ_ERR_INVALID, "%s: out must be 16-byte aligned with strides multiple of 8", fn);
   const int most = int(std::min<int64_t>(max_q_len, T));
