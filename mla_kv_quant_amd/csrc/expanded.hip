@@ -20,19 +20,20 @@ constexpr float kXMost = 256.f;              // a step's sum of weights above wh
 template <int DN>
 struct XGeo {
   static constexpr int DR = DN / 2, DK = DN + DR;
-  static constexpr int W = 4;                  // waves
-  static constexpr int ROWS = 32 * W;          // query rows of a block
-  static constexpr int KT = DN == 128 ? 32 : 64;  // keys of a step
-  static constexpr int U = KT / 32;            // units of 32 keys
+  static constexpr int W = 4;                     // waves
+  static constexpr int ROWS = 32 * W;             // query rows of a block
+  static constexpr int TK = DN == 128 ? 32 : 64;  // keys of a step
+  static constexpr int U = TK / 32;               // units of 32 keys
   static constexpr int NB = 2 * DN, PB = 2 * DR;  // bytes of a nope or value row, and of a rope row
-  static constexpr int NTILE = KT * NB, PTILE = KT * PB, KTILE = NTILE + PTILE;
-  static constexpr int RING = 4;               // steps whose keys, and values, lie in LDS
-  static constexpr int V0 = RING * KTILE;      // where the values start
+  static constexpr int NTILE = TK * NB, PTILE = TK * PB, KTILE = NTILE + PTILE;
+  static constexpr int RING = 4;                  // steps whose keys, and values, lie in LDS
+  static constexpr int V0 = RING * KTILE;         // where the values start
   static constexpr int LDS = V0 + RING * NTILE;
   static constexpr int KS = DK / 16, KN = DN / 16;  // K-steps of the scores, those of the nope part
-  static constexpr int ND = DN / 32;           // output column blocks
-  static constexpr int SM = KS * U, OM = 2 * ND * U, SLOTS = SM + OM;  // MFMAs of a step
-  static_assert(NTILE == 8192 && PTILE == 4096 && 2 * LDS <= 160 * 1024, "5 copies of 1 KB a wave, two blocks a CU");
+  static constexpr int ND = DN / 32;                // output column blocks
+  static constexpr int SM = KS * U, OM = 2 * ND * U, SL = SM + OM;  // MFMAs of a step
+  static constexpr int COPIES = 5;  // a wave's, of 1 KB each: two pieces of nope, one of rope, two of values
+  static_assert(NTILE == 2048 * W && PTILE == 1024 * W && 2 * LDS <= 160 * 1024, "pieces of a step, two blocks a CU");
 };
 
 __device__ __forceinline__ f32x16 mfma32x32x16_bf16(u32x4 a, u32x4 b, f32x16 c) {
@@ -60,11 +61,88 @@ __device__ __forceinline__ float x_sum2(uint32_t v, float acc) {  // acc + both 
                                          false);
 }
 
+struct XPlace {
+  int b, rb;           // request (-1: none), row block
+  int q0, nq, past;    // first query, queries computed, keys before the first query's own
+  int k0, nk;          // first key row, key rows
+};
+// The `want`-th row block of the batch: of up to 64 requests those that see most keys first, so that
+// the blocks that a launch ends with are short, in classes of an eighth to a quarter of the longest; in a
+// class, and of more requests, request after request, so that blocks that share keys run together
+// (4 x 2048 queries behind 14336 keys, 40 heads: 1830 us in classes of 128 keys, 1650 so).
+template <int ROWS>
+__device__ __forceinline__ XPlace x_place(const ExpandedArgs& a, uint32_t want) {
+  const int lane = threadIdx.x & 63;
+  const auto clampq = [&](int i) { return min(max(a.qo_indptr[i], 0), a.T); };
+  const auto clampk = [&](int i) { return min(max(a.kv_indptr[i], 0), a.N); };
+  XPlace p{-1, 0, 0, 0, 0, 0, 0};
+  uint32_t before = 0;
+  for (int c = 0; c < a.B; c += 64) {
+    const int i = min(c + lane, a.B - 1);
+    const int q0 = clampq(i), nq_all = max(clampq(i + 1) - q0, 0), nq = min(nq_all, a.max_q_len);
+    const int k0 = clampk(i), nk = max(clampk(i + 1) - k0, 0), past = nk - nq_all;
+    const int n = c + lane < a.B ? (nq + ROWS - 1) / ROWS : 0;
+    uint64_t hit;
+    int rb;
+    if (a.B <= 64) {
+      int most = n ? nk : 0;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+      most = __builtin_amdgcn_readfirstlane(most);
+            const int shift = max(29 - __builtin_clz(most | 1), 7);
+      // row blocks of this lane's request whose last row sees x << shift keys or more
+      const auto count = [&](int x) {
+        const int keys = x << shift;
+        if (!a.causal) return nk >= keys ? n : 0;
+        if (past + nq < keys) return 0;
+        return n - min(max((keys - past + ROWS - 1) / ROWS - 1, 0), n);
+      };
+      const auto total = [&](int x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)count(x)), 63); };
+      int x = 0;
+      if (total(0) <= want) return p;
+      for (int bit = 2; bit >= 0; --bit)
+        if (total(x | 1 << bit) > want) x |= 1 << bit;
+      const int above = count(x + 1), here = count(x) - above;
+      const uint32_t more = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)above), 63);
+      const uint32_t start = more + wave_scan((uint32_t)here) - (uint32_t)here;
+      hit = __builtin_amdgcn_ballot_w64(start <= want && want < start + (uint32_t)here);
+      rb = n - 1 - above - (int)(want - start);
+    } else {
+      const uint32_t incl = wave_scan((uint32_t)n), start = before + incl - (uint32_t)n;
+      hit = __builtin_amdgcn_ballot_w64(start <= want && want < start + (uint32_t)n);
+      rb = n - 1 - (int)(want - start);
+      before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    }
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      p.b = c + l;
+      p.rb = __builtin_amdgcn_readlane(rb, l);
+      p.q0 = __builtin_amdgcn_readlane(q0, l);
+      p.nq = __builtin_amdgcn_readlane(nq, l);
+      p.past = __builtin_amdgcn_readlane(past, l);
+      p.k0 = __builtin_amdgcn_readlane(k0, l);
+      p.nk = __builtin_amdgcn_readlane(nk, l);
+      return p;
+    }
+  }
+  return p;
+}
+
+// Copies of 16 bytes a lane to lds and lds + 1024: from base + o0 and base + 1024 + o1 (the
+// instruction's offset counts on both sides).
+__device__ __forceinline__ void x_copy2(const void* base, uint32_t o0, uint32_t o1, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:1024" ::"s"(lds),
+      "v"(o0), "v"(o1), "s"(base)
+      : "memory", "m0");
+}
+
 // LSE: for calls that ask for it, the sum of the weights before their rounding as well.
 template <int DN, bool LSE>
 __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
   using G = XGeo<DN>;
-  constexpr int NB = G::NB, PB = G::PB, KT = G::KT, KS = G::KS, KN = G::KN, ND = G::ND, U = G::U, RING = G::RING;
+  constexpr int NB = G::NB, PB = G::PB, TK = G::TK, KS = G::KS, KN = G::KN, ND = G::ND, U = G::U, RING = G::RING;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   const int tid = threadIdx.x, lane = tid & 63, la32 = lane & 31, g = lane >> 5;
@@ -75,86 +153,57 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
   const int h = item % (uint32_t)a.H;
   const uint32_t rest = item / (uint32_t)a.H;
   const int part = rest % (uint32_t)a.splits;
-  const uint32_t want = rest / (uint32_t)a.splits;  // row block of the batch
-  const auto clampq = [&](int i) { return min(max(a.qo_indptr[i], 0), a.T); };
-  const auto clampk = [&](int i) { return min(max(a.kv_indptr[i], 0), a.N); };
-  int b = -1, rb = 0;
-  {
-    uint32_t before = 0;
-    for (int c = 0; c < a.B; c += 64) {
-      const int i = min(c + lane, a.B - 1);
-      const int nq = min(max(clampq(i + 1) - clampq(i), 0), a.max_q_len);
-      const uint32_t n = c + lane < a.B ? (uint32_t)((nq + G::ROWS - 1) / G::ROWS) : 0u;
-      const uint32_t incl = wave_scan(n), start = before + incl - n;
-      const uint64_t hit = __builtin_amdgcn_ballot_w64(start <= want && want < start + n);
-      if (hit) {
-        const int l = __builtin_ctzll(hit);
-        b = c + l;
-        rb = __builtin_amdgcn_readlane((int)n, l) - 1 - (int)(want - (uint32_t)__builtin_amdgcn_readlane((int)start, l));
-        break;
-      }
-      before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-    }
-  }
-  if (b < 0) return;
-  const int q0 = __builtin_amdgcn_readfirstlane(clampq(b)), k0 = __builtin_amdgcn_readfirstlane(clampk(b));
-  const int nq_all = max(__builtin_amdgcn_readfirstlane(clampq(b + 1)) - q0, 0), nq = min(nq_all, a.max_q_len);
-  const int nk = max(__builtin_amdgcn_readfirstlane(clampk(b + 1)) - k0, 0);
-  const int row0 = rb * G::ROWS;
-  const int past = nk - nq_all;
+  const XPlace at = x_place<G::ROWS>(a, rest / (uint32_t)a.splits);
+  if (at.b < 0) return;
+  const int q0 = at.q0, nq = at.nq, k0 = at.k0, nk = at.nk, row0 = at.rb * G::ROWS;
   // keys that row r sees
-  const auto sees = [&](int r) { return a.causal ? min(max(past + r + 1, 0), nk) : nk; };
-  const int steps_all = (sees(min(row0 + G::ROWS, nq) - 1) + KT - 1) / KT;
-  const int t0 = (int)((int64_t)steps_all * part / a.splits), t1 = (int)((int64_t)steps_all * (part + 1) / a.splits);
-  const int n = t1 - t0;
-  const int first_key = KT * t0;  // steps are counted from here
+  const auto sees = [&](int r) { return a.causal ? min(max(at.past + r + 1, 0), nk) : nk; };
+  const int tiles = (sees(min(row0 + G::ROWS, nq) - 1) + TK - 1) / TK;
+  const int t0 = (int)((int64_t)tiles * part / a.splits), n = (int)((int64_t)tiles * (part + 1) / a.splits) - t0;
+  const int first_key = TK * t0;  // keys and steps are counted from here
 
   // ---- tile copies ------------------------------------------------------------------
   // This wave's pieces of a step: two of nope, one of rope, two of values, 64 chunks each.
-  const uint8_t* const kv =
-      reinterpret_cast<const uint8_t*>(a.kv + (int64_t)(k0 + first_key) * a.kv_st + (int64_t)h * a.kv_sh);
-  const uint8_t* const pe = reinterpret_cast<const uint8_t*>(a.pe + (int64_t)(k0 + first_key) * a.pe_st);
+  // Every step issues the same copies: past the last tile that one again, to places that nothing reads any
+  // more; rows past the last key read that one.
   constexpr int NC = NB / 16, PC = PB / 16;  // chunks of a row
+  const uint32_t kv_row = 2 * (uint32_t)a.kv_st, pe_row = 2 * (uint32_t)a.pe_st;  // bytes
+  // (1024 bytes before the first row, so that no offset is negative)
+  const uint8_t* const kv =
+      reinterpret_cast<const uint8_t*>(a.kv + (int64_t)(k0 + first_key) * a.kv_st + (int64_t)h * a.kv_sh) - 1024;
+  const uint8_t* const pe = reinterpret_cast<const uint8_t*>(a.pe + (int64_t)(k0 + first_key) * a.pe_st);
   const auto n_row = [&](int j) { return (64 * (2 * wave + j) + lane) / NC; };
-  const auto n_off = [&](int j, int row) { return (uint32_t)(row * 2 * (int)a.kv_st); };
-  uint32_t noff[2], voff[2], poff;
+  const int p_row = (64 * wave + lane) / PC;
+  uint32_t noff[2], voff[2], poff = p_row * pe_row + 16 * ((lane % PC) ^ k_swz<PB>(p_row));
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int r = n_row(j), c = lane % NC;
-    noff[j] = n_off(j, r) + 16 * (c ^ k_swz<NB>(r));
-    voff[j] = n_off(j, r) + NB + 16 * (c ^ v_swz<NB>(r));
+    noff[j] = r * kv_row + 1024 * (1 - j) + 16 * (c ^ k_swz<NB>(r));
+    voff[j] = r * kv_row + 1024 * (1 - j) + NB + 16 * (c ^ v_swz<NB>(r));
   }
-  const int p_row = (64 * wave + lane) / PC;
-  poff = (uint32_t)(p_row * 2 * (int)a.pe_st) + 16 * ((lane % PC) ^ k_swz<PB>(p_row));
-  // rows past the last key read that one again
-  const auto copy_keys = [&](int t, int slot) {
-    const uint8_t* const ks = kv + (int64_t)(KT * t) * (2 * a.kv_st);
-    const uint8_t* const ps = pe + (int64_t)(KT * t) * (2 * a.pe_st);
-    const uint32_t at = lds0 + slot * G::KTILE;
-    const int last = nk - 1 - first_key - KT * t;
-    uint32_t o0 = noff[0], o1 = noff[1], o2 = poff;
-    if (__builtin_expect(last < KT - 1, 0)) {
-      asm volatile("");
-      o0 -= n_off(0, max(n_row(0) - last, 0));
-      o1 -= n_off(1, max(n_row(1) - last, 0));
-      o2 -= (uint32_t)(max(p_row - last, 0) * 2 * (int)a.pe_st);
-    }
-    copy16(ks, o0, at + 1024 * (2 * wave));
-    copy16(ks, o1, at + 1024 * (2 * wave + 1));
-    copy16(ps, o2, at + G::NTILE + 1024 * wave);
+  const auto past_last = [&](int r) { return (uint32_t)max(r - (nk - 1 - first_key - TK * (n - 1)), 0); };
+  const auto tile_of = [&](const uint8_t* p, uint32_t row, int t) {
+    return p + (uint64_t)(uint32_t)min(t, n - 1) * (uint64_t)(TK * row);
   };
-  const auto copy_values = [&](int t, int slot) {
-    const uint8_t* const ks = kv + (int64_t)(KT * t) * (2 * a.kv_st);
-    const uint32_t at = lds0 + G::V0 + slot * G::NTILE;
-    const int last = nk - 1 - first_key - KT * t;
-    uint32_t o0 = voff[0], o1 = voff[1];
-    if (__builtin_expect(last < KT - 1, 0)) {
+  const auto copy_nope = [&](int t, int slot) __attribute__((always_inline)) {
+    if (__builtin_expect(t == n - 1, 0)) {  // (once: the later ones are this tile again)
       asm volatile("");
-      o0 -= n_off(0, max(n_row(0) - last, 0));
-      o1 -= n_off(1, max(n_row(1) - last, 0));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) noff[j] -= past_last(n_row(j)) * kv_row;
+      poff -= past_last(p_row) * pe_row;
     }
-    copy16(ks, o0, at + 1024 * (2 * wave));
-    copy16(ks, o1, at + 1024 * (2 * wave + 1));
+    x_copy2(tile_of(kv, kv_row, t), noff[0], noff[1], lds0 + slot * G::KTILE + 2048 * wave);
+  };
+  const auto copy_rope = [&](int t, int slot) __attribute__((always_inline)) {
+    copy16(tile_of(pe, pe_row, t), poff, lds0 + slot * G::KTILE + G::NTILE + 1024 * wave);
+  };
+  const auto copy_values = [&](int t, int slot) __attribute__((always_inline)) {
+    if (__builtin_expect(t == n - 1, 0)) {
+      asm volatile("");
+#pragma unroll
+      for (int j = 0; j < 2; ++j) voff[j] -= past_last(n_row(j)) * kv_row;
+    }
+    x_copy2(tile_of(kv, kv_row, t), voff[0], voff[1], lds0 + G::V0 + slot * G::NTILE + 2048 * wave);
   };
 
   // ---- query rows -------------------------------------------------------------------
@@ -165,17 +214,24 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
 #pragma unroll
     for (int s = 0; s < KS; ++s) qf[s] = gload<u32x4>(p + 16 * s);
   }
-  // The first steps' copies go out behind the query's loads, which are waited for here, so that
-  // no wait for them is left behind the copies: K 0, K 1, then K j + 2 and V j together.
+  // The first tiles go out behind the query's loads, which are waited for here, so that no wait for
+  // them is left behind the copies.
+  if (n > 0) {
 #pragma unroll
-  for (int t = 0; t < RING; ++t)
-    if (t < n) copy_keys(t, t);
-  if (n > 0) copy_values(0, 0);
-  if (n > 1) copy_values(1, 1);
+    for (int t = 0; t < RING; ++t) {
+      copy_nope(t, t);
+      copy_rope(t, t);
+    }
+#pragma unroll
+    for (int t = 0; t < RING - 2; ++t) copy_values(t, t);
+  }
 #pragma unroll
   for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(qf[s]));
-  const int vis = sees(row) - first_key;        // counted from first_key
-  const int vis_min = sees(row0) - first_key;   // seen by every row of the block
+  const int vis = sees(row) - first_key;       // keys that the row sees, from first_key on
+  const int vis_min = sees(row0) - first_key;  // seen by every row of the block
+  // steps of which this wave has rows that see something: in the others it only copies
+  const int row_last = min(row0 + 32 * wave + 31, nq - 1);
+  const int own = row0 + 32 * wave >= nq ? 0 : min(max((sees(row_last) - first_key + TK - 1) / TK, 0), n);
 
   f32x16 O[ND];  // O^T: columns 32 d + 8 (j / 4) + 4 g + j % 4 of the lane's row
 #pragma unroll
@@ -183,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) O[d][j] = 0.f;
   float ref = kXNoRef, sum = 0.f, usum = 0.f;  // usum (LSE): of the weights as they were
-  float most = kXMost;                         // the largest sum of a unit that needs no look at the reference
+  float most = kXMost;                         // the largest sum of a step that needs no look at the reference
   const float c2 = a.sm_scale * kLog2e;
 
   // ---- LDS operands -----------------------------------------------------------------
@@ -199,11 +255,11 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
     vbase[d] = G::V0 + r * NB + 16 * ((4 * d + 2 * ((lane >> 4) & 1) + ((la & 3) >> 1)) ^ v_swz<NB>(r)) + 8 * (la & 1);
   }
   // K-step s of unit u of the keys in `slot`
-  const auto kread = [&](int slot, int u, int s) {
+  const auto kread = [&](int slot, int u, int s) __attribute__((always_inline)) {
     return *reinterpret_cast<const u32x4*>(smem + kbase[s] + slot * G::KTILE + u * 32 * (s < KN ? NB : PB));
   };
   // columns 32 d .. of 16 keys m of the values in `slot`, transposed
-  const auto vread = [&](int slot, int m, int d) {
+  const auto vread = [&](int slot, int m, int d) __attribute__((always_inline)) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     const uint8_t* const p = smem + vbase[d] + slot * G::NTILE + 16 * m * NB;
@@ -213,48 +269,48 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
   };
 
   // ---- the parts of a step ------------------------------------------------------------
-  f32x16 zero;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) zero[j] = 0.f;
   // MFMA i of a step's scores: units in turns, so that chains of one unit are apart
   const auto score = [&](f32x16 (&S)[U], int i, u32x4 k) __attribute__((always_inline)) {
     const int u = i % U, s = i / U;
+    f32x16 zero;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) zero[j] = 0.f;
     S[u] = mfma32x32x16_bf16(k, qf[s], s == 0 ? zero : S[u]);
   };
-  const auto output = [&](const u32x4 (&P)[2 * U], int i, u32x4 v) __attribute__((always_inline)) { O[i % ND] = mfma32x32x16_bf16(v, P[i / ND], O[i % ND]); };
+  const auto output = [&](const u32x4 (&P)[2 * U], int i, u32x4 v) __attribute__((always_inline)) {
+    O[i % ND] = mfma32x32x16_bf16(v, P[i / ND], O[i % ND]);
+  };
   // positions that a row does not see
   const auto mask = [&](f32x16 (&S)[U], int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const int lim = vis - TK * t - 32 * u - 4 * g;
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (KT * t + 32 * u + 8 * (j / 4) + 4 * g + j % 4 >= vis) S[u][j] = -INFINITY;
+      for (int j = 0; j < 16; ++j) S[u][j] = 8 * (j / 4) + j % 4 < lim ? S[u][j] : -INFINITY;
+    }
   };
-  // Weights of a step in 6 (LSE 8) operations for each of 8 U pairs of keys
+  // Weights of a step in OPS operations for each of 8 U pairs of keys
   float e0, e1, us[2], uu;
   constexpr int OPS = LSE ? 8 : 6;
   const auto weigh = [&](const f32x16 (&S)[U], u32x4 (&P)[2 * U], int o) __attribute__((always_inline)) {
-    const int e = o / OPS, m = e / 4, d = e % 4, j = 8 * (m % 2) + 2 * d;
-    switch (o % OPS) {
-      case 0: e0 = fmaf(S[m / 2][j], c2, -ref); break;
-      case 1: e1 = fmaf(S[m / 2][j + 1], c2, -ref); break;
-      case 2: e0 = __builtin_amdgcn_exp2f(e0); break;
-      case 3: e1 = __builtin_amdgcn_exp2f(e1); break;
-      case 4: {
-        uint32_t w = pack_bf16(e0, e1);
-        asm volatile("" : "+v"(w));  // formed here, not where a later step uses it
-        P[m][d] = w;
-        break;
-      }
-      case 5:
-        us[e % 2] = x_sum2(P[m][d], us[e % 2]);
-        asm volatile("" : "+v"(us[e % 2]));
-        break;
-      case 6: uu += e0; break;
-      default:
-        uu += e1;
-        asm volatile("" : "+v"(uu));
-        break;
+    const int e = o / OPS, m = e / 4, d = e % 4, j = 8 * (m % 2) + 2 * d, op = o % OPS;
+    if (op == 0) e0 = fmaf(S[m / 2][j], c2, -ref);
+    if (op == 1) e1 = fmaf(S[m / 2][j + 1], c2, -ref);
+    if (op == 2) e0 = __builtin_amdgcn_exp2f(e0);
+    if (op == 3) e1 = __builtin_amdgcn_exp2f(e1);
+    if (op == 4) {
+      uint32_t w = pack_bf16(e0, e1);
+      asm volatile("" : "+v"(w));  // formed here, not where a later step uses it
+      P[m][d] = w;
+    }
+    if (op == 6) uu += e0;
+    if (op == 7) {
+      uu += e1;
+      asm volatile("" : "+v"(uu));
+    }
+    if (op == 5) {
+      us[e % 2] = x_sum2(P[m][d], us[e % 2]);
+      asm volatile("" : "+v"(us[e % 2]));
     }
   };
   // A step's sum says whether a weight passed the slack (or was the row's first): then the
@@ -271,7 +327,9 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
         for (int j = 0; j < 16; ++j) mx = fmaxf(mx, S[u][j]);
       mx = x_max_halves(mx) * c2;
       const bool over = x_max_halves(got) > most;
-      const float to = over ? fmaxf(mx, ref) : ref, f = __builtin_amdgcn_exp2f(ref - to);
+      const float to = over ? fmaxf(mx, ref) : ref;
+      // (nothing was summed before the first reference, but an infinite value may be in O)
+      const float f = ref == kXNoRef ? 1.f : __builtin_amdgcn_exp2f(ref - to);
       ref = to;
       if (over) most = fabsf(to) < 0x1p24f ? kXMost : -1.f;
       sum *= f;
@@ -294,7 +352,7 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
           }
           const uint32_t w = over ? pack_bf16(p0, p1) : P[m][d];
           P[m][d] = w;
-          s0 = x_sum2(w, s0);
+          s0 += bf16_lo(w) + bf16_hi(w);
           s1 += p0 + p1;
         }
       got = over ? s0 : got;
@@ -303,11 +361,11 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
     sum += got;
     if (LSE) usum += uu;
   };
-  // Values of a step of which a row may not see all may be anything where it does not see them, and 0
-  // times what is not finite would be NaN. So before such a step's output every wave looks for
+  // Values of a tile of which a row may not see all may be anything where it does not see them, and 0
+  // times what is not finite would be NaN. So before such a tile's output every wave looks for
   // one; where there is one, all agree, each clears those of its own pieces,
-  // and what they add to the rows that see them comes behind, from memory.
-  const auto clean = [&](int slot) __attribute__((always_inline)) {
+  // and what they add to the rows that see them comes from memory.
+  const auto clean = [&](int slot, int t) __attribute__((always_inline)) {
     u16x2_t big = {0, 0};
     uint8_t* const v = smem + G::V0 + slot * G::NTILE + 16 * lane;
 #pragma unroll
@@ -317,7 +375,7 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
       for (int e = 0; e < 4; ++e)
         big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2_t, w[e] & 0x7fff7fffu));
     }
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(big[0] >= 0x7f80 || big[1] >= 0x7f80) == 0, 1)) return false;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(big[0] >= 0x7f80 || big[1] >= 0x7f80) == 0, 1)) return;
     __syncthreads();
 #pragma unroll
     for (int k = 2 * wave; k < 2 * wave + 2; ++k) {
@@ -330,12 +388,9 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
       *reinterpret_cast<u32x4*>(v + 1024 * k) = w;
     }
     __syncthreads();
-    return true;
-  };
-  const auto add_cleared = [&](int t) __attribute__((always_inline)) {
 #pragma unroll 1
-    for (int k = KT * t; k < min(KT * (t + 1), nk - first_key); ++k) {
-      const uint8_t* const vr = kv + (int64_t)k * (2 * a.kv_st) + NB + 8 * g;
+    for (int k = TK * t; k < min(TK * (t + 1), nk - first_key); ++k) {
+      const uint8_t* const vr = kv + (int64_t)k * kv_row + 1024 + NB + 8 * g;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
@@ -343,62 +398,59 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
           const u32x2 w = gload<u32x2>(vr + 64 * d + 16 * q);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float x = e % 2 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
-            if (k < vis && !(fabsf(x) < INFINITY)) O[d][4 * q + e] += x;
+            const float y = e % 2 ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
+            if (k < vis && !(fabsf(y) < INFINITY)) O[d][4 * q + e] += y;
           }
         }
     }
   };
 
   // Step t, in ring slot I of t: the matrix cores form the scores of step t + 1 and the output of
-  // step t - 1 while the vector units turn the scores S of step t into weights.
+  // step t - 1 while the vector units turn the scores S of step t into weights. Its operands
+  // come in a ring of AHEAD + 1, of 5 in a row the second and the fourth the output's;
+  // where the last of them are under way it meets the other waves and turns to the next step's.
   // (The first step has zero weights for its output, and zero values: slot RING - 1 is cleared.)
-  bool edge_before = false;
+  constexpr int AHEAD = 4, SL = G::SL;
+  static_assert(G::SM * 2 == G::OM * 3 && SL % (AHEAD + 1) == 0, "three of the scores to two of the output");
+  u32x4 f[AHEAD + 1];
+  const auto fetch = [&](auto I, int y) __attribute__((always_inline)) {
+    constexpr int i = decltype(I)::value;
+    const int k = 2 * (y / 5) + y % 5 / 2, s = 3 * (y / 5) + y % 5 / 2;
+    f[y % (AHEAD + 1)] = y % 5 % 2 == 0 ? kread((i + 1) % RING, s % U, s / U) : vread((i + RING - 1) % RING, k / ND, k % ND);
+  };
+  // Before step t: K t + 1 and V t - 1 are there (two steps' copies may be under way), and no wave
+  // reads K t and V t - 2 any more.
+  const auto meet = [&](int slot, int t) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((RING - 2) * G::COPIES) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (__builtin_expect(TK * t > vis_min && t > 0, 0)) clean((slot + RING - 1) % RING, t - 1);
+  };
   const auto step = [&](auto I, int t, f32x16 (&S)[U], f32x16 (&Sn)[U], u32x4 (&P)[2 * U], const u32x4 (&Pb)[2 * U])
                         __attribute__((always_inline)) {
-    constexpr int i = decltype(I)::value, kslot = (i + 1) % RING, vslot = (i + RING - 1) % RING;
-    if (t + 3 < n)
-      wait_loads<10>();  // K t + 1 and V t - 1 are there; two steps' copies may be under way
-    else
-      wait_loads<0>();
-    __builtin_amdgcn_s_barrier();  // every wave's; and K t and V t - 2 are no longer read
-    asm volatile("" ::: "memory");
-    if (t + 4 < n) copy_keys(t + 4, i);
-    if (t + 2 < n) copy_values(t + 2, (i + 2) % RING);
-    const bool edge = KT * (t + 1) > vis_min;
-    if (__builtin_expect(edge, 0)) mask(S, t);
-    const bool cleared = edge_before && clean(vslot);
+    constexpr int i = decltype(I)::value;
+    const std::integral_constant<int, (i + 1) % RING> next;
+    if (__builtin_expect(TK * (t + 1) > vis_min, 0)) mask(S, t);
     us[0] = us[1] = uu = 0.f;
-    // MFMA x of the step: of 5 in a row the second and the fourth are the output's
-    constexpr int AHEAD = 4, SL = G::SLOTS, ALL = 8 * U * OPS;
-    static_assert(G::SM * 2 == G::OM * 3, "three of the scores to two of the output");
-    const auto fetch = [&](int x) __attribute__((always_inline)) {
-      const int q = x / 5, r = x % 5;
-      if (r % 2 == 0) {
-        const int k = 3 * q + r / 2;
-        return kread(kslot, k % U, k / U);
-      }
-      const int k = 2 * q + r / 2;
-      return vread(vslot, k / ND, k % ND);
-    };
-    u32x4 f[AHEAD + 1];
-#pragma unroll
-    for (int x = 0; x < AHEAD; ++x) f[x] = fetch(x);
-#pragma unroll
-    for (int x = 0; x < SL; ++x) {
-      if (x + AHEAD < SL) f[(x + AHEAD) % (AHEAD + 1)] = fetch(x + AHEAD);
-      const int q = x / 5, r = x % 5;
-      if (r % 2 == 0)
-        score(Sn, 3 * q + r / 2, f[x % (AHEAD + 1)]);
+    static_for<SL>([&](auto Y) __attribute__((always_inline)) {
+      constexpr int y = decltype(Y)::value, k = 2 * (y / 5) + y % 5 / 2, ALL = 8 * U * OPS;
+      if constexpr (y == 1) copy_nope(t + RING, i);
+      if constexpr (y == 6) copy_rope(t + RING, i);
+      if constexpr (y == 11) copy_values(t + RING - 2, (i + RING - 2) % RING);
+      if constexpr (y == SL - AHEAD) meet((i + 1) % RING, t + 1);
+      if constexpr (y + AHEAD < SL)
+        fetch(I, y + AHEAD);
       else
-        output(Pb, 2 * q + r / 2, f[x % (AHEAD + 1)]);
-#pragma unroll
-      for (int o = x * ALL / SL; o < (x + 1) * ALL / SL; ++o) weigh(S, P, o);
+        fetch(next, y + AHEAD - SL);
+      if constexpr (y % 5 % 2 == 0)
+        score(Sn, 3 * (y / 5) + y % 5 / 2, f[y % (AHEAD + 1)]);
+      else
+        output(Pb, k, f[y % (AHEAD + 1)]);
+      constexpr int o0 = y * ALL / SL, o1 = (y + 1) * ALL / SL;
+      static_for<o1 - o0>([&](auto o) __attribute__((always_inline)) { weigh(S, P, o0 + decltype(o)::value); });
       __builtin_amdgcn_sched_barrier(0);
-    }
-    if (__builtin_expect(cleared, 0)) add_cleared(t - 1);
+    });
     settle(S, P);
-    edge_before = edge;
   };
 
   if (n > 0) {
@@ -410,40 +462,46 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
     for (int k = 0; k < 2; ++k)
       *reinterpret_cast<u32x4*>(smem + G::V0 + (RING - 1) * G::NTILE + 1024 * (2 * wave + k) + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
     wait_loads<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    __syncthreads();
+    if (own > 0) {
 #pragma unroll
-    for (int x = 0; x < G::SM; ++x) {
-      score(SA, x, kread(0, x % U, x / U));
-      __builtin_amdgcn_sched_barrier(0);
+      for (int x = 0; x < G::SM; ++x) {
+        score(SA, x, kread(0, x % U, x / U));
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
+    __syncthreads();  // (K 0 is no longer read)
     int t = 0;
-    for (;;) {
-      step(std::integral_constant<int, 0>{}, t, SA, SB, PA, PB_);
-      if (++t >= n) break;
-      step(std::integral_constant<int, 1>{}, t, SB, SA, PB_, PA);
-      if (++t >= n) break;
-      step(std::integral_constant<int, 2>{}, t, SA, SB, PA, PB_);
-      if (++t >= n) break;
-      step(std::integral_constant<int, 3>{}, t, SB, SA, PB_, PA);
-      if (++t >= n) break;
-    }
-    // the last step's output
-    wait_loads<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if ((n & 1) == 0) {
+    if (own > 0) {
+      static_for<AHEAD>([&](auto Y) __attribute__((always_inline)) { fetch(std::integral_constant<int, 0>{}, decltype(Y)::value); });
+      for (;;) {
+        step(std::integral_constant<int, 0>{}, t, SA, SB, PA, PB_);
+        if (++t == own) break;
+        step(std::integral_constant<int, 1>{}, t, SB, SA, PB_, PA);
+        if (++t == own) break;
+        step(std::integral_constant<int, 2>{}, t, SA, SB, PA, PB_);
+        if (++t == own) break;
+        step(std::integral_constant<int, 3>{}, t, SB, SA, PB_, PA);
+        if (++t == own) break;
+      }
+      // the last step's output (its values were met for)
+      if ((own & 1) == 0) {
 #pragma unroll
-      for (int m = 0; m < 2 * U; ++m) PA[m] = PB_[m];
-    }
-    const int slot = (n - 1) % RING;
-    const bool cleared = edge_before && clean(slot);
+        for (int m = 0; m < 2 * U; ++m) PA[m] = PB_[m];
+      }
 #pragma unroll
-    for (int x = 0; x < G::OM; ++x) {
-      output(PA, x, vread(slot, x / ND, x % ND));
-      if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      for (int x = 0; x < G::OM; ++x) {
+        output(PA, x, vread((own - 1) % RING, x / ND, x % ND));
+        if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
     }
-    if (__builtin_expect(cleared, 0)) add_cleared(n - 1);
+    for (; t < n; ++t) {  // steps of other waves
+      copy_nope(t + RING, t % RING);
+      copy_rope(t + RING, t % RING);
+      copy_values(t + RING - 2, (t + RING - 2) % RING);
+      meet((t + 1) % RING, t + 1);
+    }
+    wait_loads<0>();  // no copy may outlive the block's LDS
   }
 
   // ---- normalise and store -----------------------------------------------------------------
@@ -451,10 +509,10 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
   const float l = x_add_halves(sum);
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   const float ul = LSE ? x_add_halves(usum) : 0.f;
-  const int64_t at = (int64_t)(q0 + row) * a.H + h;
+  const int64_t to = (int64_t)(q0 + row) * a.H + h;
   if (a.splits > 1) {
     const int64_t total = (int64_t)a.T * a.H;
-    float* const po = a.ws + (part * total + at) * DN + 4 * g;
+    float* const po = a.ws + (part * total + to) * DN + 4 * g;
     if (ok) {
 #pragma unroll
       for (int d = 0; d < ND; ++d)
@@ -462,13 +520,13 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<f32x4*>(po + 32 * d + 8 * q) =
               f32x4{O[d][4 * q] * inv, O[d][4 * q + 1] * inv, O[d][4 * q + 2] * inv, O[d][4 * q + 3] * inv};
-      float* const pl = a.ws + a.splits * total * DN + part * total + at;
+      float* const pl = a.ws + a.splits * total * DN + part * total + to;
       if (g == 0) *pl = l == 0.f ? -INFINITY : ref + __log2f(l);
       if (LSE && g == 0) pl[a.splits * total] = ul == 0.f ? -INFINITY : ref + __log2f(ul);
     }
     return;
   }
-  if (LSE && ok && g == 0) a.lse[at] = ul == 0.f ? -INFINITY : (ref + __log2f(ul)) * kLn2;
+  if (LSE && ok && g == 0) a.lse[to] = ul == 0.f ? -INFINITY : (ref + __log2f(ul)) * kLn2;
   uint16_t* const dst = a.out + (int64_t)(q0 + row) * a.o_st + (int64_t)h * a.o_sh;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
@@ -480,9 +538,9 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
     // the halves' pieces joined to 8 consecutive columns a lane: 32 d + 16 p + 8 g + (0..7)
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const auto x = __builtin_amdgcn_permlane32_swap(w[2 * p][0], w[2 * p + 1][0], false, false);
-      const auto y = __builtin_amdgcn_permlane32_swap(w[2 * p][1], w[2 * p + 1][1], false, false);
-      if (ok) *reinterpret_cast<u32x4*>(dst + 32 * d + 16 * p + 8 * g) = u32x4{x[0], y[0], x[1], y[1]};
+      const auto y = __builtin_amdgcn_permlane32_swap(w[2 * p][0], w[2 * p + 1][0], false, false);
+      const auto z = __builtin_amdgcn_permlane32_swap(w[2 * p][1], w[2 * p + 1][1], false, false);
+      if (ok) *reinterpret_cast<u32x4*>(dst + 32 * d + 16 * p + 8 * g) = u32x4{y[0], z[0], y[1], z[1]};
     }
   }
 }
@@ -531,12 +589,10 @@ struct XPlan {
   int64_t blocks;  // row blocks of the batch at most
   int splits;
 };
-template <int DN>
 XPlan expanded_plan(int64_t T, int64_t N, int B, int H, int max_q_len, int num_cus) {
-  using G = XGeo<DN>;
-  XPlan p;
-  p.blocks = std::min<int64_t>((int64_t)B * ((max_q_len + G::ROWS - 1) / G::ROWS), T / G::ROWS + B);
-  // parts of the keys: what gives each CU a block, of four tiles at least in the mean
+  constexpr int rows = XGeo<128>::ROWS;
+  XPlan p{std::min<int64_t>((int64_t)B * ((max_q_len + rows - 1) / rows), T / rows + B), 1};
+  // parts of the keys: what gives each CU a block, of 256 keys at least in the mean
   const int64_t by_cus = num_cus / std::max<int64_t>(p.blocks * H, 1), by_keys = N / ((int64_t)B * 256);
   p.splits = (int)std::max<int64_t>(1, std::min(by_cus, by_keys));
   return p;
@@ -545,12 +601,11 @@ XPlan expanded_plan(int64_t T, int64_t N, int B, int H, int max_q_len, int num_c
 template <int DN, bool LSE>
 hipError_t launch_expanded(ExpandedArgs a, int num_cus, hipStream_t stream) {
   using G = XGeo<DN>;
-  const XPlan p = expanded_plan<DN>(a.T, a.N, a.B, a.H, a.max_q_len, num_cus);
+  const XPlan p = expanded_plan(a.T, a.N, a.B, a.H, a.max_q_len, num_cus);
   a.splits = p.splits;
-  const int lds = G::LDS;
-  hipError_t e = hipFuncSetAttribute((const void*)expanded_kernel<DN, LSE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipError_t e = hipFuncSetAttribute((const void*)expanded_kernel<DN, LSE>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((expanded_kernel<DN, LSE>), dim3((unsigned)(p.blocks * a.H * a.splits)), dim3(256), lds, stream, a);
+  hipLaunchKernelGGL((expanded_kernel<DN, LSE>), dim3((unsigned)(p.blocks * a.H * a.splits)), dim3(256), G::LDS, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t rows = (int64_t)a.T * a.H, per = 256 / (DN / 4);
@@ -561,9 +616,7 @@ hipError_t launch_expanded(ExpandedArgs a, int num_cus, hipStream_t stream) {
 }  // namespace rolaq
 
 int64_t rolaq_expanded_ws_bytes(int64_t T, int64_t N, int B, int H, int DN, int max_q_len, int num_cus) {
-  using namespace rolaq;
-  const int s = DN == 128 ? expanded_plan<128>(T, N, B, H, max_q_len, num_cus).splits
-                          : expanded_plan<64>(T, N, B, H, max_q_len, num_cus).splits;
+  const int s = rolaq::expanded_plan(T, N, B, H, max_q_len, num_cus).splits;
   return s > 1 ? (int64_t)s * T * H * (DN + 2) * 4 : 0;
 }
 

@@ -95,6 +95,8 @@ def test_attention(dn, H, qlens, klens, causal):
 @pytest.mark.parametrize("dn,H,qlens,klens", [
     (128, 2, [700, 2000], [700, 2500]), (64, 2, [1500, 5], [4000, 5000]), (128, 128, [5], [300]), (128, 1, [2], [20000]),
     (64, 40, [1] * 6, [900] * 6), (64, 8, [1100] * 3, [1100] * 3),
+    (128, 128, [260, 1, 300, 257], [400, 70, 300, 600]), (64, 128, [260, 1, 300, 257], [400, 70, 300, 600]),
+    (128, 40, [1500, 3, 700, 64], [1500, 2000, 701, 65]), (64, 40, [1500, 3, 700, 64], [1500, 2000, 701, 65]),
 ])
 def test_long_and_many(dn, H, qlens, klens):
     b = Batch(dn, H, qlens, klens, seed=7)
@@ -112,21 +114,20 @@ def test_many_requests(B):
 
 
 @pytest.mark.parametrize("dn", [128, 64])
-def test_scores_that_grow_and_fall(dn):
+@pytest.mark.parametrize("H,m", [(2, 200), (128, 1030)])
+def test_scores_that_grow_and_fall(dn, H, m):
     """Scores far above and below what a row saw first, and logits of thousands."""
     for sign in (1.0, -1.0):
-        b = Batch(dn, 2, [200], [600], seed=3)
-        k = torch.linspace(0, 30, 600)[:, None] * sign
+        b = Batch(dn, H, [m], [m + 400], seed=3)
+        k = torch.linspace(0, 30, m + 400)[:, None] * sign
         b.kv[:, 0, :dn] = (k * torch.sign(b.q[100, 0, :dn].float())).to(BF)
-        lse = torch.empty(200, 2, device=DEV)
-        b.check(b.run(True, lse), True, lse)
+        lse = torch.empty(m, H, device=DEV)
+        b.check(b.run(True, lse), True, lse, rows=None if H == 2 else 40)
 
 
 @pytest.mark.parametrize("dn", [128, 64])
-@pytest.mark.parametrize("splits", [False, True])
-def test_what_a_query_does_not_see_does_not_reach_it(dn, splits):
-    m, n = (40, 1500) if splits else (300, 340)
-    H = 1 if splits else 2
+@pytest.mark.parametrize("m,n,H", [(40, 1500, 1), (300, 340, 2), (520, 560, 128)])
+def test_what_a_query_does_not_see_does_not_reach_it(dn, m, n, H):
     b = Batch(dn, H, [m, 8], [n, 8], seed=11)
     clean = b.run()
     b.check(clean, rows=50)
