@@ -89,10 +89,11 @@ __device__ __forceinline__ XPlace x_place(const ExpandedArgs& a, uint32_t want) 
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
       most = __builtin_amdgcn_readfirstlane(most);
-            const int shift = max(29 - __builtin_clz(most | 1), 7);
+      const int shift = max(29 - __builtin_clz(most | 1), 7);
       // row blocks of this lane's request whose last row sees x << shift keys or more
       const auto count = [&](int x) {
         const int keys = x << shift;
+        if (x == 0) return n;
         if (!a.causal) return nk >= keys ? n : 0;
         if (past + nq < keys) return 0;
         return n - min(max((keys - past + ROWS - 1) / ROWS - 1, 0), n);

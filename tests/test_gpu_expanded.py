@@ -171,6 +171,15 @@ def test_strides_and_what_is_left_as_it_was():
     assert torch.equal(o[:33], want[:33]) and (o[33:70] == 3).all() and torch.equal(o[70:], want[70:])
 
 
+def test_queries_before_the_first_key_that_are_cut_off_from_the_last():
+    """Of more queries than keys only the first ones, which see nothing."""
+    b = Batch(64, 2, [300, 5], [10, 5], seed=6)
+    lse = torch.full((305, 2), 5.0, device=DEV)
+    o = b.run(lse=lse, max_q_len=33)
+    assert (o[:33] == 0).all() and (lse[:33] == float("-inf")).all() and (o[33:300] == 7).all() and (lse[33:300] == 5).all()
+    b.check(b.run())
+
+
 def test_prefix_in_parts_joined_by_lse():
     """A prefix without the causal rule and the chunk with it, joined by their LSEs, are the whole."""
     m, p, H, dn = 50, 300, 4, 128
