@@ -60,6 +60,7 @@ struct Mx4WeightsArgs {
   int acc_rows;
   int64_t acc_cols;
   int add;      // to what acc holds; else in its place
+  int cost_shift;  // the launcher's: of the steps over a request's rows, where their sum would pass 32 bits
 };
 
 struct Mx4RowsArgs {

@@ -12,9 +12,14 @@
 // were off by 1e-5, now by 3e-7.)
 //
 // Few rows (64 at most, a decode step): a block keeps them in LDS and walks a range of the batch's
-// tiles, expanding as it multiplies; bound by the cache's bytes. Many rows (the last
-// queries of prompts): a wave keeps its positions expanded, and the rows come to LDS 16 at a time
-// while the last 16 are in use; bound by the matrix instructions.
+// tiles, expanding as it multiplies; bound by the cache's bytes: 49 us for 32 requests of 16384
+// positions under 16 heads of width 512, 210 MB at 4.3 TB/s. Many rows (the last queries of prompts): a
+// wave keeps its positions expanded in registers, and the rows come to LDS 64 at a time (32 of width
+// 512) while the last ones are in use, the weights of 16 rows between the products of the next 16; bound by
+// the matrix instructions, their operands' reads and the exponentials in turn: 92 us for 32 queries of 40
+// heads of width 256 in 8 requests of 8192 to 16384 positions, 69 GFLOP; 73 with the products alone,
+// 17 with one step alone (139 with 16 rows at a time and tiles of 256 positions a block, of which a part of
+// the blocks had one and the rest two).
 #include "rolaq_common.h"
 #include "mx4_args.h"
 #include "mx4_request.h"
@@ -34,7 +39,9 @@ struct WGeo {
   static constexpr int RS = R / 32;         // K-steps of the rope scores
   static constexpr int RC = (D + R) / 8;    // 16-byte chunks of a query row
   static constexpr int QT = 16 * 16 * RC;   // bytes of 16 query rows
-  static constexpr int COPIES = QT / 1024;
+  static constexpr int QR = D == 512 ? 32 : 64;  // rows in LDS at a time where they are streamed
+  static constexpr int STEP = QR / 16 * QT;      // their bytes
+  static_assert(STEP == 9 * W * 1024, "nine copies of 1 KB a wave, of whole rows");
 };
 constexpr int kWeightsFew = 64;  // the most rows of a request that stay in LDS
 
@@ -63,11 +70,13 @@ __device__ __forceinline__ float row_sum16(float v) {
 }
 
 // QT > 0: at most 16 QT rows a request, kept in LDS; 0: any number, streamed.
-template <int D, int R, int MT, int QT>
+template <int D, int R, int MOST, int QT>
 __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
   using G = WGeo<D, R>;
   constexpr int NB = G::NB, CB = G::CB, RS = G::RS, W = G::W, JS = G::JS, RC = G::RC;
-  constexpr int TILE = 16 * MT * W;  // positions of a block's tile
+  // A batch is shared out among the blocks in units of positions: whole tiles of MOST sub-tiles a wave where the rows
+  // are few; single sub-tiles a wave where they are many, for blocks to end together.
+  constexpr int TILE = 16 * W * (QT > 0 ? MOST : 1);
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_byte*)smem;
   const int lane = threadIdx.x & 63, la = lane & 15, gq = lane >> 4;
@@ -82,53 +91,72 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
   const auto tiles_of = [&](int i) {
     return i < a.B ? (uint32_t)((places(i, mx4_request(a, i)) + TILE - 1) / TILE) : 0u;
   };
+  // what one of them costs: many rows, the steps over them
+  const auto cost_of = [&](int i) {
+    if (QT > 0 || i >= a.B) return 1u;
+    const int steps = (mx4_request(a, i).nq * a.H + G::QR - 1) / G::QR;
+    return (uint32_t)(steps >> a.cost_shift) + 1u;
+  };
   uint32_t total = 0;
-  for (int c = 0; c < a.B; c += 64) total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles_of(c + lane)), 63);
+  for (int c = 0; c < a.B; c += 64)
+    total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles_of(c + lane) * cost_of(c + lane)), 63);
   // (neighbours on one XCD: they read the same query rows)
   const uint32_t per = gridDim.x / 8;
   const uint32_t j = gridDim.x % 8 == 0 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
   const uint32_t nb = min(gridDim.x, total);
   if (j >= nb) return;
-  uint32_t u = (uint32_t)((uint64_t)total * j / nb);
-  const uint32_t u_end = (uint32_t)((uint64_t)total * (j + 1) / nb);
-  int b = 0;
-  uint32_t first = 0;  // first tile of request b
-  {
-    uint32_t before = 0;
-    for (int c = 0; c < a.B; c += 64) {
-      const uint32_t n = tiles_of(c + lane), incl = wave_scan(n), start = before + incl - n;
-      const uint64_t hit = __builtin_amdgcn_ballot_w64(start <= u && u < start + n);
-      if (hit) {
-        const int l = __builtin_ctzll(hit);
-        b = c + l;
-        first = (uint32_t)__builtin_amdgcn_readlane((int)start, l);
-        break;
-      }
-      before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+  // The units of a request (n, from `start` in the batch's cost) that are this block's. Few rows: an even part of
+  // the batch. Many: a block that took a request's last units and the next one's first would go through two
+  // requests' rows and end last, so each request has blocks of its own, as many as its part of the cost says, and
+  // one too small for that goes to the block before which it ends.
+  const auto share = [&](uint32_t start, uint32_t n, uint32_t cost, uint32_t& t0, uint32_t& t1) {
+    if constexpr (QT > 0) {
+      const uint32_t lo = (uint32_t)((uint64_t)total * j / nb), hi = (uint32_t)((uint64_t)total * (j + 1) / nb);
+      t0 = max(lo, start) - start;
+      t1 = min(max(hi, start) - start, n);
+    } else {
+      const uint64_t at = 2 * (uint64_t)start * nb + total;
+      const uint32_t b0 = min((uint32_t)(at / (2 * (uint64_t)total)), nb - 1);
+      const uint32_t b1 = min((uint32_t)((at + 2 * (uint64_t)n * cost * nb) / (2 * (uint64_t)total)), nb);
+      const uint32_t blocks = b1 > b0 ? b1 - b0 : 1, k = j - b0;
+      t0 = k < blocks ? (uint32_t)((uint64_t)n * k / blocks) : n;
+      t1 = k < blocks ? (uint32_t)((uint64_t)n * (k + 1) / blocks) : 0u;
     }
-  }
+  };
+  // where a lane finds its operands of 16 rows: x = 4 s + i is block 4 s + gq's i-th quarter, x = 4 JS + s rope
+  // (the swizzle is within a block and a half, so s is a plain offset)
+  uint32_t q_at[4], pe_at[RS];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q_at[i] = 16 * (la * RC + ((4 * gq + i) ^ w_swz<D>(la)));
+#pragma unroll
+  for (int s = 0; s < RS; ++s) pe_at[s] = 16 * (la * RC + D / 8 + ((4 * s + gq) ^ w_swz<D>(la)));
+  const auto operand = [&](uint32_t rows16, int x) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4*>(smem + rows16 + (x < 4 * JS ? q_at[x % 4] + 256 * (x / 4) : pe_at[x < 4 * JS ? 0 : x - 4 * JS]));
+  };
   const uint32_t max_page = (uint32_t)((a.num_slots - 1) >> a.page_shift), max_slot = (uint32_t)(a.num_slots - 1);
   const uint32_t page_mask = (1u << a.page_shift) - 1;
 
-  while (u < u_end && b < a.B) {
+  uint32_t before = 0;
+  for (int chunk = 0; chunk < a.B; chunk += 64) {
+   const uint32_t units = tiles_of(chunk + lane), cost = cost_of(chunk + lane), incl = wave_scan(units * cost);
+   uint32_t part0, part1;
+   share(before + incl - units * cost, units, cost, part0, part1);
+   before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+   for (uint64_t hit = __builtin_amdgcn_ballot_w64(part0 < part1); hit; hit &= hit - 1) {
+    const int l = __builtin_ctzll(hit), b = chunk + l;
+    const uint32_t t_begin = (uint32_t)__builtin_amdgcn_readlane((int)part0, l);
+    const uint32_t t_end = (uint32_t)__builtin_amdgcn_readlane((int)part1, l);
     const Mx4Request rq = mx4_request(a, b);
     const int n = places(b, rq);  // positions
-    const uint32_t mine = (uint32_t)((n + TILE - 1) / TILE);
-    if (u - first >= mine) {
-      first += mine;
-      ++b;
-      continue;
-    }
-    const uint32_t t_end = min(mine, u_end - first);
     const int rows = rq.nq * a.H, qtiles = (rows + 15) / 16;
     float* const acc = a.acc + (a.req_idx ? a.req_idx[b] : b) * a.acc_st;
-    // copies of this wave's share of rows 16 qt .. to LDS at `at` (past the last row: that one again)
-    const auto copy_rows = [&](int qt, uint32_t at) {
-      for (int k = wave; k < G::COPIES; k += W) {
-        const int ci = 64 * k + lane, r = ci / RC, c = (ci - r * RC) ^ w_swz<D>(r);
-        const uint32_t row = (uint32_t)min(16 * qt + r, rows - 1), tok = row / (uint32_t)a.H, head = row - tok * a.H;
-        copy16(a.q + (int64_t)(rq.q0 + (int)tok) * a.q_st + (int64_t)head * a.q_sh + 8 * c, at + 1024 * k);
-      }
+    // Copies of 16 bytes a lane of rows r0 .. r0 + 16 N - 1, N times 16 rows, to LDS at `at`, nine a wave
+    // for every 16 * 9 W / COPIES rows (past the last row: that one again).
+    const int64_t q_row0 = (int64_t)rq.q0 * a.q_st;
+    const auto copy_piece = [&](int r0, int k, uint32_t at) __attribute__((always_inline)) {
+      const int ci = 64 * k + lane, r = ci / RC, c = (ci - r * RC) ^ w_swz<D>(r & 15);
+      const uint32_t row = (uint32_t)min(r0 + r, rows - 1), tok = row / (uint32_t)a.H, head = row - tok * a.H;
+      copy16(a.q + q_row0 + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh + 8 * c, at + 1024 * k);
     };
     // lse of row la of 16, and the positions that it sees; a row that saw nothing (lse
     // -inf), or one past the last, weighs nothing
@@ -149,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt)
         if (qt < qtiles) {
-          copy_rows(qt, lds0 + qt * G::QT);
+          for (int k = wave; k < G::QT / 1024; k += W) copy_piece(16 * qt, k, lds0 + qt * G::QT);
           qrow[qt] = row_of(qt);
         } else {
           qrow[qt] = Row{INFINITY, 0};
@@ -157,7 +185,9 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
       wait_loads<0>();
       __syncthreads();
     }
-    for (uint32_t t = u - first; t < t_end; ++t) {
+    // a tile from unit t: MT sub-tiles of 16 positions for each wave
+    const auto tile = [&](uint32_t t, auto Sub) __attribute__((always_inline)) {
+      constexpr int MT = decltype(Sub)::value;
       const int p0 = (int)t * TILE + 16 * MT * wave;  // this wave's positions
       // ---- the keys --------------------------------------------------------------------
       u32x4 code[MT][JS], pe[MT][RS];
@@ -220,8 +250,9 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
             sum[m][i] += w;
           }
       };
-      const auto query = [&](const uint8_t* rows16, int c) {
-        return *reinterpret_cast<const u32x4*>(rows16 + 16 * (la * RC + (c ^ w_swz<D>(la))));
+      const auto add_weight = [&](float c, float lse, float& to) __attribute__((always_inline)) {
+        to += __builtin_amdgcn_exp2f(fmaf(c, a.sm_scale, -lse) * kLog2e);
+        asm volatile("" : "+v"(to));  // added here, between the products
       };
       if constexpr (QT > 0) {
         if (p0 < n) {
@@ -239,7 +270,7 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
               for (int m = 0; m < MT; ++m) k[m] = values(m, s, i);
 #pragma unroll
               for (int qt = 0; qt < QT; ++qt) {
-                const u32x4 q = query(smem + qt * G::QT, 16 * s + 4 * gq + i);
+                const u32x4 q = operand(qt * G::QT, 4 * s + i);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) c[qt][m] = mfma16x16x32(k[m], q, c[qt][m]);
               }
@@ -248,7 +279,7 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
           for (int s = 0; s < RS; ++s)
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
-              const u32x4 q = query(smem + qt * G::QT, D / 8 + 4 * s + gq);
+              const u32x4 q = operand(qt * G::QT, 4 * JS + s);
 #pragma unroll
               for (int m = 0; m < MT; ++m) c[qt][m] = mfma16x16x32(pe[m][s], q, c[qt][m]);
             }
@@ -259,11 +290,37 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
       } else {
         // rows that see none of the tile's positions come first: from the first token that does
         const int tok0 = max((int)t * TILE - rq.past, 0);
-        const int qt0 = (int)min((int64_t)tok0 * a.H / 16, (int64_t)qtiles);
-        Row next{};
-        if (qt0 < qtiles) {
-          copy_rows(qt0, lds0 + (qt0 & 1) * G::QT);
-          next = row_of(qt0);
+        constexpr int QR = G::QR, SUB = QR / 16;
+        const int steps = (rows + QR - 1) / QR, s0 = (int)min((int64_t)tok0 * a.H / QR, (int64_t)steps);
+        // Whose rows lie one behind the other: a step's copies are the last one's, so much further on.
+        const bool flat = a.q_st == (int64_t)a.H * a.q_sh && a.q_sh < (1 << 22);
+        uint32_t off[9];
+#pragma unroll
+        for (int k = 0; k < 9; ++k) {
+          const int ci = 64 * (9 * wave + k) + lane, r = ci / RC;
+          off[k] = (uint32_t)(2 * (r * (int)a.q_sh + 8 * ((ci - r * RC) ^ w_swz<D>(r & 15))));
+        }
+        const auto copy_step = [&](int s) __attribute__((always_inline)) {
+          const uint32_t at = lds0 + (uint32_t)(s & 1) * G::STEP;
+          if (flat && QR * (s + 1) <= rows) {
+            const uint16_t* const from = a.q + q_row0 + (int64_t)QR * s * a.q_sh;
+#pragma unroll
+            for (int k = 0; k < 9; ++k) copy16(from, off[k], at + 1024 * (9 * wave + k));
+          } else {
+#pragma unroll 1
+            for (int k = 0; k < 9; ++k) copy_piece(QR * s, 9 * wave + k, at);
+          }
+        };
+        // lse of the rows la of a step (rows as q0 H + row in a.lse)
+        float next[SUB];
+        const auto load_lse = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+          for (int q = 0; q < SUB; ++q)
+            next[q] = a.lse[(int64_t)rq.q0 * a.H + min(QR * s + 16 * q + la, rows - 1)];
+        };
+        if (s0 < steps) {
+          copy_step(s0);
+          load_lse(s0);
         }
         u32x4 k[MT][JS][4];
 #pragma unroll
@@ -272,33 +329,57 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
           for (int s = 0; s < JS; ++s)
 #pragma unroll
             for (int i = 0; i < 4; ++i) k[m][s][i] = values(m, s, i);
-        for (int qt = qt0; qt < qtiles; ++qt) {
+        for (int step = s0; step < steps; ++step) {
           wait_loads<0>();
           __syncthreads();  // these rows are there; the last ones are no longer read
-          const Row now = next;
-          if (qt + 1 < qtiles) {
-            copy_rows(qt + 1, lds0 + ((qt + 1) & 1) * G::QT);
-            next = row_of(qt + 1);
+          float lse[SUB];
+#pragma unroll
+          for (int q = 0; q < SUB; ++q) lse[q] = next[q] == -INFINITY ? INFINITY : next[q];
+          if (step + 1 < steps) {
+            copy_step(step + 1);
+            load_lse(step + 1);
           }
-          const uint8_t* const q16 = smem + (qt & 1) * G::QT;
-          f32x4 c[MT];
+          const uint32_t rows_at = (uint32_t)(step & 1) * G::STEP;
+          const int first_row = QR * step;
+          constexpr int NS = 4 * JS + RS, AHEAD = 3;  // operands of 16 rows; how many come ahead of their use
+          const auto product = [&](f32x4 (&c)[MT], int x, u32x4 y) __attribute__((always_inline)) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m) c[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int m = 0; m < MT; ++m)
+              c[m] = mfma16x16x32(x < 4 * JS ? k[m][x / 4 % JS][x % 4] : pe[m][x < 4 * JS ? 0 : x - 4 * JS], y,
+                                  x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : c[m]);
+          };
+          if (__builtin_expect(rq.past + first_row / a.H + 1 >= p0 + 16 * MT && first_row + QR <= rows, 1)) {
+            // every row sees every position: the weights of 16 rows between the products of the next 16
+            f32x4 c[2][MT];
+            u32x4 ring[AHEAD + 1];
+            static_for<AHEAD>([&](auto Y) __attribute__((always_inline)) { ring[Y] = operand(rows_at, Y); });
+            static_for<SUB * NS>([&](auto Y) __attribute__((always_inline)) {
+              constexpr int y = decltype(Y)::value, q = y / NS, x = y % NS, ahead = y + AHEAD;
+              if constexpr (ahead < SUB * NS) ring[ahead % (AHEAD + 1)] = operand(rows_at + ahead / NS * G::QT, ahead % NS);
+              product(c[q % 2], x, ring[y % (AHEAD + 1)]);
+              if constexpr (q > 0) {
+                constexpr int v0 = x * 4 * MT / NS, v1 = (x + 1) * 4 * MT / NS;
 #pragma unroll
-          for (int s = 0; s < JS; ++s)
+                for (int v = v0; v < v1; ++v) add_weight(c[(q + 1) % 2][v / 4][v % 4], lse[q > 0 ? q - 1 : 0], sum[v / 4][v % 4]);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            });
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const u32x4 q = query(q16, 16 * s + 4 * gq + i);
+            for (int v = 0; v < 4 * MT; ++v) add_weight(c[(SUB - 1) % 2][v / 4][v % 4], lse[SUB - 1], sum[v / 4][v % 4]);
+          } else {
 #pragma unroll
-              for (int m = 0; m < MT; ++m) c[m] = mfma16x16x32(k[m][s][i], q, c[m]);
+            for (int q = 0; q < SUB; ++q) {
+              if (first_row + 16 * q >= rows) break;
+              f32x4 c[MT];
+#pragma unroll
+              for (int x = 0; x < NS; ++x) {
+                product(c, x, operand(rows_at + q * G::QT, x));
+                if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+              }
+              const int row = first_row + 16 * q + la;
+              weigh(c, Row{lse[q], row < rows ? rq.past + (int)((uint32_t)row / (uint32_t)a.H) + 1 : 0});
             }
-#pragma unroll
-          for (int s = 0; s < RS; ++s) {
-            const u32x4 q = query(q16, D / 8 + 4 * s + gq);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) c[m] = mfma16x16x32(pe[m][s], q, c[m]);
           }
-          weigh(c, now);
         }
         __syncthreads();
       }
@@ -314,18 +395,33 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
       static_assert(MT <= 4, "a lane for each position");
       const int pos = p0 + 16 * (la >> 2) + 4 * gq + (la & 3);
       if (la < 4 * MT && pos < n) acc[pos] = a.add ? acc[pos] + out : out;
+    };
+    for (uint32_t t = t_begin; t < t_end;) {
+      if constexpr (QT > 0) {
+        tile(t, std::integral_constant<int, MOST>{});
+        ++t;
+      } else {
+        const uint32_t left = t_end - t, tiles = (left + MOST - 1) / MOST, sub = (left + tiles - 1) / tiles;
+        if constexpr (MOST >= 4) {
+          if (sub == 4) tile(t, std::integral_constant<int, 4>{});
+          if (sub == 3) tile(t, std::integral_constant<int, 3>{});
+        }
+        if (sub == 2) tile(t, std::integral_constant<int, 2>{});
+        if (sub == 1) tile(t, std::integral_constant<int, 1>{});
+        t += sub;
+      }
     }
-    u = first + t_end;
+   }
   }
 }
 
 template <int D, int R, int MT, int QT>
 hipError_t launch_weights(const Mx4WeightsArgs& a, int most_blocks, hipStream_t stream) {
-  constexpr int lds = (QT > 0 ? QT : 2) * WGeo<D, R>::QT;
+  constexpr int lds = QT > 0 ? QT * WGeo<D, R>::QT : 2 * WGeo<D, R>::STEP;
   const hipError_t e = hipFuncSetAttribute((const void*)mx4_weights_kernel<D, R, MT, QT>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
-  const int64_t tiles = (a.n_indices << a.page_shift) / (64 * MT) + a.B;
+  const int64_t tiles = (a.n_indices << a.page_shift) / (64 * (QT > 0 ? MT : 1)) + a.B;
   hipLaunchKernelGGL((mx4_weights_kernel<D, R, MT, QT>), dim3((unsigned)std::min<int64_t>(tiles, most_blocks)), dim3(256),
                      lds, stream, a);
   return hipGetLastError();
@@ -338,7 +434,11 @@ hipError_t launch_weights_rows(const Mx4WeightsArgs& a, int num_cus, hipStream_t
   if (rows <= 16) return launch_weights<D, R, 2, 1>(a, 4 * num_cus, stream);
   if (rows <= 32) return launch_weights<D, R, 2, 2>(a, 4 * num_cus, stream);
   if (rows <= 64) return launch_weights<D, R, 2, 4>(a, 2 * num_cus, stream);
-  return launch_weights<D, R, D == 512 ? 2 : 4, 0>(a, 2 * num_cus, stream);
+  // (a batch's cost in 32 bits)
+  Mx4WeightsArgs m = a;
+  const int64_t units = std::min<int64_t>((a.n_indices << a.page_shift) / 64 + a.B, 1 << 30);
+  while (units * ((rows / WGeo<D, R>::QR >> m.cost_shift) + 2) >= (int64_t(1) << 32)) ++m.cost_shift;
+  return launch_weights<D, R, D == 512 ? 2 : 4, 0>(m, 2 * num_cus, stream);
 }
 
 }  // namespace rolaq

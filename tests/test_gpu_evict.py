@@ -76,6 +76,35 @@ def test_weights(D, H, lens, qlens, page):
     check_weights(b, reqs=[len(lens) + 1 - i for i in range(len(lens))], add=True)
 
 
+@pytest.mark.parametrize("D,H", [(512, 16), (256, 40)])
+def test_weights_of_many_requests_with_many_rows(D, H):
+    # more than a wave's lanes of them, short and long, with few and many rows: shares of blocks
+    lens = [1 + (37 * i) % 150 for i in range(70)] + [2500, 900, 64, 1]
+    qlens = [min(n, 1 + i % 7) for i, n in enumerate(lens)]
+    b = Batch(D, H, lens, qlens, 16, seed=12)
+    check_weights(b)
+
+
+@pytest.mark.parametrize("D,H,m", [(512, 16, 1), (512, 16, 3), (512, 16, 9), (256, 40, 1), (256, 40, 33)])
+def test_weights_of_rows_and_sums_between_others(D, H, m):
+    lens, qlens = [300, 700], [m, max(1, m - 1)]
+    b = Batch(D, H, lens, qlens, 32, seed=13)
+    lse = torch.full((b.T, H), 3.0, device=DEV)
+    apart = torch.zeros(2 * b.T, H + 3, b.D + b.R + 16, dtype=torch.bfloat16, device=DEV)
+    apart[::2, 1:1 + H, 8:8 + b.D + b.R] = b.q.to(DEV)
+    wide = torch.full((2, 1024), 7.0, device=DEV)
+    outs = []
+    for q, acc in ((b.q.to(DEV), torch.empty(2, 701, device=DEV)),
+                   (apart[::2, 1:1 + H, 8:8 + b.D + b.R], wide[:, 5:706])):
+        evict.accumulate_weights(q, lse, b.pool, 0, acc, b.kv_indptr, b.kv_indices, b.kv_lens, b.sm,
+                                 qo_indptr=b.qo, max_q_len=m, page_size=32, add=False)
+        outs.append([acc[0, :300], acc[1, :700]])
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert outs[0][0].min() > 0
+    wide[0, 5:305], wide[1, 5:705] = 7.0, 7.0
+    assert (wide == 7.0).all()
+
+
 def test_weights_of_a_decode_step_and_the_attention_calls_lse():
     b = Batch(512, 16, [100, 3000, 1], [1, 1, 1], 64, seed=9)
     check_weights(b, decode=True)
