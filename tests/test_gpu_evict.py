@@ -238,6 +238,16 @@ def test_equal_weights_go_to_the_earlier_position(n, budget):
         run_evict([n], budget, 4, 16, 16, w=w, seed=n)
 
 
+@pytest.mark.parametrize("lens", [[16384, 100], [16385, 4096, 0], [40961], [196608], [196609, 16384, 300], [300000]])
+def test_long_requests(lens):
+    # either side of every change of blocks and chunks, with equal weights across chunks
+    g = np.random.default_rng(len(lens))
+    w = (np.floor(g.random((len(lens) + 2, max(lens) + 5)) * 500) * 2.0 ** -10).astype(np.float32)
+    run_evict(lens, 5000, 7, 300, 16, w=w)
+    run_evict(lens, 400, 0, 400, 1, w=w, in_place=True)
+    run_evict(lens, 401, 400, 0, 1, w=w)
+
+
 def test_weights_that_differ_in_their_last_bits():
     for d in (1, 1 << 10, 1 << 21):
         bits = 0x3f800000 + d * np.random.default_rng(d).integers(0, 3000 if d < 1 << 21 else 3, (3, 5005))
