@@ -532,6 +532,14 @@ _ROTARY_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def _rotary_heads(x, out, name, T, dim, dtype, dev):
     """(heads, in strides, out strides) of a ``[T, heads, dim]`` or ``[T, dim]`` tensor and its output."""
+    if isinstance(x, _Tensor) and isinstance(out, _Tensor) and x.dtype is dtype and out.dtype is dtype \
+            and x.device == dev and out.device == dev:
+        shape, xs, os = x.shape, x.stride(), out.stride()
+        if out.shape == shape and shape[0] == T and shape[-1] == dim and xs[-1] == os[-1] == 1 and 0 not in os:
+            if len(shape) == 3:
+                return shape[1], xs[:2], os[:2]
+            if len(shape) == 2:
+                return 1, (xs[0], 0), (os[0], 0)
     for t, n in ((x, name), (out, name + "_out")):
         _need(t, n, dtype, dev)
         if t.ndim not in (2, 3) or t.shape != x.shape:
