@@ -65,55 +65,68 @@ struct XPlace {
   int b, rb;           // request (-1: none), row block
   int q0, nq, past;    // first query, queries computed, keys before the first query's own
   int k0, nk;          // first key row, key rows
+  int parts;           // parts of the keys of every row block
 };
-// The `want`-th row block of the batch: of up to 64 requests those that see most keys first, so that
-// the blocks that a launch ends with are short, in classes of an eighth to a quarter of the longest; in a
-// class, and of more requests, request after request, so that blocks that share keys run together
-// (4 x 2048 queries behind 14336 keys, 40 heads: 1830 us in classes of 128 keys, 1650 so).
-template <int ROWS>
+// What a launch takes, in us, of `blocks` row blocks of `longest` steps at most, `mean` in the mean, in `parts`: a
+// step of one block on a CU, and of each of several; split keys cost their rows' partials, written and read
+// (`partial` a part), and a second launch.
+__device__ __host__ inline float x_cost(float blocks, float cus, float longest, float mean, float partial, int parts) {
+  const float each = ceilf(blocks * (float)parts / cus);
+  return fmaxf(0.65f * longest, 0.6f * each * mean) / (float)parts + (parts > 1 ? 6.f + partial * (float)parts : 0.f);
+}
+// The `want`-th row block of the batch: a request's run together, as they share its keys, the last (which sees most)
+// first, and of up to 64 requests those of most keys first, so that the blocks that a launch ends with are short.
+// (Row blocks of all requests by their number of keys: 10 prompts of 800, 128 heads, 610 us against 540.)
+// Where the launch has room for parts (a.splits > 1), their number follows from the lengths.
+template <int ROWS, int TK>
 __device__ __forceinline__ XPlace x_place(const ExpandedArgs& a, uint32_t want) {
   const int lane = threadIdx.x & 63;
   const auto clampq = [&](int i) { return min(max(a.qo_indptr[i], 0), a.T); };
   const auto clampk = [&](int i) { return min(max(a.kv_indptr[i], 0), a.N); };
-  XPlace p{-1, 0, 0, 0, 0, 0, 0};
+  XPlace p{-1, 0, 0, 0, 0, 0, 0, 1};
   uint32_t before = 0;
   for (int c = 0; c < a.B; c += 64) {
     const int i = min(c + lane, a.B - 1);
     const int q0 = clampq(i), nq_all = max(clampq(i + 1) - q0, 0), nq = min(nq_all, a.max_q_len);
     const int k0 = clampk(i), nk = max(clampk(i + 1) - k0, 0), past = nk - nq_all;
     const int n = c + lane < a.B ? (nq + ROWS - 1) / ROWS : 0;
-    uint64_t hit;
-    int rb;
+    uint32_t start = 0;  // row blocks before this lane's request's
     if (a.B <= 64) {
-      int most = n ? nk : 0;
+      for (int o = 0; o < a.B; ++o) {
+        const int keys = __builtin_amdgcn_readlane(nk, o), blocks = __builtin_amdgcn_readlane(n, o);
+        start += keys > nk || (keys == nk && o < lane) ? (uint32_t)blocks : 0u;
+      }
+      if (a.splits > 1) {
+        int most = n ? nk : 0;
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
-      most = __builtin_amdgcn_readfirstlane(most);
-      const int shift = max(29 - __builtin_clz(most | 1), 7);
-      // row blocks of this lane's request whose last row sees x << shift keys or more
-      const auto count = [&](int x) {
-        const int keys = x << shift;
-        if (x == 0) return n;
-        if (!a.causal) return nk >= keys ? n : 0;
-        if (past + nq < keys) return 0;
-        return n - min(max((keys - past + ROWS - 1) / ROWS - 1, 0), n);
-      };
-      const auto total = [&](int x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)count(x)), 63); };
-      int x = 0;
-      if (total(0) <= want) return p;
-      for (int bit = 2; bit >= 0; --bit)
-        if (total(x | 1 << bit) > want) x |= 1 << bit;
-      const int above = count(x + 1), here = count(x) - above;
-      const uint32_t more = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan((uint32_t)above), 63);
-      const uint32_t start = more + wave_scan((uint32_t)here) - (uint32_t)here;
-      hit = __builtin_amdgcn_ballot_w64(start <= want && want < start + (uint32_t)here);
-      rb = n - 1 - above - (int)(want - start);
+        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+        const float steps = (float)((nk + TK - 1) / TK), longest = (float)((most + TK - 1) / TK);
+        // (a causal request's row blocks see ever fewer keys)
+        float all = (float)n * steps - (a.causal ? 0.5f * (float)n * (float)(n - 1) * (float)(ROWS / TK) : 0.f);
+        all = fmaxf(all, (float)n);
+        float blocks = (float)n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) all += __shfl_xor(all, o), blocks += __shfl_xor(blocks, o);
+        // lane s - 1 has s parts, of four steps at least
+        float us = lane < a.splits && (lane == 0 || 4.f * (float)(lane + 1) <= longest)
+                       ? x_cost(blocks * (float)a.H, (float)a.cus, longest, all / fmaxf(blocks, 1.f), a.partial, lane + 1)
+                       : INFINITY;
+        int parts = lane + 1;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const float u = __shfl_xor(us, o);
+          const int q = __shfl_xor(parts, o);
+          if (u < us || (u == us && q < parts)) us = u, parts = q;
+        }
+        p.parts = __builtin_amdgcn_readfirstlane(parts);
+      }
     } else {
-      const uint32_t incl = wave_scan((uint32_t)n), start = before + incl - (uint32_t)n;
-      hit = __builtin_amdgcn_ballot_w64(start <= want && want < start + (uint32_t)n);
-      rb = n - 1 - (int)(want - start);
+      const uint32_t incl = wave_scan((uint32_t)n);
+      start = before + incl - (uint32_t)n;
       before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(start <= want && want < start + (uint32_t)n);
+    const int rb = n - 1 - (int)(want - start);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       p.b = c + l;
@@ -150,17 +163,24 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // ---- head, row block and part of the keys ---------------------------------------
-  const uint32_t item = blockIdx.x;
+  // Where every block is resident at once, none waits for a CU to fall idle: the second one on each CU is
+  // taken from the short end, so that a CU's two take as long as another's.
+  uint32_t item = blockIdx.x;
+  const uint32_t cus = (uint32_t)a.cus;
+  if (gridDim.x > cus && gridDim.x <= 2 * cus && item >= cus) item = gridDim.x - 1 - (item - cus);
   const int h = item % (uint32_t)a.H;
   const uint32_t rest = item / (uint32_t)a.H;
-  const int part = rest % (uint32_t)a.splits;
-  const XPlace at = x_place<G::ROWS>(a, rest / (uint32_t)a.splits);
-  if (at.b < 0) return;
+  const int part = rest / (uint32_t)a.blocks;
+  const XPlace at = x_place<G::ROWS, TK>(a, rest - (uint32_t)part * (uint32_t)a.blocks);
+  const int parts = at.parts;
+  if (at.b < 0 || part >= parts) return;
+  if (a.splits > 1 && item == 0 && tid == 0)  // (for the second launch)
+    reinterpret_cast<int*>(a.ws)[(int64_t)a.splits * a.T * a.H * (DN + 2)] = parts;
   const int q0 = at.q0, nq = at.nq, k0 = at.k0, nk = at.nk, row0 = at.rb * G::ROWS;
   // keys that row r sees
   const auto sees = [&](int r) { return a.causal ? min(max(at.past + r + 1, 0), nk) : nk; };
   const int tiles = (sees(min(row0 + G::ROWS, nq) - 1) + TK - 1) / TK;
-  const int t0 = (int)((int64_t)tiles * part / a.splits), n = (int)((int64_t)tiles * (part + 1) / a.splits) - t0;
+  const int t0 = (int)((int64_t)tiles * part / parts), n = (int)((int64_t)tiles * (part + 1) / parts) - t0;
   const int first_key = TK * t0;  // keys and steps are counted from here
 
   // ---- tile copies ------------------------------------------------------------------
@@ -511,7 +531,7 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
   const float inv = l > 0.f || l != l ? 1.0f / l : 0.f;
   const float ul = LSE ? x_add_halves(usum) : 0.f;
   const int64_t to = (int64_t)(q0 + row) * a.H + h;
-  if (a.splits > 1) {
+  if (parts > 1) {
     const int64_t total = (int64_t)a.T * a.H;
     float* const po = a.ws + (part * total + to) * DN + 4 * g;
     if (ok) {
@@ -550,75 +570,112 @@ __global__ __launch_bounds__(256, 2) void expanded_kernel(ExpandedArgs a) {
 template <int DN>
 __global__ __launch_bounds__(256) void expanded_merge_kernel(ExpandedArgs a) {
   constexpr int LPR = DN / 4;  // lanes of a row
-  const int64_t total = (int64_t)a.T * a.H, at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (at >= total) return;
-  const int t = (int)(at / a.H), h = (int)(at - (int64_t)t * a.H), c = threadIdx.x % LPR;
-  // rows that belong to no request, or to none of its first max_q_len, have no partials
-  bool there = false;
-  for (int b = 0; b < a.B; ++b) {
-    const int lo = min(max(a.qo_indptr[b], 0), a.T), hi = min(max(a.qo_indptr[b + 1], 0), a.T);
-    there |= t >= lo && t < min((int64_t)hi, (int64_t)lo + a.max_q_len);
-  }
-  if (!there) return;
-  const float* const lse = a.ws + a.splits * total * DN + at;
-  float M = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, lse[s * total]);
-  float den = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float l = lse[s * total];
-    if (l == -INFINITY) continue;
-    const float w = __builtin_amdgcn_exp2f(l - M);
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws + (s * total + at) * DN + 4 * c);
-    den += w;
+  const int64_t total = (int64_t)a.T * a.H;
+  const int parts = min(reinterpret_cast<const int*>(a.ws)[a.splits * total * (DN + 2)], a.splits);
+  if (parts <= 1) return;  // (written in its place)
+  const int c = threadIdx.x % LPR;
+  const int base = (threadIdx.x & 63) - c;  // the row's first lane
+  const auto over = [](float v, auto f) {   // over the row's lanes
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fmaf(w, v[i], o[i]);
+    for (int o = 1; o < LPR; o <<= 1) v = f(v, __shfl_xor(v, o));
+    return v;
+  };
+  const auto max2 = [](float x, float y) { return fmaxf(x, y); };
+  const auto add2 = [](float x, float y) { return x + y; };
+  for (int64_t at = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR; at < total;
+       at += (int64_t)gridDim.x * (256 / LPR)) {
+    const int t = (int)(at / a.H), h = (int)(at - (int64_t)t * a.H);
+    // rows that belong to no request, or to none of its first max_q_len, have no partials
+    float there = 0.f;
+    for (int b = c; b < a.B; b += LPR) {
+      const int lo = min(max(a.qo_indptr[b], 0), a.T), hi = min(max(a.qo_indptr[b + 1], 0), a.T);
+      if (t >= lo && t < min((int64_t)hi, (int64_t)lo + a.max_q_len)) there = 1.f;
+    }
+    if (over(there, max2) == 0.f) continue;
+    // (parts s = c, c + LPR .. are this lane's)
+    const float* const lse = a.ws + a.splits * total * DN + at;
+    float M = -INFINITY;
+    for (int s = c; s < parts; s += LPR) M = fmaxf(M, lse[s * total]);
+    M = over(M, max2);
+    float den = 0.f, sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += LPR) {
+      const int mine = s0 + c;
+      const float l = mine < parts ? lse[mine * total] : -INFINITY;
+      const float wl = l == -INFINITY ? -1.f : __builtin_amdgcn_exp2f(l - M);  // (-1: a part without keys)
+      if (l != -INFINITY) den += wl;
+      if (a.lse && mine < parts) {
+        const float ul = lse[(a.splits + mine) * total];
+        if (ul != -INFINITY) sum += __builtin_amdgcn_exp2f(ul - M);
+      }
+      const int n = min(LPR, parts - s0);
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws + ((s0 + i) * total + at) * DN + 4 * c);
+        const float w = __shfl(wl, base + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = w == -1.f ? o[k] : fmaf(w, v[k], o[k]);
+      }
+    }
+    den = over(den, add2);
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    if (a.lse) {
+      sum = over(sum, add2);
+      if (c == 0) a.lse[at] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * kLn2;
+    }
+    *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + 4 * c) =
+        u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
   }
-  const float inv = den == 0.f ? 0.f : 1.f / den;
-  if (a.lse && c == 0) {
-    const float* const ul = lse + a.splits * total;
-    float sum = 0.f;
-    for (int s = 0; s < a.splits; ++s)
-      if (ul[s * total] != -INFINITY) sum += __builtin_amdgcn_exp2f(ul[s * total] - M);
-    a.lse[at] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * kLn2;
-  }
-  *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + 4 * c) =
-      u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
 }
 
+constexpr int kXMostSplits = 64;
 struct XPlan {
   int64_t blocks;  // row blocks of the batch at most
-  int splits;
+  int splits;      // parts of the keys at most
+  float partial;   // us of a part's partials
 };
-XPlan expanded_plan(int64_t T, int64_t N, int B, int H, int max_q_len, int num_cus) {
+// The lengths are known on the device alone. There is room for as many parts as pay for one request of all
+// the keys, where row blocks are fewer than the two a CU that run together (more end close together: the longest
+// come first) and requests fewer than the lanes that find them; at most four blocks a CU in all.
+XPlan expanded_plan(int64_t T, int64_t N, int B, int H, int DN, int max_q_len, int num_cus) {
   constexpr int rows = XGeo<128>::ROWS;
-  XPlan p{std::min<int64_t>((int64_t)B * ((max_q_len + rows - 1) / rows), T / rows + B), 1};
-  // parts of the keys: what gives each CU a block, of 256 keys at least in the mean
-  const int64_t by_cus = num_cus / std::max<int64_t>(p.blocks * H, 1), by_keys = N / ((int64_t)B * 256);
-  p.splits = (int)std::max<int64_t>(1, std::min(by_cus, by_keys));
+  XPlan p{std::min<int64_t>((int64_t)B * ((max_q_len + rows - 1) / rows), T / rows + B), 1, 0.f};
+  p.partial = (float)(8.0 * (double)T * H * DN / 5e6);  // written and read at 5 TB/s
+  const int64_t all = std::max<int64_t>(p.blocks * H, 1), room = all < 2 * (int64_t)num_cus ? 4 * (int64_t)num_cus / all : 1;
+  const float steps = (float)(N / (DN == 128 ? XGeo<128>::TK : XGeo<64>::TK));
+  if (B > 64) return p;
+  float best = x_cost(1.f, (float)num_cus, steps, steps, p.partial, 1);
+  for (int s = 2; s <= std::min<int64_t>(room, kXMostSplits) && 4.f * s <= steps; ++s) {
+    const float us = x_cost(1.f, (float)num_cus, steps, steps, p.partial, s);
+    if (us < best) best = us, p.splits = s;
+  }
   return p;
 }
 
 template <int DN, bool LSE>
 hipError_t launch_expanded(ExpandedArgs a, int num_cus, hipStream_t stream) {
   using G = XGeo<DN>;
-  const XPlan p = expanded_plan(a.T, a.N, a.B, a.H, a.max_q_len, num_cus);
+  const XPlan p = expanded_plan(a.T, a.N, a.B, a.H, DN, a.max_q_len, num_cus);
   a.splits = p.splits;
+  a.blocks = (int)p.blocks;
+  a.partial = p.partial;
+  a.cus = num_cus;
   hipError_t e = hipFuncSetAttribute((const void*)expanded_kernel<DN, LSE>, hipFuncAttributeMaxDynamicSharedMemorySize, G::LDS);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL((expanded_kernel<DN, LSE>), dim3((unsigned)(p.blocks * a.H * a.splits)), dim3(256), G::LDS, stream, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   const int64_t rows = (int64_t)a.T * a.H, per = 256 / (DN / 4);
-  hipLaunchKernelGGL((expanded_merge_kernel<DN>), dim3((unsigned)((rows + per - 1) / per)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((expanded_merge_kernel<DN>), dim3((unsigned)std::min<int64_t>((rows + per - 1) / per, 8 * num_cus)),
+                     dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
 }  // namespace rolaq
 
 int64_t rolaq_expanded_ws_bytes(int64_t T, int64_t N, int B, int H, int DN, int max_q_len, int num_cus) {
-  const int s = rolaq::expanded_plan(T, N, B, H, max_q_len, num_cus).splits;
-  return s > 1 ? (int64_t)s * T * H * (DN + 2) * 4 : 0;
+  const int s = rolaq::expanded_plan(T, N, B, H, DN, max_q_len, num_cus).splits;
+  return s > 1 ? (int64_t)s * T * H * (DN + 2) * 4 + 16 : 0;
 }
 
 hipError_t rolaq_launch_expanded(const rolaq::ExpandedArgs& a, int DN, int num_cus, hipStream_t stream) {

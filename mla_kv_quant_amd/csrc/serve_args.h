@@ -63,7 +63,10 @@ struct ExpandedArgs {
   float* lse;  // [T, H] or null
   float* ws;   // partials of split keys
   // set by the launcher
-  int splits;
+  int splits;     // parts of the keys at most
+  int blocks;     // row blocks at most
+  float partial;  // what a part's partials cost
+  int cus;
 };
 
 }  // namespace rolaq

@@ -214,3 +214,23 @@ def test_workspace_and_side_stream():
         o = b.run()
     side.synchronize()
     assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize("dn,H,qlens,klens", [
+    (128, 1, [20], [13000]), (64, 1, [3, 140], [17000, 200]),  # more parts than a row has lanes
+    (128, 8, [60, 282, 0, 100, 5], [60, 7000, 300, 101, 2]),  # parts by the longest request's length
+    (128, 2, [5, 130, 2], [6, 131, 3]), (64, 4, [1, 1], [1, 30]), (128, 1, [0, 0, 4], [4000, 0, 0]),  # room, not used
+    (128, 128, [400], [400]), (64, 100, [150, 180], [150, 900]),  # two blocks a CU, the second in reverse
+    (128, 128, [129, 1, 300, 128], [129, 800, 300, 500]),
+])
+@pytest.mark.parametrize("causal", [True, False])
+def test_parts_and_orders_of_row_blocks(dn, H, qlens, klens, causal):
+    b = Batch(dn, H, qlens, klens, seed=len(qlens) + H)
+    T = sum(qlens)
+    n = kernels.expanded_attend_workspace_bytes(T, sum(klens), len(qlens), H, dn, max(qlens), DEV)
+    ws = torch.full((max(n, 16),), 255, dtype=torch.uint8, device=DEV)
+    lse = torch.full((T, H), 5.0, device=DEV)
+    o = b.run(causal, lse, workspace=ws)
+    b.check(o, causal, lse, rows=40)
+    ws.fill_(127)
+    assert torch.equal(b.run(causal, workspace=ws), o)
