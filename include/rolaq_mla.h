@@ -436,6 +436,24 @@ int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_st
                                  int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
                                  int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* stream);
 
+/*
+ * The same with room for parts of a request's query rows, which many rows over few positions need to
+ * fill the device: a block goes through one part, and a second launch adds them up in order. workspace:
+ * rolaq_mx4_accumulate_weights_workspace bytes for these sizes, 16-byte aligned, contents unspecified before
+ * and after (null, or 0 bytes needed: one part). Sums of parts depend on the batch's sizes in their last bits.
+ */
+int rolaq_mx4_accumulate_weights_parts(const void* q, int64_t q_stride_t, int64_t q_stride_h, const float* lse,
+                                       const uint8_t* codes, const uint8_t* scales, const void* rope_buf, int64_t num_slots,
+                                       const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                       int64_t n_indices, int page_size, const int64_t* kv_lens, const int64_t* req_idx,
+                                       int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
+                                       int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* workspace,
+                                       int64_t workspace_bytes, void* stream);
+
+/* Bytes of its workspace for T queries of at most max_q_len a request (0: one part). Host only. */
+int rolaq_mx4_accumulate_weights_workspace(int64_t T, int B, int H, int D, int64_t n_indices, int page_size,
+                                           int max_q_len, int64_t* bytes);
+
 /* Bytes of rolaq_evict's workspace for B requests of max_kv_len positions at most. Host only. */
 int rolaq_evict_workspace(int B, int64_t max_kv_len, int64_t* bytes);
 

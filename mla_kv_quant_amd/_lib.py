@@ -68,6 +68,11 @@ SIGNATURES = {
                                      c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int,
                                      c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_int64, c_int,
                                      c_void_p],
+    "rolaq_mx4_accumulate_weights_parts": [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                           c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64,
+                                           c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64,
+                                           c_int64, c_int, c_void_p, c_int64, c_void_p],
+    "rolaq_mx4_accumulate_weights_workspace": [c_int64, c_int, c_int, c_int, c_int64, c_int, c_int, c_void_p],
     "rolaq_evict_workspace": [c_int, c_int64, c_void_p],
     "rolaq_evict": [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int,
                     c_void_p, c_int, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_void_p,

@@ -805,12 +805,25 @@ int rolaq_expanded_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_strid
                     "expanded_attend_fwd launch");
 }
 
-int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_stride_h, const float* lse,
-                                 const uint8_t* codes, const uint8_t* scales, const void* rope_buf, int64_t num_slots,
-                                 const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
-                                 int64_t n_indices, int page_size, const int64_t* kv_lens, const int64_t* req_idx,
-                                 int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
-                                 int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* stream) {
+int rolaq_mx4_accumulate_weights_workspace(int64_t T, int B, int H, int D, int64_t n_indices, int page_size, int max_q_len,
+                                           int64_t* bytes) {
+  if (T < 0 || B < 0 || H < 1 || H > kMaxHeads || (D != 512 && D != 256) || n_indices < 0 || n_indices > INT32_MAX ||
+      page_size < 1 || (page_size & (page_size - 1)) || max_q_len < 0 || !bytes)
+    return fail(ROLAQ_ERR_INVALID, "mx4_accumulate_weights_workspace: invalid sizes");
+  int page_shift = 0;
+  while ((1 << page_shift) < page_size) ++page_shift;
+  *bytes = rolaq_mx4_weights_ws_bytes(n_indices, page_shift, B, std::min<int64_t>(max_q_len, T) * H, D, cu_count());
+  g_err[0] = '\0';
+  return ROLAQ_OK;
+}
+
+int rolaq_mx4_accumulate_weights_parts(const void* q, int64_t q_stride_t, int64_t q_stride_h, const float* lse,
+                                       const uint8_t* codes, const uint8_t* scales, const void* rope_buf, int64_t num_slots,
+                                       const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                       int64_t n_indices, int page_size, const int64_t* kv_lens, const int64_t* req_idx,
+                                       int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
+                                       int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* workspace,
+                                       int64_t workspace_bytes, void* stream) {
   const char* const fn = "mx4_accumulate_weights";
   if (T < 0 || B < 0 || max_q_len < 0) return fail(ROLAQ_ERR_INVALID, "%s: negative T, B or max_q_len", fn);
   if (H < 1 || H > kMaxHeads) return fail(ROLAQ_ERR_INVALID, "%s: H must be between 1 and %d, got %d", fn, kMaxHeads, H);
@@ -832,6 +845,11 @@ int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_st
     return fail(ROLAQ_ERR_INVALID, "%s: more than 2^24 queries, or 2^29 query rows", fn);
   if (!aligned(q, 16) || q_stride_t % 8 || q_stride_h % 8 || q_stride_t < 0 || q_stride_h < 0)
     return fail(ROLAQ_ERR_INVALID, "%s: q must be 16-byte aligned with strides multiple of 8", fn);
+  int page_shift = 0;
+  while ((1 << page_shift) < page_size) ++page_shift;
+  const int64_t ws = rolaq_mx4_weights_ws_bytes(n_indices, page_shift, B, int64_t(most) * H, D, cu_count());
+  if (workspace && ws > 0 && (!aligned(workspace, 16) || workspace_bytes < ws))
+    return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
   rolaq::Mx4WeightsArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.q_st = q_stride_t;
@@ -844,7 +862,7 @@ int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_st
   a.kv_indptr = kv_indptr;
   a.kv_indices = kv_indices;
   a.n_indices = n_indices;
-  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  a.page_shift = page_shift;
   a.kv_lens = kv_lens;
   a.T = int(T);
   a.B = B;
@@ -858,8 +876,21 @@ int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_st
   a.acc_rows = int(acc_rows);
   a.acc_cols = acc_cols;
   a.add = add != 0;
+  a.ws = ws > 0 ? static_cast<float*>(workspace) : nullptr;
   return hip_status(rolaq_launch_mx4_weights(a, D, cu_count(), static_cast<hipStream_t>(stream)),
                     "mx4_accumulate_weights launch");
+}
+
+int rolaq_mx4_accumulate_weights(const void* q, int64_t q_stride_t, int64_t q_stride_h, const float* lse,
+                                 const uint8_t* codes, const uint8_t* scales, const void* rope_buf, int64_t num_slots,
+                                 const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                 int64_t n_indices, int page_size, const int64_t* kv_lens, const int64_t* req_idx,
+                                 int64_t T, int B, int H, int D, int R, int max_q_len, float sm_scale, float* acc,
+                                 int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, int add, void* stream) {
+  return rolaq_mx4_accumulate_weights_parts(q, q_stride_t, q_stride_h, lse, codes, scales, rope_buf, num_slots,
+                                            qo_indptr, kv_indptr, kv_indices, n_indices, page_size, kv_lens, req_idx, T,
+                                            B, H, D, R, max_q_len, sm_scale, acc, acc_stride, acc_rows, acc_cols, add,
+                                            nullptr, 0, stream);
 }
 
 int rolaq_evict_workspace(int B, int64_t max_kv_len, int64_t* bytes) {

@@ -100,10 +100,11 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
   uint32_t total = 0;
   for (int c = 0; c < a.B; c += 64)
     total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(tiles_of(c + lane) * cost_of(c + lane)), 63);
-  // (neighbours on one XCD: they read the same query rows)
-  const uint32_t per = gridDim.x / 8;
-  const uint32_t j = gridDim.x % 8 == 0 ? (blockIdx.x % 8) * per + blockIdx.x / 8 : blockIdx.x;
-  const uint32_t nb = min(gridDim.x, total);
+  // (each part of the rows is all blocks' over again; neighbours on one XCD: they read the same query rows)
+  const uint32_t blocks = QT > 0 ? gridDim.x : gridDim.x / (uint32_t)a.parts, per = blocks / 8;
+  const uint32_t part = QT > 0 ? 0u : blockIdx.x / blocks, in_part = blockIdx.x - part * blocks;
+  const uint32_t j = blocks % 8 == 0 ? (in_part % 8) * per + in_part / 8 : in_part;
+  const uint32_t nb = min(blocks, total);
   if (j >= nb) return;
   // The units of a request (n, from `start` in the batch's cost) that are this block's. Few rows: an even part of
   // the batch. Many: a block that took a request's last units and the next one's first would go through two
@@ -291,7 +292,8 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
         // rows that see none of the tile's positions come first: from the first token that does
         const int tok0 = max((int)t * TILE - rq.past, 0);
         constexpr int QR = G::QR, SUB = QR / 16;
-        const int steps = (rows + QR - 1) / QR, s0 = (int)min((int64_t)tok0 * a.H / QR, (int64_t)steps);
+        const int all = (rows + QR - 1) / QR, steps = (int)((int64_t)all * (part + 1) / a.parts);
+        const int s0 = (int)min(max((int64_t)tok0 * a.H / QR, (int64_t)all * part / a.parts), (int64_t)steps);
         // Whose rows lie one behind the other: a step's copies are the last one's, so much further on.
         const bool flat = a.q_st == (int64_t)a.H * a.q_sh && a.q_sh < (1 << 22);
         uint32_t off[9];
@@ -394,7 +396,12 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
         }
       static_assert(MT <= 4, "a lane for each position");
       const int pos = p0 + 16 * (la >> 2) + 4 * gq + (la & 3);
-      if (la < 4 * MT && pos < n) acc[pos] = a.add ? acc[pos] + out : out;
+      if (la < 4 * MT && pos < n) {
+        if (QT == 0 && a.parts > 1)
+          a.ws[part * a.ws_part + ((int64_t)rq.list << a.page_shift) + pos] = out;
+        else
+          acc[pos] = a.add ? acc[pos] + out : out;
+      }
     };
     for (uint32_t t = t_begin; t < t_end;) {
       if constexpr (QT > 0) {
@@ -415,33 +422,77 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
   }
 }
 
+// Sums of the rows' parts, in their order.
+__global__ __launch_bounds__(256) void mx4_weights_join_kernel(Mx4WeightsArgs a) {
+  const int b = blockIdx.y;
+  const Mx4Request rq = mx4_request(a, b);
+  const int64_t row = a.req_idx ? a.req_idx[b] : b;
+  if (row < 0 || row >= a.acc_rows) return;
+  const int n = (int)min((int64_t)rq.len, a.acc_cols);
+  const float* const ws = a.ws + ((int64_t)rq.list << a.page_shift);
+  float* const acc = a.acc + row * a.acc_st;
+  for (int pos = blockIdx.x * 256 + threadIdx.x; pos < n; pos += gridDim.x * 256) {
+    float sum = a.add ? acc[pos] : 0.f;
+#pragma unroll 8
+    for (int p = 0; p < a.parts; ++p) sum += ws[p * a.ws_part + pos];
+    acc[pos] = sum;
+  }
+}
+
+// Many rows: units of 64 positions at most, and parts of the rows: where units are fewer than the blocks that run at
+// once, as many parts as fill those, of two steps at least (7 requests of 51 to 172 positions and up to 51
+// queries of 128 heads, 26 units: 238 us in one part, 30 in 19).
+struct WeightsPlan {
+  int64_t units;
+  int parts;
+};
+static WeightsPlan weights_plan(int64_t n_indices, int page_shift, int B, int64_t rows, int step, int num_cus) {
+  // (positions stay below 2^30 a request, the units of all below 2^30 as the sums would not fit the memory)
+  WeightsPlan p{std::min<int64_t>((std::min<int64_t>(n_indices, int64_t(1) << 40 >> page_shift) << page_shift) / 64 + B, 1 << 30), 1};
+  if (rows > kWeightsFew)
+    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)num_cus / std::max<int64_t>(p.units, 1), (rows + step - 1) / step / 2));
+  return p;
+}
+
 template <int D, int R, int MT, int QT>
-hipError_t launch_weights(const Mx4WeightsArgs& a, int most_blocks, hipStream_t stream) {
+hipError_t launch_weights(const Mx4WeightsArgs& a, int64_t blocks, hipStream_t stream) {
   constexpr int lds = QT > 0 ? QT * WGeo<D, R>::QT : 2 * WGeo<D, R>::STEP;
   const hipError_t e = hipFuncSetAttribute((const void*)mx4_weights_kernel<D, R, MT, QT>,
                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
-  const int64_t tiles = (a.n_indices << a.page_shift) / (64 * (QT > 0 ? MT : 1)) + a.B;
-  hipLaunchKernelGGL((mx4_weights_kernel<D, R, MT, QT>), dim3((unsigned)std::min<int64_t>(tiles, most_blocks)), dim3(256),
-                     lds, stream, a);
+  hipLaunchKernelGGL((mx4_weights_kernel<D, R, MT, QT>), dim3((unsigned)blocks), dim3(256), lds, stream, a);
   return hipGetLastError();
 }
 
 template <int D, int R>
 hipError_t launch_weights_rows(const Mx4WeightsArgs& a, int num_cus, hipStream_t stream) {
-  const int64_t rows = (int64_t)a.max_q_len * a.H;
+  const int64_t rows = (int64_t)a.max_q_len * a.H, tiles = (a.n_indices << a.page_shift) / 128 + a.B;
   static_assert(kWeightsFew == 64, "four groups of rows");
-  if (rows <= 16) return launch_weights<D, R, 2, 1>(a, 4 * num_cus, stream);
-  if (rows <= 32) return launch_weights<D, R, 2, 2>(a, 4 * num_cus, stream);
-  if (rows <= 64) return launch_weights<D, R, 2, 4>(a, 2 * num_cus, stream);
-  // (a batch's cost in 32 bits)
+  if (rows <= 16) return launch_weights<D, R, 2, 1>(a, std::min<int64_t>(tiles, 4 * num_cus), stream);
+  if (rows <= 32) return launch_weights<D, R, 2, 2>(a, std::min<int64_t>(tiles, 4 * num_cus), stream);
+  if (rows <= 64) return launch_weights<D, R, 2, 4>(a, std::min<int64_t>(tiles, 2 * num_cus), stream);
   Mx4WeightsArgs m = a;
-  const int64_t units = std::min<int64_t>((a.n_indices << a.page_shift) / 64 + a.B, 1 << 30);
-  while (units * ((rows / WGeo<D, R>::QR >> m.cost_shift) + 2) >= (int64_t(1) << 32)) ++m.cost_shift;
-  return launch_weights<D, R, D == 512 ? 2 : 4, 0>(m, 2 * num_cus, stream);
+  const WeightsPlan p = weights_plan(a.n_indices, a.page_shift, a.B, rows, WGeo<D, R>::QR, num_cus);
+  m.parts = a.ws ? p.parts : 1;
+  m.ws_part = a.n_indices << a.page_shift;
+  // (a batch's cost in 32 bits)
+  while (p.units * ((rows / WGeo<D, R>::QR >> m.cost_shift) + 2) >= (int64_t(1) << 32)) ++m.cost_shift;
+  const int64_t blocks = std::min<int64_t>(p.units, 2 * num_cus / m.parts);
+  const hipError_t e = launch_weights<D, R, D == 512 ? 2 : 4, 0>(m, blocks * m.parts, stream);
+  if (e != hipSuccess || m.parts == 1) return e;
+  const int64_t each = std::min<int64_t>((m.ws_part + 255) / 256, 64);
+  hipLaunchKernelGGL(mx4_weights_join_kernel, dim3((unsigned)each, (unsigned)a.B), dim3(256), 0, stream, m);
+  return hipGetLastError();
 }
 
 }  // namespace rolaq
+
+int64_t rolaq_mx4_weights_ws_bytes(int64_t n_indices, int page_shift, int B, int64_t rows, int D, int num_cus) {
+  using namespace rolaq;
+  const int step = D == 512 ? WGeo<512, 64>::QR : WGeo<256, 32>::QR;
+  const int parts = weights_plan(n_indices, page_shift, B, rows, step, num_cus).parts;
+  return parts > 1 ? parts * (n_indices << page_shift) * 4 : 0;
+}
 
 hipError_t rolaq_launch_mx4_weights(const rolaq::Mx4WeightsArgs& a, int D, int num_cus, hipStream_t stream) {
   using namespace rolaq;

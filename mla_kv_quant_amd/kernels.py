@@ -631,12 +631,23 @@ def _acc_rows(acc, name, dev):
     return acc.stride(0) if acc.shape[0] > 1 else max(acc.shape[1], 1)
 
 
+def accumulate_weights_workspace_bytes(T: int, B: int, H: int, D: int, n_indices: int, page_size: int, max_q_len: int,
+                                       device) -> int:
+    """Bytes of :func:`mx4_accumulate_weights`'s workspace for these sizes on ``device`` (0: none)."""
+    n = ctypes.c_int64(0)
+    _call(torch.device(device), _lib.load().rolaq_mx4_accumulate_weights_workspace, int(T), int(B), int(H), int(D),
+          int(n_indices), int(page_size), int(max_q_len), ctypes.byref(n))
+    return n.value
+
+
 def mx4_accumulate_weights(q: torch.Tensor, lse: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                            rope_buf: torch.Tensor, qo_indptr: torch.Tensor | None, kv_indptr: torch.Tensor,
                            kv_indices: torch.Tensor, kv_lens: torch.Tensor, max_q_len: int, acc: torch.Tensor,
                            sm_scale: float, page_size: int = 1, req_idx: torch.Tensor | None = None,
-                           add: bool = True) -> torch.Tensor:
-    """Weights of the cached positions from ``q [T, H, D + R]`` with ``lse [T, H]``, summed into ``acc [rows, cols]``."""
+                           add: bool = True, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Weights of the cached positions from ``q [T, H, D + R]`` with ``lse [T, H]``, summed into ``acc [rows, cols]``.
+
+    ``workspace``: uint8, :func:`accumulate_weights_workspace_bytes` long; allocated here when not given."""
     dev = q.device
     _need(q, "q", torch.bfloat16, dev, 3)
     slots, D, R = _mx4_cache(codes, scales, rope_buf, dev)
@@ -658,10 +669,16 @@ def mx4_accumulate_weights(q: torch.Tensor, lse: torch.Tensor, codes: torch.Tens
         if req_idx.shape[0] < B:
             raise ValueError("index tensors are shorter than the batch")
     stride = _acc_rows(acc, "acc", dev)
-    _call(dev, _lib.load().rolaq_mx4_accumulate_weights, _p(q), q.stride(0), q.stride(1), _p(lse), _p(codes), _p(scales),
+    if workspace is not None:
+        _need_all(dev, ((workspace, "workspace", torch.uint8, 1),))
+    elif min(max_q_len, T) * H > 64 and 1 <= H <= 128 and page_size >= 1 and not page_size & (page_size - 1):
+        # (few rows take no parts; a call that the library refuses is left to it)
+        n = accumulate_weights_workspace_bytes(T, B, H, D, kv_indices.shape[0], page_size, max_q_len, dev)
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    _call(dev, _lib.load().rolaq_mx4_accumulate_weights_parts, _p(q), q.stride(0), q.stride(1), _p(lse), _p(codes), _p(scales),
           _p(rope_buf), slots, _p(qo_indptr), _p(kv_indptr), _p(kv_indices), kv_indices.shape[0], int(page_size),
           _p(kv_lens), _p(req_idx), T, B, H, D, R, int(max_q_len), float(sm_scale), _p(acc), stride, acc.shape[0],
-          acc.shape[1], int(bool(add)), _stream(q))
+          acc.shape[1], int(bool(add)), _p(workspace), 0 if workspace is None else workspace.shape[0], _stream(q))
     return acc
 
 

@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from mla_kv_quant_amd import evict, mx4
+from mla_kv_quant_amd import evict, kernels, mx4
 from tests.helpers import alloc_slots
 from tests.test_gpu_mx4 import Batch
 
@@ -103,6 +103,34 @@ def test_weights_of_rows_and_sums_between_others(D, H, m):
     assert outs[0][0].min() > 0
     wide[0, 5:305], wide[1, 5:705] = 7.0, 7.0
     assert (wide == 7.0).all()
+
+
+@pytest.mark.parametrize("D,H,lens,qlens", [
+    (512, 128, [170, 51, 90], [51, 20, 1]), (512, 128, [60] * 9, [57, 1, 0, 60, 2, 3, 30, 9, 5]), (512, 16, [1275], [60]),
+    (256, 40, [300], [64]), (256, 48, [65, 64, 1, 700], [2, 64, 1, 9]), (256, 20, [900], [5]),
+])
+def test_weights_of_many_rows_over_few_positions(D, H, lens, qlens):
+    b = Batch(D, H, lens, qlens, 16, seed=14)
+    check_weights(b)
+    check_weights(b, add=True, reqs=[-1] + list(range(1, len(lens))), cols=120)
+
+
+def test_workspace_of_weights():
+    b = Batch(512, 64, [200, 333], [40, 9], 16, seed=15)
+    args = (b.pool.c_codes[0], b.pool.c_scales[0], b.pool.rope_buf[0], b.qo, b.kv_indptr, b.kv_indices, b.kv_lens, 40)
+    n = kernels.accumulate_weights_workspace_bytes(b.T, 2, 64, 512, b.kv_indices.shape[0], 16, 40, DEV)
+    assert n > 0 and kernels.accumulate_weights_workspace_bytes(b.T, 2, 64, 512, 1 << 20, 16, 40, DEV) == 0
+    assert kernels.accumulate_weights_workspace_bytes(2, 2, 64, 512, 40, 16, 1, DEV) == 0
+    lse = torch.full((b.T, 64), 2.0, device=DEV)
+    outs = []
+    for fill in (0, 127, 255):
+        ws = torch.full((n,), fill, dtype=torch.uint8, device=DEV)
+        acc = torch.zeros(2, 333, device=DEV)
+        kernels.mx4_accumulate_weights(b.q.to(DEV), lse, *args, acc, b.sm, 16, workspace=ws)
+        outs.append(acc)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and outs[0][0, :200].min() > 0
+    with pytest.raises(ValueError, match="workspace"):
+        kernels.mx4_accumulate_weights(b.q.to(DEV), lse, *args, acc, b.sm, 16, workspace=ws[:n - 16])
 
 
 def test_weights_of_a_decode_step_and_the_attention_calls_lse():

@@ -224,6 +224,17 @@ def test_weights_arguments():
         refused(fn, changed(ok, **{f"i{i}": None}), "null")
 
 
+def test_weights_workspace_arguments():
+    lib = _lib.load()
+    fn = lib.rolaq_mx4_accumulate_weights_workspace
+    n = ctypes.c_int64(7)
+    ok = [100, 2, 128, 512, 40, 16, 50, ctypes.byref(n)]
+    assert fn(*ok) == _lib.ROLAQ_OK
+    assert fn(*changed(ok, i6=0)) == _lib.ROLAQ_OK and n.value == 0
+    for i, v in ((0, -1), (1, -1), (2, 0), (2, 129), (3, 384), (4, -1), (5, 48), (5, 0), (6, -1), (7, None)):
+        refused(fn, changed(ok, **{f"i{i}": v}), "invalid sizes")
+
+
 def test_evict_tensors():
     acc, ptr = torch.zeros(3, 10), torch.tensor([0, 1, 2], dtype=I32)
     idx, lens = torch.tensor([1, 2], dtype=I32), torch.tensor([1, 1])
