@@ -812,7 +812,7 @@ int rolaq_mx4_accumulate_weights_workspace(int64_t T, int B, int H, int D, int64
     return fail(ROLAQ_ERR_INVALID, "mx4_accumulate_weights_workspace: invalid sizes");
   int page_shift = 0;
   while ((1 << page_shift) < page_size) ++page_shift;
-  *bytes = rolaq_mx4_weights_ws_bytes(n_indices, page_shift, B, std::min<int64_t>(max_q_len, T) * H, D, cu_count());
+  *bytes = rolaq_mx4_weights_ws_bytes(n_indices, page_shift, B, T * H, std::min<int64_t>(max_q_len, T) * H, D, cu_count());
   g_err[0] = '\0';
   return ROLAQ_OK;
 }
@@ -847,7 +847,7 @@ int rolaq_mx4_accumulate_weights_parts(const void* q, int64_t q_stride_t, int64_
     return fail(ROLAQ_ERR_INVALID, "%s: q must be 16-byte aligned with strides multiple of 8", fn);
   int page_shift = 0;
   while ((1 << page_shift) < page_size) ++page_shift;
-  const int64_t ws = rolaq_mx4_weights_ws_bytes(n_indices, page_shift, B, int64_t(most) * H, D, cu_count());
+  const int64_t ws = rolaq_mx4_weights_ws_bytes(n_indices, page_shift, B, T * H, int64_t(most) * H, D, cu_count());
   if (workspace && ws > 0 && (!aligned(workspace, 16) || workspace_bytes < ws))
     return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
   rolaq::Mx4WeightsArgs a{};

@@ -86,8 +86,9 @@ struct Mx4RowsArgs {
 
 hipError_t rolaq_launch_mx4_attend(const rolaq::Mx4AttendArgs& a, int D, int num_cus, hipStream_t stream);
 hipError_t rolaq_launch_mx4_weights(const rolaq::Mx4WeightsArgs& a, int D, int num_cus, hipStream_t stream);
-// Bytes of workspace with which it takes parts of the rows (0: none), of `rows` a request at most.
-int64_t rolaq_mx4_weights_ws_bytes(int64_t n_indices, int page_shift, int B, int64_t rows, int D, int num_cus);
+// Bytes of workspace with which it takes parts of the rows (0: none), `all_rows`, of `rows` a request at most.
+int64_t rolaq_mx4_weights_ws_bytes(int64_t n_indices, int page_shift, int B, int64_t all_rows, int64_t rows, int D,
+                                   int num_cus);
 // Bytes of workspace that attend asks for at width D, whatever the batch.
 int64_t rolaq_mx4_attend_ws_bytes(int D, int num_cus);
 hipError_t rolaq_launch_mx4_write_plain(const rolaq::Mx4RowsArgs& a, int D, hipStream_t stream);

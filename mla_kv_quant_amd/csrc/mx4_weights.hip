@@ -26,6 +26,7 @@
 #include "mx4_tile.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace rolaq {
 
@@ -439,27 +440,35 @@ __global__ __launch_bounds__(256) void mx4_weights_join_kernel(Mx4WeightsArgs a)
   }
 }
 
-// Many rows: units of 64 positions at most, and parts of the rows: where units are fewer than the blocks that run at
-// once, as many parts as fill those, of two steps at least (7 requests of 51 to 172 positions and up to 51
-// queries of 128 heads, 26 units: 238 us in one part, 30 in 19).
+// Many rows: units of 64 positions at most, and parts of the rows. A unit's steps over its request's rows come one after
+// another, so that a launch takes as long as the longest request's, or as all units' on the blocks that run
+// at once: parts bring the first down to the second, of eight steps at least, if that saves seven (a step takes a
+// microsecond, a second launch and what it reads seven). 7 requests of 51 to 172 positions and up
+// to 51 queries of 128 heads: 238 us in one part, 30 in 19.
 struct WeightsPlan {
   int64_t units;
   int parts;
 };
-static WeightsPlan weights_plan(int64_t n_indices, int page_shift, int B, int64_t rows, int step, int num_cus) {
+static WeightsPlan weights_plan(int64_t n_indices, int page_shift, int B, int64_t all_rows, int64_t rows, int step, int num_cus) {
   // (positions stay below 2^30 a request, the units of all below 2^30 as the sums would not fit the memory)
   WeightsPlan p{std::min<int64_t>((std::min<int64_t>(n_indices, int64_t(1) << 40 >> page_shift) << page_shift) / 64 + B, 1 << 30), 1};
-  if (rows > kWeightsFew)
-    p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * (int64_t)num_cus / std::max<int64_t>(p.units, 1), (rows + step - 1) / step / 2));
+  if (rows <= kWeightsFew || B == 0) return p;
+  const int64_t steps = (rows + step - 1) / step;
+  const double mean = std::min((double)steps, (double)all_rows / B / step + 0.5);
+  const double each = std::max(8.0, (double)p.units * mean / (2.0 * num_cus));
+  const int64_t parts = (int64_t)std::ceil((double)steps / each);
+  if (parts > 1 && (double)steps - std::max(each, (double)steps / parts) > 7.0) p.parts = (int)std::min<int64_t>(parts, 2 * num_cus);
   return p;
 }
 
 template <int D, int R, int MT, int QT>
 hipError_t launch_weights(const Mx4WeightsArgs& a, int64_t blocks, hipStream_t stream) {
   constexpr int lds = QT > 0 ? QT * WGeo<D, R>::QT : 2 * WGeo<D, R>::STEP;
-  const hipError_t e = hipFuncSetAttribute((const void*)mx4_weights_kernel<D, R, MT, QT>,
-                                           hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  if (e != hipSuccess) return e;
+  if constexpr (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute((const void*)mx4_weights_kernel<D, R, MT, QT>,
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((mx4_weights_kernel<D, R, MT, QT>), dim3((unsigned)blocks), dim3(256), lds, stream, a);
   return hipGetLastError();
 }
@@ -472,7 +481,7 @@ hipError_t launch_weights_rows(const Mx4WeightsArgs& a, int num_cus, hipStream_t
   if (rows <= 32) return launch_weights<D, R, 2, 2>(a, std::min<int64_t>(tiles, 4 * num_cus), stream);
   if (rows <= 64) return launch_weights<D, R, 2, 4>(a, std::min<int64_t>(tiles, 2 * num_cus), stream);
   Mx4WeightsArgs m = a;
-  const WeightsPlan p = weights_plan(a.n_indices, a.page_shift, a.B, rows, WGeo<D, R>::QR, num_cus);
+  const WeightsPlan p = weights_plan(a.n_indices, a.page_shift, a.B, (int64_t)a.T * a.H, rows, WGeo<D, R>::QR, num_cus);
   m.parts = a.ws ? p.parts : 1;
   m.ws_part = a.n_indices << a.page_shift;
   // (a batch's cost in 32 bits)
@@ -487,10 +496,11 @@ hipError_t launch_weights_rows(const Mx4WeightsArgs& a, int num_cus, hipStream_t
 
 }  // namespace rolaq
 
-int64_t rolaq_mx4_weights_ws_bytes(int64_t n_indices, int page_shift, int B, int64_t rows, int D, int num_cus) {
+int64_t rolaq_mx4_weights_ws_bytes(int64_t n_indices, int page_shift, int B, int64_t all_rows, int64_t rows, int D,
+                                   int num_cus) {
   using namespace rolaq;
   const int step = D == 512 ? WGeo<512, 64>::QR : WGeo<256, 32>::QR;
-  const int parts = weights_plan(n_indices, page_shift, B, rows, step, num_cus).parts;
+  const int parts = weights_plan(n_indices, page_shift, B, all_rows, rows, step, num_cus).parts;
   return parts > 1 ? parts * (n_indices << page_shift) * 4 : 0;
 }
 
