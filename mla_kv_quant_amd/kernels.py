@@ -587,10 +587,9 @@ def expanded_attend_fwd(q: torch.Tensor, kv: torch.Tensor, k_pe: torch.Tensor, q
     ``workspace``: uint8, :func:`expanded_attend_workspace_bytes` long; allocated here when not given."""
     dev = q.device
     bf16 = torch.bfloat16
-    _need(q, "q", bf16, dev, 3)
-    _need(kv, "kv", bf16, dev, 3)
-    _need(k_pe, "k_pe", bf16, dev, 2)
-    _need(out, "out", bf16, dev, 3)
+    for t, name, ndim in ((q, "q", 3), (kv, "kv", 3), (k_pe, "k_pe", 2), (out, "out", 3)):
+        if not (isinstance(t, _Tensor) and t.dtype is bf16 and t.device == dev and t.ndim == ndim):
+            _need(t, name, bf16, dev, ndim)
     T, H, DK = q.shape
     N, rope, value = k_pe.shape[0], k_pe.shape[1], out.shape[2]
     nope = DK - rope
@@ -599,7 +598,8 @@ def expanded_attend_fwd(q: torch.Tensor, kv: torch.Tensor, k_pe: torch.Tensor, q
                          f"{tuple(kv.shape)}")
     if out.shape[0] < T or out.shape[1] != H:
         raise ValueError("out must be [>= T, H, value]")
-    if any(t.numel() and t.stride(-1) != 1 for t in (q, kv, k_pe, out)):
+    qs, kvs, pes, os = q.stride(), kv.stride(), k_pe.stride(), out.stride()
+    if not qs[2] == kvs[2] == pes[1] == os[2] == 1 and any(t.numel() and t.stride(-1) != 1 for t in (q, kv, k_pe, out)):
         raise ValueError("q, kv, k_pe and out must be contiguous in their last dims")
     i32 = torch.int32
     _need_all(dev, ((qo_indptr, "qo_indptr", i32, 1), (kv_indptr, "kv_indptr", i32, 1)))
@@ -617,14 +617,17 @@ def expanded_attend_fwd(q: torch.Tensor, kv: torch.Tensor, k_pe: torch.Tensor, q
         workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     else:
         _need_all(dev, ((workspace, "workspace", torch.uint8, 1),))
-    _call(dev, _lib.load().rolaq_expanded_attend_fwd, _p(q), q.stride(0), q.stride(1), _p(kv), kv.stride(0), kv.stride(1),
-          _p(k_pe), k_pe.stride(0), _p(qo_indptr), _p(kv_indptr), T, N, B, H, nope, rope, value, int(max_q_len),
-          float(sm_scale), int(bool(causal)), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace),
+    _call(dev, _lib.load().rolaq_expanded_attend_fwd, _p(q), qs[0], qs[1], _p(kv), kvs[0], kvs[1], _p(k_pe), pes[0],
+          _p(qo_indptr), _p(kv_indptr), T, N, B, H, nope, rope, value, int(max_q_len), float(sm_scale), int(bool(causal)),
+          _p(out), os[0], os[1], _p(lse), _p(workspace),
           0 if workspace is None else workspace.shape[0], _stream(q))
     return out
 
 
 def _acc_rows(acc, name, dev):
+    if isinstance(acc, _Tensor) and acc.dtype is torch.float32 and acc.device == dev and acc.ndim == 2 \
+            and acc.shape[0] > 1 and acc.stride(1) == 1 and acc.stride(0) >= acc.shape[1]:
+        return acc.stride(0)
     _need(acc, name, torch.float32, dev, 2)
     if acc.numel() and (acc.stride(1) != 1 or (acc.shape[0] > 1 and acc.stride(0) < acc.shape[1])):
         raise ValueError(f"{name} must have contiguous rows that do not overlap")
