@@ -733,6 +733,10 @@ int rolaq_rotary(const int64_t* positions, int64_t T, const uint64_t* turns, int
   a.y[0] = q_out, a.y[1] = k_out;
   a.x_st[0] = q_stride_t, a.x_sh[0] = q_stride_h, a.y_st[0] = q_out_stride_t, a.y_sh[0] = q_out_stride_h;
   a.x_st[1] = k_stride_t, a.x_sh[1] = k_stride_h, a.y_st[1] = k_out_stride_t, a.y_sh[1] = k_out_stride_h;
+  if (H == 0) {  // (the first tensor has heads)
+    a.x[0] = k, a.y[0] = k_out, a.H = Hk, a.Hk = 0;
+    a.x_st[0] = a.x_st[1], a.x_sh[0] = a.x_sh[1], a.y_st[0] = a.y_st[1], a.y_sh[0] = a.y_sh[1];
+  }
   return hip_status(rolaq_launch_rotary(a, type, interleaved != 0, cu_count(), static_cast<hipStream_t>(stream)),
                     "rotary launch");
 }
@@ -925,7 +929,7 @@ int rolaq_evict(const float* acc, int64_t acc_stride, int64_t acc_rows, int64_t 
   const int64_t ws = rolaq_evict_ws_bytes(B, max_kv_len);
   if (ws > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < ws))
     return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
-  if (int64_t(B) * std::max<int64_t>(1, (max_kv_len + 16383) / 16384) > (1 << 21))
+  if (rolaq_evict_blocks(B, max_kv_len) > (1 << 21))
     return fail(ROLAQ_ERR_INVALID, "%s: B * max_kv_len is too large for one launch", fn);
   rolaq::EvictArgs a{};
   a.acc = acc;

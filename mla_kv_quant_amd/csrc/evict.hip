@@ -331,6 +331,12 @@ hipError_t launch_evict_steps(const EvictArgs& a, hipStream_t stream) {
 
 }  // namespace rolaq
 
+int64_t rolaq_evict_blocks(int64_t B, int64_t most) {
+  using namespace rolaq;
+  const int64_t chunk = (int64_t)evict_per(most) * kEvictThreads;
+  return most <= kEvictOne ? B : B * ((most + chunk - 1) / chunk);
+}
+
 int64_t rolaq_evict_ws_bytes(int64_t B, int64_t most) {
   using namespace rolaq;
   if (most <= kEvictOne) return 0;

@@ -425,14 +425,14 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
 
 // Sums of the rows' parts, in their order.
 __global__ __launch_bounds__(256) void mx4_weights_join_kernel(Mx4WeightsArgs a) {
-  const int b = blockIdx.y;
+  const int each = gridDim.x / a.B, b = blockIdx.x / each;  // blocks of a request
   const Mx4Request rq = mx4_request(a, b);
   const int64_t row = a.req_idx ? a.req_idx[b] : b;
   if (row < 0 || row >= a.acc_rows) return;
   const int n = (int)min((int64_t)rq.len, a.acc_cols);
   const float* const ws = a.ws + ((int64_t)rq.list << a.page_shift);
   float* const acc = a.acc + row * a.acc_st;
-  for (int pos = blockIdx.x * 256 + threadIdx.x; pos < n; pos += gridDim.x * 256) {
+  for (int pos = (blockIdx.x - b * each) * 256 + threadIdx.x; pos < n; pos += each * 256) {
     float sum = a.add ? acc[pos] : 0.f;
 #pragma unroll 8
     for (int p = 0; p < a.parts; ++p) sum += ws[p * a.ws_part + pos];
@@ -489,8 +489,8 @@ hipError_t launch_weights_rows(const Mx4WeightsArgs& a, int num_cus, hipStream_t
   const int64_t blocks = std::min<int64_t>(p.units, 2 * num_cus / m.parts);
   const hipError_t e = launch_weights<D, R, D == 512 ? 2 : 4, 0>(m, blocks * m.parts, stream);
   if (e != hipSuccess || m.parts == 1) return e;
-  const int64_t each = std::min<int64_t>((m.ws_part + 255) / 256, 64);
-  hipLaunchKernelGGL(mx4_weights_join_kernel, dim3((unsigned)each, (unsigned)a.B), dim3(256), 0, stream, m);
+  const int64_t each = std::max<int64_t>(1, std::min<int64_t>((m.ws_part + 255) / 256, 2048 / a.B));
+  hipLaunchKernelGGL(mx4_weights_join_kernel, dim3((unsigned)(each * a.B)), dim3(256), 0, stream, m);
   return hipGetLastError();
 }
 

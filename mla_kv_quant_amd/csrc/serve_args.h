@@ -74,6 +74,7 @@ struct ExpandedArgs {
 enum RolaqType { ROLAQ_BF16 = 0, ROLAQ_FP16 = 1, ROLAQ_FP32 = 2 };
 
 hipError_t rolaq_launch_rotary(const rolaq::RotaryArgs& a, int type, bool interleaved, int num_cus, hipStream_t stream);
+int64_t rolaq_evict_blocks(int64_t B, int64_t most);  // of a launch
 hipError_t rolaq_launch_evict(const rolaq::EvictArgs& a, hipStream_t stream);
 // Bytes of workspace that evict asks for where a request has `most` positions at most.
 int64_t rolaq_evict_ws_bytes(int64_t B, int64_t most);

@@ -138,3 +138,32 @@ def test_values_that_are_not_finite_stay_in_their_pairs():
     same[3, 0, [8, 40]] = False
     assert torch.equal(bad[same], out[same])
     assert not torch.isfinite(bad[~same]).any()
+
+
+@pytest.mark.parametrize("interleaved", [True, False])
+@pytest.mark.parametrize("H,Hk", [(0, 1), (0, 5), (1, 40), (3, 7), (16, 16), (7, 3), (128, 2)])
+def test_heads_of_both_tensors(H, Hk, interleaved):
+    rope = rotary.Rotary(64, interleaved=interleaved, device=DEV)
+    g = torch.Generator().manual_seed(H + Hk)
+    p = torch.randint(0, 100000, (37,), generator=g).to(DEV)
+    q, k = (torch.randn(37, n, 64, generator=g).to(torch.bfloat16).to(DEV) for n in (H, Hk))
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    rotary.apply_rotary(rope, p, q, k, qo, ko)
+    if H:
+        check(qo, q, p, rope)
+    check(ko, k, p, rope)
+
+
+@pytest.mark.parametrize("T,H,dim,dtype", [(70001, 2, 32, torch.bfloat16), (20000, 17, 64, torch.float32), (9001, 5, 6, torch.float16)])
+def test_many_tokens_as_few(T, H, dim, dtype):
+    p, q, k = inputs(T, H, dim, dtype, seed=5)
+    rope = rotary.Rotary(dim, interleaved=T % 2 == 0, device=DEV)
+    qo, ko = torch.empty_like(q), torch.empty_like(k)
+    rotary.apply_rotary(rope, p, q, k, qo, ko)
+    some = torch.cat([torch.arange(3), torch.randint(0, T, (20,)), torch.arange(T - 3, T)]).to(DEV)
+    check(qo[some], q[some], p[some], rope)
+    check(ko[some], k[some], p[some], rope)
+    for i in range(0, T, 1501):
+        s = slice(i, i + 1501)
+        a, b = rotary.apply_rotary(rope, p[s], q[s], k[s], torch.empty_like(q[s]), torch.empty_like(k[s]))
+        assert torch.equal(a, qo[s]) and torch.equal(b, ko[s])
