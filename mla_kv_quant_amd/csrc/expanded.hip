@@ -61,6 +61,17 @@ __device__ __forceinline__ float x_sum2(uint32_t v, float acc) {  // acc + both 
                                          false);
 }
 
+// The largest of the lanes' v, none negative (DPP as in wave_scan).
+__device__ __forceinline__ int wave_max(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 struct XPlace {
   int b, rb;           // request (-1: none), row block
   int q0, nq, past;    // first query, queries computed, keys before the first query's own
@@ -75,7 +86,8 @@ __device__ __host__ inline float x_cost(float blocks, float cus, float longest, 
   return fmaxf(0.65f * longest, 0.6f * each * mean) / (float)parts + (parts > 1 ? 6.f + partial * (float)parts : 0.f);
 }
 // The `want`-th row block of the batch: a request's run together, as they share its keys, the last (which sees most)
-// first, and of up to 64 requests those of most keys first, so that the blocks that a launch ends with are short.
+// first, and of up to 64 requests those of more than half the most keys before the others, so that the blocks that
+// a launch ends with are short.
 // (Row blocks of all requests by their number of keys: 10 prompts of 800, 128 heads, 610 us against 540.)
 // Where the launch has room for parts (a.splits > 1), their number follows from the lengths.
 template <int ROWS, int TK>
@@ -92,14 +104,12 @@ __device__ __forceinline__ XPlace x_place(const ExpandedArgs& a, uint32_t want) 
     const int n = c + lane < a.B ? (nq + ROWS - 1) / ROWS : 0;
     uint32_t start = 0;  // row blocks before this lane's request's
     if (a.B <= 64) {
-      for (int o = 0; o < a.B; ++o) {
-        const int keys = __builtin_amdgcn_readlane(nk, o), blocks = __builtin_amdgcn_readlane(n, o);
-        start += keys > nk || (keys == nk && o < lane) ? (uint32_t)blocks : 0u;
-      }
+      const int most = wave_max(n ? nk : 0);
+      const uint32_t longer = nk > most / 2 ? (uint32_t)n : 0u, rest = (uint32_t)n - longer;
+      const uint32_t to = wave_scan(longer), behind = wave_scan(rest);  // (by all lanes)
+      const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)to, 63);
+      start = longer ? to - longer : first + behind - rest;
       if (a.splits > 1) {
-        int most = n ? nk : 0;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
         const float steps = (float)((nk + TK - 1) / TK), longest = (float)((most + TK - 1) / TK);
         // (a causal request's row blocks see ever fewer keys)
         float all = (float)n * steps - (a.causal ? 0.5f * (float)n * (float)(n - 1) * (float)(ROWS / TK) : 0.f);
