@@ -937,7 +937,6 @@ int rolaq_evict(const float* acc, int64_t acc_stride, int64_t acc_rows, int64_t 
   a.acc_st = acc_stride;
   a.acc_out_st = acc_out_stride;
   a.acc_rows = int(acc_rows);
-  a.acc_cols = acc_cols;
   a.req_idx = req_idx;
   a.kv_indptr = kv_indptr;
   a.kv_indices = kv_indices;

@@ -7,7 +7,8 @@
 // registers, expands them to bf16 (v_cvt_scalef32_pk_bf16_fp4, exact) and goes through the query
 // rows, which lie in LDS as they are, 16 at a time, on bf16 MFMA. A position's sum stays in its
 // lanes until the rows are through, so that each is written once, by one lane, in an
-// order that no other request or launch shape changes. (The scores of the attention itself, 4-bit
+// order that no other request or launch shape changes (but for parts of many rows, whose sums are joined in
+// their order). (The scores of the attention itself, 4-bit
 // codes against a query split into two e4m3 parts, are off by 2^-18 of the largest: the weights
 // were off by 1e-5, now by 3e-7.)
 //

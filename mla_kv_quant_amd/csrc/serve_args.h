@@ -25,11 +25,10 @@ struct RotaryArgs {
 };
 
 struct EvictArgs {
-  const float* acc;  // [acc_rows, acc_cols] accumulated weights, row stride acc_st
+  const float* acc;  // [acc_rows, most or more] accumulated weights, row stride acc_st
   float* acc_out;
   int64_t acc_st, acc_out_st;
   int acc_rows;
-  int64_t acc_cols;
   const int64_t* req_idx;  // [B] or null
   const int32_t* kv_indptr;
   const int32_t* kv_indices;
@@ -42,7 +41,7 @@ struct EvictArgs {
   int32_t* freed;
   int64_t freed_size;
   uint8_t* ws;
-  int64_t most;  // the most positions of a request that take part, at most acc_cols
+  int64_t most;  // the most positions of a request that take part, at most acc's columns
   int chunks;    // set by the launcher: blocks of a request
 };
 
