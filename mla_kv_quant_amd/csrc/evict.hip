@@ -348,6 +348,8 @@ hipError_t rolaq_launch_evict(const rolaq::EvictArgs& args, hipStream_t stream) 
   using namespace rolaq;
   EvictArgs a = args;
   a.chunks = 1;
+  // (where four turns of the threads reach them all: 60 requests of 80 15.3 us with sixteen, 8.8 so)
+  if (a.most <= 4 * kEvictThreads) return launch_evict<-1, 4>(a, (unsigned)a.B, stream);
   if (a.most <= kEvictOne) return launch_evict<-1, 16>(a, (unsigned)a.B, stream);
   const int per = evict_per(a.most);
   a.chunks = (int)((a.most + per * kEvictThreads - 1) / (per * kEvictThreads));

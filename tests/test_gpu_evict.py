@@ -266,7 +266,7 @@ def test_equal_weights_go_to_the_earlier_position(n, budget):
         run_evict([n], budget, 4, 16, 16, w=w, seed=n)
 
 
-@pytest.mark.parametrize("lens", [[16384, 100], [16385, 4096, 0], [40961], [196608], [196609, 16384, 300], [300000]])
+@pytest.mark.parametrize("lens", [[4091, 1000], [4092, 1025], [16384, 100], [16385, 4096, 0], [40961], [196608], [196609, 16384, 300], [300000]])
 def test_long_requests(lens):
     # either side of every change of blocks and chunks, with equal weights across chunks
     g = np.random.default_rng(len(lens))
