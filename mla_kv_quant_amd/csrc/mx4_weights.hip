@@ -478,9 +478,17 @@ template <int D, int R>
 hipError_t launch_weights_rows(const Mx4WeightsArgs& a, int num_cus, hipStream_t stream) {
   const int64_t rows = (int64_t)a.max_q_len * a.H, tiles = (a.n_indices << a.page_shift) / 128 + a.B;
   static_assert(kWeightsFew == 64, "four groups of rows");
-  if (rows <= 16) return launch_weights<D, R, 2, 1>(a, std::min<int64_t>(tiles, 4 * num_cus), stream);
-  if (rows <= 32) return launch_weights<D, R, 2, 2>(a, std::min<int64_t>(tiles, 4 * num_cus), stream);
-  if (rows <= 64) return launch_weights<D, R, 2, 4>(a, std::min<int64_t>(tiles, 2 * num_cus), stream);
+  // Few rows: as many blocks as their LDS leaves room for, four a CU at most (32 requests of 16384, 16 heads: 48.2 us
+  // with four, 51.4 with three, 55.6 with eight; 40 heads of width 512 28 with the two that fit, 35 with more).
+  const auto few = [&](int groups) {
+    const int64_t cu = std::min<int64_t>(4, (160 << 10) / (groups * WGeo<D, R>::QT));
+    return std::min<int64_t>(tiles, cu * num_cus);
+  };
+  if (rows <= 16) return launch_weights<D, R, 2, 1>(a, few(1), stream);
+  if (rows <= 32) return launch_weights<D, R, 2, 2>(a, few(2), stream);
+  // (40 heads of width 256: 20.2 us with three groups, 21.2 with four)
+  if (rows <= 48) return launch_weights<D, R, 2, 3>(a, few(3), stream);
+  if (rows <= 64) return launch_weights<D, R, 2, 4>(a, few(4), stream);
   Mx4WeightsArgs m = a;
   const WeightsPlan p = weights_plan(a.n_indices, a.page_shift, a.B, (int64_t)a.T * a.H, rows, WGeo<D, R>::QR, num_cus);
   m.parts = a.ws ? p.parts : 1;
