@@ -443,9 +443,10 @@ __global__ __launch_bounds__(256) void mx4_weights_join_kernel(Mx4WeightsArgs a)
 
 // Many rows: units of 64 positions at most, and parts of the rows. A unit's steps over its request's rows come one after
 // another, so that a launch takes as long as the longest request's, or as all units' on the blocks that run
-// at once: parts bring the first down to the second, of eight steps at least, if that saves seven (a step takes a
-// microsecond, a second launch and what it reads seven). 7 requests of 51 to 172 positions and up
-// to 51 queries of 128 heads: 238 us in one part, 30 in 19.
+// at once: parts bring the first down to the second, of three steps at least, if that saves three (a step takes
+// two microseconds, a second launch and what it reads six). 7 requests of 51 to 172 positions and up
+// to 51 queries of 128 heads: 238 us in one part, 29 in parts of a few steps; 12 of 21 positions, 20 queries of 48
+// heads: 39 and 24.
 struct WeightsPlan {
   int64_t units;
   int parts;
@@ -456,9 +457,9 @@ static WeightsPlan weights_plan(int64_t n_indices, int page_shift, int B, int64_
   if (rows <= kWeightsFew || B == 0) return p;
   const int64_t steps = (rows + step - 1) / step;
   const double mean = std::min((double)steps, (double)all_rows / B / step + 0.5);
-  const double each = std::max(8.0, (double)p.units * mean / (2.0 * num_cus));
+  const double each = std::max(3.0, (double)p.units * mean / (2.0 * num_cus));
   const int64_t parts = (int64_t)std::ceil((double)steps / each);
-  if (parts > 1 && (double)steps - std::max(each, (double)steps / parts) > 7.0) p.parts = (int)std::min<int64_t>(parts, 2 * num_cus);
+  if (parts > 1 && (double)steps - std::max(each, (double)steps / parts) > 3.0) p.parts = (int)std::min<int64_t>(parts, 2 * num_cus);
   return p;
 }
 
