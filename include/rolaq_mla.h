@@ -404,7 +404,8 @@ int rolaq_expanded_attend_workspace(int64_t T, int64_t N, int B, int H, int nope
  *   s_t = sm_scale (q_nope . k_nope_t,h + q_pe . k_pe_t),  out = softmax(s) v_h.
  * q: bf16 [T, H, nope + rope]; kv: bf16 [N, H, nope + value] (k_nope | v), as kv_b_proj gives
  * it; k_pe: bf16 [N, rope], shared by the heads; out: bf16 [T, H, value]; all 16-byte aligned
- * with strides multiples of 8, kv's and k_pe's from row to row below 2^24. lse (or null): FP32 [T, H], natural log of the sum of exp(s).
+ * with strides multiples of 8, kv's and k_pe's from row to row below 2^24. lse (or null): FP32
+ * [T, H], natural log of the sum of exp(s).
  * (nope, rope, value) = (128, 64, 128) or (64, 32, 64). Weights are rounded to bf16 and out is divided
  * by their sum as rounded; sums are FP32. A query that sees no key gets 0 and -inf (as does one whose scores are all -inf);
  * queries of no request, and past max_q_len of one, are left as they were. Keys and values that a

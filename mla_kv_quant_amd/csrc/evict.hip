@@ -293,7 +293,7 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictArgs a) {
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const uint32_t p = (uint32_t)at(i);
-    const uint32_t c = (uint32_t)__builtin_amdgcn_readfirstlane((int)count[i * kEvictWaves + __builtin_amdgcn_readfirstlane(wave)]);
+    const uint32_t c = (uint32_t)__builtin_amdgcn_readfirstlane((int)count[i * kEvictWaves + wave]);
     const uint32_t s = below(__ballot(sure(i)), more + (c & 0xffffu));
     const uint32_t e = below(__ballot(key[i] == top), equal + (c >> 16));
     const uint32_t place = s + min(e, left);  // kept ones before this position

@@ -134,293 +134,296 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
 #pragma unroll
   for (int s = 0; s < RS; ++s) pe_at[s] = 16 * (la * RC + D / 8 + ((4 * s + gq) ^ w_swz<D>(la)));
   const auto operand = [&](uint32_t rows16, int x) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4*>(smem + rows16 + (x < 4 * JS ? q_at[x % 4] + 256 * (x / 4) : pe_at[x < 4 * JS ? 0 : x - 4 * JS]));
+    const uint32_t at = x < 4 * JS ? q_at[x % 4] + 256 * (x / 4) : pe_at[x < 4 * JS ? 0 : x - 4 * JS];
+    return *reinterpret_cast<const u32x4*>(smem + rows16 + at);
   };
   const uint32_t max_page = (uint32_t)((a.num_slots - 1) >> a.page_shift), max_slot = (uint32_t)(a.num_slots - 1);
   const uint32_t page_mask = (1u << a.page_shift) - 1;
 
   uint32_t before = 0;
   for (int chunk = 0; chunk < a.B; chunk += 64) {
-   const uint32_t units = tiles_of(chunk + lane), cost = cost_of(chunk + lane), incl = wave_scan(units * cost);
-   uint32_t part0, part1;
-   share(before + incl - units * cost, units, cost, part0, part1);
-   before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-   for (uint64_t hit = __builtin_amdgcn_ballot_w64(part0 < part1); hit; hit &= hit - 1) {
-    const int l = __builtin_ctzll(hit), b = chunk + l;
-    const uint32_t t_begin = (uint32_t)__builtin_amdgcn_readlane((int)part0, l);
-    const uint32_t t_end = (uint32_t)__builtin_amdgcn_readlane((int)part1, l);
-    const Mx4Request rq = mx4_request(a, b);
-    const int n = places(b, rq);  // positions
-    const int rows = rq.nq * a.H, qtiles = (rows + 15) / 16;
-    float* const acc = a.acc + (a.req_idx ? a.req_idx[b] : b) * a.acc_st;
-    // Copies of 16 bytes a lane of rows r0 .. r0 + 16 N - 1, N times 16 rows, to LDS at `at`, nine a wave
-    // for every 16 * 9 W / COPIES rows (past the last row: that one again).
-    const int64_t q_row0 = (int64_t)rq.q0 * a.q_st;
-    const auto copy_piece = [&](int r0, int k, uint32_t at) __attribute__((always_inline)) {
-      const int ci = 64 * k + lane, r = ci / RC, c = (ci - r * RC) ^ w_swz<D>(r & 15);
-      const uint32_t row = (uint32_t)min(r0 + r, rows - 1), tok = row / (uint32_t)a.H, head = row - tok * a.H;
-      copy16(a.q + q_row0 + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh + 8 * c, at + 1024 * k);
-    };
-    // lse of row la of 16, and the positions that it sees; a row that saw nothing (lse
-    // -inf), or one past the last, weighs nothing
-    struct Row {
-      float lse;
-      int vis;
-    };
-    const auto row_of = [&](int qt) {
-      const int row = 16 * qt + la;
-      const uint32_t rc = (uint32_t)min(row, rows - 1), tok = rc / (uint32_t)a.H, head = rc - tok * a.H;
-      Row r{a.lse[(int64_t)(rq.q0 + (int)tok) * a.H + head], row < rows ? rq.past + (int)tok + 1 : 0};
-      if (r.lse == -INFINITY) r.lse = INFINITY;
-      return r;
-    };
-    Row qrow[QT > 0 ? QT : 1];
-    if constexpr (QT > 0) {
-      __syncthreads();  // the last request's rows are no longer read
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt)
-        if (qt < qtiles) {
-          for (int k = wave; k < G::QT / 1024; k += W) copy_piece(16 * qt, k, lds0 + qt * G::QT);
-          qrow[qt] = row_of(qt);
-        } else {
-          qrow[qt] = Row{INFINITY, 0};
-        }
-      wait_loads<0>();
-      __syncthreads();
-    }
-    // a tile from unit t: MT sub-tiles of 16 positions for each wave
-    const auto tile = [&](uint32_t t, auto Sub) __attribute__((always_inline)) {
-      constexpr int MT = decltype(Sub)::value;
-      const int p0 = (int)t * TILE + 16 * MT * wave;  // this wave's positions
-      // ---- the keys --------------------------------------------------------------------
-      u32x4 code[MT][JS], pe[MT][RS];
-      float scale[MT][JS];
-      uint32_t nan = 0;
-      uint32_t slot[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int pos = min(p0 + 16 * m + la, n - 1);
-        const uint32_t page = (uint32_t)a.kv_indices[rq.list + (pos >> a.page_shift)];
-        slot[m] = min((min(page, max_page) << a.page_shift) + ((uint32_t)pos & page_mask), max_slot);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint8_t* const c = a.codes + (uint64_t)slot[m] * CB + 16 * gq;
-#pragma unroll
-        for (int s = 0; s < JS; ++s) code[m][s] = gload<u32x4>(c + 64 * s);
-        const uint8_t* const r = reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)slot[m] * (2 * R) + 16 * gq;
-#pragma unroll
-        for (int s = 0; s < RS; ++s) pe[m][s] = gload<u32x4>(r + 64 * s);
-        const uint8_t* const sp = a.scales + (uint64_t)slot[m] * NB;
-        uint32_t w[JS];
-        if constexpr (JS == 4) {
-          const u32x4 v = gload<u32x4>(sp);
-          w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
-        } else {
-          const u32x2 v = gload<u32x2>(sp);
-          w[0] = v[0], w[1] = v[1];
-        }
-#pragma unroll
-        for (int s = 0; s < JS; ++s) {
-          const uint32_t e = (w[s] >> (8 * gq)) & 255u;  // of block 4 s + gq
-          scale[m][s] = __uint_as_float(e << 23);
-          nan |= e == (uint32_t)kMx4NaN ? 1u << (JS * m + s) : 0u;
-        }
-      }
-      float sum[MT][4];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum[m][i] = 0.f;
-      // dword i of the codes of block 4 s + gq of sub-tile m, as values
-      const auto values = [&](int m, int s, int i) {
-        u32x4 v = w_expand(code[m][s][i], scale[m][s]);
-        const uint32_t bad = nan >> (JS * m + s) & 1u ? 0x7fc07fc0u : 0u;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] |= bad;
-        return v;
+    const uint32_t units = tiles_of(chunk + lane), cost = cost_of(chunk + lane), incl = wave_scan(units * cost);
+    uint32_t part0, part1;
+    share(before + incl - units * cost, units, cost, part0, part1);
+    before += (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+    for (uint64_t hit = __builtin_amdgcn_ballot_w64(part0 < part1); hit; hit &= hit - 1) {
+      const int l = __builtin_ctzll(hit), b = chunk + l;
+      const uint32_t t_begin = (uint32_t)__builtin_amdgcn_readlane((int)part0, l);
+      const uint32_t t_end = (uint32_t)__builtin_amdgcn_readlane((int)part1, l);
+      const Mx4Request rq = mx4_request(a, b);
+      const int n = places(b, rq);  // positions
+      const int rows = rq.nq * a.H, qtiles = (rows + 15) / 16;
+      float* const acc = a.acc + (a.req_idx ? a.req_idx[b] : b) * a.acc_st;
+      // Copies of 16 bytes a lane of rows r0 .. r0 + 16 N - 1, N times 16 rows, to LDS at `at`, nine a wave
+      // for every 16 * 9 W / COPIES rows (past the last row: that one again).
+      const int64_t q_row0 = (int64_t)rq.q0 * a.q_st;
+      const auto copy_piece = [&](int r0, int k, uint32_t at) __attribute__((always_inline)) {
+        const int ci = 64 * k + lane, r = ci / RC, c = (ci - r * RC) ^ w_swz<D>(r & 15);
+        const uint32_t row = (uint32_t)min(r0 + r, rows - 1), tok = row / (uint32_t)a.H, head = row - tok * a.H;
+        copy16(a.q + q_row0 + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh + 8 * c, at + 1024 * k);
       };
-      // the scores of 16 rows, C[position 4 gq + i][row la], to weights
-      const auto weigh = [&](const f32x4 (&c)[MT], const Row& r) {
-        // positions that not every row sees (a row past the last sees none)
-        const bool edge = __builtin_amdgcn_ballot_w64(r.vis < p0 + 16 * MT) != 0;
+      // lse of row la of 16, and the positions that it sees; a row that saw nothing (lse
+      // -inf), or one past the last, weighs nothing
+      struct Row {
+        float lse;
+        int vis;
+      };
+      const auto row_of = [&](int qt) {
+        const int row = 16 * qt + la;
+        const uint32_t rc = (uint32_t)min(row, rows - 1), tok = rc / (uint32_t)a.H, head = rc - tok * a.H;
+        Row r{a.lse[(int64_t)(rq.q0 + (int)tok) * a.H + head], row < rows ? rq.past + (int)tok + 1 : 0};
+        if (r.lse == -INFINITY) r.lse = INFINITY;
+        return r;
+      };
+      Row qrow[QT > 0 ? QT : 1];
+      if constexpr (QT > 0) {
+        __syncthreads();  // the last request's rows are no longer read
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+          if (qt < qtiles) {
+            for (int k = wave; k < G::QT / 1024; k += W) copy_piece(16 * qt, k, lds0 + qt * G::QT);
+            qrow[qt] = row_of(qt);
+          } else {
+            qrow[qt] = Row{INFINITY, 0};
+          }
+        wait_loads<0>();
+        __syncthreads();
+      }
+      // a tile from unit t: MT sub-tiles of 16 positions for each wave
+      const auto tile = [&](uint32_t t, auto Sub) __attribute__((always_inline)) {
+        constexpr int MT = decltype(Sub)::value;
+        const int p0 = (int)t * TILE + 16 * MT * wave;  // this wave's positions
+        // ---- the keys --------------------------------------------------------------------
+        u32x4 code[MT][JS], pe[MT][RS];
+        float scale[MT][JS];
+        uint32_t nan = 0;
+        uint32_t slot[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int pos = min(p0 + 16 * m + la, n - 1);
+          const uint32_t page = (uint32_t)a.kv_indices[rq.list + (pos >> a.page_shift)];
+          slot[m] = min((min(page, max_page) << a.page_shift) + ((uint32_t)pos & page_mask), max_slot);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint8_t* const c = a.codes + (uint64_t)slot[m] * CB + 16 * gq;
+#pragma unroll
+          for (int s = 0; s < JS; ++s) code[m][s] = gload<u32x4>(c + 64 * s);
+          const uint8_t* const r = reinterpret_cast<const uint8_t*>(a.rope) + (uint64_t)slot[m] * (2 * R) + 16 * gq;
+#pragma unroll
+          for (int s = 0; s < RS; ++s) pe[m][s] = gload<u32x4>(r + 64 * s);
+          const uint8_t* const sp = a.scales + (uint64_t)slot[m] * NB;
+          uint32_t w[JS];
+          if constexpr (JS == 4) {
+            const u32x4 v = gload<u32x4>(sp);
+            w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+          } else {
+            const u32x2 v = gload<u32x2>(sp);
+            w[0] = v[0], w[1] = v[1];
+          }
+#pragma unroll
+          for (int s = 0; s < JS; ++s) {
+            const uint32_t e = (w[s] >> (8 * gq)) & 255u;  // of block 4 s + gq
+            scale[m][s] = __uint_as_float(e << 23);
+            nan |= e == (uint32_t)kMx4NaN ? 1u << (JS * m + s) : 0u;
+          }
+        }
+        float sum[MT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[m][i] = 0.f;
+        // dword i of the codes of block 4 s + gq of sub-tile m, as values
+        const auto values = [&](int m, int s, int i) {
+          u32x4 v = w_expand(code[m][s][i], scale[m][s]);
+          const uint32_t bad = nan >> (JS * m + s) & 1u ? 0x7fc07fc0u : 0u;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] |= bad;
+          return v;
+        };
+        // the scores of 16 rows, C[position 4 gq + i][row la], to weights
+        const auto weigh = [&](const f32x4 (&c)[MT], const Row& r) {
+          // positions that not every row sees (a row past the last sees none)
+          const bool edge = __builtin_amdgcn_ballot_w64(r.vis < p0 + 16 * MT) != 0;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float w = __builtin_amdgcn_exp2f(fmaf(c[m][i], a.sm_scale, -r.lse) * kLog2e);
+              if (edge) w = p0 + 16 * m + 4 * gq + i < r.vis ? w : 0.f;
+              sum[m][i] += w;
+            }
+        };
+        const auto add_weight = [&](float c, float lse, float& to) __attribute__((always_inline)) {
+          to += __builtin_amdgcn_exp2f(fmaf(c, a.sm_scale, -lse) * kLog2e);
+          asm volatile("" : "+v"(to));  // added here, between the products
+        };
+        if constexpr (QT > 0) {
+          if (p0 < n) {
+            f32x4 c[QT][MT];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+              for (int m = 0; m < MT; ++m) c[qt][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < JS; ++s)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                u32x4 k[MT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) k[m] = values(m, s, i);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                  const u32x4 q = operand(qt * G::QT, 4 * s + i);
+#pragma unroll
+                  for (int m = 0; m < MT; ++m) c[qt][m] = mfma16x16x32(k[m], q, c[qt][m]);
+                }
+              }
+#pragma unroll
+            for (int s = 0; s < RS; ++s)
+#pragma unroll
+              for (int qt = 0; qt < QT; ++qt) {
+                const u32x4 q = operand(qt * G::QT, 4 * JS + s);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) c[qt][m] = mfma16x16x32(pe[m][s], q, c[qt][m]);
+              }
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt)
+              if (QT == 1 || qt < qtiles) weigh(c[qt], qrow[qt]);
+          }
+        } else {
+          // rows that see none of the tile's positions come first: from the first token that does
+          const int tok0 = max((int)t * TILE - rq.past, 0);
+          constexpr int QR = G::QR, SUB = QR / 16;
+          const int all = (rows + QR - 1) / QR, steps = (int)((int64_t)all * (part + 1) / a.parts);
+          const int s0 = (int)min(max((int64_t)tok0 * a.H / QR, (int64_t)all * part / a.parts), (int64_t)steps);
+          // Whose rows lie one behind the other: a step's copies are the last one's, so much further on.
+          const bool flat = a.q_st == (int64_t)a.H * a.q_sh && a.q_sh < (1 << 22);
+          uint32_t off[9];
+#pragma unroll
+          for (int k = 0; k < 9; ++k) {
+            const int ci = 64 * (9 * wave + k) + lane, r = ci / RC;
+            off[k] = (uint32_t)(2 * (r * (int)a.q_sh + 8 * ((ci - r * RC) ^ w_swz<D>(r & 15))));
+          }
+          const auto copy_step = [&](int s) __attribute__((always_inline)) {
+            const uint32_t at = lds0 + (uint32_t)(s & 1) * G::STEP;
+            if (flat && QR * (s + 1) <= rows) {
+              const uint16_t* const from = a.q + q_row0 + (int64_t)QR * s * a.q_sh;
+#pragma unroll
+              for (int k = 0; k < 9; ++k) copy16(from, off[k], at + 1024 * (9 * wave + k));
+            } else {
+#pragma unroll 1
+              for (int k = 0; k < 9; ++k) copy_piece(QR * s, 9 * wave + k, at);
+            }
+          };
+          // lse of the rows la of a step (rows as q0 H + row in a.lse)
+          float next[SUB];
+          const auto load_lse = [&](int s) __attribute__((always_inline)) {
+#pragma unroll
+            for (int q = 0; q < SUB; ++q)
+              next[q] = a.lse[(int64_t)rq.q0 * a.H + min(QR * s + 16 * q + la, rows - 1)];
+          };
+          if (s0 < steps) {
+            copy_step(s0);
+            load_lse(s0);
+          }
+          u32x4 k[MT][JS][4];
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int s = 0; s < JS; ++s)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) k[m][s][i] = values(m, s, i);
+          for (int step = s0; step < steps; ++step) {
+            wait_loads<0>();
+            __syncthreads();  // these rows are there; the last ones are no longer read
+            float lse[SUB];
+#pragma unroll
+            for (int q = 0; q < SUB; ++q) lse[q] = next[q] == -INFINITY ? INFINITY : next[q];
+            if (step + 1 < steps) {
+              copy_step(step + 1);
+              load_lse(step + 1);
+            }
+            const uint32_t rows_at = (uint32_t)(step & 1) * G::STEP;
+            const int first_row = QR * step;
+            constexpr int NS = 4 * JS + RS, AHEAD = 3;  // operands of 16 rows; how many come ahead of their use
+            const auto product = [&](f32x4 (&c)[MT], int x, u32x4 y) __attribute__((always_inline)) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m)
+                c[m] = mfma16x16x32(x < 4 * JS ? k[m][x / 4 % JS][x % 4] : pe[m][x < 4 * JS ? 0 : x - 4 * JS], y,
+                                    x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : c[m]);
+            };
+            if (__builtin_expect(rq.past + first_row / a.H + 1 >= p0 + 16 * MT && first_row + QR <= rows, 1)) {
+              // every row sees every position: the weights of 16 rows between the products of the next 16
+              f32x4 c[2][MT];
+              u32x4 ring[AHEAD + 1];
+              static_for<AHEAD>([&](auto Y) __attribute__((always_inline)) { ring[Y] = operand(rows_at, Y); });
+              static_for<SUB * NS>([&](auto Y) __attribute__((always_inline)) {
+                constexpr int y = decltype(Y)::value, q = y / NS, x = y % NS, ahead = y + AHEAD;
+                if constexpr (ahead < SUB * NS)
+                  ring[ahead % (AHEAD + 1)] = operand(rows_at + ahead / NS * G::QT, ahead % NS);
+                product(c[q % 2], x, ring[y % (AHEAD + 1)]);
+                if constexpr (q > 0) {
+                  constexpr int v0 = x * 4 * MT / NS, v1 = (x + 1) * 4 * MT / NS;
+#pragma unroll
+                  for (int v = v0; v < v1; ++v)
+                    add_weight(c[(q + 1) % 2][v / 4][v % 4], lse[q > 0 ? q - 1 : 0], sum[v / 4][v % 4]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+              });
+#pragma unroll
+              for (int v = 0; v < 4 * MT; ++v) add_weight(c[(SUB - 1) % 2][v / 4][v % 4], lse[SUB - 1], sum[v / 4][v % 4]);
+            } else {
+#pragma unroll
+              for (int q = 0; q < SUB; ++q) {
+                if (first_row + 16 * q >= rows) break;
+                f32x4 c[MT];
+#pragma unroll
+                for (int x = 0; x < NS; ++x) {
+                  product(c, x, operand(rows_at + q * G::QT, x));
+                  if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+                const int row = first_row + 16 * q + la;
+                weigh(c, Row{lse[q], row < rows ? rq.past + (int)((uint32_t)row / (uint32_t)a.H) + 1 : 0});
+              }
+            }
+          }
+          __syncthreads();
+        }
+        // ---- sums over the rows, a position to each lane that writes ------------------------
+        float out = 0.f;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float w = __builtin_amdgcn_exp2f(fmaf(c[m][i], a.sm_scale, -r.lse) * kLog2e);
-            if (edge) w = p0 + 16 * m + 4 * gq + i < r.vis ? w : 0.f;
-            sum[m][i] += w;
+            const float s = row_sum16(sum[m][i]);
+            if (la == 4 * m + i) out = s;
           }
+        static_assert(MT <= 4, "a lane for each position");
+        const int pos = p0 + 16 * (la >> 2) + 4 * gq + (la & 3);
+        if (la < 4 * MT && pos < n) {
+          if (QT == 0 && a.parts > 1)
+            a.ws[part * a.ws_part + ((int64_t)rq.list << a.page_shift) + pos] = out;
+          else
+            acc[pos] = a.add ? acc[pos] + out : out;
+        }
       };
-      const auto add_weight = [&](float c, float lse, float& to) __attribute__((always_inline)) {
-        to += __builtin_amdgcn_exp2f(fmaf(c, a.sm_scale, -lse) * kLog2e);
-        asm volatile("" : "+v"(to));  // added here, between the products
-      };
-      if constexpr (QT > 0) {
-        if (p0 < n) {
-          f32x4 c[QT][MT];
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) c[qt][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < JS; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              u32x4 k[MT];
-#pragma unroll
-              for (int m = 0; m < MT; ++m) k[m] = values(m, s, i);
-#pragma unroll
-              for (int qt = 0; qt < QT; ++qt) {
-                const u32x4 q = operand(qt * G::QT, 4 * s + i);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) c[qt][m] = mfma16x16x32(k[m], q, c[qt][m]);
-              }
-            }
-#pragma unroll
-          for (int s = 0; s < RS; ++s)
-#pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-              const u32x4 q = operand(qt * G::QT, 4 * JS + s);
-#pragma unroll
-              for (int m = 0; m < MT; ++m) c[qt][m] = mfma16x16x32(pe[m][s], q, c[qt][m]);
-            }
-#pragma unroll
-          for (int qt = 0; qt < QT; ++qt)
-            if (QT == 1 || qt < qtiles) weigh(c[qt], qrow[qt]);
-        }
-      } else {
-        // rows that see none of the tile's positions come first: from the first token that does
-        const int tok0 = max((int)t * TILE - rq.past, 0);
-        constexpr int QR = G::QR, SUB = QR / 16;
-        const int all = (rows + QR - 1) / QR, steps = (int)((int64_t)all * (part + 1) / a.parts);
-        const int s0 = (int)min(max((int64_t)tok0 * a.H / QR, (int64_t)all * part / a.parts), (int64_t)steps);
-        // Whose rows lie one behind the other: a step's copies are the last one's, so much further on.
-        const bool flat = a.q_st == (int64_t)a.H * a.q_sh && a.q_sh < (1 << 22);
-        uint32_t off[9];
-#pragma unroll
-        for (int k = 0; k < 9; ++k) {
-          const int ci = 64 * (9 * wave + k) + lane, r = ci / RC;
-          off[k] = (uint32_t)(2 * (r * (int)a.q_sh + 8 * ((ci - r * RC) ^ w_swz<D>(r & 15))));
-        }
-        const auto copy_step = [&](int s) __attribute__((always_inline)) {
-          const uint32_t at = lds0 + (uint32_t)(s & 1) * G::STEP;
-          if (flat && QR * (s + 1) <= rows) {
-            const uint16_t* const from = a.q + q_row0 + (int64_t)QR * s * a.q_sh;
-#pragma unroll
-            for (int k = 0; k < 9; ++k) copy16(from, off[k], at + 1024 * (9 * wave + k));
-          } else {
-#pragma unroll 1
-            for (int k = 0; k < 9; ++k) copy_piece(QR * s, 9 * wave + k, at);
+      for (uint32_t t = t_begin; t < t_end;) {
+        if constexpr (QT > 0) {
+          tile(t, std::integral_constant<int, MOST>{});
+          ++t;
+        } else {
+          const uint32_t left = t_end - t, tiles = (left + MOST - 1) / MOST, sub = (left + tiles - 1) / tiles;
+          if constexpr (MOST >= 4) {
+            if (sub == 4) tile(t, std::integral_constant<int, 4>{});
+            if (sub == 3) tile(t, std::integral_constant<int, 3>{});
           }
-        };
-        // lse of the rows la of a step (rows as q0 H + row in a.lse)
-        float next[SUB];
-        const auto load_lse = [&](int s) __attribute__((always_inline)) {
-#pragma unroll
-          for (int q = 0; q < SUB; ++q)
-            next[q] = a.lse[(int64_t)rq.q0 * a.H + min(QR * s + 16 * q + la, rows - 1)];
-        };
-        if (s0 < steps) {
-          copy_step(s0);
-          load_lse(s0);
+          if (sub == 2) tile(t, std::integral_constant<int, 2>{});
+          if (sub == 1) tile(t, std::integral_constant<int, 1>{});
+          t += sub;
         }
-        u32x4 k[MT][JS][4];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int s = 0; s < JS; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) k[m][s][i] = values(m, s, i);
-        for (int step = s0; step < steps; ++step) {
-          wait_loads<0>();
-          __syncthreads();  // these rows are there; the last ones are no longer read
-          float lse[SUB];
-#pragma unroll
-          for (int q = 0; q < SUB; ++q) lse[q] = next[q] == -INFINITY ? INFINITY : next[q];
-          if (step + 1 < steps) {
-            copy_step(step + 1);
-            load_lse(step + 1);
-          }
-          const uint32_t rows_at = (uint32_t)(step & 1) * G::STEP;
-          const int first_row = QR * step;
-          constexpr int NS = 4 * JS + RS, AHEAD = 3;  // operands of 16 rows; how many come ahead of their use
-          const auto product = [&](f32x4 (&c)[MT], int x, u32x4 y) __attribute__((always_inline)) {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-              c[m] = mfma16x16x32(x < 4 * JS ? k[m][x / 4 % JS][x % 4] : pe[m][x < 4 * JS ? 0 : x - 4 * JS], y,
-                                  x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : c[m]);
-          };
-          if (__builtin_expect(rq.past + first_row / a.H + 1 >= p0 + 16 * MT && first_row + QR <= rows, 1)) {
-            // every row sees every position: the weights of 16 rows between the products of the next 16
-            f32x4 c[2][MT];
-            u32x4 ring[AHEAD + 1];
-            static_for<AHEAD>([&](auto Y) __attribute__((always_inline)) { ring[Y] = operand(rows_at, Y); });
-            static_for<SUB * NS>([&](auto Y) __attribute__((always_inline)) {
-              constexpr int y = decltype(Y)::value, q = y / NS, x = y % NS, ahead = y + AHEAD;
-              if constexpr (ahead < SUB * NS) ring[ahead % (AHEAD + 1)] = operand(rows_at + ahead / NS * G::QT, ahead % NS);
-              product(c[q % 2], x, ring[y % (AHEAD + 1)]);
-              if constexpr (q > 0) {
-                constexpr int v0 = x * 4 * MT / NS, v1 = (x + 1) * 4 * MT / NS;
-#pragma unroll
-                for (int v = v0; v < v1; ++v) add_weight(c[(q + 1) % 2][v / 4][v % 4], lse[q > 0 ? q - 1 : 0], sum[v / 4][v % 4]);
-              }
-              __builtin_amdgcn_sched_barrier(0);
-            });
-#pragma unroll
-            for (int v = 0; v < 4 * MT; ++v) add_weight(c[(SUB - 1) % 2][v / 4][v % 4], lse[SUB - 1], sum[v / 4][v % 4]);
-          } else {
-#pragma unroll
-            for (int q = 0; q < SUB; ++q) {
-              if (first_row + 16 * q >= rows) break;
-              f32x4 c[MT];
-#pragma unroll
-              for (int x = 0; x < NS; ++x) {
-                product(c, x, operand(rows_at + q * G::QT, x));
-                if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-              }
-              const int row = first_row + 16 * q + la;
-              weigh(c, Row{lse[q], row < rows ? rq.past + (int)((uint32_t)row / (uint32_t)a.H) + 1 : 0});
-            }
-          }
-        }
-        __syncthreads();
-      }
-      // ---- sums over the rows, a position to each lane that writes ------------------------
-      float out = 0.f;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float s = row_sum16(sum[m][i]);
-          if (la == 4 * m + i) out = s;
-        }
-      static_assert(MT <= 4, "a lane for each position");
-      const int pos = p0 + 16 * (la >> 2) + 4 * gq + (la & 3);
-      if (la < 4 * MT && pos < n) {
-        if (QT == 0 && a.parts > 1)
-          a.ws[part * a.ws_part + ((int64_t)rq.list << a.page_shift) + pos] = out;
-        else
-          acc[pos] = a.add ? acc[pos] + out : out;
-      }
-    };
-    for (uint32_t t = t_begin; t < t_end;) {
-      if constexpr (QT > 0) {
-        tile(t, std::integral_constant<int, MOST>{});
-        ++t;
-      } else {
-        const uint32_t left = t_end - t, tiles = (left + MOST - 1) / MOST, sub = (left + tiles - 1) / tiles;
-        if constexpr (MOST >= 4) {
-          if (sub == 4) tile(t, std::integral_constant<int, 4>{});
-          if (sub == 3) tile(t, std::integral_constant<int, 3>{});
-        }
-        if (sub == 2) tile(t, std::integral_constant<int, 2>{});
-        if (sub == 1) tile(t, std::integral_constant<int, 1>{});
-        t += sub;
       }
     }
-   }
   }
 }
 
@@ -451,15 +454,18 @@ struct WeightsPlan {
   int64_t units;
   int parts;
 };
-static WeightsPlan weights_plan(int64_t n_indices, int page_shift, int B, int64_t all_rows, int64_t rows, int step, int num_cus) {
+static WeightsPlan weights_plan(int64_t n_indices, int page_shift, int B, int64_t all_rows, int64_t rows, int step,
+                                int num_cus) {
   // (positions stay below 2^30 a request, the units of all below 2^30 as the sums would not fit the memory)
-  WeightsPlan p{std::min<int64_t>((std::min<int64_t>(n_indices, int64_t(1) << 40 >> page_shift) << page_shift) / 64 + B, 1 << 30), 1};
+  const int64_t positions = std::min<int64_t>(n_indices, int64_t(1) << 40 >> page_shift) << page_shift;
+  WeightsPlan p{std::min<int64_t>(positions / 64 + B, 1 << 30), 1};
   if (rows <= kWeightsFew || B == 0) return p;
   const int64_t steps = (rows + step - 1) / step;
   const double mean = std::min((double)steps, (double)all_rows / B / step + 0.5);
   const double each = std::max(3.0, (double)p.units * mean / (2.0 * num_cus));
   const int64_t parts = (int64_t)std::ceil((double)steps / each);
-  if (parts > 1 && (double)steps - std::max(each, (double)steps / parts) > 3.0) p.parts = (int)std::min<int64_t>(parts, 2 * num_cus);
+  if (parts > 1 && (double)steps - std::max(each, (double)steps / parts) > 3.0)
+    p.parts = (int)std::min<int64_t>(parts, 2 * num_cus);
   return p;
 }
 

@@ -114,7 +114,8 @@ def test_two_streams_at_once():
         kept, _, freed = evict.evict(w, ptrs[2], ids, n, 1000 + i)
         return acc, o, kept, freed[:40000 - 1000 - i].clone()
 
-    ptrs, ids, n = [offsets([40]), offsets([6000]), offsets([40000])], torch.arange(40000, dtype=I32, device=DEV), torch.tensor([40000], device=DEV)
+    ptrs = [offsets([40]), offsets([6000]), offsets([40000])]
+    ids, n = torch.arange(40000, dtype=I32, device=DEV), torch.tensor([40000], device=DEV)
     want = [work(0), work(1)]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in b]
