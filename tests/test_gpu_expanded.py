@@ -234,3 +234,25 @@ def test_parts_and_orders_of_row_blocks(dn, H, qlens, klens, causal):
     b.check(o, causal, lse, rows=40)
     ws.fill_(127)
     assert torch.equal(b.run(causal, workspace=ws), o)
+
+
+@pytest.mark.parametrize("dn,H,qlens,klens", [(128, 2, [300, 40], [500, 3000]), (64, 3, [70, 129], [90, 129]), (128, 1, [8], [6000])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_outputs_that_overflow_or_hold_the_largest_values(dn, H, qlens, klens, causal):
+    """Outputs that are not finite are as the formula has them, those beside them are not touched."""
+    b = Batch(dn, H, qlens, klens, seed=17)
+    big = torch.finfo(BF).max
+    clean = b.run(causal)
+    b.kv[:, 0, dn + 1] = big  # every value of a column: sums of outputs pass the range, the outputs do not
+    b.kv[:, 0, dn + 2] = big
+    o = b.run(causal)
+    ok = torch.ones(H, dn, dtype=torch.bool)
+    ok[0, 1:3] = False
+    assert torch.equal(o[:, ok], clean[:, ok])
+    seen = torch.cat([torch.arange(m) + n - m >= 0 for m, n in zip(qlens, klens)]) if causal else slice(None)
+    assert (o[seen, 0, 1].float() >= big * (1 - 2.0 ** -7)).all()
+    b.q[3] = float("nan")
+    lse = torch.zeros(sum(qlens), H, device=DEV)
+    o2 = b.run(causal, lse)
+    rest = torch.arange(sum(qlens)) != 3
+    assert torch.equal(o2[rest], o[rest]) and torch.isnan(o2[3]).all() and torch.isfinite(lse[rest]).all()
