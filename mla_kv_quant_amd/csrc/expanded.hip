@@ -13,8 +13,8 @@
 // sums are of the weights as rounded to bf16, by which the output's weights add up to one.
 //
 // Bound: matrix instructions at the clock that the power limit leaves, two waves to a SIMD: 16 heads of 4 x 4096
-// queries 340 to 400 us by card (344 GFLOP, 0.86 to 1.02 PFLOP/s; a large library product reaches 1.24), 55 % of the
-// cycles at 1.77 GHz with one under way; 40 heads of 4 x 2048 behind 14336, 64 wide, 1.63 ms (0.99). Without the
+// queries 330 to 400 us by card (344 GFLOP, 0.86 to 1.04 PFLOP/s; a large library product reaches 1.24), 55 % of the
+// cycles at 1.77 GHz with one under way; 40 heads of 4 x 2048 behind 14336, 64 wide, 1.57 to 1.61 ms (1.0). Without the
 // weights' arithmetic it takes 20 to 30 % less, without the copies 15 %, without the reads of keys and values 6 %.
 // 256 rows a block, 64 rows a wave (one wave to a SIMD), rings of 8 steps and operands read 9
 // instructions ahead were no faster (480 us for 430 with 64 rows).
