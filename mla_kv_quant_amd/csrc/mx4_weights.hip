@@ -59,16 +59,18 @@ __device__ __forceinline__ u32x4 w_expand(uint32_t v, float f) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v, f, 3))};
 }
 
-// Sum over the 16 lanes of a row of lanes, on each of them.
+// Sum over the 16 lanes of a row of lanes, the same bits on each of them: both sides of an exchange add the same
+// two sums. (Which lane writes a position follows from where its tile starts, so from the batch; sums of rotated lanes
+// differed by lane in their last bit.)
 template <int CTRL>
-__device__ __forceinline__ float add_ror(float v) {
+__device__ __forceinline__ float add_dpp(float v) {
   return v + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xF, 0xF, false));
 }
 __device__ __forceinline__ float row_sum16(float v) {
-  v = add_ror<0x121>(v);
-  v = add_ror<0x122>(v);
-  v = add_ror<0x124>(v);
-  return add_ror<0x128>(v);
+  v = add_dpp<0xB1>(v);     // quad_perm 1, 0, 3, 2
+  v = add_dpp<0x4E>(v);     // quad_perm 2, 3, 0, 1
+  v = add_dpp<0x141>(v);    // row_half_mirror: the other four of eight
+  return add_dpp<0x140>(v);  // row_mirror: the other eight
 }
 
 // QT > 0: at most 16 QT rows a request, kept in LDS; 0: any number, streamed.
