@@ -472,7 +472,9 @@ int rolaq_evict_workspace(int B, int64_t max_kv_len, int64_t* bytes);
  *                 left as they were. May be acc itself (same address and stride), else must not overlap it.
  * kept, with offsets b * budget, is a page list of pages of one slot. Rows r of one call must
  * differ. acc and acc_out: FP32 [acc_rows, acc_cols]. workspace: rolaq_evict_workspace bytes,
- * 16-byte aligned, not shared with a call that overlaps. No allocation, no synchronisation.
+ * 16-byte aligned, not shared with a call that overlaps. No allocation, no synchronisation. Outputs and workspace
+ * overlap neither each other nor an input, acc_out on acc apart: in particular kept_lens is not kv_lens,
+ * and kept and freed are not parts of kv_indices (calls where they do are refused).
  */
 int rolaq_evict(const float* acc, int64_t acc_stride, int64_t acc_rows, int64_t acc_cols, float* acc_out,
                 int64_t acc_out_stride, const int64_t* req_idx, const int32_t* kv_indptr, const int32_t* kv_indices,

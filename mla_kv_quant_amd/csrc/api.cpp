@@ -7,6 +7,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <utility>
 
 #include "../../include/rolaq_mla.h"
 
@@ -702,6 +703,42 @@ int rolaq_mx4_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
 
 // ---- rotary positions, expanded attention, accumulated weights, eviction ---------------
 
+namespace {
+
+// Rows of memory: `rows` of `width` bytes each, `stride` (width or more) apart.
+struct Rows {
+  const char* name;
+  uintptr_t at;
+  int64_t rows, width, stride;
+};
+
+Rows flat(const char* name, const void* p, int64_t bytes) {
+  return {name, reinterpret_cast<uintptr_t>(p), bytes > 0 && p ? 1 : 0, bytes, bytes};
+}
+
+// Whether two of them share a byte. Those of one stride (parts of the columns of one tensor) by their distance
+// modulo it; else row by row, where their ranges meet at all.
+bool meet(Rows a, Rows b) {
+  if (a.rows == 0 || b.rows == 0 || a.width == 0 || b.width == 0) return false;
+  const auto end = [](const Rows& r) { return r.at + uintptr_t(r.rows - 1) * r.stride + r.width; };
+  if (end(a) <= b.at || end(b) <= a.at) return false;
+  if (a.stride == b.stride && a.rows > 1 && b.rows > 1) {
+    if (b.at < a.at) std::swap(a, b);
+    const int64_t k = int64_t((b.at - a.at) / a.stride), d = int64_t((b.at - a.at) % a.stride);
+    // (row j of b begins d behind row j + k of a)
+    return (d < a.width && k < a.rows) || (d + b.width > a.stride && k + 1 < a.rows);
+  }
+  if (a.rows > b.rows) std::swap(a, b);
+  for (int64_t i = 0; i < a.rows; ++i) {
+    const uintptr_t lo = a.at + uintptr_t(i) * a.stride, hi = lo + a.width;
+    const int64_t j = lo < b.at + b.width ? 0 : int64_t((lo - b.at - b.width) / b.stride) + 1;  // the first to end behind lo
+    if (j < b.rows && b.at + uintptr_t(j) * b.stride < hi) return true;
+  }
+  return false;
+}
+
+}  // namespace
+
 extern "C" {
 
 int rolaq_rotary(const int64_t* positions, int64_t T, const uint64_t* turns, int dim, float scale, int interleaved,
@@ -931,6 +968,20 @@ int rolaq_evict(const float* acc, int64_t acc_stride, int64_t acc_rows, int64_t 
     return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
   if (rolaq_evict_blocks(B, max_kv_len) > (1 << 21))
     return fail(ROLAQ_ERR_INVALID, "%s: B * max_kv_len is too large for one launch", fn);
+  // Blocks read lengths and lists of other requests than the one that they write for, in no order.
+  const Rows in[] = {{"acc", reinterpret_cast<uintptr_t>(acc), acc_rows, 4 * acc_cols, 4 * acc_stride},
+                     flat("req_idx", req_idx, 8 * int64_t(B)), flat("kv_indptr", kv_indptr, 4 * (int64_t(B) + 1)),
+                     flat("kv_indices", kv_indices, 4 * n_indices), flat("kv_lens", kv_lens, 8 * int64_t(B))};
+  const Rows out[] = {{"acc_out", reinterpret_cast<uintptr_t>(acc_out), acc_rows, 4 * acc_cols, 4 * acc_out_stride},
+                      flat("kept", kept, 4 * int64_t(B) * budget), flat("kept_lens", kept_lens, 8 * int64_t(B)),
+                      flat("freed", freed, 4 * freed_size), flat("workspace", workspace, ws)};
+  for (const Rows& o : out) {
+    for (const Rows& i : in)
+      if (!(&o == &out[0] && &i == &in[0] && acc == acc_out && acc_stride == acc_out_stride) && meet(o, i))
+        return fail(ROLAQ_ERR_INVALID, "%s: %s must not overlap %s", fn, o.name, i.name);
+    for (const Rows* p = out; p != &o; ++p)
+      if (meet(o, *p)) return fail(ROLAQ_ERR_INVALID, "%s: %s must not overlap %s", fn, o.name, p->name);
+  }
   rolaq::EvictArgs a{};
   a.acc = acc;
   a.acc_out = acc_out;

@@ -52,7 +52,8 @@ def evict(acc, kv_indptr, kv_indices, kv_lens, budget: int, sink: int = 4, recen
     ``acc_out`` (``acc`` itself if not given) receives the weights of what stays in its new columns, and 0 in the
     others up to the old length. ``max_kv_len``: the most positions of a request (``acc``'s columns if not given), longer
     requests are cut there: their other positions are neither kept nor freed. Lists, lengths and rows as for
-    :func:`accumulate_weights`. Outputs that are not given are allocated.
+    :func:`accumulate_weights`. Outputs that are not given are allocated; none may overlap another or an input (``kept_lens``
+    is not ``kv_lens``, ``kept`` no part of ``kv_indices``), ``acc_out`` on ``acc`` itself apart.
     """
     dev = acc.device
     kv_lens = _as_int64(kv_lens)
