@@ -48,10 +48,13 @@ def evict(acc, kv_indptr, kv_indices, kv_lens, budget: int, sink: int = 4, recen
     ``recent`` and, of the others, those of largest ``acc`` (the earlier of equal ones; NaN counts as the largest).
     ``kept``: int32 ``[B, budget]`` slots in order of position, of which ``kept_lens`` (int64 ``[B]``) are set:
     a page list of pages of one slot, with ``b * budget`` as its offsets. ``freed``: int32, the other slots, request
-    after request; ``sum(max(kv_lens - budget, 0))`` of them, later entries (and slots past its end) are left out.
+    after request: ``n - kept_lens`` of each, ``n`` being its length, cut as below. Later entries of one that is given are
+    left as they were (and slots past its end left out), of one that is allocated here they are -1.
     ``acc_out`` (``acc`` itself if not given) receives the weights of what stays in its new columns, and 0 in the
-    others up to the old length. ``max_kv_len``: the most positions of a request (``acc``'s columns if not given), longer
-    requests are cut there: their other positions are neither kept nor freed. Lists, lengths and rows as for
+    others up to the old length. ``max_kv_len``: the most positions of a request (``acc``'s columns if not given, and at
+    most those). A longer request is cut there, as one that is longer than its page list reaches is at that: the
+    positions past it, its newest ones, are neither kept nor freed, and ``recent`` counts from the cut. Lists,
+    lengths and rows as for
     :func:`accumulate_weights`. Outputs that are not given are allocated; none may overlap another or an input (``kept_lens``
     is not ``kv_lens``, ``kept`` no part of ``kv_indices``), ``acc_out`` on ``acc`` itself apart.
     """
@@ -65,7 +68,7 @@ def evict(acc, kv_indptr, kv_indices, kv_lens, budget: int, sink: int = 4, recen
     if kept_lens is None:
         kept_lens = torch.empty(B, dtype=torch.int64, device=dev)
     if freed is None:
-        freed = torch.empty(kv_indices.shape[0] * page_size, dtype=torch.int32, device=dev)
+        freed = torch.full((kv_indices.shape[0] * page_size,), -1, dtype=torch.int32, device=dev)
     req = None if req_pool_indices is None else _as_int64(req_pool_indices)
     kernels.evict(acc, kv_indptr, kv_indices, kv_lens, budget, sink, recent, page_size, req,
                   acc.shape[1] if max_kv_len is None else min(max_kv_len, acc.shape[1]), acc if acc_out is None else acc_out,

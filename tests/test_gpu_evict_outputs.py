@@ -49,3 +49,28 @@ def test_outputs_on_inputs_are_refused():
     with pytest.raises(ValueError, match="acc_out must not overlap acc"):
         evict.evict(acc[:, :400], ptr, ids, n, 60, acc_out=acc[:, 100:])
     assert n.tolist() == [500, 300]
+
+
+@pytest.mark.parametrize("lens,cols,kw,cut", [
+    ([500, 90, 300], 500, {}, [500, 90, 300]), ([500, 90, 300], 200, {}, [200, 90, 200]),
+    ([500, 90, 300], 500, {"max_kv_len": 250}, [250, 90, 250]), ([20000, 90], 18000, {}, [18000, 90]),
+    ([20000, 400], 20000, {"max_kv_len": 17000}, [17000, 400]), ([30, 90], 100, {}, [30, 90]),
+])
+def test_how_many_are_freed(lens, cols, kw, cut):
+    acc, ptr, ids, n = batch(lens, cols)
+    torch.full((ids.numel(),), 5, dtype=I32, device=DEV)  # (what an allocation may find)
+    kept, kept_lens, freed = evict.evict(acc, ptr, ids, n, 64, **kw)
+    gone = freed[freed >= 0]
+    assert gone.numel() == (torch.tensor(cut) - kept_lens.cpu()).sum() and (freed[gone.numel():] == -1).all()
+    at, seen = 0, ids.tolist()
+    for b, m in enumerate(cut):
+        own = seen[sum(lens[:b]):sum(lens[:b]) + m]
+        rest = m - int(kept_lens[b])
+        assert sorted(kept[b, :int(kept_lens[b])].tolist() + gone[at:at + rest].tolist()) == sorted(own)
+        at += rest
+
+
+def test_requests_longer_than_their_lists():
+    acc, ptr, ids, _ = batch([500, 300], 600)
+    kept, kept_lens, freed = evict.evict(acc, ptr, ids, torch.tensor([600, 10 ** 9], device=DEV), 64)
+    assert kept_lens.tolist() == [64, 64] and (freed >= 0).sum() == 800 - 128
