@@ -425,7 +425,8 @@ int rolaq_expanded_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_strid
  * query rows:
  *   acc[r, t] = (add ? acc[r, t] : 0) + sum over the queries i and heads h that see t of exp(s_t - lse[i, h]),
  * s_t, who sees what, the cache, the index lists and their bounds as in rolaq_mx4_attend_fwd, whose
- * lse ([T, H], contiguous) this takes; rows with lse = -inf count for nothing. r = req_idx[b] (null: b):
+ * lse ([T, H], contiguous) this takes; rows with lse = -inf count for nothing, whatever q holds there.
+ * r = req_idx[b] (null: b):
  * a request whose r is outside 0 .. acc_rows - 1 is left out, positions from acc_cols on are not
  * counted; rows r of one call must differ. acc: FP32, row stride acc_stride. A request's sums do not depend
  * on the batch. No workspace, no allocation, no synchronisation.

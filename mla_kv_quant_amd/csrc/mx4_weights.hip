@@ -164,8 +164,8 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
         const uint32_t row = (uint32_t)min(r0 + r, rows - 1), tok = row / (uint32_t)a.H, head = row - tok * a.H;
         copy16(a.q + q_row0 + (int64_t)tok * a.q_st + (int64_t)head * a.q_sh + 8 * c, at + 1024 * k);
       };
-      // lse of row la of 16, and the positions that it sees; a row that saw nothing (lse
-      // -inf), or one past the last, weighs nothing
+      // lse of row la of 16, and the positions that it sees; a row that saw nothing (lse -inf, whatever its query
+      // holds), or one past the last, sees none
       struct Row {
         float lse;
         int vis;
@@ -173,9 +173,8 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
       const auto row_of = [&](int qt) {
         const int row = 16 * qt + la;
         const uint32_t rc = (uint32_t)min(row, rows - 1), tok = rc / (uint32_t)a.H, head = rc - tok * a.H;
-        Row r{a.lse[(int64_t)(rq.q0 + (int)tok) * a.H + head], row < rows ? rq.past + (int)tok + 1 : 0};
-        if (r.lse == -INFINITY) r.lse = INFINITY;
-        return r;
+        const float lse = a.lse[(int64_t)(rq.q0 + (int)tok) * a.H + head];
+        return Row{lse, row < rows && lse != -INFINITY ? rq.past + (int)tok + 1 : 0};
       };
       Row qrow[QT > 0 ? QT : 1];
       if constexpr (QT > 0) {
@@ -245,7 +244,7 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
         };
         // the scores of 16 rows, C[position 4 gq + i][row la], to weights
         const auto weigh = [&](const f32x4 (&c)[MT], const Row& r) {
-          // positions that not every row sees (a row past the last sees none)
+          // positions that not every row sees
           const bool edge = __builtin_amdgcn_ballot_w64(r.vis < p0 + 16 * MT) != 0;
 #pragma unroll
           for (int m = 0; m < MT; ++m)
@@ -340,8 +339,13 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
             wait_loads<0>();
             __syncthreads();  // these rows are there; the last ones are no longer read
             float lse[SUB];
+            bool none = false;
 #pragma unroll
-            for (int q = 0; q < SUB; ++q) lse[q] = next[q] == -INFINITY ? INFINITY : next[q];
+            for (int q = 0; q < SUB; ++q) {
+              lse[q] = next[q];
+              none = none || lse[q] == -INFINITY;
+            }
+            const bool all_weigh = __builtin_amdgcn_ballot_w64(none) == 0;
             if (step + 1 < steps) {
               copy_step(step + 1);
               load_lse(step + 1);
@@ -355,7 +359,7 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
                 c[m] = mfma16x16x32(x < 4 * JS ? k[m][x / 4 % JS][x % 4] : pe[m][x < 4 * JS ? 0 : x - 4 * JS], y,
                                     x == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : c[m]);
             };
-            if (__builtin_expect(rq.past + first_row / a.H + 1 >= p0 + 16 * MT && first_row + QR <= rows, 1)) {
+            if (__builtin_expect(all_weigh && rq.past + first_row / a.H + 1 >= p0 + 16 * MT && first_row + QR <= rows, 1)) {
               // every row sees every position: the weights of 16 rows between the products of the next 16
               f32x4 c[2][MT];
               u32x4 ring[AHEAD + 1];
@@ -386,7 +390,8 @@ __global__ __launch_bounds__(256, 2) void mx4_weights_kernel(Mx4WeightsArgs a) {
                   if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
                 const int row = first_row + 16 * q + la;
-                weigh(c, Row{lse[q], row < rows ? rq.past + (int)((uint32_t)row / (uint32_t)a.H) + 1 : 0});
+                weigh(c, Row{lse[q], row < rows && lse[q] != -INFINITY
+                                         ? rq.past + (int)((uint32_t)row / (uint32_t)a.H) + 1 : 0});
               }
             }
           }

@@ -27,9 +27,10 @@ def accumulate_weights(q, lse, pool, layer_id, acc, kv_indptr, kv_indices, kv_le
     """Add to ``acc`` the attention weight that each cached position gets from ``q``, over all queries and heads.
 
     ``q``, the index lists, ``kv_lens``, ``qo_indptr`` and ``max_q_len`` as for ``mx4.attend_fwd``, and ``lse`` as it
-    returned for these queries (rows with -inf count for nothing). ``acc``: FP32 ``[rows, columns]``; position ``t`` of
-    request ``b`` is column ``t`` of row ``req_pool_indices[b]`` (row ``b`` if not given). Rows of one call must differ; a
-    request whose row does not exist is left out, as are positions past the columns. With ``add=False`` the sums
+    returned for these queries (rows with -inf count for nothing, whatever ``q`` holds there: a batch's padding).
+    ``acc``: FP32 ``[rows, columns]``; position ``t`` of request ``b`` is column ``t`` of row ``req_pool_indices[b]`` (row
+    ``b`` if not given). Rows of one call must differ; a request whose row does not exist is left out, as are
+    positions past the columns. With ``add=False`` the sums
     take the place of what the cached positions' columns held. Returns ``acc``.
     """
     li = layer_id - pool.start_layer
