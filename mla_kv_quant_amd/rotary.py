@@ -26,14 +26,27 @@ from . import kernels
 _PER_TURN = Fraction("0.1591549430918953357688837633725143620344596457404564487476673441")
 
 
-def _yarn_ramp(dim, base, original, beta_fast, beta_slow):
+# what a scaling of each kind may state (besides the rotary base, where it is ``base``)
+_STATED = {
+    "default": (),
+    "linear": ("factor", "original_max_position_embeddings"),
+    "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "truncate", "mscale", "mscale_all_dim",
+             "attention_factor"),
+    "longrope": ("factor", "original_max_position_embeddings", "long_factor", "short_factor", "long", "attention_factor"),
+}
+
+
+def _yarn_ramp(dim, base, original, beta_fast, beta_slow, truncate):
     """0 for pairs that turn more than ``beta_fast`` times over the ``original`` length, 1 for those that turn
-    less than ``beta_slow`` times, linear in the pair's number between."""
+    less than ``beta_slow`` times, linear in the pair's number between (``truncate``: between whole numbers)."""
 
     def pair(turns):
         return dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), dim - 1)
+    low, high = pair(beta_fast), pair(beta_slow)
+    if truncate:
+        low, high = math.floor(low), math.ceil(high)
+    low, high = max(low, 0), min(high, dim - 1)
     width = high - low if high > low else 0.001
     return [min(max((i - low) / width, 0.0), 1.0) for i in range(dim // 2)]
 
@@ -43,18 +56,27 @@ def frequencies(dim: int, base: float = 10000.0, scaling: dict | None = None):
     factor of sines and cosines.
 
     ``scaling``: a configuration's ``rope_scaling`` (its kind under ``type`` or ``rope_type``): ``linear``
-    (``factor``), ``yarn`` (``factor``, ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, and
+    (``factor``), ``yarn`` (``factor``, ``original_max_position_embeddings``, ``beta_fast``, ``beta_slow``, ``truncate``, and
     ``mscale`` / ``mscale_all_dim`` or ``attention_factor``), ``longrope`` (``long_factor`` and ``short_factor``, a
     divisor for each pair, ``factor`` and ``original_max_position_embeddings``, or ``attention_factor``; ``long`` says
-    which of the two lists, the first by default), ``default`` or None.
+    which of the two lists, the first by default), ``default`` or None. An entry that its kind does not have, or one
+    that is missing, is refused: configurations that keep the context's factor or original length outside of
+    ``rope_scaling`` have to add them. Entries of None count as missing.
     """
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary width must be even and positive, got {dim}")
     if not (math.isfinite(base) and base > 1):
         raise ValueError(f"rotary base must be finite and above 1, got {base}")
     f = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
-    s = scaling or {}
+    s = {k: v for k, v in (scaling or {}).items() if v is not None}
     kind = s.get("type", s.get("rope_type", "default"))
+    if kind not in _STATED:
+        raise ValueError(f"unknown rope scaling {kind!r}")
+    unknown = sorted(set(s) - {"type", "rope_type", "rope_theta", *_STATED[kind]})
+    if unknown:
+        raise ValueError(f"rope scaling {kind!r} has no {', '.join(unknown)}")
+    if s.get("rope_theta", base) != base:
+        raise ValueError(f"rope scaling states rope_theta {s['rope_theta']!r}, base is {base!r}")
     if kind == "default":
         return f, 1.0
 
@@ -69,30 +91,33 @@ def frequencies(dim: int, base: float = 10000.0, scaling: dict | None = None):
         return [x / factor for x in f], 1.0
     if kind == "yarn":
         factor, original = number("factor"), number("original_max_position_embeddings")
-        ramp = _yarn_ramp(dim, base, original, number("beta_fast", 32.0), number("beta_slow", 1.0))
+        ramp = _yarn_ramp(dim, base, original, number("beta_fast", 32.0), number("beta_slow", 1.0),
+                          s.get("truncate", True))
 
         def mscale(m):
             return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
 
-        if s.get("attention_factor") is not None:
+        by_m, by_all = s.get("mscale"), s.get("mscale_all_dim")
+        if "attention_factor" in s:
             scale = number("attention_factor")
-        elif s.get("mscale") and s.get("mscale_all_dim"):
+        elif by_m and by_all:
             scale = mscale(number("mscale")) / mscale(number("mscale_all_dim"))
+        elif by_all or (by_m and by_m != 1):
+            # (published code differs in what the other one is then)
+            raise ValueError("rope scaling 'yarn' needs mscale and mscale_all_dim together, or attention_factor")
         else:
             scale = mscale(1.0)
         return [x / factor * r + x * (1.0 - r) for x, r in zip(f, ramp)], scale
-    if kind == "longrope":
-        by = s.get("long_factor" if s.get("long", True) else "short_factor")
-        if not isinstance(by, (list, tuple)) or len(by) != dim // 2 or not all(
-                isinstance(v, (int, float)) and math.isfinite(v) and v > 0 for v in by):
-            raise ValueError(f"rope scaling 'longrope' needs {dim // 2} positive factors")
-        if s.get("attention_factor") is not None:
-            scale = number("attention_factor")
-        else:
-            factor, original = number("factor", 1.0), number("original_max_position_embeddings", least=1.0)
-            scale = math.sqrt(1.0 + math.log(factor) / math.log(original)) if factor > 1 else 1.0
-        return [x / v for x, v in zip(f, by)], scale
-    raise ValueError(f"unknown rope scaling {kind!r}")
+    by = s.get("long_factor" if s.get("long", True) else "short_factor")
+    if not isinstance(by, (list, tuple)) or len(by) != dim // 2 or not all(
+            isinstance(v, (int, float)) and math.isfinite(v) and v > 0 for v in by):
+        raise ValueError(f"rope scaling 'longrope' needs {dim // 2} positive factors")
+    if "attention_factor" in s:
+        scale = number("attention_factor")
+    else:
+        factor, original = number("factor"), number("original_max_position_embeddings", least=1.0)
+        scale = math.sqrt(1.0 + math.log(factor) / math.log(original)) if factor > 1 else 1.0
+    return [x / v for x, v in zip(f, by)], scale
 
 
 class Rotary:
