@@ -23,7 +23,7 @@ from .writer import _as_int64
 
 
 def accumulate_weights(q, lse, pool, layer_id, acc, kv_indptr, kv_indices, kv_lens, sm_scale, qo_indptr=None,
-                       max_q_len: int = 1, page_size: int = 1, req_pool_indices=None, add: bool = True):
+                       max_q_len: int = 1, page_size: int = 1, req_pool_indices=None, add: bool = True, workspace=None):
     """Add to ``acc`` the attention weight that each cached position gets from ``q``, over all queries and heads.
 
     ``q``, the index lists, ``kv_lens``, ``qo_indptr`` and ``max_q_len`` as for ``mx4.attend_fwd``, and ``lse`` as it
@@ -31,13 +31,15 @@ def accumulate_weights(q, lse, pool, layer_id, acc, kv_indptr, kv_indices, kv_le
     ``acc``: FP32 ``[rows, columns]``; position ``t`` of request ``b`` is column ``t`` of row ``req_pool_indices[b]`` (row
     ``b`` if not given). Rows of one call must differ; a request whose row does not exist is left out, as are
     positions past the columns. With ``add=False`` the sums
-    take the place of what the cached positions' columns held. Returns ``acc``.
+    take the place of what the cached positions' columns held. ``workspace``: uint8, of
+    ``kernels.accumulate_weights_workspace_bytes`` and used by no other call at the same time; allocated on the
+    current stream when not given and needed. Returns ``acc``.
     """
     li = layer_id - pool.start_layer
     req = None if req_pool_indices is None else _as_int64(req_pool_indices)
     return kernels.mx4_accumulate_weights(q, lse, pool.c_codes[li], pool.c_scales[li], pool.rope_buf[li], qo_indptr,
                                           kv_indptr, kv_indices, _as_int64(kv_lens), max_q_len, acc, sm_scale, page_size,
-                                          req, add)
+                                          req, add, workspace)
 
 
 def evict(acc, kv_indptr, kv_indices, kv_lens, budget: int, sink: int = 4, recent: int = 16, page_size: int = 1,
@@ -57,7 +59,10 @@ def evict(acc, kv_indptr, kv_indices, kv_lens, budget: int, sink: int = 4, recen
     positions past it, its newest ones, are neither kept nor freed, and ``recent`` counts from the cut. Lists,
     lengths and rows as for
     :func:`accumulate_weights`. Outputs that are not given are allocated; none may overlap another or an input (``kept_lens``
-    is not ``kv_lens``, ``kept`` no part of ``kv_indices``), ``acc_out`` on ``acc`` itself apart.
+    is not ``kv_lens``, ``kept`` no part of ``kv_indices``), ``acc_out`` on ``acc`` itself apart. ``workspace``: uint8, of
+    ``kernels.evict_workspace_bytes`` for this ``max_kv_len``, used by no other call at the same time; allocated on the
+    current stream when not given and needed. It follows from ``max_kv_len``, not from the lengths, as do the
+    launches: one up to 16384, else four. Where ``acc`` has more columns than the batch is long, state it.
     """
     dev = acc.device
     kv_lens = _as_int64(kv_lens)

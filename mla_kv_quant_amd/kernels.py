@@ -685,11 +685,20 @@ def mx4_accumulate_weights(q: torch.Tensor, lse: torch.Tensor, codes: torch.Tens
     return acc
 
 
+def evict_workspace_bytes(B: int, max_kv_len: int, device) -> int:
+    """Bytes of :func:`evict`'s workspace for ``B`` requests of ``max_kv_len`` positions at most (0: none)."""
+    n = ctypes.c_int64(0)
+    _call(torch.device(device), _lib.load().rolaq_evict_workspace, int(B), int(max_kv_len), ctypes.byref(n))
+    return n.value
+
+
 def evict(acc: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor, kv_lens: torch.Tensor, budget: int,
           sink: int, recent: int, page_size: int, req_idx: torch.Tensor | None, max_kv_len: int, acc_out: torch.Tensor,
           kept: torch.Tensor, kept_lens: torch.Tensor, freed: torch.Tensor,
           workspace: torch.Tensor | None = None) -> None:
-    """The positions that stay of every request: slots in ``kept [B, budget]``, weights in ``acc_out``, the rest in ``freed``."""
+    """The positions that stay of every request: slots in ``kept [B, budget]``, weights in ``acc_out``, the rest in ``freed``.
+
+    ``workspace``: uint8, :func:`evict_workspace_bytes` long; allocated here when not given."""
     dev = acc.device
     i32, i64 = torch.int32, torch.int64
     _need_all(dev, ((kv_indptr, "kv_indptr", i32, 1), (kv_indices, "kv_indices", i32, 1), (kv_lens, "kv_lens", i64, 1),
@@ -707,10 +716,9 @@ def evict(acc: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor, 
     if acc_out.shape != acc.shape:
         raise ValueError("acc_out must have acc's shape")
     if workspace is None:
-        n = ctypes.c_int64(0)
-        if 0 <= max_kv_len <= 1 << 30:  # (a call that the library refuses is left to it)
-            _call(dev, _lib.load().rolaq_evict_workspace, B, int(max_kv_len), ctypes.byref(n))
-        workspace = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
+        # (a call that the library refuses is left to it)
+        n = evict_workspace_bytes(B, max_kv_len, dev) if 0 <= max_kv_len <= 1 << 30 else 0
+        workspace = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     else:
         _need_all(dev, ((workspace, "workspace", torch.uint8, 1),))
     _call(dev, _lib.load().rolaq_evict, _p(acc), stride, acc.shape[0], acc.shape[1], _p(acc_out), out_stride, _p(req_idx),
