@@ -817,7 +817,8 @@ int rolaq_expanded_attend_fwd(const void* q, int64_t q_stride_t, int64_t q_strid
   const int64_t ws = rolaq_expanded_ws_bytes(T, N, B, H, nope, most, cu_count());
   if (ws > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < ws))
     return fail(ROLAQ_ERR_INVALID, "%s: workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)ws);
-  if ((T / 32 + B) * H > (1 << 24))  // (2^32 threads and more are too many for one launch)
+  // (2^32 threads and more are too many for one launch; it has a block for 128 queries at most)
+  if ((T / 32 + B) * H > (1 << 24) || (T / 128 + B) * H >= (1 << 24))
     return fail(ROLAQ_ERR_INVALID, "%s: T * H is too large for one launch", fn);
   rolaq::ExpandedArgs a{};
   a.q = static_cast<const uint16_t*>(q);
