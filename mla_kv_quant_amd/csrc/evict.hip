@@ -309,8 +309,11 @@ __global__ __launch_bounds__(kEvictThreads) void evict_kernel(EvictArgs a) {
 }
 
 // Positions of a block where several share a request. In chunks of 4096 four times as many blocks count as in
-// chunks of 16384, and each reads four times as many histograms: 32 against 36 us for 131072 positions,
-// 38 against 40 for 200000, 43 against 39 for 262144 (the reads grow with the square).
+// chunks of 16384, and each reads four times as many histograms (the reads grow with the square): 30.1 against 34.0 us
+// for one request of 131072 positions, 35.9 / 37.5 for 196608, 36.6 / 38.2 for 200000, 38.8 / 38.2 for 212992,
+// 38.7 / 39.2 for 229376, 41.7 / 37.6 for 262144; four requests 33.5 / 35.0, 37.4 / 39.0, 38.3 / 39.9, 40.6 / 40.0,
+// 40.5 / 40.9, 43.8 / 39.4. The limit lies where they first meet, by whole chunks of 16384. (It does not look at the number of
+// requests: 16 of 131072 positions take 50.0 / 40.7, 16 of 65536 28.4 / 36.3.)
 static int evict_per(int64_t most) { return most <= kEvictSmall ? 4 : 16; }
 
 template <int STEP, int PER>

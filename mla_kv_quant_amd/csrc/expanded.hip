@@ -9,8 +9,11 @@
 // query's scores and they become the next product's operand, O^T += V^T P^T, where they are (values
 // are read transposed from LDS). One stream of matrix instructions interleaves a step's scores with the
 // output of the step before and has its weights formed in between: exp2 of scaled scores less a
-// reference that moves only when a step's sum of weights passes 256, so that no maximum is formed;
-// sums are of the weights as rounded to bf16, by which the output's weights add up to one.
+// reference that moves only when a step's sum of weights passes 256, so that no maximum is formed.
+// Weights are rounded to bf16, the type of the values that they are multiplied with (fp16 is three bits
+// finer, but has no place for values above 65504, and two bf16 parts would double the second product); sums are of the
+// weights as rounded, by which the output's weights add up to one. Outputs are off by 0.0019 to 0.0022 of their norm;
+// rounded once from the exact ones they would be by 0.0017.
 //
 // Bound: matrix instructions at the clock that the power limit leaves, two waves to a SIMD: 16 heads of 4 x 4096
 // queries 330 to 400 us by card (344 GFLOP, 0.86 to 1.04 PFLOP/s; a large library product reaches 1.24), 55 % of the
@@ -18,7 +21,10 @@
 // weights' arithmetic it takes 20 to 30 % less, without the copies 15 %, without the reads of keys and values 6 %.
 // 256 rows a block, 64 rows a wave (one wave to a SIMD), rings of 8 steps and operands read 9
 // instructions ahead were no faster (480 us for 430 with 64 rows).
-// Few rows behind long keys: bound by the keys' bytes (8 x 16 queries behind 4096, 16 heads: 59 us, 275 MB).
+// Few rows behind long keys: bound by the keys' bytes (8 x 16 queries behind 4096, 16 heads: 59 us, 275 MB). A row block
+// of up to 32 rows leaves three of its waves to copy alone.
+// (Of the 256 registers a wave has, 6 to 120 are spilled, in the repeated pass of blocks with outputs that are not finite
+// alone.)
 #include "rolaq_common.h"
 #include "mx4_request.h"
 #include "mx4_tile.h"

@@ -137,7 +137,7 @@ hipError_t launch_rotary(RotaryArgs a, int num_cus, hipStream_t stream) {
   const int64_t wanted = (threads + a.T * a.groups - 1) / (a.T * a.groups);
   a.slots = (int)std::min<int64_t>({(int64_t)room, (int64_t)a.H, std::max<int64_t>(wanted, (a.H + 3) / 4)});
   a.tokens = std::max(1, 256 / (a.groups * a.slots));
-  // (as many as are resident)
+  // (eight blocks a CU: two turns of the four of the 16-byte bf16 kernels that are resident, by their 103 and 124 registers)
   const int64_t blocks = std::min<int64_t>((a.T + a.tokens - 1) / a.tokens, 8 * num_cus);
   hipLaunchKernelGGL((rotary_kernel<TYPE, TWO, V>), dim3((unsigned)blocks), dim3(256), 0, stream, a);
   return hipGetLastError();
