@@ -17,7 +17,7 @@
 // positions under 16 heads of width 512, 210 MB at 4.3 TB/s. Many rows (the last queries of prompts): a
 // wave keeps its positions expanded in registers, and the rows come to LDS 64 at a time (32 of width
 // 512) while the last ones are in use, the weights of 16 rows between the products of the next 16; bound by
-// the matrix instructions, their operands' reads and the exponentials in turn: 88 to 90 us (95 under the profiler) for
+// the matrix instructions, their operands' reads and the exponentials in turn: 88 to 91 us (95 under the profiler) for
 // 32 queries of 40 heads of width 256 in 8 requests of 8192 to 16384 positions, 69 GFLOP; 73 with the products alone,
 // 17 with one step alone (139 with 16 rows at a time and tiles of 256 positions a block, of which a part of
 // the blocks had one and the rest two). At width 256 46 registers are spilled there, which steps load before their
